@@ -1,0 +1,534 @@
+// The linear layer with its epilogue, and its backward products.
+//
+//   y = act(x W^T + bias) + residual
+//   dz = dy act'(z);  dx = dz W;  dW = dz^T x;  dbias = sum over rows of dz
+//
+// Sums are held in fp32 by the matrix cores; z, y, dz and the gradients are rounded once, to
+// the tensors' dtype, as they are stored.  z is stored for the backward pass: dz is formed
+// from its rounded values, which moves act' by at most one rounding of its argument.
+#include "hbt_matmul.hpp"
+
+namespace hbt {
+namespace mm {
+namespace {
+
+// ---- activations ---------------------------------------------------------------------
+// 1 / (1 + exp(-t)).  2-byte results take the hardware exponential and reciprocal (about one
+// fp32 ulp each, far below their rounding); fp32 results the accurate functions.
+template <int D>
+__device__ __forceinline__ float sigmoid(float t) {
+    if constexpr (D == HBT_DTYPE_F32) return 1.0f / (1.0f + expf(-t));
+    else return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t * -1.44269504f));
+}
+constexpr float kGeluC = 0.79788456f;  // sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;
+
+template <int D>
+__device__ __forceinline__ float activate(float z, int act) {
+    switch (act) {
+        case HBT_ACT_RELU: return z < 0.0f ? 0.0f : z;  // a NaN stays one
+        case HBT_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+        // (1 + tanh(u)) / 2 = sigmoid(2 u)
+        case HBT_ACT_GELU_TANH: return z * sigmoid<D>(2.0f * kGeluC * (z + kGeluA * z * z * z));
+        case HBT_ACT_SILU: return z * sigmoid<D>(z);
+        default: return z;
+    }
+}
+template <int D>
+__device__ __forceinline__ float slope(float z, int act) {
+    switch (act) {
+        case HBT_ACT_RELU: return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
+        case HBT_ACT_GELU:
+            return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * expf(-0.5f * z * z) * 0.39894228f;
+        case HBT_ACT_GELU_TANH: {
+            const float s = sigmoid<D>(2.0f * kGeluC * (z + kGeluA * z * z * z));
+            return s + z * s * (1.0f - s) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * z * z);
+        }
+        case HBT_ACT_SILU: {
+            const float s = sigmoid<D>(z);
+            return s * (1.0f + z * (1.0f - s));
+        }
+        default: return 1.0f;
+    }
+}
+
+// ---- the product ---------------------------------------------------------------------
+struct ProductArgs {
+    const void* a;
+    const void* b;
+    const void* bias;
+    const void* residual;
+    void* y;
+    void* z;
+    float* partial;  // [splits][m][ldp], when the sum over k is split
+    int64_t lda, ldb, ldr, ldy, ldz, ldp, m, n, k, k_split;
+    int tiles_m, tiles_n, act;
+};
+
+// Four results of row i from column j: bias, activation, residual, each store rounded once.
+template <int D>
+__device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_t j, f32x4 v) {
+    if (j + 4 <= p.n) {
+        if (p.bias != nullptr) v += load4<D>(p.bias, j);
+        if (p.z != nullptr) store4<D>(p.z, i * p.ldz + j, v);
+        if (p.act != HBT_ACT_NONE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = activate<D>(v[e], p.act);
+        }
+        if (p.residual != nullptr) v += load4<D>(p.residual, i * p.ldr + j);
+        store4<D>(p.y, i * p.ldy + j, v);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+        if (j + e >= p.n) break;
+        float x = v[e];
+        if (p.bias != nullptr) x += load_elem<D>(p.bias, j + e);
+        if (p.z != nullptr) store_elem<D>(p.z, i * p.ldz + j + e, x);
+        x = activate<D>(x, p.act);
+        if (p.residual != nullptr) x += load_elem<D>(p.residual, i * p.ldr + j + e);
+        store_elem<D>(p.y, i * p.ldy + j + e, x);
+    }
+}
+
+template <int D, bool kA, bool kB, class T>
+__global__ __launch_bounds__(T::kThreads) void product_kernel(ProductArgs p) {
+    extern __shared__ __align__(16) char lds[];
+    const int t = xcd_tile(blockIdx.x, gridDim.x);
+    int tm, tn;
+    band_order<8>(t, p.tiles_m, p.tiles_n, tm, tn);
+    const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
+    const int64_t k0 = blockIdx.y * p.k_split, k1 = min(p.k, k0 + p.k_split);
+    f32x4 acc[T::TM][T::TN];
+    tile_product<D, kA, kB, T>(p.a, p.lda, m0, p.m, p.b, p.ldb, n0, p.n, k0, k1, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t mw = m0 + (wave / T::WN) * (T::BM / T::WM) + (lane & 15);
+    const int64_t nw = n0 + (wave % T::WN) * (T::BN / T::WN) + 4 * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) {
+        const int64_t m = mw + 16 * i;
+        if (m >= p.m) continue;
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j) {
+            const int64_t n = nw + 16 * j;
+            if (n >= p.n) continue;
+            if (p.partial != nullptr)
+                *reinterpret_cast<f32x4*>(p.partial + (blockIdx.y * p.m + m) * p.ldp + n) = acc[i][j];
+            else
+                epilogue<D>(p, m, n, acc[i][j]);
+        }
+    }
+}
+
+// Joins the parts of a split sum, in their order, and finishes the result.
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(ProductArgs p, int splits) {
+    const int64_t units = p.ldp / 4, total = p.m * units;
+    for (int64_t u = blockIdx.x * int64_t(256) + threadIdx.x; u < total; u += int64_t(gridDim.x) * 256) {
+        const int64_t m = u / units, n = u % units * 4;
+        f32x4 v = *reinterpret_cast<const f32x4*>(p.partial + m * p.ldp + n);
+        for (int s = 1; s < splits; ++s)
+            v += *reinterpret_cast<const f32x4*>(p.partial + (s * p.m + m) * p.ldp + n);
+        epilogue<D>(p, m, n, v);
+    }
+}
+
+// ---- few rows ------------------------------------------------------------------------
+// At most 16 rows of x: the product is the read of W.  A workgroup of 8 waves forms 16
+// columns of y; its waves take k-steps in turn straight from global memory, each wave
+// instruction covering 64 bytes of 16 rows of W, and their sums meet in LDS.
+template <int D>
+__global__ __launch_bounds__(512) void thin_kernel(ProductArgs p) {
+    constexpr int E = unit_elems<D>(), kStep = 4 * E, kWaves = 8, kUnroll = 4, B = elem_bytes<D>();
+    __shared__ f32x4 sums[kWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, q = lane >> 4;
+    const int64_t n0 = int64_t(blockIdx.x) * 16;
+    const bool w_in = n0 + row < p.n, x_in = row < p.m;
+    const char* w = static_cast<const char*>(p.b) + ((n0 + (w_in ? row : 0)) * p.ldb + q * E) * B;
+    const char* x = static_cast<const char*>(p.a) + ((x_in ? row : 0) * p.lda + q * E) * B;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const int64_t whole = p.k / kStep;
+    int64_t s = wave;
+    for (; s + (kUnroll - 1) * kWaves < whole; s += kUnroll * kWaves) {
+        u32x4 fw[kUnroll], fx[kUnroll];
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i) {
+            const int64_t at = (s + i * kWaves) * kStep * B;
+            fw[i] = load16(w + at);
+            fx[i] = load16(x + at);
+        }
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i) {
+            if (!x_in) fx[i] = u32x4{0, 0, 0, 0};
+            acc = mma<D>(fw[i], fx[i], acc);
+        }
+    }
+    for (; s < whole; s += kWaves) {
+        const u32x4 fw = load16(w + s * kStep * B);
+        u32x4 fx = load16(x + s * kStep * B);
+        if (!x_in) fx = u32x4{0, 0, 0, 0};
+        acc = mma<D>(fw, fx, acc);
+    }
+    if (wave == whole % kWaves && whole * kStep < p.k) {  // the last, partial step
+        u32x4 fw = {0, 0, 0, 0}, fx = {0, 0, 0, 0};
+        const int64_t at = whole * kStep;
+        for (int e = 0; e < E; ++e) {
+            if (at + q * E + e >= p.k) break;
+            if constexpr (B == 4) {
+                fw[e] = reinterpret_cast<const uint32_t*>(w)[at + e];
+                if (x_in) fx[e] = reinterpret_cast<const uint32_t*>(x)[at + e];
+            } else {
+                fw[e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(w)[at + e]) << (16 * (e % 2));
+                if (x_in) fx[e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(x)[at + e]) << (16 * (e % 2));
+            }
+        }
+        acc = mma<D>(fw, fx, acc);
+    }
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) acc += sums[i][lane];
+        const int64_t n = n0 + 4 * q;
+        if (x_in && n < p.n) epilogue<D>(p, row, n, acc);
+    }
+}
+
+// ---- the gradient before the products ---------------------------------------------------
+struct SlopeArgs {
+    const void* dy;
+    const void* z;
+    void* dz;
+    float* partial;  // [row blocks][ldp] column sums, or null
+    int64_t lddy, ldz, lddz, ldp, m, n;
+    int rows_per_block, act;
+};
+
+// dz = dy act'(z) over a block of rows by 256 columns (four a lane), and the block's column
+// sums in row order: each of four waves adds every fourth row, and the four meet in LDS.
+template <int D>
+__global__ __launch_bounds__(256) void slope_kernel(SlopeArgs p) {
+    __shared__ f32x4 sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t j = (int64_t(blockIdx.x) * 64 + lane) * 4;
+    const int64_t first = int64_t(blockIdx.y) * p.rows_per_block, last = min(p.m, first + p.rows_per_block);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (j + 4 <= p.n) {
+#pragma unroll 4
+        for (int64_t i = first + wave; i < last; i += 4) {
+            f32x4 g = load4<D>(p.dy, i * p.lddy + j);
+            if (p.act != HBT_ACT_NONE) {
+                const f32x4 z = load4<D>(p.z, i * p.ldz + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) g[e] *= slope<D>(z[e], p.act);
+            }
+            if (p.dz != nullptr) store4<D>(p.dz, i * p.lddz + j, g);
+            sum += g;
+        }
+    } else if (j < p.n) {
+        for (int64_t i = first + wave; i < last; i += 4) {
+            for (int e = 0; e < 3; ++e) {
+                if (j + e >= p.n) break;
+                float g = load_elem<D>(p.dy, i * p.lddy + j + e);
+                if (p.act != HBT_ACT_NONE) g *= slope<D>(load_elem<D>(p.z, i * p.ldz + j + e), p.act);
+                if (p.dz != nullptr) store_elem<D>(p.dz, i * p.lddz + j + e, g);
+                sum[e] += g;
+            }
+        }
+    }
+    if (p.partial == nullptr) return;
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && j < p.n) {
+        sum = ((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane];
+        *reinterpret_cast<f32x4*>(p.partial + blockIdx.y * p.ldp + j) = sum;  // ldp: a multiple of 4
+    }
+}
+
+// dbias: the row blocks' column sums, added in their order.
+template <int D>
+__global__ __launch_bounds__(256) void bias_kernel(const float* partial, int64_t ldp, int blocks, void* db, int64_t n) {
+    __shared__ float sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t j = int64_t(blockIdx.x) * 64 + lane;
+    float sum = 0.0f;
+    if (j < n) {
+        for (int b = wave; b < blocks; b += 4) sum += partial[b * ldp + j];
+    }
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && j < n)
+        store_elem<D>(db, j, ((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]);
+}
+
+// ---- host ----------------------------------------------------------------------------
+using Tile256 = Tile<256, 256, 2, 4>;
+using Tile128 = Tile<128, 128, 2, 2>;
+using Tile64 = Tile<64, 64, 2, 2>;
+
+struct Choice {
+    int tile;    // 256, 128 or 64
+    int splits;  // parts the sum over k is split into
+};
+
+constexpr int kMaxSplits = 16;
+
+Choice choose(int64_t m, int64_t n, int64_t k, int dtype) {
+    const int bk = dtype == HBT_DTYPE_F32 ? 32 : 64;
+    const int64_t cus = 256;
+    const auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+    if (dtype != HBT_DTYPE_F32 && tiles(256) >= cus) return {256, 1};
+    const int tile = tiles(128) >= cus ? 128 : 64;
+    const int64_t count = tiles(tile), steps = (k + bk - 1) / bk;
+    int64_t splits = 1;
+    if (count < cus) splits = std::min<int64_t>({2 * cus / std::max<int64_t>(count, 1), steps / 8, kMaxSplits});
+    return {tile, static_cast<int>(std::max<int64_t>(splits, 1))};
+}
+
+template <int D, bool kA, bool kB, class T>
+int32_t launch_tile(const char* who, ProductArgs& p, int splits, hipStream_t stream) {
+    constexpr int kLds = lds_bytes<D, T>();
+    p.tiles_m = static_cast<int>((p.m + T::BM - 1) / T::BM);
+    p.tiles_n = static_cast<int>((p.n + T::BN - 1) / T::BN);
+    if constexpr (kLds > 65536) {
+        static const hipError_t set = hipFuncSetAttribute(
+            reinterpret_cast<const void*>(product_kernel<D, kA, kB, T>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+        if (set != hipSuccess) return check_hip(set, who);
+    }
+    product_kernel<D, kA, kB, T><<<dim3(p.tiles_m * p.tiles_n, splits), T::kThreads, kLds, stream>>>(p);
+    return check_launch(who);
+}
+
+template <int D, bool kA, bool kB>
+int32_t launch_product(const char* who, ProductArgs& p, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+    Choice c = choose(p.m, p.n, p.k, D);
+    constexpr int BK = tile_k<D>();
+    p.ldp = (p.n + 3) / 4 * 4;
+    while (c.splits > 1 && 4 * c.splits * p.m * p.ldp > workspace_bytes) --c.splits;
+    p.k_split = p.k;
+    p.partial = nullptr;
+    if (c.splits > 1) {
+        p.k_split = ((p.k + c.splits - 1) / c.splits + BK - 1) / BK * BK;
+        c.splits = static_cast<int>((p.k + p.k_split - 1) / p.k_split);
+        if (c.splits > 1) p.partial = static_cast<float*>(workspace);
+    }
+    int32_t status;
+    if constexpr (D == HBT_DTYPE_F32) {
+        status = c.tile == 128 ? launch_tile<D, kA, kB, Tile128>(who, p, c.splits, stream)
+                               : launch_tile<D, kA, kB, Tile64>(who, p, c.splits, stream);
+    } else {
+        status = c.tile == 256   ? launch_tile<D, kA, kB, Tile256>(who, p, c.splits, stream)
+                 : c.tile == 128 ? launch_tile<D, kA, kB, Tile128>(who, p, c.splits, stream)
+                                 : launch_tile<D, kA, kB, Tile64>(who, p, c.splits, stream);
+    }
+    if (status != HBT_OK || c.splits == 1) return status;
+    const int64_t blocks = std::min<int64_t>((p.m * (p.ldp / 4) + 255) / 256, 4096);
+    join_kernel<D><<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(p, c.splits);
+    return check_launch(who);
+}
+
+int32_t fail(const char* who, const char* what) {
+    set_error("%s: %s", who, what);
+    return HBT_ERR_INVALID_ARGUMENT;
+}
+
+// Rows of a tile are addressed by 31-bit byte offsets from its first one.
+constexpr int64_t kMaxLd = int64_t(1) << 20;
+// Tile and column-block counts stay far inside a grid's limits.
+constexpr int64_t kMaxSide = int64_t(1) << 27;
+
+int32_t check_matrix(const char* who, const void* p, int64_t rows, int64_t cols, int64_t ld, const char* name) {
+    if (rows == 0 || cols == 0) return HBT_OK;
+    if (p == nullptr) {
+        set_error("%s: %s is null", who, name);
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    if (ld < cols) {
+        set_error("%s: rows of %s overlap (%lld elements apart, %lld long)", who, name, static_cast<long long>(ld),
+                  static_cast<long long>(cols));
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    if (ld > kMaxLd) {
+        set_error("%s: rows of %s are %lld elements apart; at most %lld", who, name, static_cast<long long>(ld),
+                  static_cast<long long>(kMaxLd));
+        return HBT_ERR_UNSUPPORTED;
+    }
+    return HBT_OK;
+}
+
+int32_t check_sizes(const char* who, int64_t m, int64_t n, int64_t k, int32_t dtype) {
+    if (m < 0 || n < 0 || k < 0) return fail(who, "a size is negative");
+    if (dtype != HBT_DTYPE_F32 && dtype != HBT_DTYPE_BF16 && dtype != HBT_DTYPE_F16) {
+        set_error("%s: dtype %d is not F32, BF16 or F16", who, dtype);
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    if (m > kMaxSide || n > kMaxSide || k > kMaxSide || ((m + 63) / 64) * ((n + 63) / 64) > 0x7FFFFFFF) {
+        set_error("%s: sizes %lld x %lld x %lld are past the launch limits", who, static_cast<long long>(m),
+                  static_cast<long long>(n), static_cast<long long>(k));
+        return HBT_ERR_UNSUPPORTED;
+    }
+    return HBT_OK;
+}
+
+int64_t split_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype) {
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    const Choice c = choose(m, n, k, dtype);
+    return c.splits == 1 ? 0 : 4 * c.splits * m * ((n + 3) / 4 * 4);
+}
+
+// Rows per block of the slope pass: enough blocks for the device, few enough partial sums.
+int rows_per_block(int64_t m, int64_t n) {
+    const int64_t columns = (n + 255) / 256;
+    int64_t rows = m * columns / 2048;
+    rows = std::min<int64_t>(std::max<int64_t>(rows, 16), 256);
+    while ((m + rows - 1) / rows > 65535) rows *= 2;
+    return static_cast<int>(rows);
+}
+
+template <typename F>
+int32_t by_dtype(int32_t dtype, F&& f) {
+    if (dtype == HBT_DTYPE_F32) return f(std::integral_constant<int, HBT_DTYPE_F32>{});
+    if (dtype == HBT_DTYPE_BF16) return f(std::integral_constant<int, HBT_DTYPE_BF16>{});
+    return f(std::integral_constant<int, HBT_DTYPE_F16>{});
+}
+
+}  // namespace
+}  // namespace mm
+}  // namespace hbt
+
+using namespace hbt;
+using namespace hbt::mm;
+
+extern "C" {
+
+int64_t hbt_linear_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t which) {
+    if (tokens < 0 || inner < 0 || outer < 0) return -1;
+    if (dtype != HBT_DTYPE_F32 && dtype != HBT_DTYPE_BF16 && dtype != HBT_DTYPE_F16) return -1;
+    switch (which) {
+        case HBT_LINEAR_FORWARD: return tokens <= 16 ? 0 : split_bytes(tokens, outer, inner, dtype);
+        case HBT_LINEAR_SLOPE: {
+            if (tokens == 0 || outer == 0) return 0;
+            const int64_t rows = rows_per_block(tokens, outer);
+            return 4 * ((tokens + rows - 1) / rows) * ((outer + 3) / 4 * 4);
+        }
+        case HBT_LINEAR_GRAD_INPUT: return split_bytes(tokens, inner, outer, dtype);
+        case HBT_LINEAR_GRAD_WEIGHT: return split_bytes(outer, inner, tokens, dtype);
+        default: return -1;
+    }
+}
+
+int32_t hbt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
+                   int64_t ldr, void* y, int64_t ldy, void* z, int64_t ldz, int64_t tokens, int64_t inner,
+                   int64_t outer, int32_t dtype, int32_t activation, void* workspace, int64_t workspace_bytes,
+                   void* stream) {
+    clear_error();
+    const char* who = "hbt_linear";
+    int32_t status = check_sizes(who, tokens, outer, inner, dtype);
+    if (status != HBT_OK) return status;
+    if (activation < HBT_ACT_NONE || activation > HBT_ACT_SILU) return fail(who, "unknown activation");
+    if (tokens == 0 || outer == 0) return HBT_OK;
+    if ((status = check_matrix(who, x, tokens, inner, ldx, "x")) != HBT_OK ||
+        (status = check_matrix(who, w, outer, inner, ldw, "w")) != HBT_OK ||
+        (status = check_matrix(who, y, tokens, outer, ldy, "y")) != HBT_OK)
+        return status;
+    if (residual != nullptr && (status = check_matrix(who, residual, tokens, outer, ldr, "residual")) != HBT_OK)
+        return status;
+    if (z != nullptr && (status = check_matrix(who, z, tokens, outer, ldz, "z")) != HBT_OK) return status;
+    ProductArgs p{};
+    p.a = x, p.b = w, p.bias = bias, p.residual = residual, p.y = y, p.z = z;
+    p.lda = ldx, p.ldb = ldw, p.ldr = ldr, p.ldy = ldy, p.ldz = ldz;
+    p.m = tokens, p.n = outer, p.k = inner, p.act = activation;
+    const hipStream_t s = as_stream(stream);
+    return by_dtype(dtype, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if (tokens <= 16) {
+            thin_kernel<D><<<dim3(static_cast<unsigned>((outer + 15) / 16)), 512, 0, s>>>(p);
+            return check_launch(who);
+        }
+        return launch_product<D, true, true>(who, p, workspace, workspace == nullptr ? 0 : workspace_bytes, s);
+    });
+}
+
+int32_t hbt_linear_slope(const void* dy, int64_t lddy, const void* z, int64_t ldz, void* dz, int64_t lddz, void* dbias,
+                         int64_t tokens, int64_t outer, int32_t dtype, int32_t activation, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* who = "hbt_linear_slope";
+    int32_t status = check_sizes(who, tokens, outer, 0, dtype);
+    if (status != HBT_OK) return status;
+    if (activation < HBT_ACT_NONE || activation > HBT_ACT_SILU) return fail(who, "unknown activation");
+    if (outer == 0) return HBT_OK;
+    if ((status = check_matrix(who, dy, tokens, outer, lddy, "dy")) != HBT_OK) return status;
+    if (activation != HBT_ACT_NONE && (status = check_matrix(who, z, tokens, outer, ldz, "z")) != HBT_OK)
+        return status;
+    if (dz != nullptr && (status = check_matrix(who, dz, tokens, outer, lddz, "dz")) != HBT_OK) return status;
+    SlopeArgs p{};
+    p.dy = dy, p.z = z, p.dz = dz, p.lddy = lddy, p.ldz = ldz, p.lddz = lddz;
+    p.m = tokens, p.n = outer, p.act = activation, p.ldp = (outer + 3) / 4 * 4;
+    p.rows_per_block = rows_per_block(std::max<int64_t>(tokens, 1), outer);
+    const int64_t blocks = (tokens + p.rows_per_block - 1) / p.rows_per_block;
+    if (dbias != nullptr && tokens > 0) {
+        if (workspace == nullptr || workspace_bytes < 4 * blocks * p.ldp) return fail(who, "the workspace is too small");
+        p.partial = static_cast<float*>(workspace);
+    }
+    const hipStream_t s = as_stream(stream);
+    return by_dtype(dtype, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if (blocks > 0) {
+            slope_kernel<D><<<dim3(static_cast<unsigned>((outer + 255) / 256), static_cast<unsigned>(blocks)), 256, 0,
+                              s>>>(p);
+            const int32_t launched = check_launch(who);
+            if (launched != HBT_OK) return launched;
+        }
+        if (dbias == nullptr) return HBT_OK;
+        bias_kernel<D><<<dim3(static_cast<unsigned>((outer + 63) / 64)), 256, 0, s>>>(
+            p.partial, p.ldp, static_cast<int>(blocks), dbias, outer);
+        return check_launch(who);
+    });
+}
+
+int32_t hbt_linear_grad_input(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx,
+                              int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* who = "hbt_linear_grad_input";
+    int32_t status = check_sizes(who, tokens, inner, outer, dtype);
+    if (status != HBT_OK) return status;
+    if (tokens == 0 || inner == 0) return HBT_OK;
+    if ((status = check_matrix(who, dz, tokens, outer, lddz, "dz")) != HBT_OK ||
+        (status = check_matrix(who, w, outer, inner, ldw, "w")) != HBT_OK ||
+        (status = check_matrix(who, dx, tokens, inner, lddx, "dx")) != HBT_OK)
+        return status;
+    ProductArgs p{};
+    p.a = dz, p.b = w, p.y = dx, p.lda = lddz, p.ldb = ldw, p.ldy = lddx;
+    p.m = tokens, p.n = inner, p.k = outer, p.act = HBT_ACT_NONE;
+    return by_dtype(dtype, [&](auto d) {
+        return launch_product<decltype(d)::value, true, false>(who, p, workspace,
+                                                               workspace == nullptr ? 0 : workspace_bytes,
+                                                               as_stream(stream));
+    });
+}
+
+int32_t hbt_linear_grad_weight(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw,
+                               int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* who = "hbt_linear_grad_weight";
+    int32_t status = check_sizes(who, outer, inner, tokens, dtype);
+    if (status != HBT_OK) return status;
+    if (outer == 0 || inner == 0) return HBT_OK;
+    if ((status = check_matrix(who, dz, tokens, outer, lddz, "dz")) != HBT_OK ||
+        (status = check_matrix(who, x, tokens, inner, ldx, "x")) != HBT_OK ||
+        (status = check_matrix(who, dw, outer, inner, lddw, "dw")) != HBT_OK)
+        return status;
+    ProductArgs p{};
+    p.a = dz, p.b = x, p.y = dw, p.lda = lddz, p.ldb = ldx, p.ldy = lddw;
+    p.m = outer, p.n = inner, p.k = tokens, p.act = HBT_ACT_NONE;
+    return by_dtype(dtype, [&](auto d) {
+        return launch_product<decltype(d)::value, false, false>(who, p, workspace,
+                                                                workspace == nullptr ? 0 : workspace_bytes,
+                                                                as_stream(stream));
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,319 @@
+// Tile products on the matrix cores (gfx950), shared by the linear layer and the
+// orthogonalised update.
+//
+// A workgroup forms one BM x BN tile of C[m][n] = sum_k A(m, k) B(n, k).  Each operand is
+// stored either k-major (the k of one row consecutive: x and W of y = x W^T) or
+// row-major in the other sense (the rows of one k consecutive: both operands of
+// dW = dz^T x), so the three products of a layer and its backward pass, and the Gram and
+// iterate products of a Newton-Schulz step, read every matrix where it lies.
+//
+// Global memory goes through registers into one of two LDS buffers, in 16-byte units: the
+// next tile but one is in flight while the current one feeds the matrix cores, with one
+// barrier per k-tile.  A unit out of range is read at an offset past the buffer's end,
+// which returns zeros; a unit that straddles an edge is read element by element.
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "hbt_common.hpp"
+
+namespace hbt {
+namespace mm {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+template <int D>
+constexpr int elem_bytes() { return D == HBT_DTYPE_F32 ? 4 : 2; }
+// Elements of a 16-byte unit.
+template <int D>
+constexpr int unit_elems() { return 16 / elem_bytes<D>(); }
+// Elements of k per tile: 128 bytes.
+template <int D>
+constexpr int tile_k() { return 128 / elem_bytes<D>(); }
+
+template <int D>
+__device__ __forceinline__ float load_elem(const void* p, int64_t i) {
+    if constexpr (D == HBT_DTYPE_F32) return static_cast<const float*>(p)[i];
+    else return b16_to_f32<D == HBT_DTYPE_F16>(static_cast<const uint16_t*>(p)[i]);
+}
+template <int D>
+__device__ __forceinline__ void store_elem(void* p, int64_t i, float v) {
+    if constexpr (D == HBT_DTYPE_F32) static_cast<float*>(p)[i] = v;
+    else static_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(f32_to_b16<D == HBT_DTYPE_F16>(v));
+}
+// Four consecutive elements from any element boundary.
+template <int D>
+__device__ __forceinline__ f32x4 load4(const void* p, int64_t i) {
+    f32x4 v;
+    if constexpr (D == HBT_DTYPE_F32) {
+        typedef float u __attribute__((ext_vector_type(4), aligned(4)));
+        const u x = *reinterpret_cast<const u*>(static_cast<const float*>(p) + i);
+        v = f32x4{x[0], x[1], x[2], x[3]};
+    } else {
+        typedef uint32_t u __attribute__((ext_vector_type(2), aligned(2)));
+        const u x = *reinterpret_cast<const u*>(static_cast<const uint16_t*>(p) + i);
+        constexpr bool H = D == HBT_DTYPE_F16;
+        v = f32x4{b16_to_f32<H>(x[0] & 0xFFFFu), b16_to_f32<H>(x[0] >> 16), b16_to_f32<H>(x[1] & 0xFFFFu),
+                  b16_to_f32<H>(x[1] >> 16)};
+    }
+    return v;
+}
+template <int D>
+__device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
+    if constexpr (D == HBT_DTYPE_F32) {
+        typedef float u __attribute__((ext_vector_type(4), aligned(4)));
+        *reinterpret_cast<u*>(static_cast<float*>(p) + i) = u{v[0], v[1], v[2], v[3]};
+    } else {
+        typedef uint32_t u __attribute__((ext_vector_type(2), aligned(2)));
+        *reinterpret_cast<u*>(static_cast<uint16_t*>(p) + i) =
+            u{pack2_rounded<D>(v[0], v[1]), pack2_rounded<D>(v[2], v[3])};
+    }
+}
+
+// 16 bytes from any element boundary.
+__device__ __forceinline__ u32x4 load16(const char* at) {
+    typedef uint32_t u __attribute__((ext_vector_type(4), aligned(2)));
+    const u v = *reinterpret_cast<const u*>(at);
+    return u32x4{v[0], v[1], v[2], v[3]};
+}
+
+// c += a b over one 16-byte fragment pair: 32 values of k in 2-byte types (one
+// instruction), 16 in fp32 (four).  Lane l holds row l % 16 of each operand and the unit of
+// k that its quarter l / 16 names; the order of k inside a fragment is the same in both.
+// The result has element [4 (l / 16) + r][l % 16] of (first operand's row, second's).
+template <int D>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (D == HBT_DTYPE_F16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
+                                                      0, 0, 0);
+    } else if constexpr (D == HBT_DTYPE_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                       c, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+        return c;
+    }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
+}
+// An offset past every buffer's end: reads zeros.
+constexpr uint32_t kNowhere = 0xFFFFFF00u;
+
+// One operand's share of a tile: ROWS rows (m or n) by tile_k of k, moved by THREADS lanes.
+// kKMajor: element (row, k) at base[row * ld + k]; else at base[k * ld + row].
+template <int D, bool kKMajor, int ROWS, int THREADS>
+struct Operand {
+    static constexpr int E = unit_elems<D>(), BK = tile_k<D>(), B = elem_bytes<D>();
+    static constexpr int kUnitsPerLine = kKMajor ? BK / E : ROWS / E;  // units per LDS line
+    static constexpr int kLineBytes = kUnitsPerLine * 16;
+    static constexpr int kUnits = ROWS * BK / E / THREADS;  // units per lane
+    static constexpr int kBytes = ROWS * BK * B;
+    static_assert(ROWS * BK / E % THREADS == 0, "whole units per lane");
+
+    const char* base;      // the tile's first row (k-major) or column at k = 0
+    int64_t ld;            // elements between rows (k-major) or between k
+    int rows;              // rows of the operand from the tile's first one
+    uint32_t offset[kUnits];
+    u32x4 held[kUnits];
+    bool straddles;        // some lane's unit crosses the last row (not k-major)
+
+    // LDS position of a unit: lines are XOR-swizzled in units so that the 16 rows of a
+    // fragment read (k-major), or the four k of a transposing read, fall on distinct banks.
+    static __device__ __forceinline__ int swizzle(int line) {
+        if constexpr (kKMajor) return line & 7;
+        else if constexpr (B == 2) return (line & 3) << 1;
+        else return ((line >> 2) & 3) << 2;
+    }
+
+    __device__ __forceinline__ void init(const void* p, int64_t ld_, int64_t row0, int64_t row_count, int tid) {
+        ld = ld_;
+        rows = static_cast<int>(row_count - row0 < ROWS ? row_count - row0 : ROWS);
+        base = static_cast<const char*>(p) + (kKMajor ? row0 * ld_ : row0) * B;
+        straddles = !kKMajor && rows < ROWS && rows % E != 0;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
+            const bool in = kKMajor ? line < rows : (at + 1) * E <= rows;
+            offset[i] = in ? static_cast<uint32_t>(line * ld * B) + at * 16 : kNowhere;
+        }
+    }
+
+    // The lane's units of the k-tile [k0, k0 + BK), of which `left` values of k exist.
+    __device__ __forceinline__ void load(int64_t k0, int left, int tid) {
+        const char* at_k = base + (kKMajor ? k0 : k0 * ld) * B;
+        const auto buffer = buffer_at(at_k);
+        if (left >= BK) {
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i)
+                held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset[i], 0, 0));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
+                const bool in = kKMajor ? (at + 1) * E <= left : line < left;
+                held[i] = __builtin_bit_cast(
+                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, in ? offset[i] : kNowhere, 0, 0));
+            }
+        }
+        if (straddles || (kKMajor && left < BK && left % E != 0)) load_edge(at_k, left, tid);
+    }
+
+    // Units that cross the last row or the last k, element by element.
+    __device__ __forceinline__ void load_edge(const char* at_k, int left, int tid) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
+            const int have = (kKMajor ? left : rows) - at * E;  // elements of the unit that exist
+            const bool line_in = kKMajor ? line < rows : line < left;
+            if (line_in && have > 0 && have < E) {
+                u32x4 v = {0, 0, 0, 0};
+                const int64_t first = line * ld + at * E;
+#pragma unroll
+                for (int e = 0; e < E - 1; ++e) {
+                    if (e < have) {
+                        if constexpr (B == 4) v[e] = reinterpret_cast<const uint32_t*>(at_k)[first + e];
+                        else v[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(at_k)[first + e])
+                                         << (16 * (e % 2));
+                    }
+                }
+                held[i] = v;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
+            *reinterpret_cast<u32x4*>(lds + line * kLineBytes + ((at ^ swizzle(line)) << 4)) = held[i];
+        }
+    }
+
+    // The fragment of rows [row, row + 16), k-units 4 * step .. 4 * step + 3 of the tile.
+    static __device__ __forceinline__ u32x4 fragment(const char* lds, int row, int step, int lane) {
+        const int q = step * 4 + (lane >> 4);
+        if constexpr (kKMajor) {
+            const int line = row + (lane & 15);
+            return *reinterpret_cast<const u32x4*>(lds + line * kLineBytes + ((q ^ swizzle(line)) << 4));
+        } else if constexpr (B == 2) {
+            // A transposing read takes 4 values of k by 16 rows per quarter wave: lane i of it
+            // addresses k = i / 4, rows 4 (i % 4) .. + 3, and receives row i's four values.
+            const int i = lane & 15, line = q * 8 + (i >> 2), r = row + (i & 3) * 4;
+            const int at = line * kLineBytes + (((r >> 3) ^ swizzle(line)) << 4) + (r & 7) * 2;
+            using lds_ptr = __attribute__((address_space(3))) s16x4*;
+            // line + 4 has the same swizzle, so the second half is four lines further.
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<char*>(lds) + at));
+            const s16x4 hi =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<char*>(lds) + at + 4 * kLineBytes));
+            const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+            return u32x4{a[0], a[1], b[0], b[1]};
+        } else {
+            const int r = row + (lane & 15), line = q * 4;  // the four lines share a swizzle
+            const char* at = lds + line * kLineBytes + (((r >> 2) ^ swizzle(line)) << 4) + (r & 3) * 4;
+            u32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint32_t*>(at + j * kLineBytes);
+            return v;
+        }
+    }
+};
+
+// A workgroup's tile: BM x BN by WM x WN waves.
+template <int BM_, int BN_, int WM_, int WN_>
+struct Tile {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kThreads = 64 * WM * WN;
+    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;  // 16 x 16 results per wave
+};
+
+template <int D, class T>
+constexpr int lds_bytes() { return 2 * (T::BM + T::BN) * 128; }
+
+// Forms the tile at rows m0 of A and n0 of B over k in [k0, k1) into acc: acc[i][j] holds, in
+// lane l, element m = 16 i + l % 16, n = 16 j + 4 (l / 16) + r (r = 0..3) of the wave's part.
+template <int D, bool kA, bool kB, class T>
+__device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t m0, int64_t m_count, const void* b,
+                                             int64_t ldb, int64_t n0, int64_t n_count, int64_t k0, int64_t k1,
+                                             char* lds, f32x4 (&acc)[T::TM][T::TN]) {
+    constexpr int BK = tile_k<D>(), kThreads = T::kThreads, kSteps = 2;
+    using OpA = Operand<D, kA, T::BM, kThreads>;
+    using OpB = Operand<D, kB, T::BN, kThreads>;
+    constexpr int kBuffer = OpA::kBytes + OpB::kBytes;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = (wave / T::WN) * (T::BM / T::WM), wn = (wave % T::WN) * (T::BN / T::WN);
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (k0 >= k1) return;
+    OpA oa;
+    OpB ob;
+    oa.init(a, lda, m0, m_count, tid);
+    ob.init(b, ldb, n0, n_count, tid);
+    const int tiles = static_cast<int>((k1 - k0 + BK - 1) / BK);
+    const auto left_of = [&](int t) { return static_cast<int>(min<int64_t>(k1 - k0 - int64_t(t) * BK, BK)); };
+    oa.load(k0, left_of(0), tid);
+    ob.load(k0, left_of(0), tid);
+    oa.store(lds, tid);
+    ob.store(lds + OpA::kBytes, tid);
+    if (tiles > 1) {
+        oa.load(k0 + BK, left_of(1), tid);
+        ob.load(k0 + BK, left_of(1), tid);
+    }
+    __syncthreads();
+    for (int t = 0; t < tiles; ++t) {
+        const char* now = lds + (t & 1) * kBuffer;
+        char* next = lds + ((t & 1) ^ 1) * kBuffer;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            u32x4 fa[T::TM], fb[T::TN];
+#pragma unroll
+            for (int j = 0; j < T::TN; ++j) fb[j] = OpB::fragment(now + OpA::kBytes, wn + 16 * j, s, lane);
+#pragma unroll
+            for (int i = 0; i < T::TM; ++i) fa[i] = OpA::fragment(now, wm + 16 * i, s, lane);
+#pragma unroll
+            for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+                for (int j = 0; j < T::TN; ++j) acc[i][j] = mma<D>(fb[j], fa[i], acc[i][j]);
+            if (s == 0 && t + 1 < tiles) {
+                // Every wave has passed the barrier that ended the reads of this buffer.
+                oa.store(next, tid);
+                ob.store(next + OpA::kBytes, tid);
+                if (t + 2 < tiles) {
+                    const int64_t k = k0 + int64_t(t + 2) * BK;
+                    oa.load(k, left_of(t + 2), tid);
+                    ob.load(k, left_of(t + 2), tid);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- the order of tiles --------------------------------------------------------------
+// Workgroup b of `count` as a tile index such that each XCD (workgroups b mod 8) takes one
+// run of consecutive tiles: neighbours share their operands in that XCD's L2.
+__device__ __forceinline__ int xcd_tile(int b, int count) {
+    const int xcd = b & 7, q = count >> 3, r = count & 7;
+    return xcd * q + min(xcd, r) + (b >> 3);
+}
+// Tile t of a tiles_m x tiles_n grid, in bands of kBand tile rows walked column by column.
+template <int kBand>
+__device__ __forceinline__ void band_order(int t, int tiles_m, int tiles_n, int& m, int& n) {
+    const int width = kBand * tiles_n, band = t / width, first = band * kBand;
+    const int height = min(tiles_m - first, kBand), within = t - band * width;
+    m = first + within % height;
+    n = within / height;
+}
+
+}  // namespace mm
+}  // namespace hbt

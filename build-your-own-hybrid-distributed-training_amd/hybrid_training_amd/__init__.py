@@ -34,6 +34,7 @@ from .flat_param import (FlatParameter, FlatParamHandle, PieceLayout, ShardedTen
 from .grad_scaler import GradScaler, GradScalerState
 from .graphs import StepGraph
 from .groups import GroupHandle
+from .linear import FusedLinear, fused_linear
 from .manifest import (
     CheckpointManifest,
     FileRecord,

@@ -1,0 +1,222 @@
+"""The linear layer with its bias, activation and residual in the product's epilogue.
+
+:func:`fused_linear` computes ``act(x W^T + bias) + residual`` in one kernel (``hbt_linear``),
+and its backward pass in at most four: ``dz = dy act'(z)`` with the bias gradient
+(``hbt_linear_slope``), ``dx = dz W`` and ``dW = dz^T x``.  :class:`FusedLinear` is the module
+around it, with ``torch.nn.Linear``'s parameters and initialisation.
+
+Sums are held in float32; every stored value is rounded once to the tensors' dtype.  With an
+activation the backward pass keeps ``z = x W^T + bias`` in that dtype and forms ``act'`` from
+it.  No atomics run, so equal inputs give equal bits.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _native
+from .errors import ShardingError, UnsupportedFeatureError, format_error
+
+__all__ = ["ACTIVATIONS", "FusedLinear", "fused_linear"]
+
+#: Activation names and their HBT_ACT_* codes.  ``gelu`` is the exact (erf) form, ``gelu_tanh``
+#: the tanh approximation GPT-2 trains with.
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+#: Elements between rows that the kernels address (hbt_linear's limit).
+_MAX_LD = 1 << 20
+_FORWARD, _SLOPE, _GRAD_INPUT, _GRAD_WEIGHT = 0, 1, 2, 3
+
+
+def _rows(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
+    """``t`` as rows of ``cols`` consecutive elements and the distance between them: a view
+    where its strides allow one, else a dense copy."""
+    t = t.detach()
+    if t.dim() != 2:
+        t = t.reshape(-1, cols) if cols else t.reshape(math.prod(t.shape[:-1]), 0)
+    rows = t.shape[0]
+    if cols <= 1 or t.stride(1) == 1:
+        if rows <= 1:
+            return t, max(cols, 1)
+        ld = t.stride(0)
+        if max(cols, 1) <= ld <= _MAX_LD:
+            return t, ld
+    t = t.contiguous()
+    return t, max(cols, 1)
+
+
+def _workspace(tokens: int, inner: int, outer: int, dtype: int, which: int,
+               device: torch.device) -> tuple[torch.Tensor | None, int, int]:
+    """(tensor to keep, address, bytes) of the working storage one call can use."""
+    nbytes = _native.library().hbt_linear_workspace(tokens, inner, outer, dtype, which)
+    if nbytes <= 0:
+        return None, 0, 0
+    space = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return space, space.data_ptr(), nbytes
+
+
+def _check(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
+           activation: str) -> None:
+    who = "linear.fused_linear"
+    if activation not in ACTIVATIONS:
+        raise UnsupportedFeatureError(format_error(who, "unknown activation", expected=sorted(ACTIVATIONS),
+                                                   observed=activation))
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ShardingError(
+            format_error(who, "x must end in the weight's inner size",
+                         expected="x [..., inner] and weight [outer, inner]",
+                         observed=f"x {tuple(x.shape)}, weight {tuple(weight.shape)}"))
+    outer = weight.shape[0]
+    if bias is not None and tuple(bias.shape) != (outer,):
+        raise ShardingError(format_error(who, "the bias must hold one value per output", expected=(outer,),
+                                         observed=tuple(bias.shape)))
+    if residual is not None and residual.shape != (*x.shape[:-1], outer):
+        raise ShardingError(format_error(who, "the residual must have the result's shape",
+                                         expected=(*x.shape[:-1], outer), observed=tuple(residual.shape)))
+    for t in (x, weight, bias, residual):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _native.require_device_tensor(t, who)
+        if t.dtype != x.dtype or t.dtype not in _DTYPES:
+            raise UnsupportedFeatureError(
+                format_error(who, "x, weight, bias and residual share one dtype of bfloat16, float16 or float32",
+                             observed=[str(v.dtype) for v in (x, weight, bias, residual) if v is not None]))
+        if t.device != x.device:
+            raise ShardingError(format_error(who, "x, weight, bias and residual must be on one device",
+                                             expected=str(x.device), observed=str(t.device)))
+
+
+def _forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
+             activation: str, keep: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The result and, with ``keep``, z."""
+    outer, inner = weight.shape
+    shape = (*x.shape[:-1], outer)
+    rows, ldx = _rows(x, inner)
+    tokens = rows.shape[0]
+    w, ldw = _rows(weight, inner)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    z = torch.empty((tokens, outer), dtype=x.dtype, device=x.device) if keep else None
+    if tokens == 0 or outer == 0:
+        return y, z
+    b = None if bias is None else bias.detach().contiguous()
+    r, ldr = (None, 0) if residual is None else _rows(residual, outer)
+    code = _native.dtype_code(x.dtype)
+    device = x.device
+    with _native.device_guard(device):
+        space, address, nbytes = _workspace(tokens, inner, outer, code, _FORWARD, device)
+        status = _native.library().hbt_linear(
+            rows.data_ptr(), ldx, w.data_ptr(), ldw, None if b is None else b.data_ptr(),
+            None if r is None else r.data_ptr(), ldr, y.data_ptr(), outer, None if z is None else z.data_ptr(), outer,
+            tokens, inner, outer, code, ACTIVATIONS[activation], address, nbytes, _native.stream_of(device))
+    if status:
+        _native.check(status, "linear.hbt_linear")
+    return y, z
+
+
+class _FusedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        y, z = _forward(x, weight, bias, residual, activation, keep=activation != "none")
+        ctx.activation = activation
+        ctx.save_for_backward(x, weight, z)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
+        outer, inner = weight.shape
+        device, dtype = x.device, x.dtype
+        code = _native.dtype_code(dtype)
+        g, ldg = _rows(dy, outer)
+        tokens = g.shape[0]
+        activation = ACTIVATIONS[ctx.activation]
+        lib = _native.library()
+        dx = dw = db = None
+        with _native.device_guard(device):
+            stream = _native.stream_of(device)
+            dz, lddz = g, ldg
+            form = activation != 0 and (want_x or want_w)
+            if form:
+                # rows on 16-byte boundaries, which the products read fastest
+                unit = 16 // g.element_size()
+                lddz = max(unit, (outer + unit - 1) // unit * unit)
+                dz = torch.empty((tokens, lddz), dtype=dtype, device=device)
+            if want_b:
+                db = torch.empty(outer, dtype=dtype, device=device)
+            if form or want_b:
+                space, address, nbytes = (_workspace(tokens, inner, outer, code, _SLOPE, device) if want_b
+                                          else (None, 0, 0))
+                _native.check(lib.hbt_linear_slope(
+                    g.data_ptr(), ldg, None if z is None else z.data_ptr(), outer, dz.data_ptr() if form else None,
+                    lddz, None if db is None else db.data_ptr(), tokens, outer, code, activation, address, nbytes,
+                    stream), "linear.hbt_linear_slope")
+            if want_x:
+                w, ldw = _rows(weight, inner)
+                dx = torch.empty(x.shape, dtype=dtype, device=device)
+                space, address, nbytes = _workspace(tokens, inner, outer, code, _GRAD_INPUT, device)
+                _native.check(lib.hbt_linear_grad_input(
+                    dz.data_ptr(), lddz, w.data_ptr(), ldw, dx.data_ptr(), max(inner, 1), tokens, inner, outer, code,
+                    address, nbytes, stream), "linear.hbt_linear_grad_input")
+            if want_w:
+                rows, ldx = _rows(x, inner)
+                dw = torch.empty((outer, inner), dtype=dtype, device=device)
+                space, address, nbytes = _workspace(tokens, inner, outer, code, _GRAD_WEIGHT, device)
+                _native.check(lib.hbt_linear_grad_weight(
+                    dz.data_ptr(), lddz, rows.data_ptr(), ldx, dw.data_ptr(), max(inner, 1), tokens, inner, outer,
+                    code, address, nbytes, stream), "linear.hbt_linear_grad_weight")
+        return dx, dw, db, dy if want_r else None, None
+
+
+def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                 activation: str = "none", residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x weight^T + bias) + residual`` in one kernel, differentiable once.
+
+    ``x`` is ``[..., inner]``, ``weight`` ``[outer, inner]``, ``bias`` ``[outer]`` and
+    ``residual`` ``[..., outer]``, all of one dtype: bfloat16, float16 or float32.  Any strides
+    are accepted; rows of consecutive elements up to 2**20 apart are read where they lie, other
+    layouts through a dense copy.  ``activation`` is one of :data:`ACTIVATIONS`.
+    """
+    _check(x, weight, bias, residual, activation)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _FusedLinear.apply(x, weight, bias, residual, activation)
+    return _forward(x, weight, bias, residual, activation, keep=False)[0]
+
+
+class FusedLinear(nn.Module):
+    """``torch.nn.Linear`` with an activation, and a residual given to :meth:`forward`, in its
+    product's epilogue.  Parameters, their names and their initialisation are
+    ``torch.nn.Linear``'s."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, *, activation: str = "none",
+                 device: torch.device | str | None = None, dtype: torch.dtype | None = None) -> None:
+        super().__init__()
+        if activation not in ACTIVATIONS:
+            raise UnsupportedFeatureError(format_error("linear.FusedLinear", "unknown activation",
+                                                       expected=sorted(ACTIVATIONS), observed=activation))
+        self.in_features, self.out_features, self.activation = in_features, out_features, activation
+        self.weight = nn.Parameter(torch.empty(out_features, in_features, device=device, dtype=dtype))
+        self.bias = nn.Parameter(torch.empty(out_features, device=device, dtype=dtype)) if bias else None
+        self.reset_parameters()
+
+    def reset_parameters(self) -> None:
+        """Uniform in +-1/sqrt(in_features), weight and bias."""
+        bound = 1 / math.sqrt(self.in_features) if self.in_features > 0 else 0.0
+        with torch.no_grad():
+            self.weight.uniform_(-bound, bound)
+            if self.bias is not None:
+                self.bias.uniform_(-bound, bound)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        return fused_linear(x, self.weight, self.bias, activation=self.activation, residual=residual)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, "
+                f"bias={self.bias is not None}, activation={self.activation!r}")
