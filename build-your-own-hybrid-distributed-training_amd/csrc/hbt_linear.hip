@@ -91,7 +91,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_
     }
 }
 
-template <int D, bool kA, bool kB, class T>
+template <int D, bool kA, bool kB, class T, bool kEdge>
 __global__ __launch_bounds__(T::kThreads) void product_kernel(ProductArgs p) {
     extern __shared__ __align__(16) char lds[];
     const int t = xcd_tile(blockIdx.x, gridDim.x);
@@ -100,24 +100,13 @@ __global__ __launch_bounds__(T::kThreads) void product_kernel(ProductArgs p) {
     const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
     const int64_t k0 = blockIdx.y * p.k_split, k1 = min(p.k, k0 + p.k_split);
     f32x4 acc[T::TM][T::TN];
-    tile_product<D, kA, kB, T>(p.a, p.lda, m0, p.m, p.b, p.ldb, n0, p.n, k0, k1, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t mw = m0 + (wave / T::WN) * (T::BM / T::WM) + (lane & 15);
-    const int64_t nw = n0 + (wave % T::WN) * (T::BN / T::WN) + 4 * (lane >> 4);
-#pragma unroll
-    for (int i = 0; i < T::TM; ++i) {
-        const int64_t m = mw + 16 * i;
-        if (m >= p.m) continue;
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j) {
-            const int64_t n = nw + 16 * j;
-            if (n >= p.n) continue;
-            if (p.partial != nullptr)
-                *reinterpret_cast<f32x4*>(p.partial + (blockIdx.y * p.m + m) * p.ldp + n) = acc[i][j];
-            else
-                epilogue<D>(p, m, n, acc[i][j]);
-        }
-    }
+    tile_product<D, kA, kB, T, kEdge>(p.a, p.lda, m0, p.m, p.b, p.ldb, n0, p.n, k0, k1, lds, acc);
+    finish_tile<D, T>(lds, acc, [&](int i, int j, f32x4 v) {
+        const int64_t m = m0 + i, n = n0 + j;
+        if (m >= p.m || n >= p.n) return;
+        if (p.partial != nullptr) *reinterpret_cast<f32x4*>(p.partial + (blockIdx.y * p.m + m) * p.ldp + n) = v;
+        else epilogue<D>(p, m, n, v);
+    });
 }
 
 // Joins the parts of a split sum, in their order, and finishes the result.
@@ -273,11 +262,11 @@ struct Choice {
 
 constexpr int kMaxSplits = 16;
 
-Choice choose(int64_t m, int64_t n, int64_t k, int dtype) {
+Choice choose(int64_t m, int64_t n, int64_t k, int dtype, bool whole_units) {
     const int bk = dtype == HBT_DTYPE_F32 ? 32 : 64;
     const int64_t cus = 256;
     const auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-    if (dtype != HBT_DTYPE_F32 && tiles(256) >= cus) return {256, 1};
+    if (dtype != HBT_DTYPE_F32 && whole_units && tiles(256) >= cus) return {256, 1};
     const int tile = tiles(128) >= cus ? 128 : 64;
     const int64_t count = tiles(tile), steps = (k + bk - 1) / bk;
     int64_t splits = 1;
@@ -285,24 +274,30 @@ Choice choose(int64_t m, int64_t n, int64_t k, int dtype) {
     return {tile, static_cast<int>(std::max<int64_t>(splits, 1))};
 }
 
-template <int D, bool kA, bool kB, class T>
+// Whether no unit of an operand that is not k-major crosses its last row.
+template <bool kA, bool kB>
+bool whole_units(int64_t m, int64_t n) { return (kA || m % 8 == 0) && (kB || n % 8 == 0); }
+
+template <int D, bool kA, bool kB, class T, bool kEdge>
 int32_t launch_tile(const char* who, ProductArgs& p, int splits, hipStream_t stream) {
     constexpr int kLds = lds_bytes<D, T>();
     p.tiles_m = static_cast<int>((p.m + T::BM - 1) / T::BM);
     p.tiles_n = static_cast<int>((p.n + T::BN - 1) / T::BN);
+    const auto kernel = product_kernel<D, kA, kB, T, kEdge>;
     if constexpr (kLds > 65536) {
-        static const hipError_t set = hipFuncSetAttribute(
-            reinterpret_cast<const void*>(product_kernel<D, kA, kB, T>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+        static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
         if (set != hipSuccess) return check_hip(set, who);
     }
-    product_kernel<D, kA, kB, T><<<dim3(p.tiles_m * p.tiles_n, splits), T::kThreads, kLds, stream>>>(p);
+    kernel<<<dim3(p.tiles_m * p.tiles_n, splits), T::kThreads, kLds, stream>>>(p);
     return check_launch(who);
 }
 
 template <int D, bool kA, bool kB>
 int32_t launch_product(const char* who, ProductArgs& p, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-    Choice c = choose(p.m, p.n, p.k, D);
     constexpr int BK = tile_k<D>();
+    constexpr bool kEdge = !kA || !kB;
+    Choice c = choose(p.m, p.n, p.k, D, whole_units<kA, kB>(p.m, p.n));
     p.ldp = (p.n + 3) / 4 * 4;
     while (c.splits > 1 && 4 * c.splits * p.m * p.ldp > workspace_bytes) --c.splits;
     p.k_split = p.k;
@@ -312,15 +307,10 @@ int32_t launch_product(const char* who, ProductArgs& p, void* workspace, int64_t
         c.splits = static_cast<int>((p.k + p.k_split - 1) / p.k_split);
         if (c.splits > 1) p.partial = static_cast<float*>(workspace);
     }
-    int32_t status;
-    if constexpr (D == HBT_DTYPE_F32) {
-        status = c.tile == 128 ? launch_tile<D, kA, kB, Tile128>(who, p, c.splits, stream)
-                               : launch_tile<D, kA, kB, Tile64>(who, p, c.splits, stream);
-    } else {
-        status = c.tile == 256   ? launch_tile<D, kA, kB, Tile256>(who, p, c.splits, stream)
-                 : c.tile == 128 ? launch_tile<D, kA, kB, Tile128>(who, p, c.splits, stream)
-                                 : launch_tile<D, kA, kB, Tile64>(who, p, c.splits, stream);
-    }
+    int32_t status = HBT_OK;
+    if (c.tile == 64) status = launch_tile<D, kA, kB, Tile64, kEdge>(who, p, c.splits, stream);
+    else if (c.tile == 128) status = launch_tile<D, kA, kB, Tile128, kEdge>(who, p, c.splits, stream);
+    else if constexpr (D != HBT_DTYPE_F32) status = launch_tile<D, kA, kB, Tile256, false>(who, p, c.splits, stream);
     if (status != HBT_OK || c.splits == 1) return status;
     const int64_t blocks = std::min<int64_t>((p.m * (p.ldp / 4) + 255) / 256, 4096);
     join_kernel<D><<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(p, c.splits);
@@ -370,9 +360,10 @@ int32_t check_sizes(const char* who, int64_t m, int64_t n, int64_t k, int32_t dt
     return HBT_OK;
 }
 
+template <bool kA, bool kB>
 int64_t split_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype) {
     if (m <= 0 || n <= 0 || k <= 0) return 0;
-    const Choice c = choose(m, n, k, dtype);
+    const Choice c = choose(m, n, k, dtype, whole_units<kA, kB>(m, n));
     return c.splits == 1 ? 0 : 4 * c.splits * m * ((n + 3) / 4 * 4);
 }
 
@@ -383,6 +374,33 @@ int rows_per_block(int64_t m, int64_t n) {
     rows = std::min<int64_t>(std::max<int64_t>(rows, 16), 256);
     while ((m + rows - 1) / rows > 65535) rows *= 2;
     return static_cast<int>(rows);
+}
+
+// The backward pass's working storage: dz with rows on 16-byte boundaries when an activation
+// makes it differ from dy, then a region that the bias sums and each product's split take in
+// turn.
+struct BackwardSpace {
+    int64_t lddz, dz_bytes, shared_bytes;
+};
+
+BackwardSpace backward_space(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t activation,
+                             int32_t wants) {
+    BackwardSpace b{};
+    if (tokens <= 0 || outer <= 0) return b;
+    const int64_t unit = dtype == HBT_DTYPE_F32 ? 4 : 8, size = dtype == HBT_DTYPE_F32 ? 4 : 2;
+    if (activation != HBT_ACT_NONE && (wants & (HBT_LINEAR_DX | HBT_LINEAR_DW)) != 0) {
+        b.lddz = (outer + unit - 1) / unit * unit;
+        b.dz_bytes = (tokens * b.lddz * size + 255) / 256 * 256;
+    }
+    if (wants & HBT_LINEAR_DBIAS) {
+        const int64_t rows = rows_per_block(tokens, outer);
+        b.shared_bytes = 4 * ((tokens + rows - 1) / rows) * ((outer + 3) / 4 * 4);
+    }
+    if (wants & HBT_LINEAR_DX)
+        b.shared_bytes = std::max(b.shared_bytes, split_bytes<true, false>(tokens, inner, outer, dtype));
+    if (wants & HBT_LINEAR_DW)
+        b.shared_bytes = std::max(b.shared_bytes, split_bytes<false, false>(outer, inner, tokens, dtype));
+    return b;
 }
 
 template <typename F>
@@ -401,20 +419,19 @@ using namespace hbt::mm;
 
 extern "C" {
 
-int64_t hbt_linear_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t which) {
+int64_t hbt_linear_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype) {
     if (tokens < 0 || inner < 0 || outer < 0) return -1;
     if (dtype != HBT_DTYPE_F32 && dtype != HBT_DTYPE_BF16 && dtype != HBT_DTYPE_F16) return -1;
-    switch (which) {
-        case HBT_LINEAR_FORWARD: return tokens <= 16 ? 0 : split_bytes(tokens, outer, inner, dtype);
-        case HBT_LINEAR_SLOPE: {
-            if (tokens == 0 || outer == 0) return 0;
-            const int64_t rows = rows_per_block(tokens, outer);
-            return 4 * ((tokens + rows - 1) / rows) * ((outer + 3) / 4 * 4);
-        }
-        case HBT_LINEAR_GRAD_INPUT: return split_bytes(tokens, inner, outer, dtype);
-        case HBT_LINEAR_GRAD_WEIGHT: return split_bytes(outer, inner, tokens, dtype);
-        default: return -1;
-    }
+    return tokens <= 16 ? 0 : split_bytes<true, true>(tokens, outer, inner, dtype);
+}
+
+int64_t hbt_linear_backward_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t activation,
+                                      int32_t wants) {
+    if (tokens < 0 || inner < 0 || outer < 0 || wants < 0 || wants > 7) return -1;
+    if (dtype != HBT_DTYPE_F32 && dtype != HBT_DTYPE_BF16 && dtype != HBT_DTYPE_F16) return -1;
+    if (activation < HBT_ACT_NONE || activation > HBT_ACT_SILU) return -1;
+    const BackwardSpace b = backward_space(tokens, inner, outer, dtype, activation, wants);
+    return b.dz_bytes + b.shared_bytes;
 }
 
 int32_t hbt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
@@ -439,7 +456,7 @@ int32_t hbt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const
     p.lda = ldx, p.ldb = ldw, p.ldr = ldr, p.ldy = ldy, p.ldz = ldz;
     p.m = tokens, p.n = outer, p.k = inner, p.act = activation;
     const hipStream_t s = as_stream(stream);
-    return by_dtype(dtype, [&](auto d) {
+    return by_dtype(dtype, [&](auto d) -> int32_t {
         constexpr int D = decltype(d)::value;
         if (tokens <= 16) {
             thin_kernel<D><<<dim3(static_cast<unsigned>((outer + 15) / 16)), 512, 0, s>>>(p);
@@ -449,85 +466,70 @@ int32_t hbt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const
     });
 }
 
-int32_t hbt_linear_slope(const void* dy, int64_t lddy, const void* z, int64_t ldz, void* dz, int64_t lddz, void* dbias,
-                         int64_t tokens, int64_t outer, int32_t dtype, int32_t activation, void* workspace,
-                         int64_t workspace_bytes, void* stream) {
+int32_t hbt_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                            const void* z, int64_t ldz, void* dx, int64_t lddx, void* dw, int64_t lddw, void* dbias,
+                            int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t activation,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
     clear_error();
-    const char* who = "hbt_linear_slope";
-    int32_t status = check_sizes(who, tokens, outer, 0, dtype);
+    const char* who = "hbt_linear_backward";
+    int32_t status = check_sizes(who, tokens, outer, inner, dtype);
     if (status != HBT_OK) return status;
     if (activation < HBT_ACT_NONE || activation > HBT_ACT_SILU) return fail(who, "unknown activation");
-    if (outer == 0) return HBT_OK;
     if ((status = check_matrix(who, dy, tokens, outer, lddy, "dy")) != HBT_OK) return status;
     if (activation != HBT_ACT_NONE && (status = check_matrix(who, z, tokens, outer, ldz, "z")) != HBT_OK)
         return status;
-    if (dz != nullptr && (status = check_matrix(who, dz, tokens, outer, lddz, "dz")) != HBT_OK) return status;
-    SlopeArgs p{};
-    p.dy = dy, p.z = z, p.dz = dz, p.lddy = lddy, p.ldz = ldz, p.lddz = lddz;
-    p.m = tokens, p.n = outer, p.act = activation, p.ldp = (outer + 3) / 4 * 4;
-    p.rows_per_block = rows_per_block(std::max<int64_t>(tokens, 1), outer);
-    const int64_t blocks = (tokens + p.rows_per_block - 1) / p.rows_per_block;
-    if (dbias != nullptr && tokens > 0) {
-        if (workspace == nullptr || workspace_bytes < 4 * blocks * p.ldp) return fail(who, "the workspace is too small");
-        p.partial = static_cast<float*>(workspace);
-    }
+    if (dx != nullptr && ((status = check_matrix(who, dx, tokens, inner, lddx, "dx")) != HBT_OK ||
+                          (status = check_matrix(who, w, outer, inner, ldw, "w")) != HBT_OK))
+        return status;
+    if (dw != nullptr && ((status = check_matrix(who, dw, outer, inner, lddw, "dw")) != HBT_OK ||
+                          (status = check_matrix(who, x, tokens, inner, ldx, "x")) != HBT_OK))
+        return status;
+    const int32_t wants = (dx != nullptr ? HBT_LINEAR_DX : 0) | (dw != nullptr ? HBT_LINEAR_DW : 0) |
+                          (dbias != nullptr ? HBT_LINEAR_DBIAS : 0);
+    const BackwardSpace space = backward_space(tokens, inner, outer, dtype, activation, wants);
+    const int64_t need = space.dz_bytes + space.shared_bytes;
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return fail(who, "the workspace is smaller than hbt_linear_backward_workspace's");
+    char* shared = static_cast<char*>(workspace) + space.dz_bytes;
     const hipStream_t s = as_stream(stream);
-    return by_dtype(dtype, [&](auto d) {
+    return by_dtype(dtype, [&](auto d) -> int32_t {
         constexpr int D = decltype(d)::value;
-        if (blocks > 0) {
+        SlopeArgs p{};
+        p.dy = dy, p.z = z, p.dz = space.dz_bytes > 0 ? workspace : nullptr;
+        p.lddy = lddy, p.ldz = ldz, p.lddz = space.lddz, p.ldp = (outer + 3) / 4 * 4;
+        p.partial = dbias != nullptr ? reinterpret_cast<float*>(shared) : nullptr;
+        p.m = tokens, p.n = outer, p.act = activation;
+        int64_t blocks = 0;
+        if (tokens > 0 && outer > 0 && (p.dz != nullptr || dbias != nullptr)) {
+            p.rows_per_block = rows_per_block(tokens, outer);
+            blocks = (tokens + p.rows_per_block - 1) / p.rows_per_block;
             slope_kernel<D><<<dim3(static_cast<unsigned>((outer + 255) / 256), static_cast<unsigned>(blocks)), 256, 0,
                               s>>>(p);
             const int32_t launched = check_launch(who);
             if (launched != HBT_OK) return launched;
         }
-        if (dbias == nullptr) return HBT_OK;
-        bias_kernel<D><<<dim3(static_cast<unsigned>((outer + 63) / 64)), 256, 0, s>>>(
-            p.partial, p.ldp, static_cast<int>(blocks), dbias, outer);
-        return check_launch(who);
-    });
-}
-
-int32_t hbt_linear_grad_input(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx,
-                              int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, void* workspace,
-                              int64_t workspace_bytes, void* stream) {
-    clear_error();
-    const char* who = "hbt_linear_grad_input";
-    int32_t status = check_sizes(who, tokens, inner, outer, dtype);
-    if (status != HBT_OK) return status;
-    if (tokens == 0 || inner == 0) return HBT_OK;
-    if ((status = check_matrix(who, dz, tokens, outer, lddz, "dz")) != HBT_OK ||
-        (status = check_matrix(who, w, outer, inner, ldw, "w")) != HBT_OK ||
-        (status = check_matrix(who, dx, tokens, inner, lddx, "dx")) != HBT_OK)
-        return status;
-    ProductArgs p{};
-    p.a = dz, p.b = w, p.y = dx, p.lda = lddz, p.ldb = ldw, p.ldy = lddx;
-    p.m = tokens, p.n = inner, p.k = outer, p.act = HBT_ACT_NONE;
-    return by_dtype(dtype, [&](auto d) {
-        return launch_product<decltype(d)::value, true, false>(who, p, workspace,
-                                                               workspace == nullptr ? 0 : workspace_bytes,
-                                                               as_stream(stream));
-    });
-}
-
-int32_t hbt_linear_grad_weight(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw,
-                               int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, void* workspace,
-                               int64_t workspace_bytes, void* stream) {
-    clear_error();
-    const char* who = "hbt_linear_grad_weight";
-    int32_t status = check_sizes(who, outer, inner, tokens, dtype);
-    if (status != HBT_OK) return status;
-    if (outer == 0 || inner == 0) return HBT_OK;
-    if ((status = check_matrix(who, dz, tokens, outer, lddz, "dz")) != HBT_OK ||
-        (status = check_matrix(who, x, tokens, inner, ldx, "x")) != HBT_OK ||
-        (status = check_matrix(who, dw, outer, inner, lddw, "dw")) != HBT_OK)
-        return status;
-    ProductArgs p{};
-    p.a = dz, p.b = x, p.y = dw, p.lda = lddz, p.ldb = ldx, p.ldy = lddw;
-    p.m = outer, p.n = inner, p.k = tokens, p.act = HBT_ACT_NONE;
-    return by_dtype(dtype, [&](auto d) {
-        return launch_product<decltype(d)::value, false, false>(who, p, workspace,
-                                                                workspace == nullptr ? 0 : workspace_bytes,
-                                                                as_stream(stream));
+        if (dbias != nullptr && outer > 0) {
+            bias_kernel<D><<<dim3(static_cast<unsigned>((outer + 63) / 64)), 256, 0, s>>>(
+                p.partial, p.ldp, static_cast<int>(blocks), dbias, outer);
+            const int32_t launched = check_launch(who);
+            if (launched != HBT_OK) return launched;
+        }
+        const void* dz = p.dz != nullptr ? p.dz : dy;
+        const int64_t lddz = p.dz != nullptr ? space.lddz : lddy;
+        if (dx != nullptr && tokens > 0 && inner > 0) {
+            ProductArgs q{};
+            q.a = dz, q.b = w, q.y = dx, q.lda = lddz, q.ldb = ldw, q.ldy = lddx;
+            q.m = tokens, q.n = inner, q.k = outer;
+            const int32_t launched = launch_product<D, true, false>(who, q, shared, space.shared_bytes, s);
+            if (launched != HBT_OK) return launched;
+        }
+        if (dw != nullptr && outer > 0 && inner > 0) {
+            ProductArgs q{};
+            q.a = dz, q.b = x, q.y = dw, q.lda = lddz, q.ldb = ldx, q.ldy = lddw;
+            q.m = outer, q.n = inner, q.k = tokens;
+            return launch_product<D, false, false>(who, q, shared, space.shared_bytes, s);
+        }
+        return HBT_OK;
     });
 }
 

@@ -111,7 +111,8 @@ constexpr uint32_t kNowhere = 0xFFFFFF00u;
 
 // One operand's share of a tile: ROWS rows (m or n) by tile_k of k, moved by THREADS lanes.
 // kKMajor: element (row, k) at base[row * ld + k]; else at base[k * ld + row].
-template <int D, bool kKMajor, int ROWS, int THREADS>
+// kEdge: units may cross the last row of an operand that is not k-major.
+template <int D, bool kKMajor, int ROWS, int THREADS, bool kEdge>
 struct Operand {
     static constexpr int E = unit_elems<D>(), BK = tile_k<D>(), B = elem_bytes<D>();
     static constexpr int kUnitsPerLine = kKMajor ? BK / E : ROWS / E;  // units per LDS line
@@ -125,7 +126,7 @@ struct Operand {
     int rows;              // rows of the operand from the tile's first one
     uint32_t offset[kUnits];
     u32x4 held[kUnits];
-    bool straddles;        // some lane's unit crosses the last row (not k-major)
+    bool straddles;        // some lane's unit crosses the last row (kEdge, not k-major)
 
     // LDS position of a unit: lines are XOR-swizzled in units so that the 16 rows of a
     // fragment read (k-major), or the four k of a transposing read, fall on distinct banks.
@@ -139,7 +140,7 @@ struct Operand {
         ld = ld_;
         rows = static_cast<int>(row_count - row0 < ROWS ? row_count - row0 : ROWS);
         base = static_cast<const char*>(p) + (kKMajor ? row0 * ld_ : row0) * B;
-        straddles = !kKMajor && rows < ROWS && rows % E != 0;
+        straddles = kEdge && !kKMajor && rows < ROWS && rows % E != 0;
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
@@ -148,24 +149,30 @@ struct Operand {
         }
     }
 
-    // The lane's units of the k-tile [k0, k0 + BK), of which `left` values of k exist.
-    __device__ __forceinline__ void load(int64_t k0, int left, int tid) {
+    // The lane's units of the whole k-tile at k0.
+    __device__ __forceinline__ void load(int64_t k0, int tid) {
         const char* at_k = base + (kKMajor ? k0 : k0 * ld) * B;
         const auto buffer = buffer_at(at_k);
-        if (left >= BK) {
 #pragma unroll
-            for (int i = 0; i < kUnits; ++i)
-                held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset[i], 0, 0));
-        } else {
-#pragma unroll
-            for (int i = 0; i < kUnits; ++i) {
-                const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
-                const bool in = kKMajor ? (at + 1) * E <= left : line < left;
-                held[i] = __builtin_bit_cast(
-                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, in ? offset[i] : kNowhere, 0, 0));
-            }
+        for (int i = 0; i < kUnits; ++i)
+            held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset[i], 0, 0));
+        if constexpr (kEdge && !kKMajor) {
+            if (straddles) load_edge(at_k, BK, tid);
         }
-        if (straddles || (kKMajor && left < BK && left % E != 0)) load_edge(at_k, left, tid);
+    }
+
+    // The lane's units of the k-tile at k0, of which only `left` values of k exist.
+    __device__ __forceinline__ void load_part(int64_t k0, int left, int tid) {
+        const char* at_k = base + (kKMajor ? k0 : k0 * ld) * B;
+        const auto buffer = buffer_at(at_k);
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
+            const bool in = kKMajor ? (at + 1) * E <= left : line < left;
+            held[i] = __builtin_bit_cast(
+                u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, in ? offset[i] : kNowhere, 0, 0));
+        }
+        if (straddles || (kKMajor && left % E != 0)) load_edge(at_k, left, tid);
     }
 
     // Units that cross the last row or the last k, element by element.
@@ -240,13 +247,14 @@ constexpr int lds_bytes() { return 2 * (T::BM + T::BN) * 128; }
 
 // Forms the tile at rows m0 of A and n0 of B over k in [k0, k1) into acc: acc[i][j] holds, in
 // lane l, element m = 16 i + l % 16, n = 16 j + 4 (l / 16) + r (r = 0..3) of the wave's part.
-template <int D, bool kA, bool kB, class T>
+// A partial k-tile comes first, so that the loop moves whole ones only.
+template <int D, bool kA, bool kB, class T, bool kEdge>
 __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t m0, int64_t m_count, const void* b,
                                              int64_t ldb, int64_t n0, int64_t n_count, int64_t k0, int64_t k1,
                                              char* lds, f32x4 (&acc)[T::TM][T::TN]) {
     constexpr int BK = tile_k<D>(), kThreads = T::kThreads, kSteps = 2;
-    using OpA = Operand<D, kA, T::BM, kThreads>;
-    using OpB = Operand<D, kB, T::BN, kThreads>;
+    using OpA = Operand<D, kA, T::BM, kThreads, kEdge>;
+    using OpB = Operand<D, kB, T::BN, kThreads, kEdge>;
     constexpr int kBuffer = OpA::kBytes + OpB::kBytes;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = (wave / T::WN) * (T::BM / T::WM), wn = (wave % T::WN) * (T::BN / T::WN);
@@ -260,14 +268,20 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
     oa.init(a, lda, m0, m_count, tid);
     ob.init(b, ldb, n0, n_count, tid);
     const int tiles = static_cast<int>((k1 - k0 + BK - 1) / BK);
-    const auto left_of = [&](int t) { return static_cast<int>(min<int64_t>(k1 - k0 - int64_t(t) * BK, BK)); };
-    oa.load(k0, left_of(0), tid);
-    ob.load(k0, left_of(0), tid);
+    const int part = static_cast<int>((k1 - k0) % BK);
+    if (part != 0) {
+        oa.load_part(k0, part, tid);
+        ob.load_part(k0, part, tid);
+    } else {
+        oa.load(k0, tid);
+        ob.load(k0, tid);
+    }
     oa.store(lds, tid);
     ob.store(lds + OpA::kBytes, tid);
+    int64_t k = k0 + (part != 0 ? part : BK);  // the next k-tile to load
     if (tiles > 1) {
-        oa.load(k0 + BK, left_of(1), tid);
-        ob.load(k0 + BK, left_of(1), tid);
+        oa.load(k, tid);
+        ob.load(k, tid);
     }
     __syncthreads();
     for (int t = 0; t < tiles; ++t) {
@@ -289,13 +303,44 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
                 oa.store(next, tid);
                 ob.store(next + OpA::kBytes, tid);
                 if (t + 2 < tiles) {
-                    const int64_t k = k0 + int64_t(t + 2) * BK;
-                    oa.load(k, left_of(t + 2), tid);
-                    ob.load(k, left_of(t + 2), tid);
+                    k += BK;
+                    oa.load(k, tid);
+                    ob.load(k, tid);
                 }
             }
         }
         __syncthreads();
+    }
+}
+
+// Hands the tile's results to `store(m, n, v)`, four consecutive n at a time, each in one lane,
+// rows in order: the accumulators pass through LDS (free by now), so the code that finishes a
+// result stands once, in a loop, and a wave's loads and stores cover whole rows.
+template <int D, class T, class Store>
+__device__ __forceinline__ void finish_tile(char* lds, const f32x4 (&acc)[T::TM][T::TN], Store&& store) {
+    constexpr int kRowUnits = T::BN / 4, kPhases = T::BM * T::BN * 4 > lds_bytes<D, T>() ? T::WM : 1;
+    constexpr int kRows = T::BM / kPhases;
+    static_assert(kRows * T::BN * 4 <= lds_bytes<D, T>(), "a phase fits the tile's LDS");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = (wave / T::WN) * (T::BM / T::WM), wn = (wave % T::WN) * (T::BN / T::WN);
+    f32x4* out = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+    for (int phase = 0; phase < kPhases; ++phase) {
+        if (phase > 0) __syncthreads();
+        if (kPhases == 1 || wave / T::WN == phase) {
+#pragma unroll
+            for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+                for (int j = 0; j < T::TN; ++j) {
+                    const int m = wm - phase * kRows + 16 * i + (lane & 15), unit = wn / 4 + 4 * j + (lane >> 4);
+                    out[m * kRowUnits + (unit ^ (m & 15))] = acc[i][j];
+                }
+        }
+        __syncthreads();
+        for (int u = tid; u < kRows * kRowUnits; u += T::kThreads) {
+            const int m = u / kRowUnits, unit = u % kRowUnits;
+            store(phase * kRows + m, unit * 4, out[m * kRowUnits + (unit ^ (m & 15))]);
+        }
     }
 }
 

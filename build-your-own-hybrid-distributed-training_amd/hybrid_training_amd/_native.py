@@ -283,26 +283,17 @@ EXPORTED_SYMBOLS: dict[str, tuple[object, tuple[object, ...]]] = {
     "hbt_sgd_scalar_record_f64": (_c_i32, (_c_void_p, _c_f64, _c_f64, _c_f64, _c_f64, _c_f64, _c_i32)),
     "hbt_exchange_capture_mode": (_c_i32, (_c_i32, ctypes.POINTER(_c_i32))),
     "hbt_write_words": (_c_i32, (_c_void_p, ctypes.POINTER(ctypes.c_uint32), _c_i64, _c_void_p)),
-    "hbt_linear_workspace": (_c_i64, (_c_i64, _c_i64, _c_i64, _c_i32, _c_i32)),
+    "hbt_linear_workspace": (_c_i64, (_c_i64, _c_i64, _c_i64, _c_i32)),
     "hbt_linear": (
         _c_i32,
         (_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64,
          _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_void_p, _c_i64, _c_void_p),
     ),
-    "hbt_linear_slope": (
+    "hbt_linear_backward_workspace": (_c_i64, (_c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32)),
+    "hbt_linear_backward": (
         _c_i32,
-        (_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_i64, _c_i32, _c_i32,
-         _c_void_p, _c_i64, _c_void_p),
-    ),
-    "hbt_linear_grad_input": (
-        _c_i32,
-        (_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_void_p, _c_i64,
-         _c_void_p),
-    ),
-    "hbt_linear_grad_weight": (
-        _c_i32,
-        (_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_void_p, _c_i64,
-         _c_void_p),
+        (_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p,
+         _c_i64, _c_void_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_void_p, _c_i64, _c_void_p),
     ),
 }
 

@@ -1,8 +1,8 @@
 """The linear layer with its bias, activation and residual in the product's epilogue.
 
 :func:`fused_linear` computes ``act(x W^T + bias) + residual`` in one kernel (``hbt_linear``),
-and its backward pass in at most four: ``dz = dy act'(z)`` with the bias gradient
-(``hbt_linear_slope``), ``dx = dz W`` and ``dW = dz^T x``.  :class:`FusedLinear` is the module
+and its backward pass ``dz = dy act'(z)``, ``dx = dz W``, ``dW = dz^T x`` and the bias gradient in
+one call (``hbt_linear_backward``).  :class:`FusedLinear` is the module
 around it, with ``torch.nn.Linear``'s parameters and initialisation.
 
 Sums are held in float32; every stored value is rounded once to the tensors' dtype.  With an
@@ -30,7 +30,7 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 #: Elements between rows that the kernels address (hbt_linear's limit).
 _MAX_LD = 1 << 20
-_FORWARD, _SLOPE, _GRAD_INPUT, _GRAD_WEIGHT = 0, 1, 2, 3
+_DX, _DW, _DBIAS = 1, 2, 4
 
 
 def _rows(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
@@ -50,14 +50,12 @@ def _rows(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
     return t, max(cols, 1)
 
 
-def _workspace(tokens: int, inner: int, outer: int, dtype: int, which: int,
-               device: torch.device) -> tuple[torch.Tensor | None, int, int]:
-    """(tensor to keep, address, bytes) of the working storage one call can use."""
-    nbytes = _native.library().hbt_linear_workspace(tokens, inner, outer, dtype, which)
+def _workspace(nbytes: int, device: torch.device) -> tuple[torch.Tensor | None, int]:
+    """(tensor to keep, address) of working storage, or nothing where none is needed."""
     if nbytes <= 0:
-        return None, 0, 0
+        return None, 0
     space = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return space, space.data_ptr(), nbytes
+    return space, space.data_ptr()
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
@@ -109,8 +107,10 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, r
     code = _native.dtype_code(x.dtype)
     device = x.device
     with _native.device_guard(device):
-        space, address, nbytes = _workspace(tokens, inner, outer, code, _FORWARD, device)
-        status = _native.library().hbt_linear(
+        lib = _native.library()
+        nbytes = lib.hbt_linear_workspace(tokens, inner, outer, code)
+        space, address = _workspace(nbytes, device)
+        status = lib.hbt_linear(
             rows.data_ptr(), ldx, w.data_ptr(), ldw, None if b is None else b.data_ptr(),
             None if r is None else r.data_ptr(), ldr, y.data_ptr(), outer, None if z is None else z.data_ptr(), outer,
             tokens, inner, outer, code, ACTIVATIONS[activation], address, nbytes, _native.stream_of(device))
@@ -132,46 +132,37 @@ class _FusedLinear(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
-        outer, inner = weight.shape
-        device, dtype = x.device, x.dtype
-        code = _native.dtype_code(dtype)
-        g, ldg = _rows(dy, outer)
-        tokens = g.shape[0]
-        activation = ACTIVATIONS[ctx.activation]
-        lib = _native.library()
         dx = dw = db = None
-        with _native.device_guard(device):
-            stream = _native.stream_of(device)
-            dz, lddz = g, ldg
-            form = activation != 0 and (want_x or want_w)
-            if form:
-                # rows on 16-byte boundaries, which the products read fastest
-                unit = 16 // g.element_size()
-                lddz = max(unit, (outer + unit - 1) // unit * unit)
-                dz = torch.empty((tokens, lddz), dtype=dtype, device=device)
-            if want_b:
-                db = torch.empty(outer, dtype=dtype, device=device)
-            if form or want_b:
-                space, address, nbytes = (_workspace(tokens, inner, outer, code, _SLOPE, device) if want_b
-                                          else (None, 0, 0))
-                _native.check(lib.hbt_linear_slope(
-                    g.data_ptr(), ldg, None if z is None else z.data_ptr(), outer, dz.data_ptr() if form else None,
-                    lddz, None if db is None else db.data_ptr(), tokens, outer, code, activation, address, nbytes,
-                    stream), "linear.hbt_linear_slope")
+        if want_x or want_w or want_b:
+            outer, inner = weight.shape
+            device, dtype = x.device, x.dtype
+            g, ldg = _rows(dy, outer)
+            tokens = g.shape[0]
+            wants, xs, ws, ldx, ldw, across = 0, None, None, 0, 0, max(inner, 1)
             if want_x:
-                w, ldw = _rows(weight, inner)
+                wants |= _DX
+                ws, ldw = _rows(weight, inner)
                 dx = torch.empty(x.shape, dtype=dtype, device=device)
-                space, address, nbytes = _workspace(tokens, inner, outer, code, _GRAD_INPUT, device)
-                _native.check(lib.hbt_linear_grad_input(
-                    dz.data_ptr(), lddz, w.data_ptr(), ldw, dx.data_ptr(), max(inner, 1), tokens, inner, outer, code,
-                    address, nbytes, stream), "linear.hbt_linear_grad_input")
             if want_w:
-                rows, ldx = _rows(x, inner)
+                wants |= _DW
+                xs, ldx = _rows(x, inner)
                 dw = torch.empty((outer, inner), dtype=dtype, device=device)
-                space, address, nbytes = _workspace(tokens, inner, outer, code, _GRAD_WEIGHT, device)
-                _native.check(lib.hbt_linear_grad_weight(
-                    dz.data_ptr(), lddz, rows.data_ptr(), ldx, dw.data_ptr(), max(inner, 1), tokens, inner, outer,
-                    code, address, nbytes, stream), "linear.hbt_linear_grad_weight")
+            if want_b:
+                wants |= _DBIAS
+                db = torch.empty(outer, dtype=dtype, device=device)
+            code, activation = _native.dtype_code(dtype), ACTIVATIONS[ctx.activation]
+            lib = _native.library()
+            with _native.device_guard(device):
+                nbytes = lib.hbt_linear_backward_workspace(tokens, inner, outer, code, activation, wants)
+                space, address = _workspace(nbytes, device)
+                status = lib.hbt_linear_backward(
+                    g.data_ptr(), ldg, None if xs is None else xs.data_ptr(), ldx,
+                    None if ws is None else ws.data_ptr(), ldw, None if z is None else z.data_ptr(), max(outer, 1),
+                    None if dx is None else dx.data_ptr(), across, None if dw is None else dw.data_ptr(), across,
+                    None if db is None else db.data_ptr(), tokens, inner, outer, code, activation, address, nbytes,
+                    _native.stream_of(device))
+            if status:
+                _native.check(status, "linear.hbt_linear_backward")
         return dx, dw, db, dy if want_r else None, None
 
 

@@ -643,46 +643,44 @@ int32_t hbt_exchange_capture_mode(int32_t mode, int32_t* previous);
  * y may not overlap x or w; y may be the residual itself.
  *
  * Small results of a long sum split it over workgroups: `workspace` (16-byte aligned) then
- * holds the fp32 parts.  hbt_linear_workspace gives the bytes that each entry point can use
- * for these sizes (`which`: HBT_LINEAR_*; -1 for bad arguments); with a smaller workspace,
- * or NULL, the sum is split less or not at all, which is slower and rounds in another order.
+ * holds the fp32 parts.  hbt_linear_workspace gives the bytes that a call of these sizes can
+ * use (-1 for bad arguments); with a smaller workspace, or NULL, the sum is split less or not
+ * at all, which is slower and rounds in another order.
  * ---------------------------------------------------------------------------- */
 #define HBT_ACT_NONE 0
 #define HBT_ACT_RELU 1
 #define HBT_ACT_GELU 2
 #define HBT_ACT_GELU_TANH 3
 #define HBT_ACT_SILU 4
-#define HBT_LINEAR_FORWARD 0
-#define HBT_LINEAR_SLOPE 1
-#define HBT_LINEAR_GRAD_INPUT 2
-#define HBT_LINEAR_GRAD_WEIGHT 3
-int64_t hbt_linear_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t which);
+int64_t hbt_linear_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype);
 int32_t hbt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
                    int64_t ldr, void* y, int64_t ldy, void* z, int64_t ldz, int64_t tokens, int64_t inner,
                    int64_t outer, int32_t dtype, int32_t activation, void* workspace, int64_t workspace_bytes,
                    void* stream);
 
 /* ------------------------------------------------------------------------------
- * The backward pass of hbt_linear, in three calls that a caller may leave out singly.
+ * The backward pass of hbt_linear: dz = dy act'(z); dx = dz W; dw = dz^T x; dbias = the column
+ * sums of dz.
  *
  * Replaces: autograd's backward of the layers above (tests/distributed/test_fsdp.py:42-46),
  *   whose weight and bias gradients FlatParamHandle.reduce_scatter_gradient
  *   (parallel/fsdp.py:704-769) and the DDP buckets (parallel/ddp.py:513) take.
- * hbt_linear_slope: dz = dy act'(z), rounded once, and dbias = the column sums of the
- *   unrounded dz, added in a fixed order.  dz or dbias may be NULL (dz may be dy); z is read
- *   only with an activation.  dbias needs the whole workspace.  With tokens = 0 dbias is 0.
- * hbt_linear_grad_input: dx = dz W.  hbt_linear_grad_weight: dw = dz^T x (0 with no tokens).
- * Layouts, dtypes, workspaces and limits are hbt_linear's.  No atomics: results repeat bitwise.
+ * dx, dw and dbias may each be NULL, which leaves it out; z is read only with an activation,
+ * w only for dx and x only for dw.  dz is rounded once to the dtype for the products; dbias
+ * sums the unrounded values in a fixed order.  With tokens = 0, dw and dbias are 0.
+ * `workspace` (256-byte aligned) holds at least hbt_linear_backward_workspace's bytes for
+ * these sizes and `wants`, the HBT_LINEAR_* of the results asked for (-1 for bad arguments).
+ * Layouts, dtypes and limits are hbt_linear's.  No atomics: results repeat bitwise.
  * ---------------------------------------------------------------------------- */
-int32_t hbt_linear_slope(const void* dy, int64_t lddy, const void* z, int64_t ldz, void* dz, int64_t lddz, void* dbias,
-                         int64_t tokens, int64_t outer, int32_t dtype, int32_t activation, void* workspace,
-                         int64_t workspace_bytes, void* stream);
-int32_t hbt_linear_grad_input(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx,
-                              int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, void* workspace,
-                              int64_t workspace_bytes, void* stream);
-int32_t hbt_linear_grad_weight(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw,
-                               int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, void* workspace,
-                               int64_t workspace_bytes, void* stream);
+#define HBT_LINEAR_DX 1
+#define HBT_LINEAR_DW 2
+#define HBT_LINEAR_DBIAS 4
+int64_t hbt_linear_backward_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t activation,
+                                      int32_t wants);
+int32_t hbt_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                            const void* z, int64_t ldz, void* dx, int64_t lddx, void* dw, int64_t lddw, void* dbias,
+                            int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t activation,
+                            void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
