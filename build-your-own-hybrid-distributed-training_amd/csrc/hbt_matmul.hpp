@@ -316,8 +316,14 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
 // Hands the tile's results to `store(m, n, v)`, four consecutive n at a time, each in one lane,
 // rows in order: the accumulators pass through LDS (free by now), so the code that finishes a
 // result stands once, in a loop, and a wave's loads and stores cover whole rows.
-template <int D, class T, class Store>
-__device__ __forceinline__ void finish_tile(char* lds, const f32x4 (&acc)[T::TM][T::TN], Store&& store) {
+//
+// `mirror(n, m, v)`, unless it is NoMirror or `mirrored` is false, then gets the transposed
+// tile, four consecutive m at a time: a wave takes sixteen n by four units of m, so its LDS
+// reads fall on distinct banks and its stores cover 32 bytes of a row.
+struct NoMirror {};
+template <int D, class T, class Store, class Mirror = NoMirror>
+__device__ __forceinline__ void finish_tile(char* lds, const f32x4 (&acc)[T::TM][T::TN], Store&& store,
+                                            bool mirrored = false, Mirror&& mirror = Mirror{}) {
     constexpr int kRowUnits = T::BN / 4, kPhases = T::BM * T::BN * 4 > lds_bytes<D, T>() ? T::WM : 1;
     constexpr int kRows = T::BM / kPhases;
     static_assert(kRows * T::BN * 4 <= lds_bytes<D, T>(), "a phase fits the tile's LDS");
@@ -340,6 +346,20 @@ __device__ __forceinline__ void finish_tile(char* lds, const f32x4 (&acc)[T::TM]
         for (int u = tid; u < kRows * kRowUnits; u += T::kThreads) {
             const int m = u / kRowUnits, unit = u % kRowUnits;
             store(phase * kRows + m, unit * 4, out[m * kRowUnits + (unit ^ (m & 15))]);
+        }
+        if constexpr (!std::is_same_v<std::decay_t<Mirror>, NoMirror>) {
+            if (mirrored) {
+                const float* flat = reinterpret_cast<const float*>(lds);
+                for (int u = tid; u < T::BN * kRows / 4; u += T::kThreads) {
+                    const int block = u >> 6, n = block % (T::BN / 16) * 16 + (u & 15);
+                    const int m = (block / (T::BN / 16) * 4 + ((u >> 4) & 3)) * 4;
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        v[e] = flat[((m + e) * kRowUnits + ((n >> 2) ^ ((m + e) & 15))) * 4 + (n & 3)];
+                    mirror(n, phase * kRows + m, v);
+                }
+            }
         }
     }
 }

@@ -1,0 +1,712 @@
+// Orthogonalised updates: momentum, Newton-Schulz products, the step.
+//
+//   v' = mu v + (1 - mu) g;  u = (1 - mu) g + mu v' (Nesterov) or v';  x = u / max(|u|, eps)
+//   `steps` times:  A = x x^T (or x^T x, over the shorter side),  B = b A + c A A,  x = a x + B x
+//   w' = decay w - lr scale x
+//
+// The iterate x is held in fp32.  The products read copies of x, A and B rounded to the product
+// type: fp16 (11 bits, and the values are bounded: singular values stay below 1.3, and x is
+// scaled by a power of two near the square root of its longer side, which puts its elements near
+// 1 and the first iterate's above fp16's subnormals) or, on request, fp32.  Rounding x itself
+// to 16 bits would be amplified by 3.4 a step in the directions that start small: on matrices with
+// a decaying spectrum fp16 products then end 6e-3 to 9e-3 off, and 3e-4 to 2e-3 with x in fp32.
+//
+// Every phase takes all matrices of one orientation in one launch: the tiles of up to 16
+// matrices of any sizes, found in a table in the launch's arguments.
+#include "hbt_matmul.hpp"
+
+namespace hbt {
+namespace mm {
+namespace {
+
+constexpr int kMaxMatrices = HBT_MAX_TENSORS_PER_LAUNCH;
+constexpr int kChunk = 4096;  // elements per norm partial
+constexpr int kMaxSteps = 64;
+
+// ---- the direction and its norm --------------------------------------------------------
+struct DirectionEntry {
+    const void* g;
+    float* v;        // null: u is the input itself
+    float* u;        // fp32, dense
+    double* partial;
+    int64_t numel, first_block;
+};
+struct DirectionArgs {
+    DirectionEntry entry[kMaxMatrices];
+    const float* grad_mul;
+    const float* slot;  // null, or the momentum and its complement are its third and fourth float
+    float unscale, momentum, rest;
+    int count, nesterov;
+};
+
+template <int N, class Entry>
+__device__ __forceinline__ int find_entry(const Entry (&entry)[N], int count, int64_t block) {
+    int e = 0;
+    while (e + 1 < count && entry[e + 1].first_block <= block) ++e;
+    return e;
+}
+
+// One pass over the gradients: the momentum, the direction, and its squares summed in fp64.
+template <int GD>
+__global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
+    const int64_t block = blockIdx.x;
+    const DirectionEntry& t = p.entry[find_entry(p.entry, p.count, block)];
+    const int64_t chunk = block - t.first_block, base = chunk * kChunk;
+    const float mul = p.grad_mul != nullptr ? *p.grad_mul : 1.0f;
+    const float mu = p.slot != nullptr ? p.slot[2] : p.momentum, rest = p.slot != nullptr ? p.slot[3] : p.rest;
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < kChunk / 1024; ++k) {
+        const int64_t i = base + k * 1024 + threadIdx.x * 4;
+        if (i >= t.numel) break;
+        f32x4 u;
+        if (i + 4 <= t.numel) {
+            u = load4<GD>(t.g, i) * p.unscale * mul;
+            if (t.v != nullptr) {
+                f32x4 v = load4<HBT_DTYPE_F32>(t.v, i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = mu * v[e] + rest * u[e];
+                    u[e] = p.nesterov ? mu * v[e] + rest * u[e] : v[e];
+                }
+                store4<HBT_DTYPE_F32>(t.v, i, v);
+            }
+            store4<HBT_DTYPE_F32>(t.u, i, u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += double(u[e]) * double(u[e]);
+        } else {
+            for (int64_t j = i; j < t.numel; ++j) {
+                float x = load_elem<GD>(t.g, j) * p.unscale * mul;
+                if (t.v != nullptr) {
+                    const float v = mu * t.v[j] + rest * x;
+                    x = p.nesterov ? mu * v + rest * x : v;
+                    t.v[j] = v;
+                }
+                t.u[j] = x;
+                sum += double(x) * double(x);
+            }
+        }
+    }
+    const double total = block_sum<256>(sum);
+    if (threadIdx.x == 0) t.partial[chunk] = total;
+}
+
+struct NormEntry {
+    const double* partial;
+    float* factor;
+    int64_t chunks;
+    float scale;  // the power of two the iterate is held at
+};
+struct NormArgs {
+    NormEntry entry[kMaxMatrices];
+    double eps;
+};
+
+// scale / norm within float's range; 0 for a zero norm, whose u is 0 and stays 0.
+__device__ __forceinline__ float factor_of(float scale, double norm) {
+    const double f = scale / norm;
+    return norm == 0.0 ? 0.0f : (f > 3.4028234e38 ? 3.4028234e38f : static_cast<float>(f));
+}
+
+// factor = scale / max(|u|, eps), one workgroup a matrix, partials in a fixed order.
+__global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
+    const NormEntry& t = p.entry[blockIdx.x];
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < t.chunks; i += 1024) sum += t.partial[i];
+    const double total = block_sum<1024>(sum);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(total);
+        const double floor = norm < p.eps ? p.eps : norm;  // a NaN norm stays one
+        *t.factor = factor_of(t.scale, floor);
+    }
+}
+
+struct StartEntry {
+    const float* u;
+    void* x;
+    const float* factor;
+    int64_t rows, cols, ld, first_block;
+};
+struct StartArgs {
+    StartEntry entry[kMaxMatrices];
+    int count;
+};
+
+// The first iterate in the product type, rows on 16-byte boundaries: eight columns a lane.
+template <int D>
+__global__ __launch_bounds__(256) void start_kernel(StartArgs p) {
+    const int64_t block = blockIdx.x;
+    const StartEntry& t = p.entry[find_entry(p.entry, p.count, block)];
+    const int64_t units = t.ld / 8, i = (block - t.first_block) * 256 + threadIdx.x;
+    if (i >= t.rows * units) return;
+    const int64_t row = i / units, col = i % units * 8;
+    const float f = *t.factor;
+    const float* u = t.u + row * t.cols + col;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (col + 4 * h + 4 <= t.cols) {
+            v = load4<HBT_DTYPE_F32>(u, 4 * h) * f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (col + 4 * h + e < t.cols) v[e] = u[4 * h + e] * f;
+        }
+        store4<D>(t.x, row * t.ld + col + 4 * h, v);
+    }
+}
+
+// ---- the products ----------------------------------------------------------------------
+enum Phase { kGram, kSquare, kIterate };
+
+struct Problem {
+    const void* x;        // the iterate in the product type, [rows][ldx]
+    void* x_next;
+    void* gram;           // [side][ldg], side the shorter one
+    void* poly;
+    float* state;         // the fp32 iterate [rows][cols] (fp16 products), or null
+    const float* factor;  // first step: the state is still u, to be multiplied by this
+    void* out;            // last step: the parameter or the result, [rows][cols]
+    int rows, cols, ldx, first_block;
+    float gram_scale;     // 1 / scale^2
+    float out_scale;      // the step's multiple of x, over scale
+};
+struct ProductArgs {
+    Problem problem[kMaxMatrices];
+    const float* slot;    // null, or decay and learning rate are its first two floats
+    float a, b, c, decay, lr;
+    int count, first, last, update, out_dtype;
+};
+
+// Elements j .. j + 3 of a row of `cols`, in either rounding: all four, or those that exist.
+template <int D>
+__device__ __forceinline__ f32x4 load_row(const void* p, int64_t i, int have) {
+    if (have >= 4) return load4<D>(p, i);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < 3; ++e)
+        if (e < have) v[e] = load_elem<D>(p, i + e);
+    return v;
+}
+template <int D>
+__device__ __forceinline__ void store_row(void* p, int64_t i, int have, f32x4 v) {
+    if (have >= 4) {
+        store4<D>(p, i, v);
+        return;
+    }
+    for (int e = 0; e < 3; ++e)
+        if (e < have) store_elem<D>(p, i + e, v[e]);
+}
+
+// w' = decay w - lr out_scale x, or the result out_scale x itself.
+template <int D>
+__device__ __forceinline__ void finish(const ProductArgs& p, const Problem& t, float decay, float lr, int64_t i,
+                                       int have, f32x4 x) {
+    if (p.update) x = load_row<D>(t.out, i, have) * decay - x * (lr * t.out_scale);
+    else x *= t.out_scale;
+    store_row<D>(t.out, i, have, x);
+}
+
+// kWide: rows <= columns, so A = x x^T and x' = a x + B x; else A = x^T x and x' = a x + x B.
+template <int D, class T, Phase kPhase, bool kWide>
+__global__ __launch_bounds__(T::kThreads) void newton_schulz_kernel(ProductArgs p) {
+    extern __shared__ __align__(16) char lds[];
+    const int block = xcd_tile(blockIdx.x, gridDim.x);
+    const Problem& t = p.problem[find_entry(p.problem, p.count, block)];
+    const int tile = block - t.first_block, side = kWide ? t.rows : t.cols;
+    const int ldg = (side + 7) / 8 * 8;
+    int tm, tn;
+    if constexpr (kPhase == kIterate) {
+        band_order<8>(tile, (t.rows + T::BM - 1) / T::BM, (t.cols + T::BN - 1) / T::BN, tm, tn);
+    } else {  // the lower triangle of a symmetric result, row by row
+        tm = static_cast<int>((sqrtf(8.0f * tile + 1.0f) - 1.0f) * 0.5f);
+        while (tm * (tm + 1) / 2 > tile) --tm;
+        while ((tm + 1) * (tm + 2) / 2 <= tile) ++tm;
+        tn = tile - tm * (tm + 1) / 2;
+    }
+    const int m0 = tm * T::BM, n0 = tn * T::BN;
+    f32x4 acc[T::TM][T::TN];
+    if constexpr (kPhase == kGram) {
+        // Columns past the last one are padding of x's rows: read, never stored.
+        const int count = kWide ? side : t.ldx, k = kWide ? t.cols : t.rows;
+        tile_product<D, kWide, kWide, T, false>(t.x, t.ldx, m0, count, t.x, t.ldx, n0, count, 0, k, lds, acc);
+    } else if constexpr (kPhase == kSquare) {
+        tile_product<D, true, true, T, false>(t.gram, ldg, m0, side, t.gram, ldg, n0, side, 0, side, lds, acc);
+    } else if constexpr (kWide) {
+        tile_product<D, true, false, T, false>(t.poly, ldg, m0, side, t.x, t.ldx, n0, t.ldx, 0, side, lds, acc);
+    } else {
+        tile_product<D, true, true, T, false>(t.x, t.ldx, m0, t.rows, t.poly, ldg, n0, side, 0, side, lds, acc);
+    }
+    if constexpr (kPhase == kIterate) {
+        const float factor = p.first && t.state != nullptr ? *t.factor : 1.0f;
+        const float decay = p.slot != nullptr ? p.slot[0] : p.decay, lr = p.slot != nullptr ? p.slot[1] : p.lr;
+        finish_tile<D, T>(lds, acc, [&](int i, int j, f32x4 v) {
+            const int m = m0 + i, n = n0 + j, have = t.cols - n;
+            if (m >= t.rows || have <= 0) return;
+            const int64_t dense = int64_t(m) * t.cols + n, padded = int64_t(m) * t.ldx + n;
+            const f32x4 x = D == HBT_DTYPE_F32 ? load4<D>(t.x, padded)
+                                               : load_row<HBT_DTYPE_F32>(t.state, dense, have) * factor;
+            v += x * p.a;
+            if (p.last) {
+                if (p.out_dtype == HBT_DTYPE_F32) finish<HBT_DTYPE_F32>(p, t, decay, lr, dense, have, v);
+                else if (p.out_dtype == HBT_DTYPE_BF16) finish<HBT_DTYPE_BF16>(p, t, decay, lr, dense, have, v);
+                else finish<HBT_DTYPE_F16>(p, t, decay, lr, dense, have, v);
+            } else {
+                if constexpr (D != HBT_DTYPE_F32) store_row<HBT_DTYPE_F32>(t.state, dense, have, v);
+                store4<D>(t.x_next, padded, v);
+            }
+        });
+    } else {
+        void* out = kPhase == kGram ? t.gram : t.poly;
+        const auto value = [&](int m, int n, f32x4 v) {
+            if constexpr (kPhase == kGram) return v * t.gram_scale;
+            else return load4<D>(t.gram, int64_t(m) * ldg + n) * p.b + v * p.c;
+        };
+        const auto store = [&](int i, int j, f32x4 v) {
+            const int m = m0 + i, n = n0 + j;
+            if (m < side && n < side) store4<D>(out, int64_t(m) * ldg + n, value(m, n, v));
+        };
+        // Off the diagonal the mirror image is stored too: the products are bitwise symmetric.
+        finish_tile<D, T>(lds, acc, store, tm != tn, [&](int j, int i, f32x4 v) {
+            const int n = n0 + j, m = m0 + i;
+            if (n < side && m < side) store4<D>(out, int64_t(n) * ldg + m, value(n, m, v));
+        });
+    }
+}
+
+// ---- small matrices --------------------------------------------------------------------
+// A matrix whose sides are at most 64 and 128 is one workgroup's whole step, in fp32: it stays
+// in LDS from its gradient to its parameter, so a model of small matrices is one launch.  The
+// products are 16 x 16 tiles of fp32 matrix instructions over LDS, zero-padded to whole tiles.
+constexpr int kSmallSide = 64, kSmallLong = 128;
+constexpr int kSmallLd = kSmallSide + 4, kSmallXLd = kSmallLong + 4;  // 16 rows by 4 k: distinct banks
+constexpr int kSmallLds = 4 * (kSmallSide * kSmallXLd + 2 * kSmallSide * kSmallLd);
+
+struct SmallEntry {
+    const void* g;
+    float* v;
+    void* out;
+    int rows, cols;
+    float scale;
+};
+struct SmallArgs {
+    SmallEntry entry[kMaxMatrices];
+    const float* grad_mul;
+    const float* slot;
+    double eps;
+    float unscale, momentum, rest, a, b, c, decay, lr;
+    int nesterov, steps, update, out_dtype;
+};
+
+template <int GD>
+__global__ __launch_bounds__(512) void small_kernel(SmallArgs p) {
+    extern __shared__ __align__(16) char lds[];
+    float* x = reinterpret_cast<float*>(lds);
+    float* gram = x + kSmallSide * kSmallXLd;
+    float* poly = gram + kSmallSide * kSmallLd;
+    const SmallEntry& t = p.entry[blockIdx.x];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 15, q = lane >> 4;
+    const bool wide = t.rows <= t.cols;
+    const int side = wide ? t.rows : t.cols, len = wide ? t.cols : t.rows;
+    const int side16 = (side + 15) / 16, len16 = (len + 15) / 16, numel = t.rows * t.cols;
+    const float mul = p.grad_mul != nullptr ? *p.grad_mul : 1.0f;
+    const float mu = p.slot != nullptr ? p.slot[2] : p.momentum, rest = p.slot != nullptr ? p.slot[3] : p.rest;
+    const auto place = [&](int i) {  // element i of the matrix in x, its shorter side as rows
+        const int r = i / t.cols, c = i % t.cols;
+        return wide ? r * kSmallXLd + c : c * kSmallXLd + r;
+    };
+    for (int i = tid; i < kSmallSide * kSmallXLd; i += 512) x[i] = 0.0f;
+    __syncthreads();
+    double sum = 0.0;
+    for (int i = tid; i < numel; i += 512) {
+        float u = load_elem<GD>(t.g, i) * p.unscale * mul;
+        if (t.v != nullptr) {
+            const float v = mu * t.v[i] + rest * u;
+            u = p.nesterov ? mu * v + rest * u : v;
+            t.v[i] = v;
+        }
+        x[place(i)] = u;
+        sum += double(u) * double(u);
+    }
+    const double total = block_sum<512>(sum);
+    __shared__ float factor;
+    if (tid == 0) {
+        const double norm = sqrt(total);
+        const double floor = norm < p.eps ? p.eps : norm;
+        factor = factor_of(1.0f, floor);
+    }
+    __syncthreads();
+    for (int i = tid; i < numel; i += 512) x[place(i)] *= factor;
+    __syncthreads();
+    for (int s = 0; s < p.steps; ++s) {
+        for (int tile = wave; tile < side16 * side16; tile += 8) {  // A = x x^T
+            const float* a = x + (tile / side16 * 16 + row) * kSmallXLd + q;
+            const float* b = x + (tile % side16 * 16 + row) * kSmallXLd + q;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < len16 * 16; k += 4) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], b[k], acc, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) gram[(tile / side16 * 16 + 4 * q + e) * kSmallLd + tile % side16 * 16 + row] = acc[e];
+        }
+        __syncthreads();
+        for (int tile = wave; tile < side16 * side16; tile += 8) {  // B = b A + c A A, A symmetric
+            const float* a = gram + (tile / side16 * 16 + row) * kSmallLd + q;
+            const float* b = gram + (tile % side16 * 16 + row) * kSmallLd + q;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < side16 * 16; k += 4) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], b[k], acc, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int at = (tile / side16 * 16 + 4 * q + e) * kSmallLd + tile % side16 * 16 + row;
+                poly[at] = p.b * gram[at] + p.c * acc[e];
+            }
+        }
+        __syncthreads();
+        for (int col = wave; col < len16; col += 8) {  // 16 columns of x = a x + B x, this wave's alone
+            f32x4 acc[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < side16 * 16; k += 4) {
+                const float b = x[(k + q) * kSmallXLd + col * 16 + row];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < side16)
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(poly[(i * 16 + row) * kSmallLd + k + q], b, acc[i],
+                                                                      0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i >= side16) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float* at = x + (i * 16 + 4 * q + e) * kSmallXLd + col * 16 + row;
+                    *at = p.a * *at + acc[i][e];
+                }
+            }
+        }
+        __syncthreads();
+    }
+    const float decay = p.slot != nullptr ? p.slot[0] : p.decay, lr = p.slot != nullptr ? p.slot[1] : p.lr;
+    const auto finish_all = [&](auto d) {
+        constexpr int PD = decltype(d)::value;
+        for (int i = tid; i < numel; i += 512) {
+            float w = x[place(i)] * t.scale;
+            if (p.update) w = load_elem<PD>(t.out, i) * decay - lr * w;
+            store_elem<PD>(t.out, i, w);
+        }
+    };
+    if (p.out_dtype == HBT_DTYPE_F32) finish_all(std::integral_constant<int, HBT_DTYPE_F32>{});
+    else if (p.out_dtype == HBT_DTYPE_BF16) finish_all(std::integral_constant<int, HBT_DTYPE_BF16>{});
+    else finish_all(std::integral_constant<int, HBT_DTYPE_F16>{});
+}
+
+// ---- host ----------------------------------------------------------------------------
+using Tile256 = Tile<256, 256, 2, 4>;
+using Tile128 = Tile<128, 128, 2, 2>;
+using Tile64 = Tile<64, 64, 2, 2>;
+
+struct Plan {
+    int64_t state, x0, x1, gram, poly, partial, factor, end;  // offsets of one matrix's storage
+    int64_t chunks, ldx, ldg;
+};
+
+Plan plan_of(int64_t rows, int64_t cols, int product, int64_t at) {
+    const auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const int64_t size = product == HBT_DTYPE_F32 ? 4 : 2, side = std::min(rows, cols);
+    Plan p{};
+    p.ldx = (cols + 7) / 8 * 8;
+    p.ldg = (side + 7) / 8 * 8;
+    p.chunks = (rows * cols + kChunk - 1) / kChunk;
+    p.state = take(rows * cols * 4);
+    p.x0 = take(rows * p.ldx * size);
+    p.x1 = take(rows * p.ldx * size);
+    p.gram = take(side * p.ldg * size);
+    p.poly = take(side * p.ldg * size);
+    p.partial = take(p.chunks * 8);
+    p.factor = take(4);
+    p.end = at;
+    return p;
+}
+
+// The power of two that brings an orthogonal matrix's elements near 1 in fp16.
+float iterate_scale(int64_t rows, int64_t cols, int product) {
+    if (product == HBT_DTYPE_F32) return 1.0f;
+    float s = 1.0f;
+    while (s * s * 4.0f <= static_cast<float>(std::max(rows, cols))) s *= 2.0f;
+    return s;
+}
+
+// A matrix's own product type: fp16's rounding errors average over a side longer than 64, and a
+// shorter side's products cost nothing beside its memory traffic, so those are formed in fp32.
+int product_of(int64_t rows, int64_t cols, int product) {
+    return std::min(rows, cols) <= 64 ? HBT_DTYPE_F32 : product;
+}
+
+bool is_small(int64_t rows, int64_t cols) {
+    return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= kSmallLong;
+}
+
+struct Matrices {
+    const void* const* grads;
+    float* const* momenta;
+    void* const* outs;
+    const int64_t* rows;
+    const int64_t* cols;
+    const float* scales;
+    int count;
+};
+
+int64_t tiles_of(const Problem& t, int size, Phase phase) {
+    const auto n = [&](int64_t extent) { return (extent + size - 1) / size; };
+    if (phase == kIterate) return n(t.rows) * n(t.cols);
+    const int64_t s = n(std::min(t.rows, t.cols));
+    return s * (s + 1) / 2;
+}
+
+template <int D, class T, Phase kPhase, bool kWide>
+int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t stream) {
+    constexpr int kLds = lds_bytes<D, T>();
+    int64_t blocks = 0;
+    for (int i = 0; i < p.count; ++i) {
+        p.problem[i].first_block = static_cast<int>(blocks);
+        blocks += tiles_of(p.problem[i], size, kPhase);
+    }
+    const auto kernel = newton_schulz_kernel<D, T, kPhase, kWide>;
+    if constexpr (kLds > 65536) {
+        static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+        if (set != hipSuccess) return check_hip(set, who);
+    }
+    kernel<<<dim3(static_cast<unsigned>(blocks)), T::kThreads, kLds, stream>>>(p);
+    return check_launch(who);
+}
+
+template <int D, Phase kPhase, bool kWide>
+int32_t launch_phase(const char* who, ProductArgs& p, hipStream_t stream) {
+    if (p.count == 0) return HBT_OK;
+    int64_t tiles256 = 0, tiles128 = 0;
+    for (int i = 0; i < p.count; ++i) {
+        tiles256 += tiles_of(p.problem[i], 256, kPhase);
+        tiles128 += tiles_of(p.problem[i], 128, kPhase);
+    }
+    if constexpr (D != HBT_DTYPE_F32) {
+        if (tiles256 >= 256) return launch_phase_tile<D, Tile256, kPhase, kWide>(who, p, 256, stream);
+    }
+    if (tiles128 >= 256) return launch_phase_tile<D, Tile128, kPhase, kWide>(who, p, 128, stream);
+    return launch_phase_tile<D, Tile64, kPhase, kWide>(who, p, 64, stream);
+}
+
+// The small matrices of a call, all in one launch.
+int32_t run_small(const char* who, const Matrices& t, int32_t grad_dtype, const DirectionArgs& direction,
+                  const ProductArgs& common, int steps, double eps, hipStream_t stream) {
+    SmallArgs p{};
+    int n = 0;
+    for (int i = 0; i < t.count; ++i) {
+        if (t.rows[i] * t.cols[i] == 0 || !is_small(t.rows[i], t.cols[i])) continue;
+        p.entry[n++] = {t.grads[i], t.momenta == nullptr ? nullptr : t.momenta[i], t.outs[i],
+                        static_cast<int>(t.rows[i]), static_cast<int>(t.cols[i]),
+                        t.scales == nullptr ? 1.0f : t.scales[i]};
+    }
+    if (n == 0) return HBT_OK;
+    p.grad_mul = direction.grad_mul, p.slot = direction.slot, p.eps = eps;
+    p.unscale = direction.unscale, p.momentum = direction.momentum, p.rest = direction.rest;
+    p.a = common.a, p.b = common.b, p.c = common.c, p.decay = common.decay, p.lr = common.lr;
+    p.nesterov = direction.nesterov, p.steps = steps, p.update = common.update, p.out_dtype = common.out_dtype;
+    const auto launch = [&](auto d) {
+        const auto kernel = small_kernel<decltype(d)::value>;
+        static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds);
+        if (set != hipSuccess) return check_hip(set, who);
+        kernel<<<dim3(n), 512, kSmallLds, stream>>>(p);
+        return check_launch(who);
+    };
+    if (grad_dtype == HBT_DTYPE_F32) return launch(std::integral_constant<int, HBT_DTYPE_F32>{});
+    if (grad_dtype == HBT_DTYPE_BF16) return launch(std::integral_constant<int, HBT_DTYPE_BF16>{});
+    return launch(std::integral_constant<int, HBT_DTYPE_F16>{});
+}
+
+// The matrices whose products read type D.
+template <int D>
+int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t product, DirectionArgs& direction,
+            ProductArgs& common, int steps, double eps, char* workspace, hipStream_t stream) {
+    NormArgs norm{};
+    StartArgs start{};
+    ProductArgs wide = common, tall = common;
+    wide.count = tall.count = 0;
+    norm.eps = eps;
+    int64_t at = 0, direction_blocks = 0, start_blocks = 0;
+    int n = 0;
+    for (int i = 0; i < t.count; ++i) {
+        const int64_t rows = t.rows[i], cols = t.cols[i];
+        if (rows == 0 || cols == 0 || is_small(rows, cols)) continue;
+        const int kind = product_of(rows, cols, product);
+        const Plan plan = plan_of(rows, cols, kind, at);
+        at = plan.end;
+        if (kind != D) continue;
+        const float scale = iterate_scale(rows, cols, D);
+        float* state = reinterpret_cast<float*>(workspace + plan.state);
+        float* factor = reinterpret_cast<float*>(workspace + plan.factor);
+        double* partial = reinterpret_cast<double*>(workspace + plan.partial);
+        direction.entry[n] = {t.grads[i], t.momenta == nullptr ? nullptr : t.momenta[i], state, partial, rows * cols,
+                              direction_blocks};
+        direction_blocks += plan.chunks;
+        norm.entry[n] = {partial, factor, plan.chunks, scale};
+        start.entry[n] = {state, workspace + plan.x0, factor, rows, cols, plan.ldx, start_blocks};
+        start_blocks += (rows * (plan.ldx / 8) + 255) / 256;
+        ++n;
+        ProductArgs& group = rows <= cols ? wide : tall;
+        group.problem[group.count++] = {workspace + plan.x0, workspace + plan.x1, workspace + plan.gram,
+                                        workspace + plan.poly, D == HBT_DTYPE_F32 ? nullptr : state, factor, t.outs[i],
+                                        static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(plan.ldx), 0,
+                                        1.0f / (scale * scale), (t.scales == nullptr ? 1.0f : t.scales[i]) / scale};
+    }
+    if (n == 0) return HBT_OK;
+    direction.count = start.count = n;
+    const dim3 direction_grid(static_cast<unsigned>(direction_blocks));
+    if (grad_dtype == HBT_DTYPE_F32) direction_kernel<HBT_DTYPE_F32><<<direction_grid, 256, 0, stream>>>(direction);
+    else if (grad_dtype == HBT_DTYPE_BF16) direction_kernel<HBT_DTYPE_BF16><<<direction_grid, 256, 0, stream>>>(direction);
+    else direction_kernel<HBT_DTYPE_F16><<<direction_grid, 256, 0, stream>>>(direction);
+    int32_t status = check_launch(who);
+    if (status != HBT_OK) return status;
+    norm_kernel<<<dim3(n), 1024, 0, stream>>>(norm);
+    if ((status = check_launch(who)) != HBT_OK) return status;
+    start_kernel<D><<<dim3(static_cast<unsigned>(start_blocks)), 256, 0, stream>>>(start);
+    if ((status = check_launch(who)) != HBT_OK) return status;
+    for (int s = 0; s < steps; ++s) {
+        for (ProductArgs* g : {&wide, &tall}) g->first = s == 0, g->last = s == steps - 1;
+        if ((status = launch_phase<D, kGram, true>(who, wide, stream)) != HBT_OK ||
+            (status = launch_phase<D, kGram, false>(who, tall, stream)) != HBT_OK ||
+            (status = launch_phase<D, kSquare, true>(who, wide, stream)) != HBT_OK ||
+            (status = launch_phase<D, kSquare, false>(who, tall, stream)) != HBT_OK ||
+            (status = launch_phase<D, kIterate, true>(who, wide, stream)) != HBT_OK ||
+            (status = launch_phase<D, kIterate, false>(who, tall, stream)) != HBT_OK)
+            return status;
+        for (ProductArgs* g : {&wide, &tall})
+            for (int i = 0; i < g->count; ++i) {
+                const void* x = g->problem[i].x;
+                g->problem[i].x = g->problem[i].x_next;
+                g->problem[i].x_next = const_cast<void*>(x);
+            }
+    }
+    return HBT_OK;
+}
+
+int32_t invalid(const char* who, const char* what) {
+    set_error("%s: %s", who, what);
+    return HBT_ERR_INVALID_ARGUMENT;
+}
+
+bool known(int32_t dtype) { return dtype == HBT_DTYPE_F32 || dtype == HBT_DTYPE_BF16 || dtype == HBT_DTYPE_F16; }
+
+// Sides that keep 16-byte units of a tile's rows inside 31-bit offsets, and element counts whose
+// workgroups fit one launch.
+constexpr int64_t kMaxSide = int64_t(1) << 20;
+constexpr int64_t kMaxElements = int64_t(1) << 34;
+
+int32_t check_matrices(const char* who, const Matrices& t, int32_t product, int32_t steps, int64_t* bytes) {
+    if (t.count < 0 || t.count > kMaxMatrices) {
+        set_error("%s: count %d is outside 0..%d", who, t.count, kMaxMatrices);
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    if (t.count > 0 && (t.rows == nullptr || t.cols == nullptr)) return invalid(who, "a table is null");
+    if (product != HBT_DTYPE_F16 && product != HBT_DTYPE_F32) {
+        set_error("%s: product dtype %d is not F16 or F32", who, product);
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    if (steps < 1 || steps > kMaxSteps) {
+        set_error("%s: %d steps are outside 1..%d", who, steps, kMaxSteps);
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    int64_t at = 0, elements = 0;
+    for (int i = 0; i < t.count; ++i) {
+        const int64_t rows = t.rows[i], cols = t.cols[i];
+        if (rows < 0 || cols < 0) return invalid(who, "a size is negative");
+        if (rows == 0 || cols == 0) continue;
+        if (rows > kMaxSide || cols > kMaxSide || (elements += rows * cols) > kMaxElements) {
+            set_error("%s: matrix %d (%lld x %lld) is past the limits of one call", who, i,
+                      static_cast<long long>(rows), static_cast<long long>(cols));
+            return HBT_ERR_UNSUPPORTED;
+        }
+        if (!is_small(rows, cols)) at = plan_of(rows, cols, product_of(rows, cols, product), at).end;
+    }
+    *bytes = at;
+    return HBT_OK;
+}
+
+int32_t dispatch(const char* who, const Matrices& t, int32_t grad_dtype, int32_t product, DirectionArgs& direction,
+                 ProductArgs& common, int steps, double eps, void* workspace, int64_t workspace_bytes, void* stream) {
+    int64_t need = 0;
+    const int32_t status = check_matrices(who, t, product, steps, &need);
+    if (status != HBT_OK) return status;
+    if (!known(grad_dtype) || !known(common.out_dtype)) return invalid(who, "dtypes are F32, BF16 or F16");
+    if (!(eps >= 0.0)) return invalid(who, "eps is negative");
+    for (int i = 0; i < t.count; ++i) {
+        if (t.rows[i] == 0 || t.cols[i] == 0) continue;
+        if (t.grads == nullptr || t.outs == nullptr || t.grads[i] == nullptr || t.outs[i] == nullptr ||
+            (t.momenta != nullptr && t.momenta[i] == nullptr))
+            return invalid(who, "a matrix is null");
+    }
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return invalid(who, "the workspace is smaller than hbt_orthogonal_workspace's");
+    char* space = static_cast<char*>(workspace);
+    const hipStream_t s = as_stream(stream);
+    int32_t launched = run_small(who, t, grad_dtype, direction, common, steps, eps, s);
+    if (launched == HBT_OK)
+        launched = run<HBT_DTYPE_F32>(who, t, grad_dtype, product, direction, common, steps, eps, space, s);
+    if (launched == HBT_OK && product != HBT_DTYPE_F32)
+        launched = run<HBT_DTYPE_F16>(who, t, grad_dtype, product, direction, common, steps, eps, space, s);
+    return launched;
+}
+
+}  // namespace
+}  // namespace mm
+}  // namespace hbt
+
+using namespace hbt;
+using namespace hbt::mm;
+
+extern "C" {
+
+int64_t hbt_orthogonal_workspace(const int64_t* rows, const int64_t* cols, int32_t count, int32_t product_dtype) {
+    clear_error();
+    Matrices t{};
+    t.rows = rows, t.cols = cols, t.count = count;
+    int64_t bytes = 0;
+    return check_matrices("hbt_orthogonal_workspace", t, product_dtype, 1, &bytes) == HBT_OK ? bytes : -1;
+}
+
+int32_t hbt_orthogonalize(const void* const* inputs, void* const* outputs, const int64_t* rows, const int64_t* cols,
+                          int32_t count, int32_t in_dtype, int32_t out_dtype, int32_t product_dtype, int32_t steps,
+                          float a, float b, float c, double eps, void* workspace, int64_t workspace_bytes,
+                          void* stream) {
+    clear_error();
+    Matrices t{inputs, nullptr, outputs, rows, cols, nullptr, count};
+    DirectionArgs direction{};
+    direction.unscale = 1.0f;
+    ProductArgs common{};
+    common.a = a, common.b = b, common.c = c, common.out_dtype = out_dtype;
+    return dispatch("hbt_orthogonalize", t, in_dtype, product_dtype, direction, common, steps, eps, workspace,
+                    workspace_bytes, stream);
+}
+
+int32_t hbt_muon_step(void* const* params, const void* const* grads, float* const* momenta, const int64_t* rows,
+                      const int64_t* cols, const float* scales, int32_t count, int32_t param_dtype, int32_t grad_dtype,
+                      int32_t product_dtype, float unscale, const float* grad_mul, float momentum,
+                      float one_minus_momentum, int32_t nesterov, int32_t steps, float a, float b, float c, double eps, float decay, float lr, const float* slot,
+                      void* workspace, int64_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* who = "hbt_muon_step";
+    if (count > 0 && momenta == nullptr) return invalid(who, "a table is null");
+    Matrices t{grads, momenta, params, rows, cols, scales, count};
+    DirectionArgs direction{};
+    direction.unscale = unscale, direction.grad_mul = grad_mul, direction.slot = slot;
+    direction.momentum = momentum, direction.rest = one_minus_momentum, direction.nesterov = nesterov;
+    ProductArgs common{};
+    common.a = a, common.b = b, common.c = c, common.out_dtype = param_dtype, common.update = 1;
+    common.decay = decay, common.lr = lr, common.slot = slot;
+    return dispatch(who, t, grad_dtype, product_dtype, direction, common, steps, eps, workspace, workspace_bytes,
+                    stream);
+}
+
+}  // extern "C"

@@ -58,8 +58,8 @@ const char* hbt_last_error(void) { return hbt::g_last_error.c_str(); }
 // Bumped whenever an exported signature or a table layout changes.
 int32_t hbt_abi_version(void) { return 22; }
 
-// Entry points declared in include/hbt.h (hbt_last_error .. hbt_linear_backward).
-int32_t hbt_symbol_count(void) { return 44; }
+// Entry points declared in include/hbt.h (hbt_last_error .. hbt_muon_step).
+int32_t hbt_symbol_count(void) { return 47; }
 
 int64_t hbt_grid_slices(int64_t blocks, int32_t threads, int64_t* first, int64_t* count, int64_t capacity) {
     if (threads <= 0) return -1;

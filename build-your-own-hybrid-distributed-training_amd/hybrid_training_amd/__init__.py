@@ -14,6 +14,7 @@ from .config import (
     FSDPConfig,
     GradScalerConfig,
     MixedPrecisionConfig,
+    MuonConfig,
     OptimizerConfig,
     resolve_dtype,
 )
@@ -44,6 +45,7 @@ from .manifest import (
     shard_filename,
     validate_shard_filename,
 )
+from .muon import MuonOptimizer, orthogonalize
 from .optim import (
     NormContribution,
     ShardedOptimizer,

@@ -295,6 +295,19 @@ EXPORTED_SYMBOLS: dict[str, tuple[object, tuple[object, ...]]] = {
         (_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p,
          _c_i64, _c_void_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_void_p, _c_i64, _c_void_p),
     ),
+    "hbt_orthogonal_workspace": (_c_i64, (_i64_array, _i64_array, _c_i32, _c_i32)),
+    "hbt_orthogonalize": (
+        _c_i32,
+        (_ptr_array, _ptr_array, _i64_array, _i64_array, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_f32, _c_f32,
+         _c_f64, _c_void_p, _c_i64, _c_void_p),
+    ),
+    "hbt_muon_step": (
+        _c_i32,
+        (_ptr_array, _ptr_array, _ptr_array, _i64_array, _i64_array, ctypes.POINTER(_c_f32), _c_i32, _c_i32, _c_i32,
+         _c_i32, _c_f32, _c_void_p, _c_f32, _c_f32, _c_i32, _c_i32, _c_f32, _c_f32, _c_f32, _c_f64, _c_f32, _c_f32,
+         _c_void_p,
+         _c_void_p, _c_i64, _c_void_p),
+    ),
 }
 
 _LOCK = threading.Lock()

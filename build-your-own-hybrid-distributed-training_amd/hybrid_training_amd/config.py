@@ -9,6 +9,7 @@ configuration built for the reference builds here unchanged.
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 
 import torch
@@ -20,7 +21,9 @@ __all__ = [
     "FSDPConfig",
     "GradScalerConfig",
     "MixedPrecisionConfig",
+    "MuonConfig",
     "OptimizerConfig",
+    "check_newton_schulz",
     "resolve_dtype",
 ]
 
@@ -197,3 +200,51 @@ class OptimizerConfig:
             _fail("OptimizerConfig", "betas must be two values in [0, 1)",
                   "(b1, b2) with 0 <= b < 1", self.betas, "e.g. (0.9, 0.999)")
         object.__setattr__(self, "betas", betas)
+
+
+def check_newton_schulz(owner: str, steps: int, coefficients: tuple[float, float, float], eps: float) -> None:
+    """Refuse step counts, coefficients and norm floors the products cannot use."""
+    if int(steps) != steps or not 1 <= steps <= 64:
+        _fail(owner, "steps must be a whole number from 1 to 64", "1..64", steps,
+              "5 steps bring every singular value of an update near 1")
+    if len(tuple(coefficients)) != 3 or not all(math.isfinite(c) for c in coefficients):
+        _fail(owner, "coefficients must be three finite values", "(a, b, c)", coefficients,
+              "x becomes a x + (b A + c A A) x")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        _fail(owner, "eps must be finite and non-negative", ">= 0", eps, "the norm is held at eps or above")
+
+
+@dataclass(frozen=True)
+class MuonConfig:
+    """Orthogonalised-momentum hyper-parameters (no counterpart in the reference).
+
+    ``scale`` says what multiplies the learning rate of a rows x cols matrix: ``"rms"``,
+    ``0.2 sqrt(max(rows, cols))``, gives updates the size of AdamW's, so AdamW's learning rate
+    and weight decay carry over; ``"spectral"`` is ``sqrt(max(1, rows / cols))``.
+    ``product_dtype`` is what the matrix cores read: ``"float16"`` or ``"float32"``.
+    """
+
+    learning_rate: float = 1e-3
+    weight_decay: float = 0.0
+    momentum: float = 0.95
+    nesterov: bool = True
+    steps: int = 5
+    coefficients: tuple[float, float, float] = (3.4445, -4.7750, 2.0315)
+    eps: float = 1e-12
+    scale: str = "rms"
+    product_dtype: str = "float16"
+
+    def __post_init__(self) -> None:
+        if self.learning_rate <= 0:
+            _fail("MuonConfig", "learning_rate must be positive", "> 0", self.learning_rate,
+                  "a step needs a learning rate above zero")
+        if not 0.0 <= self.momentum < 1.0:
+            _fail("MuonConfig", "momentum must lie in [0, 1)", "0 <= m < 1", self.momentum, "0.95 is usual")
+        if self.scale not in ("rms", "spectral"):
+            _fail("MuonConfig", "unknown update scale", ["rms", "spectral"], self.scale,
+                  "rms matches AdamW's update size")
+        if resolve_dtype(self.product_dtype) not in (torch.float16, torch.float32):
+            _fail("MuonConfig", "the products read float16 or float32", ["float16", "float32"], self.product_dtype,
+                  "float16 is the fast one; sums are float32 either way")
+        check_newton_schulz("MuonConfig", self.steps, self.coefficients, self.eps)
+        object.__setattr__(self, "coefficients", tuple(float(c) for c in self.coefficients))

@@ -682,6 +682,44 @@ int32_t hbt_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t
                             int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t activation,
                             void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------
+ * Matrices orthogonalised by Newton-Schulz products, and the optimizer step that moves its
+ * parameters along them.
+ *
+ * Replaces: for matrix parameters, the update of ShardedOptimizer.step
+ *   (optim/sharded_optimizer.py:340-355) by an orthogonalised one; the reference has AdamW and
+ *   SGD only.
+ * Up to HBT_MAX_TENSORS_PER_LAUNCH dense row-major matrices of any sizes, rows[i] x cols[i]
+ * (sides at most 2^20, at most 2^34 elements a call; an empty one is skipped):
+ *   x = u / max(|u|, eps) (Frobenius norm);  `steps` (1..64) times
+ *     A = x x^T, or x^T x when rows > cols;  B = b A + c A A;  x = a x + B x, or a x + x B
+ * hbt_orthogonalize: u = inputs[i] (in_dtype), outputs[i] = x (out_dtype).  An output may be
+ * its input.
+ * hbt_muon_step, on parameters of param_dtype, gradients of grad_dtype and fp32 momenta:
+ *   g = grads[i] unscale (*grad_mul);  v = momentum v + one_minus_momentum g
+ *   u = one_minus_momentum g + momentum v with nesterov, else v
+ *   params[i] = decay params[i] - lr scales[i] x     (scales NULL = 1; grad_mul NULL = 1)
+ * in fp32, each result rounded once.  `slot`: NULL, or device memory holding the fp32 decay,
+ * lr, momentum and one_minus_momentum, read in place of the arguments when the kernels run, for a step recorded
+ * into a HIP graph.
+ * Dtypes: F32, BF16 or F16 each.  Sums are held in fp32 and the norm in fp64; x is carried in
+ * fp32.  The products read x, A and B rounded to product_dtype: F16, or F32; a matrix whose
+ * shorter side is at most 64 takes F32 either way.  A non-finite
+ * gradient makes its whole matrix non-finite.  No atomics: results repeat bitwise.
+ * `workspace` (256-byte aligned) holds at least hbt_orthogonal_workspace's bytes for these
+ * matrices (-1 for bad arguments).
+ * ---------------------------------------------------------------------------- */
+int64_t hbt_orthogonal_workspace(const int64_t* rows, const int64_t* cols, int32_t count, int32_t product_dtype);
+int32_t hbt_orthogonalize(const void* const* inputs, void* const* outputs, const int64_t* rows, const int64_t* cols,
+                          int32_t count, int32_t in_dtype, int32_t out_dtype, int32_t product_dtype, int32_t steps,
+                          float a, float b, float c, double eps, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+int32_t hbt_muon_step(void* const* params, const void* const* grads, float* const* momenta, const int64_t* rows,
+                      const int64_t* cols, const float* scales, int32_t count, int32_t param_dtype, int32_t grad_dtype,
+                      int32_t product_dtype, float unscale, const float* grad_mul, float momentum,
+                      float one_minus_momentum, int32_t nesterov, int32_t steps, float a, float b, float c, double eps, float decay, float lr, const float* slot,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
