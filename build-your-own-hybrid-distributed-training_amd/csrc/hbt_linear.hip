@@ -91,7 +91,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_
     }
 }
 
-template <int D, bool kA, bool kB, class T, bool kEdge>
+template <int D, bool kA, bool kB, class T, bool kAsync>
 __global__ __launch_bounds__(T::kThreads) void product_kernel(ProductArgs p) {
     extern __shared__ __align__(16) char lds[];
     const int t = xcd_tile(blockIdx.x, gridDim.x);
@@ -100,8 +100,8 @@ __global__ __launch_bounds__(T::kThreads) void product_kernel(ProductArgs p) {
     const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
     const int64_t k0 = blockIdx.y * p.k_split, k1 = min(p.k, k0 + p.k_split);
     f32x4 acc[T::TM][T::TN];
-    tile_product<D, kA, kB, T, kEdge>(p.a, p.lda, m0, p.m, p.b, p.ldb, n0, p.n, k0, k1, lds, acc);
-    finish_tile<D, T>(lds, acc, [&](int i, int j, f32x4 v) {
+    tile_product<D, kA, kB, T, kAsync>(p.a, p.lda, m0, p.m, p.b, p.ldb, n0, p.n, k0, k1, lds, acc);
+    finish_tile<T, kAsync>(lds, acc, [&](int i, int j, f32x4 v) {
         const int64_t m = m0 + i, n = n0 + j;
         if (m >= p.m || n >= p.n) return;
         if (p.partial != nullptr) *reinterpret_cast<f32x4*>(p.partial + (blockIdx.y * p.m + m) * p.ldp + n) = v;
@@ -251,9 +251,9 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* partial, int64_t
 }
 
 // ---- host ----------------------------------------------------------------------------
-using Tile256 = Tile<256, 256, 2, 4>;
-using Tile128 = Tile<128, 128, 2, 2>;
-using Tile64 = Tile<64, 64, 2, 2>;
+using Tile256 = Tile<256, 256, 2, 4, 2>;
+using Tile128 = Tile<128, 128, 2, 2, 2>;
+using Tile64 = Tile<64, 64, 2, 2, 4>;
 
 struct Choice {
     int tile;    // 256, 128 or 64
@@ -262,11 +262,11 @@ struct Choice {
 
 constexpr int kMaxSplits = 16;
 
-Choice choose(int64_t m, int64_t n, int64_t k, int dtype, bool whole_units) {
+Choice choose(int64_t m, int64_t n, int64_t k, int dtype, bool aligned) {
     const int bk = dtype == HBT_DTYPE_F32 ? 32 : 64;
     const int64_t cus = 256;
     const auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-    if (dtype != HBT_DTYPE_F32 && whole_units && tiles(256) >= cus) return {256, 1};
+    if (dtype != HBT_DTYPE_F32 && aligned && tiles(256) >= cus) return {256, 1};
     const int tile = tiles(128) >= cus ? 128 : 64;
     const int64_t count = tiles(tile), steps = (k + bk - 1) / bk;
     int64_t splits = 1;
@@ -274,16 +274,19 @@ Choice choose(int64_t m, int64_t n, int64_t k, int dtype, bool whole_units) {
     return {tile, static_cast<int>(std::max<int64_t>(splits, 1))};
 }
 
-// Whether no unit of an operand that is not k-major crosses its last row.
-template <bool kA, bool kB>
-bool whole_units(int64_t m, int64_t n) { return (kA || m % 8 == 0) && (kB || n % 8 == 0); }
+// Whether an operand's 16-byte units can be loaded straight into LDS: rows on 16 bytes, and, where
+// it is not k-major, no unit across its last row.
+bool is_aligned(const void* p, int64_t ld, bool k_major, int64_t rows, int dtype) {
+    const int64_t unit = dtype == HBT_DTYPE_F32 ? 4 : 8;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % unit == 0 && (k_major || rows % unit == 0);
+}
 
-template <int D, bool kA, bool kB, class T, bool kEdge>
+template <int D, bool kA, bool kB, class T, bool kAsync>
 int32_t launch_tile(const char* who, ProductArgs& p, int splits, hipStream_t stream) {
-    constexpr int kLds = lds_bytes<D, T>();
+    constexpr int kLds = lds_bytes<T, kAsync>();
     p.tiles_m = static_cast<int>((p.m + T::BM - 1) / T::BM);
     p.tiles_n = static_cast<int>((p.n + T::BN - 1) / T::BN);
-    const auto kernel = product_kernel<D, kA, kB, T, kEdge>;
+    const auto kernel = product_kernel<D, kA, kB, T, kAsync>;
     if constexpr (kLds > 65536) {
         static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
@@ -296,8 +299,8 @@ int32_t launch_tile(const char* who, ProductArgs& p, int splits, hipStream_t str
 template <int D, bool kA, bool kB>
 int32_t launch_product(const char* who, ProductArgs& p, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
     constexpr int BK = tile_k<D>();
-    constexpr bool kEdge = !kA || !kB;
-    Choice c = choose(p.m, p.n, p.k, D, whole_units<kA, kB>(p.m, p.n));
+    const bool aligned = is_aligned(p.a, p.lda, kA, p.m, D) && is_aligned(p.b, p.ldb, kB, p.n, D);
+    Choice c = choose(p.m, p.n, p.k, D, aligned);
     p.ldp = (p.n + 3) / 4 * 4;
     while (c.splits > 1 && 4 * c.splits * p.m * p.ldp > workspace_bytes) --c.splits;
     p.k_split = p.k;
@@ -308,9 +311,15 @@ int32_t launch_product(const char* who, ProductArgs& p, void* workspace, int64_t
         if (c.splits > 1) p.partial = static_cast<float*>(workspace);
     }
     int32_t status = HBT_OK;
-    if (c.tile == 64) status = launch_tile<D, kA, kB, Tile64, kEdge>(who, p, c.splits, stream);
-    else if (c.tile == 128) status = launch_tile<D, kA, kB, Tile128, kEdge>(who, p, c.splits, stream);
-    else if constexpr (D != HBT_DTYPE_F32) status = launch_tile<D, kA, kB, Tile256, false>(who, p, c.splits, stream);
+    if (c.tile == 64) {
+        status = aligned ? launch_tile<D, kA, kB, Tile64, true>(who, p, c.splits, stream)
+                         : launch_tile<D, kA, kB, Tile64, false>(who, p, c.splits, stream);
+    } else if (c.tile == 128) {
+        status = aligned ? launch_tile<D, kA, kB, Tile128, true>(who, p, c.splits, stream)
+                         : launch_tile<D, kA, kB, Tile128, false>(who, p, c.splits, stream);
+    } else if constexpr (D != HBT_DTYPE_F32) {
+        status = launch_tile<D, kA, kB, Tile256, true>(who, p, c.splits, stream);
+    }
     if (status != HBT_OK || c.splits == 1) return status;
     const int64_t blocks = std::min<int64_t>((p.m * (p.ldp / 4) + 255) / 256, 4096);
     join_kernel<D><<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(p, c.splits);
@@ -360,11 +369,11 @@ int32_t check_sizes(const char* who, int64_t m, int64_t n, int64_t k, int32_t dt
     return HBT_OK;
 }
 
-template <bool kA, bool kB>
+// What the split of a product's sum can use, aligned or not.
 int64_t split_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype) {
     if (m <= 0 || n <= 0 || k <= 0) return 0;
-    const Choice c = choose(m, n, k, dtype, whole_units<kA, kB>(m, n));
-    return c.splits == 1 ? 0 : 4 * c.splits * m * ((n + 3) / 4 * 4);
+    const int splits = std::max(choose(m, n, k, dtype, true).splits, choose(m, n, k, dtype, false).splits);
+    return splits == 1 ? 0 : 4 * splits * m * ((n + 3) / 4 * 4);
 }
 
 // Rows per block of the slope pass: enough blocks for the device, few enough partial sums.
@@ -397,9 +406,9 @@ BackwardSpace backward_space(int64_t tokens, int64_t inner, int64_t outer, int32
         b.shared_bytes = 4 * ((tokens + rows - 1) / rows) * ((outer + 3) / 4 * 4);
     }
     if (wants & HBT_LINEAR_DX)
-        b.shared_bytes = std::max(b.shared_bytes, split_bytes<true, false>(tokens, inner, outer, dtype));
+        b.shared_bytes = std::max(b.shared_bytes, split_bytes(tokens, inner, outer, dtype));
     if (wants & HBT_LINEAR_DW)
-        b.shared_bytes = std::max(b.shared_bytes, split_bytes<false, false>(outer, inner, tokens, dtype));
+        b.shared_bytes = std::max(b.shared_bytes, split_bytes(outer, inner, tokens, dtype));
     return b;
 }
 
@@ -422,7 +431,7 @@ extern "C" {
 int64_t hbt_linear_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype) {
     if (tokens < 0 || inner < 0 || outer < 0) return -1;
     if (dtype != HBT_DTYPE_F32 && dtype != HBT_DTYPE_BF16 && dtype != HBT_DTYPE_F16) return -1;
-    return tokens <= 16 ? 0 : split_bytes<true, true>(tokens, outer, inner, dtype);
+    return tokens <= 16 ? 0 : split_bytes(tokens, outer, inner, dtype);
 }
 
 int64_t hbt_linear_backward_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t activation,

@@ -7,10 +7,11 @@
 // dW = dz^T x), so the three products of a layer and its backward pass, and the Gram and
 // iterate products of a Newton-Schulz step, read every matrix where it lies.
 //
-// Global memory goes through registers into one of two LDS buffers, in 16-byte units: the
-// next tile but one is in flight while the current one feeds the matrix cores, with one
-// barrier per k-tile.  A unit out of range is read at an offset past the buffer's end,
-// which returns zeros; a unit that straddles an edge is read element by element.
+// Operands whose rows start on 16 bytes go straight from global memory into one of the tile's
+// LDS stages (buffer loads with an LDS destination), several k-tiles ahead of the matrix cores,
+// with one barrier per k-tile.  Others go through registers into two stages: unaligned 16-byte
+// units are loaded as they lie, and a unit that straddles an edge element by element.  A unit
+// out of range is read at an offset past the buffer's end, which returns zeros.
 #pragma once
 
 #include <algorithm>
@@ -111,8 +112,9 @@ constexpr uint32_t kNowhere = 0xFFFFFF00u;
 
 // One operand's share of a tile: ROWS rows (m or n) by tile_k of k, moved by THREADS lanes.
 // kKMajor: element (row, k) at base[row * ld + k]; else at base[k * ld + row].
-// kEdge: units may cross the last row of an operand that is not k-major.
-template <int D, bool kKMajor, int ROWS, int THREADS, bool kEdge>
+// kAsync: rows and base on 16 bytes, and whole units (the rows of an operand that is not
+// k-major a multiple of a unit, or padded to one).
+template <int D, bool kKMajor, int ROWS, int THREADS, bool kAsync>
 struct Operand {
     static constexpr int E = unit_elems<D>(), BK = tile_k<D>(), B = elem_bytes<D>();
     static constexpr int kUnitsPerLine = kKMajor ? BK / E : ROWS / E;  // units per LDS line
@@ -126,7 +128,7 @@ struct Operand {
     int rows;              // rows of the operand from the tile's first one
     uint32_t offset[kUnits];
     u32x4 held[kUnits];
-    bool straddles;        // some lane's unit crosses the last row (kEdge, not k-major)
+    bool straddles;        // some lane's unit crosses the last row (not k-major)
 
     // LDS position of a unit: lines are XOR-swizzled in units so that the 16 rows of a
     // fragment read (k-major), or the four k of a transposing read, fall on distinct banks.
@@ -136,14 +138,21 @@ struct Operand {
         else return ((line >> 2) & 3) << 2;
     }
 
+    // The unit of its line that unit u of the lane order is.  An asynchronous load writes lane l's
+    // 16 bytes l units after its wave's LDS address, so there the swizzle picks what a lane loads.
+    static __device__ __forceinline__ int column(int u) {
+        const int line = u / kUnitsPerLine, at = u % kUnitsPerLine;
+        return kAsync ? at ^ swizzle(line) : at;
+    }
+
     __device__ __forceinline__ void init(const void* p, int64_t ld_, int64_t row0, int64_t row_count, int tid) {
         ld = ld_;
         rows = static_cast<int>(row_count - row0 < ROWS ? row_count - row0 : ROWS);
         base = static_cast<const char*>(p) + (kKMajor ? row0 * ld_ : row0) * B;
-        straddles = kEdge && !kKMajor && rows < ROWS && rows % E != 0;
+        straddles = !kAsync && !kKMajor && rows < ROWS && rows % E != 0;
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
+            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = column(u);
             const bool in = kKMajor ? line < rows : (at + 1) * E <= rows;
             offset[i] = in ? static_cast<uint32_t>(line * ld * B) + at * 16 : kNowhere;
         }
@@ -156,8 +165,24 @@ struct Operand {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i)
             held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset[i], 0, 0));
-        if constexpr (kEdge && !kKMajor) {
+        if constexpr (!kAsync && !kKMajor) {
             if (straddles) load_edge(at_k, BK, tid);
+        }
+    }
+
+    // The whole k-tile at k0 into the LDS stage at byte address `lds`, without waiting: kUnits
+    // loads a wave.  They are written as assembly because the compiler makes every LDS read wait
+    // for all such loads; they have no register results, and wait_loads() below waits for them.
+    __device__ __forceinline__ void load_async(int64_t k0, uint32_t lds, int wave) const {
+        const uint64_t at_k = reinterpret_cast<uint64_t>(base + (kKMajor ? k0 : k0 * ld) * B);
+        const u32x4 buffer = {static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at_k))),
+                              static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at_k >> 32))),
+                              0x7FFFFFFFu, 0x00020000u};
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (i * THREADS + wave * 64) * 16);
+            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :: "s"(to), "v"(offset[i]), "s"(buffer) : "memory");  // nothing else here uses m0
         }
     }
 
@@ -167,7 +192,7 @@ struct Operand {
         const auto buffer = buffer_at(at_k);
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
+            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = column(u);
             const bool in = kKMajor ? (at + 1) * E <= left : line < left;
             held[i] = __builtin_bit_cast(
                 u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, in ? offset[i] : kNowhere, 0, 0));
@@ -179,7 +204,7 @@ struct Operand {
     __device__ __forceinline__ void load_edge(const char* at_k, int left, int tid) {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
+            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = column(u);
             const int have = (kKMajor ? left : rows) - at * E;  // elements of the unit that exist
             const bool line_in = kKMajor ? line < rows : line < left;
             if (line_in && have > 0 && have < E) {
@@ -201,8 +226,8 @@ struct Operand {
     __device__ __forceinline__ void store(char* lds, int tid) const {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = u % kUnitsPerLine;
-            *reinterpret_cast<u32x4*>(lds + line * kLineBytes + ((at ^ swizzle(line)) << 4)) = held[i];
+            const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = column(u) ^ swizzle(line);
+            *reinterpret_cast<u32x4*>(lds + line * kLineBytes + (at << 4)) = held[i];
         }
     }
 
@@ -235,27 +260,47 @@ struct Operand {
     }
 };
 
-// A workgroup's tile: BM x BN by WM x WN waves.
-template <int BM_, int BN_, int WM_, int WN_>
+// Waits until at most N of the wave's global loads are in flight, and for its LDS reads.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
+}
+
+// A workgroup's tile: BM x BN by WM x WN waves, with kStages_ LDS stages for asynchronous loads.
+template <int BM_, int BN_, int WM_, int WN_, int kStages_>
 struct Tile {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kThreads = 64 * WM * WN;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kThreads = 64 * WM * WN, kStages = kStages_;
     static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;  // 16 x 16 results per wave
+    static constexpr int kStageBytes = (BM + BN) * 128;
 };
 
-template <int D, class T>
-constexpr int lds_bytes() { return 2 * (T::BM + T::BN) * 128; }
+template <class T, bool kAsync>
+constexpr int lds_bytes() { return (kAsync ? T::kStages : 2) * T::kStageBytes; }
+
+template <int D, class T, class OpA, class OpB>
+__device__ __forceinline__ void multiply(const char* now, int step, int wm, int wn, int lane,
+                                         f32x4 (&acc)[T::TM][T::TN]) {
+    u32x4 fa[T::TM], fb[T::TN];
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j) fb[j] = OpB::fragment(now + OpA::kBytes, wn + 16 * j, step, lane);
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) fa[i] = OpA::fragment(now, wm + 16 * i, step, lane);
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j) acc[i][j] = mma<D>(fb[j], fa[i], acc[i][j]);
+}
 
 // Forms the tile at rows m0 of A and n0 of B over k in [k0, k1) into acc: acc[i][j] holds, in
 // lane l, element m = 16 i + l % 16, n = 16 j + 4 (l / 16) + r (r = 0..3) of the wave's part.
-// A partial k-tile comes first, so that the loop moves whole ones only.
-template <int D, bool kA, bool kB, class T, bool kEdge>
+// A partial k-tile comes first and goes through registers, so that the loop moves whole ones.
+template <int D, bool kA, bool kB, class T, bool kAsync>
 __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t m0, int64_t m_count, const void* b,
                                              int64_t ldb, int64_t n0, int64_t n_count, int64_t k0, int64_t k1,
                                              char* lds, f32x4 (&acc)[T::TM][T::TN]) {
-    constexpr int BK = tile_k<D>(), kThreads = T::kThreads, kSteps = 2;
-    using OpA = Operand<D, kA, T::BM, kThreads, kEdge>;
-    using OpB = Operand<D, kB, T::BN, kThreads, kEdge>;
-    constexpr int kBuffer = OpA::kBytes + OpB::kBytes;
+    constexpr int BK = tile_k<D>(), kThreads = T::kThreads;
+    using OpA = Operand<D, kA, T::BM, kThreads, kAsync>;
+    using OpB = Operand<D, kB, T::BN, kThreads, kAsync>;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = (wave / T::WN) * (T::BM / T::WM), wn = (wave % T::WN) * (T::BN / T::WN);
 #pragma unroll
@@ -269,37 +314,66 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
     ob.init(b, ldb, n0, n_count, tid);
     const int tiles = static_cast<int>((k1 - k0 + BK - 1) / BK);
     const int part = static_cast<int>((k1 - k0) % BK);
-    if (part != 0) {
-        oa.load_part(k0, part, tid);
-        ob.load_part(k0, part, tid);
+    int64_t k = k0;  // the next k-tile to load
+    if constexpr (kAsync) {
+        constexpr int kLoads = OpA::kUnits + OpB::kUnits, kAhead = T::kStages - 1;
+        const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+            (__attribute__((address_space(3))) char*)lds));
+        const auto issue = [&](int stage) {
+            oa.load_async(k, at + stage * T::kStageBytes, wave);
+            ob.load_async(k, at + stage * T::kStageBytes + OpA::kBytes, wave);
+            k += BK;
+        };
+        if (part != 0) {
+            oa.load_part(k, part, tid);
+            ob.load_part(k, part, tid);
+            oa.store(lds, tid);
+            ob.store(lds + OpA::kBytes, tid);
+            k += part;
+        } else {
+            issue(0);
+        }
+#pragma unroll
+        for (int s = 1; s < kAhead; ++s)
+            if (s < tiles) issue(s);
+        int stage = 0;
+        for (int t = 0; t < tiles; ++t) {
+            // Tile t has landed once at most the kAhead - 1 later ones are in flight; past the
+            // barrier it has for every wave, and every wave has read tile t - 1, whose stage the
+            // next load takes.
+            if (t + kAhead <= tiles) wait_loads<kLoads * (kAhead - 1)>();
+            else wait_loads<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const int free = stage == 0 ? T::kStages - 1 : stage - 1;
+            if (t + kAhead < tiles) issue(free);
+            const char* now = lds + stage * T::kStageBytes;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) multiply<D, T, OpA, OpB>(now, s, wm, wn, lane, acc);
+            stage = stage + 1 == T::kStages ? 0 : stage + 1;
+        }
     } else {
-        oa.load(k0, tid);
-        ob.load(k0, tid);
-    }
-    oa.store(lds, tid);
-    ob.store(lds + OpA::kBytes, tid);
-    int64_t k = k0 + (part != 0 ? part : BK);  // the next k-tile to load
-    if (tiles > 1) {
-        oa.load(k, tid);
-        ob.load(k, tid);
-    }
-    __syncthreads();
-    for (int t = 0; t < tiles; ++t) {
-        const char* now = lds + (t & 1) * kBuffer;
-        char* next = lds + ((t & 1) ^ 1) * kBuffer;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            u32x4 fa[T::TM], fb[T::TN];
-#pragma unroll
-            for (int j = 0; j < T::TN; ++j) fb[j] = OpB::fragment(now + OpA::kBytes, wn + 16 * j, s, lane);
-#pragma unroll
-            for (int i = 0; i < T::TM; ++i) fa[i] = OpA::fragment(now, wm + 16 * i, s, lane);
-#pragma unroll
-            for (int i = 0; i < T::TM; ++i)
-#pragma unroll
-                for (int j = 0; j < T::TN; ++j) acc[i][j] = mma<D>(fb[j], fa[i], acc[i][j]);
-            if (s == 0 && t + 1 < tiles) {
-                // Every wave has passed the barrier that ended the reads of this buffer.
+        if (part != 0) {
+            oa.load_part(k, part, tid);
+            ob.load_part(k, part, tid);
+        } else {
+            oa.load(k, tid);
+            ob.load(k, tid);
+        }
+        k += part != 0 ? part : BK;
+        oa.store(lds, tid);
+        ob.store(lds + OpA::kBytes, tid);
+        if (tiles > 1) {
+            oa.load(k, tid);
+            ob.load(k, tid);
+        }
+        __syncthreads();
+        for (int t = 0; t < tiles; ++t) {
+            const char* now = lds + (t & 1) * T::kStageBytes;
+            char* next = lds + ((t & 1) ^ 1) * T::kStageBytes;
+            multiply<D, T, OpA, OpB>(now, 0, wm, wn, lane, acc);
+            if (t + 1 < tiles) {
+                // Every wave has passed the barrier that ended the reads of this stage.
                 oa.store(next, tid);
                 ob.store(next + OpA::kBytes, tid);
                 if (t + 2 < tiles) {
@@ -308,9 +382,11 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
                     ob.load(k, tid);
                 }
             }
+            multiply<D, T, OpA, OpB>(now, 1, wm, wn, lane, acc);
+            if (t + 1 < tiles) __syncthreads();
         }
-        __syncthreads();
     }
+    __syncthreads();  // the LDS is free
 }
 
 // Hands the tile's results to `store(m, n, v)`, four consecutive n at a time, each in one lane,
@@ -321,12 +397,12 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
 // tile, four consecutive m at a time: a wave takes sixteen n by four units of m, so its LDS
 // reads fall on distinct banks and its stores cover 32 bytes of a row.
 struct NoMirror {};
-template <int D, class T, class Store, class Mirror = NoMirror>
+template <class T, bool kAsync, class Store, class Mirror = NoMirror>
 __device__ __forceinline__ void finish_tile(char* lds, const f32x4 (&acc)[T::TM][T::TN], Store&& store,
                                             bool mirrored = false, Mirror&& mirror = Mirror{}) {
-    constexpr int kRowUnits = T::BN / 4, kPhases = T::BM * T::BN * 4 > lds_bytes<D, T>() ? T::WM : 1;
+    constexpr int kRowUnits = T::BN / 4, kPhases = T::BM * T::BN * 4 > lds_bytes<T, kAsync>() ? T::WM : 1;
     constexpr int kRows = T::BM / kPhases;
-    static_assert(kRows * T::BN * 4 <= lds_bytes<D, T>(), "a phase fits the tile's LDS");
+    static_assert(kRows * T::BN * 4 <= lds_bytes<T, kAsync>(), "a phase fits the tile's LDS");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = (wave / T::WN) * (T::BM / T::WM), wn = (wave % T::WN) * (T::BN / T::WN);
     f32x4* out = reinterpret_cast<f32x4*>(lds);

@@ -228,18 +228,18 @@ __global__ __launch_bounds__(T::kThreads) void newton_schulz_kernel(ProductArgs 
     if constexpr (kPhase == kGram) {
         // Columns past the last one are padding of x's rows: read, never stored.
         const int count = kWide ? side : t.ldx, k = kWide ? t.cols : t.rows;
-        tile_product<D, kWide, kWide, T, false>(t.x, t.ldx, m0, count, t.x, t.ldx, n0, count, 0, k, lds, acc);
+        tile_product<D, kWide, kWide, T, true>(t.x, t.ldx, m0, count, t.x, t.ldx, n0, count, 0, k, lds, acc);
     } else if constexpr (kPhase == kSquare) {
-        tile_product<D, true, true, T, false>(t.gram, ldg, m0, side, t.gram, ldg, n0, side, 0, side, lds, acc);
+        tile_product<D, true, true, T, true>(t.gram, ldg, m0, side, t.gram, ldg, n0, side, 0, side, lds, acc);
     } else if constexpr (kWide) {
-        tile_product<D, true, false, T, false>(t.poly, ldg, m0, side, t.x, t.ldx, n0, t.ldx, 0, side, lds, acc);
+        tile_product<D, true, false, T, true>(t.poly, ldg, m0, side, t.x, t.ldx, n0, t.ldx, 0, side, lds, acc);
     } else {
-        tile_product<D, true, true, T, false>(t.x, t.ldx, m0, t.rows, t.poly, ldg, n0, side, 0, side, lds, acc);
+        tile_product<D, true, true, T, true>(t.x, t.ldx, m0, t.rows, t.poly, ldg, n0, side, 0, side, lds, acc);
     }
     if constexpr (kPhase == kIterate) {
         const float factor = p.first && t.state != nullptr ? *t.factor : 1.0f;
         const float decay = p.slot != nullptr ? p.slot[0] : p.decay, lr = p.slot != nullptr ? p.slot[1] : p.lr;
-        finish_tile<D, T>(lds, acc, [&](int i, int j, f32x4 v) {
+        finish_tile<T, true>(lds, acc, [&](int i, int j, f32x4 v) {
             const int m = m0 + i, n = n0 + j, have = t.cols - n;
             if (m >= t.rows || have <= 0) return;
             const int64_t dense = int64_t(m) * t.cols + n, padded = int64_t(m) * t.ldx + n;
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(T::kThreads) void newton_schulz_kernel(ProductArgs 
             if (m < side && n < side) store4<D>(out, int64_t(m) * ldg + n, value(m, n, v));
         };
         // Off the diagonal the mirror image is stored too: the products are bitwise symmetric.
-        finish_tile<D, T>(lds, acc, store, tm != tn, [&](int j, int i, f32x4 v) {
+        finish_tile<T, true>(lds, acc, store, tm != tn, [&](int j, int i, f32x4 v) {
             const int n = n0 + j, m = m0 + i;
             if (n < side && m < side) store4<D>(out, int64_t(n) * ldg + m, value(n, m, v));
         });
@@ -398,9 +398,9 @@ __global__ __launch_bounds__(512) void small_kernel(SmallArgs p) {
 }
 
 // ---- host ----------------------------------------------------------------------------
-using Tile256 = Tile<256, 256, 2, 4>;
-using Tile128 = Tile<128, 128, 2, 2>;
-using Tile64 = Tile<64, 64, 2, 2>;
+using Tile256 = Tile<256, 256, 2, 4, 2>;
+using Tile128 = Tile<128, 128, 2, 2, 2>;
+using Tile64 = Tile<64, 64, 2, 2, 4>;
 
 struct Plan {
     int64_t state, x0, x1, gram, poly, partial, factor, end;  // offsets of one matrix's storage
@@ -466,7 +466,7 @@ int64_t tiles_of(const Problem& t, int size, Phase phase) {
 
 template <int D, class T, Phase kPhase, bool kWide>
 int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t stream) {
-    constexpr int kLds = lds_bytes<D, T>();
+    constexpr int kLds = lds_bytes<T, true>();
     int64_t blocks = 0;
     for (int i = 0; i < p.count; ++i) {
         p.problem[i].first_block = static_cast<int>(blocks);
