@@ -92,7 +92,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_
 }
 
 template <int D, bool kA, bool kB, class T, bool kAsync>
-__global__ __launch_bounds__(T::kThreads) void product_kernel(ProductArgs p) {
+__global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs p) {
     extern __shared__ __align__(16) char lds[];
     const int t = xcd_tile(blockIdx.x, gridDim.x);
     int tm, tn;

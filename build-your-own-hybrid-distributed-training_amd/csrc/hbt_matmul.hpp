@@ -121,6 +121,7 @@ struct Operand {
     static constexpr int kLineBytes = kUnitsPerLine * 16;
     static constexpr int kUnits = ROWS * BK / E / THREADS;  // units per lane
     static constexpr int kBytes = ROWS * BK * B;
+    static constexpr int kReads = kKMajor ? 1 : B;  // LDS reads per fragment: two transposing, or four
     static_assert(ROWS * BK / E % THREADS == 0, "whole units per lane");
 
     const char* base;      // the tile's first row (k-major) or column at k = 0
@@ -277,18 +278,27 @@ struct Tile {
 template <class T, bool kAsync>
 constexpr int lds_bytes() { return (kAsync ? T::kStages : 2) * T::kStageBytes; }
 
-template <int D, class T, class OpA, class OpB>
-__device__ __forceinline__ void multiply(const char* now, int step, int wm, int wn, int lane,
-                                         f32x4 (&acc)[T::TM][T::TN]) {
-    u32x4 fa[T::TM], fb[T::TN];
+// N fragments of consecutive sixteens of rows.
+template <class Op, int N>
+__device__ __forceinline__ void read(u32x4 (&f)[N], const char* lds, int row, int step, int lane) {
 #pragma unroll
-    for (int j = 0; j < T::TN; ++j) fb[j] = OpB::fragment(now + OpA::kBytes, wn + 16 * j, step, lane);
+    for (int i = 0; i < N; ++i) f[i] = Op::fragment(lds, row + 16 * i, step, lane);
+}
+template <int D, class T, int kFirst, int N>
+__device__ __forceinline__ void multiply(const u32x4 (&a)[N], const u32x4 (&b)[T::TN], f32x4 (&acc)[T::TM][T::TN]) {
 #pragma unroll
-    for (int i = 0; i < T::TM; ++i) fa[i] = OpA::fragment(now, wm + 16 * i, step, lane);
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int i = 0; i < T::TM; ++i)
+        for (int j = 0; j < T::TN; ++j) acc[kFirst + i][j] = mma<D>(b[j], a[i], acc[kFirst + i][j]);
+}
+// Asks the scheduler to spread LDS reads among matrix instructions.
+template <int kReads, int kMmas>
+__device__ __forceinline__ void interleave() {
 #pragma unroll
-        for (int j = 0; j < T::TN; ++j) acc[i][j] = mma<D>(fb[j], fa[i], acc[i][j]);
+    for (int i = 0; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
+        __builtin_amdgcn_sched_group_barrier(0x008, kMmas / kReads > 0 ? kMmas / kReads : 1, 0);
+    }
 }
 
 // Forms the tile at rows m0 of A and n0 of B over k in [k0, k1) into acc: acc[i][j] holds, in
@@ -298,7 +308,7 @@ template <int D, bool kA, bool kB, class T, bool kAsync>
 __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t m0, int64_t m_count, const void* b,
                                              int64_t ldb, int64_t n0, int64_t n_count, int64_t k0, int64_t k1,
                                              char* lds, f32x4 (&acc)[T::TM][T::TN]) {
-    constexpr int BK = tile_k<D>(), kThreads = T::kThreads;
+    constexpr int BK = tile_k<D>(), B = elem_bytes<D>(), kThreads = T::kThreads;
     using OpA = Operand<D, kA, T::BM, kThreads, kAsync>;
     using OpB = Operand<D, kB, T::BN, kThreads, kAsync>;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -334,23 +344,51 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
             issue(0);
         }
 #pragma unroll
-        for (int s = 1; s < kAhead; ++s)
+        for (int s = 1; s <= kAhead; ++s)
             if (s < tiles) issue(s);
-        int stage = 0;
-        for (int t = 0; t < tiles; ++t) {
-            // Tile t has landed once at most the kAhead - 1 later ones are in flight; past the
-            // barrier it has for every wave, and every wave has read tile t - 1, whose stage the
-            // next load takes.
+        const auto landed = [&](int t) {  // tile t is in LDS for every wave
             if (t + kAhead <= tiles) wait_loads<kLoads * (kAhead - 1)>();
             else wait_loads<0>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            const int free = stage == 0 ? T::kStages - 1 : stage - 1;
-            if (t + kAhead < tiles) issue(free);
+        };
+        if (kAhead < tiles) wait_loads<kLoads * kAhead>();
+        else wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        // Each k-tile is two steps of two halves of the wave's rows.  While one half's matrix
+        // instructions run, the fragments of the next are read: two sets of each operand's are held.
+        constexpr int kHalf = T::TM / 2, kReadsA = OpA::kReads * kHalf, kReadsB = OpB::kReads * T::TN;
+        constexpr int kMmas = kHalf * T::TN * (B == 4 ? 4 : 1);
+        u32x4 a0[kHalf], a1[kHalf], b0[T::TN], b1[T::TN];
+        read<OpB>(b0, lds + OpA::kBytes, wn, 0, lane);
+        read<OpA>(a0, lds, wm, 0, lane);
+        int stage = 0;
+        for (int t = 0; t < tiles; ++t) {
             const char* now = lds + stage * T::kStageBytes;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) multiply<D, T, OpA, OpB>(now, s, wm, wn, lane, acc);
-            stage = stage + 1 == T::kStages ? 0 : stage + 1;
+            read<OpA>(a1, now, wm + 16 * kHalf, 0, lane);
+            multiply<D, T, 0>(a0, b0, acc);
+            interleave<kReadsA, kMmas>();
+            read<OpB>(b1, now + OpA::kBytes, wn, 1, lane);
+            read<OpA>(a0, now, wm, 1, lane);
+            multiply<D, T, kHalf>(a1, b0, acc);
+            interleave<kReadsA + kReadsB, kMmas>();
+            read<OpA>(a1, now, wm + 16 * kHalf, 1, lane);
+            multiply<D, T, 0>(a0, b1, acc);
+            interleave<kReadsA, kMmas>();
+            if (t + 1 < tiles) {
+                // At most the kAhead - 1 tiles after t + 1 are in flight, so it has landed; past the
+                // barrier it has for every wave, and every wave holds the last of tile t, whose
+                // stage the next load takes.
+                landed(t + 1);
+                if (t + 1 + kAhead < tiles) issue(stage);
+                stage = stage + 1 == T::kStages ? 0 : stage + 1;
+                const char* next = lds + stage * T::kStageBytes;
+                read<OpB>(b0, next + OpA::kBytes, wn, 0, lane);
+                read<OpA>(a0, next, wm, 0, lane);
+            }
+            multiply<D, T, kHalf>(a1, b1, acc);
+            interleave<kReadsA + kReadsB, kMmas>();
         }
     } else {
         if (part != 0) {
@@ -371,7 +409,10 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
         for (int t = 0; t < tiles; ++t) {
             const char* now = lds + (t & 1) * T::kStageBytes;
             char* next = lds + ((t & 1) ^ 1) * T::kStageBytes;
-            multiply<D, T, OpA, OpB>(now, 0, wm, wn, lane, acc);
+            u32x4 fa[T::TM], fb[T::TN];
+            read<OpB>(fb, now + OpA::kBytes, wn, 0, lane);
+            read<OpA>(fa, now, wm, 0, lane);
+            multiply<D, T, 0>(fa, fb, acc);
             if (t + 1 < tiles) {
                 // Every wave has passed the barrier that ended the reads of this stage.
                 oa.store(next, tid);
@@ -382,7 +423,9 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
                     ob.load(k, tid);
                 }
             }
-            multiply<D, T, OpA, OpB>(now, 1, wm, wn, lane, acc);
+            read<OpB>(fb, now + OpA::kBytes, wn, 1, lane);
+            read<OpA>(fa, now, wm, 1, lane);
+            multiply<D, T, 0>(fa, fb, acc);
             if (t + 1 < tiles) __syncthreads();
         }
     }

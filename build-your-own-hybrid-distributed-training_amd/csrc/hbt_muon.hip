@@ -23,35 +23,44 @@ constexpr int kMaxMatrices = HBT_MAX_TENSORS_PER_LAUNCH;
 constexpr int kChunk = 4096;  // elements per norm partial
 constexpr int kMaxSteps = 64;
 
+// The first workgroup of every matrix of a launch, the unused ones past every workgroup.
+struct FirstBlocks {
+    int first[kMaxMatrices];
+    void clear() {
+        for (int& f : first) f = 0x7FFFFFFF;
+    }
+};
+// The matrix of a workgroup: one wide scalar load and a sum of comparisons.
+__device__ __forceinline__ int find_entry(const FirstBlocks& blocks, int block) {
+    int e = -1;
+#pragma unroll
+    for (int i = 0; i < kMaxMatrices; ++i) e += blocks.first[i] <= block ? 1 : 0;
+    return e;
+}
+
 // ---- the direction and its norm --------------------------------------------------------
 struct DirectionEntry {
     const void* g;
     float* v;        // null: u is the input itself
     float* u;        // fp32, dense
     double* partial;
-    int64_t numel, first_block;
+    int64_t numel;
 };
 struct DirectionArgs {
+    FirstBlocks blocks;
     DirectionEntry entry[kMaxMatrices];
     const float* grad_mul;
     const float* slot;  // null, or the momentum and its complement are its third and fourth float
     float unscale, momentum, rest;
-    int count, nesterov;
+    int nesterov;
 };
-
-template <int N, class Entry>
-__device__ __forceinline__ int find_entry(const Entry (&entry)[N], int count, int64_t block) {
-    int e = 0;
-    while (e + 1 < count && entry[e + 1].first_block <= block) ++e;
-    return e;
-}
 
 // One pass over the gradients: the momentum, the direction, and its squares summed in fp64.
 template <int GD>
 __global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
-    const int64_t block = blockIdx.x;
-    const DirectionEntry& t = p.entry[find_entry(p.entry, p.count, block)];
-    const int64_t chunk = block - t.first_block, base = chunk * kChunk;
+    const int block = blockIdx.x, e = find_entry(p.blocks, block);
+    const DirectionEntry& t = p.entry[e];
+    const int64_t chunk = block - p.blocks.first[e], base = chunk * kChunk;
     const float mul = p.grad_mul != nullptr ? *p.grad_mul : 1.0f;
     const float mu = p.slot != nullptr ? p.slot[2] : p.momentum, rest = p.slot != nullptr ? p.slot[3] : p.rest;
     double sum = 0.0;
@@ -125,19 +134,19 @@ struct StartEntry {
     const float* u;
     void* x;
     const float* factor;
-    int64_t rows, cols, ld, first_block;
+    int64_t rows, cols, ld;
 };
 struct StartArgs {
+    FirstBlocks blocks;
     StartEntry entry[kMaxMatrices];
-    int count;
 };
 
 // The first iterate in the product type, rows on 16-byte boundaries: eight columns a lane.
 template <int D>
 __global__ __launch_bounds__(256) void start_kernel(StartArgs p) {
-    const int64_t block = blockIdx.x;
-    const StartEntry& t = p.entry[find_entry(p.entry, p.count, block)];
-    const int64_t units = t.ld / 8, i = (block - t.first_block) * 256 + threadIdx.x;
+    const int block = blockIdx.x, e = find_entry(p.blocks, block);
+    const StartEntry& t = p.entry[e];
+    const int64_t units = t.ld / 8, i = int64_t(block - p.blocks.first[e]) * 256 + threadIdx.x;
     if (i >= t.rows * units) return;
     const int64_t row = i / units, col = i % units * 8;
     const float f = *t.factor;
@@ -167,11 +176,12 @@ struct Problem {
     float* state;         // the fp32 iterate [rows][cols] (fp16 products), or null
     const float* factor;  // first step: the state is still u, to be multiplied by this
     void* out;            // last step: the parameter or the result, [rows][cols]
-    int rows, cols, ldx, first_block;
+    int rows, cols, ldx;
     float gram_scale;     // 1 / scale^2
     float out_scale;      // the step's multiple of x, over scale
 };
 struct ProductArgs {
+    FirstBlocks blocks;
     Problem problem[kMaxMatrices];
     const float* slot;    // null, or decay and learning rate are its first two floats
     float a, b, c, decay, lr;
@@ -208,11 +218,12 @@ __device__ __forceinline__ void finish(const ProductArgs& p, const Problem& t, f
 
 // kWide: rows <= columns, so A = x x^T and x' = a x + B x; else A = x^T x and x' = a x + x B.
 template <int D, class T, Phase kPhase, bool kWide>
-__global__ __launch_bounds__(T::kThreads) void newton_schulz_kernel(ProductArgs p) {
+__global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductArgs p) {
     extern __shared__ __align__(16) char lds[];
     const int block = xcd_tile(blockIdx.x, gridDim.x);
-    const Problem& t = p.problem[find_entry(p.problem, p.count, block)];
-    const int tile = block - t.first_block, side = kWide ? t.rows : t.cols;
+    const int e = find_entry(p.blocks, block);
+    const Problem& t = p.problem[e];
+    const int tile = block - p.blocks.first[e], side = kWide ? t.rows : t.cols;
     const int ldg = (side + 7) / 8 * 8;
     int tm, tn;
     if constexpr (kPhase == kIterate) {
@@ -468,8 +479,9 @@ template <int D, class T, Phase kPhase, bool kWide>
 int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t stream) {
     constexpr int kLds = lds_bytes<T, true>();
     int64_t blocks = 0;
+    p.blocks.clear();
     for (int i = 0; i < p.count; ++i) {
-        p.problem[i].first_block = static_cast<int>(blocks);
+        p.blocks.first[i] = static_cast<int>(blocks);
         blocks += tiles_of(p.problem[i], size, kPhase);
     }
     const auto kernel = newton_schulz_kernel<D, T, kPhase, kWide>;
@@ -535,6 +547,8 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
     ProductArgs wide = common, tall = common;
     wide.count = tall.count = 0;
     norm.eps = eps;
+    direction.blocks.clear();
+    start.blocks.clear();
     int64_t at = 0, direction_blocks = 0, start_blocks = 0;
     int n = 0;
     for (int i = 0; i < t.count; ++i) {
@@ -548,21 +562,21 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
         float* state = reinterpret_cast<float*>(workspace + plan.state);
         float* factor = reinterpret_cast<float*>(workspace + plan.factor);
         double* partial = reinterpret_cast<double*>(workspace + plan.partial);
-        direction.entry[n] = {t.grads[i], t.momenta == nullptr ? nullptr : t.momenta[i], state, partial, rows * cols,
-                              direction_blocks};
+        direction.entry[n] = {t.grads[i], t.momenta == nullptr ? nullptr : t.momenta[i], state, partial, rows * cols};
+        direction.blocks.first[n] = static_cast<int>(direction_blocks);
         direction_blocks += plan.chunks;
         norm.entry[n] = {partial, factor, plan.chunks, scale};
-        start.entry[n] = {state, workspace + plan.x0, factor, rows, cols, plan.ldx, start_blocks};
+        start.entry[n] = {state, workspace + plan.x0, factor, rows, cols, plan.ldx};
+        start.blocks.first[n] = static_cast<int>(start_blocks);
         start_blocks += (rows * (plan.ldx / 8) + 255) / 256;
         ++n;
         ProductArgs& group = rows <= cols ? wide : tall;
         group.problem[group.count++] = {workspace + plan.x0, workspace + plan.x1, workspace + plan.gram,
                                         workspace + plan.poly, D == HBT_DTYPE_F32 ? nullptr : state, factor, t.outs[i],
-                                        static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(plan.ldx), 0,
+                                        static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(plan.ldx),
                                         1.0f / (scale * scale), (t.scales == nullptr ? 1.0f : t.scales[i]) / scale};
     }
     if (n == 0) return HBT_OK;
-    direction.count = start.count = n;
     const dim3 direction_grid(static_cast<unsigned>(direction_blocks));
     if (grad_dtype == HBT_DTYPE_F32) direction_kernel<HBT_DTYPE_F32><<<direction_grid, 256, 0, stream>>>(direction);
     else if (grad_dtype == HBT_DTYPE_BF16) direction_kernel<HBT_DTYPE_BF16><<<direction_grid, 256, 0, stream>>>(direction);
