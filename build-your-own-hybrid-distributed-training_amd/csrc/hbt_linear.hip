@@ -65,30 +65,25 @@ struct ProductArgs {
     int tiles_m, tiles_n, act;
 };
 
+// The residual of four results of row i from column j.
+template <int D>
+__device__ __forceinline__ f32x4 residual_of(const ProductArgs& p, int64_t i, int64_t j) {
+    if (p.residual == nullptr) return f32x4{0.f, 0.f, 0.f, 0.f};
+    return load_row<D>(p.residual, i * p.ldr + j, static_cast<int>(min<int64_t>(p.n - j, 4)));
+}
+
 // Four results of row i from column j: bias, activation, residual, each store rounded once.
 template <int D>
-__device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_t j, f32x4 v) {
-    if (j + 4 <= p.n) {
-        if (p.bias != nullptr) v += load4<D>(p.bias, j);
-        if (p.z != nullptr) store4<D>(p.z, i * p.ldz + j, v);
-        if (p.act != HBT_ACT_NONE) {
+__device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_t j, f32x4 v, f32x4 residual) {
+    const int have = static_cast<int>(min<int64_t>(p.n - j, 4));
+    if (p.bias != nullptr) v += load_row<D>(p.bias, j, have);
+    if (p.z != nullptr) store_row<D>(p.z, i * p.ldz + j, have, v);
+    if (p.act != HBT_ACT_NONE) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = activate<D>(v[e], p.act);
-        }
-        if (p.residual != nullptr) v += load4<D>(p.residual, i * p.ldr + j);
-        store4<D>(p.y, i * p.ldy + j, v);
-        return;
+        for (int e = 0; e < 4; ++e) v[e] = activate<D>(v[e], p.act);
     }
-#pragma unroll
-    for (int e = 0; e < 3; ++e) {
-        if (j + e >= p.n) break;
-        float x = v[e];
-        if (p.bias != nullptr) x += load_elem<D>(p.bias, j + e);
-        if (p.z != nullptr) store_elem<D>(p.z, i * p.ldz + j + e, x);
-        x = activate<D>(x, p.act);
-        if (p.residual != nullptr) x += load_elem<D>(p.residual, i * p.ldr + j + e);
-        store_elem<D>(p.y, i * p.ldy + j + e, x);
-    }
+    if (p.residual != nullptr) v += residual;
+    store_row<D>(p.y, i * p.ldy + j, have, v);
 }
 
 template <int D, bool kA, bool kB, class T, bool kAsync>
@@ -101,12 +96,19 @@ __global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs p) 
     const int64_t k0 = blockIdx.y * p.k_split, k1 = min(p.k, k0 + p.k_split);
     f32x4 acc[T::TM][T::TN];
     tile_product<D, kA, kB, T, kAsync>(p.a, p.lda, m0, p.m, p.b, p.ldb, n0, p.n, k0, k1, lds, acc);
-    finish_tile<T, kAsync>(lds, acc, [&](int i, int j, f32x4 v) {
-        const int64_t m = m0 + i, n = n0 + j;
-        if (m >= p.m || n >= p.n) return;
-        if (p.partial != nullptr) *reinterpret_cast<f32x4*>(p.partial + (blockIdx.y * p.m + m) * p.ldp + n) = v;
-        else epilogue<D>(p, m, n, v);
-    });
+    finish_tile<T, kAsync, 2>(
+        lds, acc,
+        [&](int i, int j) {
+            const int64_t m = m0 + i, n = n0 + j;
+            return m < p.m && n < p.n && p.partial == nullptr ? residual_of<D>(p, m, n) : f32x4{0.f, 0.f, 0.f, 0.f};
+        },
+        [&](int i, int j, f32x4 v, f32x4 residual) {
+            const int64_t m = m0 + i, n = n0 + j;
+            if (m >= p.m || n >= p.n) return v;
+            if (p.partial != nullptr) *reinterpret_cast<f32x4*>(p.partial + (blockIdx.y * p.m + m) * p.ldp + n) = v;
+            else epilogue<D>(p, m, n, v, residual);
+            return v;
+        });
 }
 
 // Joins the parts of a split sum, in their order, and finishes the result.
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(256) void join_kernel(ProductArgs p, int splits) {
         f32x4 v = *reinterpret_cast<const f32x4*>(p.partial + m * p.ldp + n);
         for (int s = 1; s < splits; ++s)
             v += *reinterpret_cast<const f32x4*>(p.partial + (s * p.m + m) * p.ldp + n);
-        epilogue<D>(p, m, n, v);
+        epilogue<D>(p, m, n, v, residual_of<D>(p, m, n));
     }
 }
 
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(512) void thin_kernel(ProductArgs p) {
 #pragma unroll
         for (int i = 1; i < kWaves; ++i) acc += sums[i][lane];
         const int64_t n = n0 + 4 * q;
-        if (x_in && n < p.n) epilogue<D>(p, row, n, acc);
+        if (x_in && n < p.n) epilogue<D>(p, row, n, acc, residual_of<D>(p, row, n));
     }
 }
 

@@ -84,6 +84,27 @@ __device__ __forceinline__ u32x4 load16(const char* at) {
     return u32x4{v[0], v[1], v[2], v[3]};
 }
 
+// Elements i .. i + 3, or as many of them as exist.
+template <int D>
+__device__ __forceinline__ f32x4 load_row(const void* p, int64_t i, int have) {
+    if (have >= 4) return load4<D>(p, i);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < have) v[e] = load_elem<D>(p, i + e);
+    return v;
+}
+template <int D>
+__device__ __forceinline__ void store_row(void* p, int64_t i, int have, f32x4 v) {
+    if (have >= 4) {
+        store4<D>(p, i, v);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < have) store_elem<D>(p, i + e, v[e]);
+}
+
 // c += a b over one 16-byte fragment pair: 32 values of k in 2-byte types (one
 // instruction), 16 in fp32 (four).  Lane l holds row l % 16 of each operand and the unit of
 // k that its quarter l / 16 names; the order of k inside a fragment is the same in both.
@@ -432,20 +453,24 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
     __syncthreads();  // the LDS is free
 }
 
-// Hands the tile's results to `store(m, n, v)`, four consecutive n at a time, each in one lane,
-// rows in order: the accumulators pass through LDS (free by now), so the code that finishes a
-// result stands once, in a loop, and a wave's loads and stores cover whole rows.
+// Finishes the tile, four consecutive n of a row at a time: `load(m, n)` fetches what the result
+// is combined with, `store(m, n, v, loaded)` stores it and returns the value kept.  The
+// accumulators pass through LDS (free by now), so that this code stands once and a wave's loads
+// and stores cover whole rows; a lane issues the loads of up to kMostBatch units before it uses the first.
 //
-// `mirror(n, m, v)`, unless it is NoMirror or `mirrored` is false, then gets the transposed
-// tile, four consecutive m at a time: a wave takes sixteen n by four units of m, so its LDS
-// reads fall on distinct banks and its stores cover 32 bytes of a row.
+// `mirror(n, m, v)`, unless it is NoMirror or `mirrored` is false, then gets the kept values
+// transposed, four consecutive m at a time: a wave takes sixteen n by four units of m, so its
+// LDS reads fall on distinct banks and its stores cover 32 bytes of a row.
 struct NoMirror {};
-template <class T, bool kAsync, class Store, class Mirror = NoMirror>
-__device__ __forceinline__ void finish_tile(char* lds, const f32x4 (&acc)[T::TM][T::TN], Store&& store,
+template <class T, bool kAsync, int kMostBatch, class Load, class Store, class Mirror = NoMirror>
+__device__ __forceinline__ void finish_tile(char* lds, const f32x4 (&acc)[T::TM][T::TN], Load&& load, Store&& store,
                                             bool mirrored = false, Mirror&& mirror = Mirror{}) {
+    constexpr bool kMirror = !std::is_same_v<std::decay_t<Mirror>, NoMirror>;
     constexpr int kRowUnits = T::BN / 4, kPhases = T::BM * T::BN * 4 > lds_bytes<T, kAsync>() ? T::WM : 1;
-    constexpr int kRows = T::BM / kPhases;
+    constexpr int kRows = T::BM / kPhases, kUnits = kRows * kRowUnits / T::kThreads, kBatch = kUnits < kMostBatch ? kUnits : kMostBatch;
     static_assert(kRows * T::BN * 4 <= lds_bytes<T, kAsync>(), "a phase fits the tile's LDS");
+    static_assert(kRows * kRowUnits % (T::kThreads * kBatch) == 0, "whole batches");
+    using Loaded = decltype(load(0, 0));
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = (wave / T::WN) * (T::BM / T::WM), wn = (wave % T::WN) * (T::BN / T::WN);
     f32x4* out = reinterpret_cast<f32x4*>(lds);
@@ -462,13 +487,29 @@ __device__ __forceinline__ void finish_tile(char* lds, const f32x4 (&acc)[T::TM]
                 }
         }
         __syncthreads();
-        for (int u = tid; u < kRows * kRowUnits; u += T::kThreads) {
-            const int m = u / kRowUnits, unit = u % kRowUnits;
-            store(phase * kRows + m, unit * 4, out[m * kRowUnits + (unit ^ (m & 15))]);
+#pragma unroll 1
+        for (int first = tid; first < kRows * kRowUnits; first += kBatch * T::kThreads) {
+            Loaded loaded[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int u = first + b * T::kThreads;
+                loaded[b] = load(phase * kRows + u / kRowUnits, u % kRowUnits * 4);
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int u = first + b * T::kThreads, m = u / kRowUnits, unit = u % kRowUnits;
+                f32x4& at = out[m * kRowUnits + (unit ^ (m & 15))];
+                const f32x4 kept = store(phase * kRows + m, unit * 4, at, loaded[b]);
+                if constexpr (kMirror) {
+                    if (mirrored) at = kept;
+                }
+            }
         }
-        if constexpr (!std::is_same_v<std::decay_t<Mirror>, NoMirror>) {
+        if constexpr (kMirror) {
             if (mirrored) {
+                __syncthreads();
                 const float* flat = reinterpret_cast<const float*>(lds);
+#pragma unroll 4
                 for (int u = tid; u < T::BN * kRows / 4; u += T::kThreads) {
                     const int block = u >> 6, n = block % (T::BN / 16) * 16 + (u & 15);
                     const int m = (block / (T::BN / 16) * 4 + ((u >> 4) & 3)) * 4;

@@ -13,6 +13,8 @@
 //
 // Every phase takes all matrices of one orientation in one launch: the tiles of up to 16
 // matrices of any sizes, found in a table in the launch's arguments.
+#include <numeric>
+
 #include "hbt_matmul.hpp"
 
 namespace hbt {
@@ -180,50 +182,37 @@ struct Problem {
     float gram_scale;     // 1 / scale^2
     float out_scale;      // the step's multiple of x, over scale
 };
+struct Run {
+    int first, count, tiles;  // its matrices, and the tiles of each
+};
 struct ProductArgs {
     FirstBlocks blocks;
+    Run run[kMaxMatrices];
     Problem problem[kMaxMatrices];
     const float* slot;    // null, or decay and learning rate are its first two floats
     float a, b, c, decay, lr;
     int count, first, last, update, out_dtype;
 };
 
-// Elements j .. j + 3 of a row of `cols`, in either rounding: all four, or those that exist.
-template <int D>
-__device__ __forceinline__ f32x4 load_row(const void* p, int64_t i, int have) {
-    if (have >= 4) return load4<D>(p, i);
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int e = 0; e < 3; ++e)
-        if (e < have) v[e] = load_elem<D>(p, i + e);
-    return v;
-}
-template <int D>
-__device__ __forceinline__ void store_row(void* p, int64_t i, int have, f32x4 v) {
-    if (have >= 4) {
-        store4<D>(p, i, v);
-        return;
-    }
-    for (int e = 0; e < 3; ++e)
-        if (e < have) store_elem<D>(p, i + e, v[e]);
-}
-
-// w' = decay w - lr out_scale x, or the result out_scale x itself.
-template <int D>
-__device__ __forceinline__ void finish(const ProductArgs& p, const Problem& t, float decay, float lr, int64_t i,
-                                       int have, f32x4 x) {
-    if (p.update) x = load_row<D>(t.out, i, have) * decay - x * (lr * t.out_scale);
-    else x *= t.out_scale;
-    store_row<D>(t.out, i, have, x);
+template <typename F>
+__device__ __forceinline__ auto by_dtype(int dtype, F&& f) {
+    if (dtype == HBT_DTYPE_F32) return f(std::integral_constant<int, HBT_DTYPE_F32>{});
+    if (dtype == HBT_DTYPE_BF16) return f(std::integral_constant<int, HBT_DTYPE_BF16>{});
+    return f(std::integral_constant<int, HBT_DTYPE_F16>{});
 }
 
 // kWide: rows <= columns, so A = x x^T and x' = a x + B x; else A = x^T x and x' = a x + x B.
 template <int D, class T, Phase kPhase, bool kWide>
 __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductArgs p) {
     extern __shared__ __align__(16) char lds[];
-    const int block = xcd_tile(blockIdx.x, gridDim.x);
-    const int e = find_entry(p.blocks, block);
-    const Problem& t = p.problem[e];
-    const int tile = block - p.blocks.first[e], side = kWide ? t.rows : t.cols;
+    // Matrices of one shape share a run of workgroups, which starts at a multiple of 8: each XCD
+    // takes consecutive tiles of it, and every XCD its part of each run, whose sums differ in length.
+    const int r = find_entry(p.blocks, blockIdx.x), local = blockIdx.x - p.blocks.first[r];
+    const Run& run = p.run[r];
+    if (local >= run.count * run.tiles) return;
+    const int global = xcd_tile(local, run.count * run.tiles);
+    const Problem& t = p.problem[run.first + global / run.tiles];
+    const int tile = global % run.tiles, side = kWide ? t.rows : t.cols;
     const int ldg = (side + 7) / 8 * 8;
     int tm, tn;
     if constexpr (kPhase == kIterate) {
@@ -250,37 +239,61 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
     if constexpr (kPhase == kIterate) {
         const float factor = p.first && t.state != nullptr ? *t.factor : 1.0f;
         const float decay = p.slot != nullptr ? p.slot[0] : p.decay, lr = p.slot != nullptr ? p.slot[1] : p.lr;
-        finish_tile<T, true>(lds, acc, [&](int i, int j, f32x4 v) {
-            const int m = m0 + i, n = n0 + j, have = t.cols - n;
-            if (m >= t.rows || have <= 0) return;
-            const int64_t dense = int64_t(m) * t.cols + n, padded = int64_t(m) * t.ldx + n;
-            const f32x4 x = D == HBT_DTYPE_F32 ? load4<D>(t.x, padded)
-                                               : load_row<HBT_DTYPE_F32>(t.state, dense, have) * factor;
-            v += x * p.a;
-            if (p.last) {
-                if (p.out_dtype == HBT_DTYPE_F32) finish<HBT_DTYPE_F32>(p, t, decay, lr, dense, have, v);
-                else if (p.out_dtype == HBT_DTYPE_BF16) finish<HBT_DTYPE_BF16>(p, t, decay, lr, dense, have, v);
-                else finish<HBT_DTYPE_F16>(p, t, decay, lr, dense, have, v);
-            } else {
-                if constexpr (D != HBT_DTYPE_F32) store_row<HBT_DTYPE_F32>(t.state, dense, have, v);
-                store4<D>(t.x_next, padded, v);
-            }
-        });
+        struct Loaded {
+            f32x4 x, w;
+        };
+        finish_tile<T, true, 8>(
+            lds, acc,
+            [&](int i, int j) {
+                Loaded l{};
+                const int m = m0 + i, n = n0 + j, have = t.cols - n;
+                if (m >= t.rows || have <= 0) return l;
+                const int64_t dense = int64_t(m) * t.cols + n;
+                l.x = D == HBT_DTYPE_F32 ? load4<D>(t.x, int64_t(m) * t.ldx + n)
+                                         : load_row<HBT_DTYPE_F32>(t.state, dense, have) * factor;
+                if (p.last && p.update)
+                    l.w = by_dtype(p.out_dtype, [&](auto d) { return load_row<decltype(d)::value>(t.out, dense, have); });
+                return l;
+            },
+            [&](int i, int j, f32x4 v, const Loaded& l) {
+                const int m = m0 + i, n = n0 + j, have = t.cols - n;
+                if (m >= t.rows || have <= 0) return v;
+                const int64_t dense = int64_t(m) * t.cols + n;
+                v += l.x * p.a;
+                if (p.last) {
+                    // w' = decay w - lr out_scale x, or the result out_scale x itself
+                    v = p.update ? l.w * decay - v * (lr * t.out_scale) : v * t.out_scale;
+                    by_dtype(p.out_dtype, [&](auto d) { store_row<decltype(d)::value>(t.out, dense, have, v); });
+                } else {
+                    if constexpr (D != HBT_DTYPE_F32) store_row<HBT_DTYPE_F32>(t.state, dense, have, v);
+                    store4<D>(t.x_next, int64_t(m) * t.ldx + n, v);
+                }
+                return v;
+            });
     } else {
         void* out = kPhase == kGram ? t.gram : t.poly;
-        const auto value = [&](int m, int n, f32x4 v) {
-            if constexpr (kPhase == kGram) return v * t.gram_scale;
-            else return load4<D>(t.gram, int64_t(m) * ldg + n) * p.b + v * p.c;
-        };
-        const auto store = [&](int i, int j, f32x4 v) {
-            const int m = m0 + i, n = n0 + j;
-            if (m < side && n < side) store4<D>(out, int64_t(m) * ldg + n, value(m, n, v));
-        };
         // Off the diagonal the mirror image is stored too: the products are bitwise symmetric.
-        finish_tile<T, true>(lds, acc, store, tm != tn, [&](int j, int i, f32x4 v) {
-            const int n = n0 + j, m = m0 + i;
-            if (n < side && m < side) store4<D>(out, int64_t(n) * ldg + m, value(n, m, v));
-        });
+        finish_tile<T, true, 8>(
+            lds, acc,
+            [&](int i, int j) {
+                const int m = m0 + i, n = n0 + j;
+                f32x4 l = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (kPhase == kSquare) {
+                    if (m < side && n < side) l = load4<D>(t.gram, int64_t(m) * ldg + n);
+                }
+                return l;
+            },
+            [&](int i, int j, f32x4 v, f32x4 l) {
+                const int m = m0 + i, n = n0 + j;
+                v = kPhase == kGram ? v * t.gram_scale : l * p.b + v * p.c;
+                if (m < side && n < side) store4<D>(out, int64_t(m) * ldg + n, v);
+                return v;
+            },
+            tm != tn,
+            [&](int j, int i, f32x4 v) {
+                const int n = n0 + j, m = m0 + i;
+                if (n < side && m < side) store4<D>(out, int64_t(n) * ldg + m, v);
+            });
     }
 }
 
@@ -480,9 +493,13 @@ int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t
     constexpr int kLds = lds_bytes<T, true>();
     int64_t blocks = 0;
     p.blocks.clear();
-    for (int i = 0; i < p.count; ++i) {
-        p.blocks.first[i] = static_cast<int>(blocks);
-        blocks += tiles_of(p.problem[i], size, kPhase);
+    for (int i = 0, r = 0; i < p.count; i += p.run[r++].count) {
+        const Problem& t = p.problem[i];
+        int n = 1;
+        while (i + n < p.count && p.problem[i + n].rows == t.rows && p.problem[i + n].cols == t.cols) ++n;
+        p.run[r] = {i, n, static_cast<int>(tiles_of(t, size, kPhase))};
+        p.blocks.first[r] = static_cast<int>(blocks);
+        blocks += (int64_t(n) * p.run[r].tiles + 7) / 8 * 8;
     }
     const auto kernel = newton_schulz_kernel<D, T, kPhase, kWide>;
     if constexpr (kLds > 65536) {
@@ -549,9 +566,17 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
     norm.eps = eps;
     direction.blocks.clear();
     start.blocks.clear();
+    // Longest sums first: a launch's last workgroups are then its shortest.
+    int order[kMaxMatrices];
+    std::iota(order, order + t.count, 0);
+    std::stable_sort(order, order + t.count, [&](int i, int j) {
+        const int64_t a = std::max(t.rows[i], t.cols[i]), b = std::max(t.rows[j], t.cols[j]);
+        return a != b ? a > b : t.rows[i] * t.cols[i] > t.rows[j] * t.cols[j];
+    });
     int64_t at = 0, direction_blocks = 0, start_blocks = 0;
     int n = 0;
-    for (int i = 0; i < t.count; ++i) {
+    for (int k = 0; k < t.count; ++k) {
+        const int i = order[k];
         const int64_t rows = t.rows[i], cols = t.cols[i];
         if (rows == 0 || cols == 0 || is_small(rows, cols)) continue;
         const int kind = product_of(rows, cols, product);
