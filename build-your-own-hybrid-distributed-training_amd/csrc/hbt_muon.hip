@@ -11,7 +11,7 @@
 // to 16 bits would be amplified by 3.4 a step in the directions that start small: on matrices with
 // a decaying spectrum fp16 products then end 6e-3 to 9e-3 off, and 3e-4 to 2e-3 with x in fp32.
 //
-// Every phase takes all matrices of one orientation in one launch: the tiles of up to 16
+// Every phase takes all matrices of one orientation in one launch: the tiles of up to 32
 // matrices of any sizes, found in a table in the launch's arguments.
 #include <numeric>
 
@@ -21,7 +21,7 @@ namespace hbt {
 namespace mm {
 namespace {
 
-constexpr int kMaxMatrices = HBT_MAX_TENSORS_PER_LAUNCH;
+constexpr int kMaxMatrices = HBT_MAX_MATRICES;
 constexpr int kChunk = 4096;  // elements per norm partial
 constexpr int kMaxSteps = 64;
 

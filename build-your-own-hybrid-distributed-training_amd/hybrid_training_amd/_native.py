@@ -54,6 +54,7 @@ __all__ = [
     "EXPORTED_SYMBOLS",
     "GraphRecording",
     "MAX_LOCAL_RANKS",
+    "MAX_MATRICES",
     "MAX_NORM_PARTS",
     "MAX_TENSORS_PER_LAUNCH",
     "PIECES_PER_NORM_CHUNK",
@@ -70,6 +71,7 @@ __all__ = [
 
 ABI_VERSION = 22
 MAX_TENSORS_PER_LAUNCH = 16
+MAX_MATRICES = 32
 MAX_LOCAL_RANKS = 64
 MAX_NORM_PARTS = 128
 CLIP_MAX_ELEMENTS = 1048576

@@ -8,7 +8,7 @@ Newton-Schulz products from ``x = u / |u|``::
     A = x x^T (over the shorter side);  x = a x + (b A + c A A) x
 
 and the parameter moves by ``-lr * scale * x`` after its weight decay.  One call updates up to
-16 matrices of any sizes (``hbt_muon_step``): the momentum and the norm in one pass over the
+32 matrices of any sizes (``hbt_muon_step``): the momentum and the norm in one pass over the
 gradients, the products on the matrix cores with every matrix of a phase in one launch, the
 parameter written by the last product's epilogue.
 
@@ -52,7 +52,7 @@ __all__ = ["MuonOptimizer", "orthogonalize"]
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 #: Working storage one call may ask for before a list of matrices is split (a single matrix may
-#: need more): 16 matrices of a few thousand squared fit.
+#: need more): 32 matrices of a few thousand squared fit.
 _WORKSPACE_CAP = 4 << 30
 #: Sides the kernels address (hbt_orthogonalize's limit).
 _MAX_SIDE = 1 << 20
@@ -60,7 +60,7 @@ _MAX_SIDE = 1 << 20
 
 def _call_groups(shapes: Sequence[tuple[int, int]], product: int) -> list[tuple[list[int], int]]:
     """(indices, workspace bytes) of the calls a list of matrices is split into, in order: at
-    most ``MAX_TENSORS_PER_LAUNCH`` matrices and ``_WORKSPACE_CAP`` bytes each."""
+    most ``MAX_MATRICES`` matrices and ``_WORKSPACE_CAP`` bytes each."""
     lib = _native.library()
 
     def need(indices: list[int]) -> int:
@@ -72,8 +72,8 @@ def _call_groups(shapes: Sequence[tuple[int, int]], product: int) -> list[tuple[
         return nbytes
 
     groups: list[tuple[list[int], int]] = []
-    for first in range(0, len(shapes), _native.MAX_TENSORS_PER_LAUNCH):
-        indices = list(range(first, min(first + _native.MAX_TENSORS_PER_LAUNCH, len(shapes))))
+    for first in range(0, len(shapes), _native.MAX_MATRICES):
+        indices = list(range(first, min(first + _native.MAX_MATRICES, len(shapes))))
         nbytes = need(indices)
         if nbytes <= _WORKSPACE_CAP:
             groups.append((indices, nbytes))
@@ -288,7 +288,7 @@ class MuonOptimizer(ShardedOptimizer):
                                     self._device, "muon.hbt_scale_inplace")
 
     def _step_batch(self, batch, pdtype, gdtype, unscale, grad_mul, recording) -> None:
-        """Matrices of one group and dtype pair, in calls of up to 16."""
+        """Matrices of one group and dtype pair, in calls of up to 32."""
         lib = _native.library()
         stream = _native.stream_of(self._device)
         group = batch[0][0]

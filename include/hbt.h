@@ -37,6 +37,7 @@ extern "C" {
 
 /* ---- per-call limits ---------------------------------------------------------- */
 #define HBT_MAX_TENSORS_PER_LAUNCH 16 /* AdamW / norm tables; the host splits larger lists */
+#define HBT_MAX_MATRICES 32           /* orthogonalised matrices; the host splits larger lists */
 
 /* Message describing the last failed call on this thread ("" if none). */
 const char* hbt_last_error(void);
@@ -689,7 +690,7 @@ int32_t hbt_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t
  * Replaces: for matrix parameters, the update of ShardedOptimizer.step
  *   (optim/sharded_optimizer.py:340-355) by an orthogonalised one; the reference has AdamW and
  *   SGD only.
- * Up to HBT_MAX_TENSORS_PER_LAUNCH dense row-major matrices of any sizes, rows[i] x cols[i]
+ * Up to HBT_MAX_MATRICES dense row-major matrices of any sizes, rows[i] x cols[i]
  * (sides at most 2^20, at most 2^34 elements a call; an empty one is skipped):
  *   x = u / max(|u|, eps) (Frobenius norm);  `steps` (1..64) times
  *     A = x x^T, or x^T x when rows > cols;  B = b A + c A A;  x = a x + B x, or a x + x B
