@@ -4,12 +4,13 @@
 //   `steps` times:  A = x x^T (or x^T x, over the shorter side),  B = b A + c A A,  x = a x + B x
 //   w' = decay w - lr scale x
 //
-// The iterate x is held in fp32.  The products read copies of x, A and B rounded to the product
+// The iterate x is held in 32 bits: fp32, or, beside fp16 products, the fp16 value they read and
+// the fp16 rounding error of it (22 bits of mantissa).  The products read copies of x, A and B rounded to the product
 // type: fp16 (11 bits, and the values are bounded: singular values stay below 1.3, and x is
 // scaled by a power of two near the square root of its longer side, which puts its elements near
 // 1 and the first iterate's above fp16's subnormals) or, on request, fp32.  Rounding x itself
 // to 16 bits would be amplified by 3.4 a step in the directions that start small: on matrices with
-// a decaying spectrum fp16 products then end 6e-3 to 9e-3 off, and 3e-4 to 2e-3 with x in fp32.
+// a decaying spectrum fp16 products then end 6e-3 to 9e-3 off, and 3e-4 to 2e-3 with x in 32.
 //
 // Every phase takes all matrices of one orientation in one launch: the tiles of up to 32
 // matrices of any sizes, found in a table in the launch's arguments.
@@ -44,9 +45,9 @@ __device__ __forceinline__ int find_entry(const FirstBlocks& blocks, int block) 
 struct DirectionEntry {
     const void* g;
     float* v;        // null: u is the input itself
-    float* u;        // fp32, dense
+    float* u;        // fp32, [rows][ld]
     double* partial;
-    int64_t numel;
+    int64_t rows, cols, ld;
 };
 struct DirectionArgs {
     FirstBlocks blocks;
@@ -58,45 +59,52 @@ struct DirectionArgs {
 };
 
 // One pass over the gradients: the momentum, the direction, and its squares summed in fp64.
+// A lane takes four columns of a row at a time; gradients and momenta lie dense, at any
+// alignment, the directions on rows of whole 16-byte units.
 template <int GD>
 __global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
-    const int block = blockIdx.x, e = find_entry(p.blocks, block);
-    const DirectionEntry& t = p.entry[e];
-    const int64_t chunk = block - p.blocks.first[e], base = chunk * kChunk;
+    const int block = blockIdx.x, entry = find_entry(p.blocks, block);
+    const DirectionEntry& t = p.entry[entry];
+    const int chunk = block - p.blocks.first[entry];
+    const uint32_t units = static_cast<uint32_t>(t.ld / 4);
+    const int64_t first = int64_t(chunk) * (kChunk / 4), row0 = first / units;
+    const uint32_t unit0 = static_cast<uint32_t>(first - row0 * units);
     const float mul = p.grad_mul != nullptr ? *p.grad_mul : 1.0f;
     const float mu = p.slot != nullptr ? p.slot[2] : p.momentum, rest = p.slot != nullptr ? p.slot[3] : p.rest;
+    constexpr int kUnits = kChunk / 1024;
+    int64_t at[kUnits], to[kUnits];
+    int have[kUnits];
+    f32x4 g[kUnits], v[kUnits];
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+        const uint32_t local = unit0 + k * 256 + threadIdx.x, down = local / units;
+        const int64_t row = row0 + down;
+        const int col = static_cast<int>(local - down * units) * 4;
+        have[k] = row < t.rows ? static_cast<int>(min<int64_t>(t.cols - col, 4)) : 0;
+        at[k] = row * t.cols + col;
+        to[k] = row * t.ld + col;
+        if (have[k] > 0) {
+            g[k] = load_row<GD>(t.g, at[k], have[k]);
+            if (t.v != nullptr) v[k] = load_row<HBT_DTYPE_F32>(t.v, at[k], have[k]);
+        }
+    }
     double sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < kChunk / 1024; ++k) {
-        const int64_t i = base + k * 1024 + threadIdx.x * 4;
-        if (i >= t.numel) break;
-        f32x4 u;
-        if (i + 4 <= t.numel) {
-            u = load4<GD>(t.g, i) * p.unscale * mul;
-            if (t.v != nullptr) {
-                f32x4 v = load4<HBT_DTYPE_F32>(t.v, i);
+    for (int k = 0; k < kUnits; ++k) {
+        if (have[k] <= 0) continue;
+        f32x4 u = g[k] * p.unscale * mul;
+        if (t.v != nullptr) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = mu * v[e] + rest * u[e];
-                    u[e] = p.nesterov ? mu * v[e] + rest * u[e] : v[e];
-                }
-                store4<HBT_DTYPE_F32>(t.v, i, v);
+            for (int e = 0; e < 4; ++e) {
+                v[k][e] = mu * v[k][e] + rest * u[e];
+                u[e] = p.nesterov ? mu * v[k][e] + rest * u[e] : v[k][e];
             }
-            store4<HBT_DTYPE_F32>(t.u, i, u);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum += double(u[e]) * double(u[e]);
-        } else {
-            for (int64_t j = i; j < t.numel; ++j) {
-                float x = load_elem<GD>(t.g, j) * p.unscale * mul;
-                if (t.v != nullptr) {
-                    const float v = mu * t.v[j] + rest * x;
-                    x = p.nesterov ? mu * v + rest * x : v;
-                    t.v[j] = v;
-                }
-                t.u[j] = x;
-                sum += double(x) * double(x);
-            }
+            store_row<HBT_DTYPE_F32>(t.v, at[k], have[k], v[k]);
         }
+        *reinterpret_cast<f32x4*>(t.u + to[k]) = u;  // past the last column: padding
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < have[k]) sum += double(u[e]) * double(u[e]);
     }
     const double total = block_sum<256>(sum);
     if (threadIdx.x == 0) t.partial[chunk] = total;
@@ -132,38 +140,50 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
     }
 }
 
+// The fp16 value of x and what it leaves, itself in fp16.
+__device__ __forceinline__ void split(f32x4 x, u32x2& high, u32x2& low) {
+    high = u32x2{pack2_rounded<HBT_DTYPE_F16>(x[0], x[1]), pack2_rounded<HBT_DTYPE_F16>(x[2], x[3])};
+    f32x4 left;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) left[e] = x[e] - f16_to_f32((high[e / 2] >> (16 * (e % 2))) & 0xFFFFu);
+    low = u32x2{pack2_rounded<HBT_DTYPE_F16>(left[0], left[1]), pack2_rounded<HBT_DTYPE_F16>(left[2], left[3])};
+}
+
 struct StartEntry {
     const float* u;
     void* x;
+    void* low;  // the rest of x beside fp16 values
     const float* factor;
-    int64_t rows, cols, ld;
+    int64_t units;  // of four elements: whole rows with their padding
 };
 struct StartArgs {
     FirstBlocks blocks;
     StartEntry entry[kMaxMatrices];
 };
 
-// The first iterate in the product type, rows on 16-byte boundaries: eight columns a lane.
+// The first iterate in the product type.
 template <int D>
 __global__ __launch_bounds__(256) void start_kernel(StartArgs p) {
-    const int block = blockIdx.x, e = find_entry(p.blocks, block);
-    const StartEntry& t = p.entry[e];
-    const int64_t units = t.ld / 8, i = int64_t(block - p.blocks.first[e]) * 256 + threadIdx.x;
-    if (i >= t.rows * units) return;
-    const int64_t row = i / units, col = i % units * 8;
+    const int block = blockIdx.x, entry = find_entry(p.blocks, block);
+    const StartEntry& t = p.entry[entry];
+    const int64_t base = int64_t(block - p.blocks.first[entry]) * 1024 + threadIdx.x;
     const float f = *t.factor;
-    const float* u = t.u + row * t.cols + col;
+    f32x4 x[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (col + 4 * h + 4 <= t.cols) {
-            v = load4<HBT_DTYPE_F32>(u, 4 * h) * f;
+    for (int k = 0; k < 4; ++k)
+        if (base + k * 256 < t.units) x[k] = reinterpret_cast<const f32x4*>(t.u)[base + k * 256] * f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t i = base + k * 256;
+        if (i >= t.units) break;
+        if constexpr (D == HBT_DTYPE_F32) {
+            static_cast<f32x4*>(t.x)[i] = x[k];
         } else {
-#pragma unroll
-            for (int e = 0; e < 3; ++e)
-                if (col + 4 * h + e < t.cols) v[e] = u[4 * h + e] * f;
+            u32x2 high, low;
+            split(x[k], high, low);
+            static_cast<u32x2*>(t.x)[i] = high;
+            static_cast<u32x2*>(t.low)[i] = low;
         }
-        store4<D>(t.x, row * t.ld + col + 4 * h, v);
     }
 }
 
@@ -175,8 +195,7 @@ struct Problem {
     void* x_next;
     void* gram;           // [side][ldg], side the shorter one
     void* poly;
-    float* state;         // the fp32 iterate [rows][cols] (fp16 products), or null
-    const float* factor;  // first step: the state is still u, to be multiplied by this
+    void* low;            // what x's fp16 values leave of it, [rows][ldx], or null
     void* out;            // last step: the parameter or the result, [rows][cols]
     int rows, cols, ldx;
     float gram_scale;     // 1 / scale^2
@@ -191,7 +210,7 @@ struct ProductArgs {
     Problem problem[kMaxMatrices];
     const float* slot;    // null, or decay and learning rate are its first two floats
     float a, b, c, decay, lr;
-    int count, first, last, update, out_dtype;
+    int count, last, update, out_dtype;
 };
 
 template <typename F>
@@ -237,7 +256,6 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
         tile_product<D, true, true, T, true>(t.x, t.ldx, m0, t.rows, t.poly, ldg, n0, side, 0, side, lds, acc);
     }
     if constexpr (kPhase == kIterate) {
-        const float factor = p.first && t.state != nullptr ? *t.factor : 1.0f;
         const float decay = p.slot != nullptr ? p.slot[0] : p.decay, lr = p.slot != nullptr ? p.slot[1] : p.lr;
         struct Loaded {
             f32x4 x, w;
@@ -248,25 +266,33 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
                 Loaded l{};
                 const int m = m0 + i, n = n0 + j, have = t.cols - n;
                 if (m >= t.rows || have <= 0) return l;
-                const int64_t dense = int64_t(m) * t.cols + n;
-                l.x = D == HBT_DTYPE_F32 ? load4<D>(t.x, int64_t(m) * t.ldx + n)
-                                         : load_row<HBT_DTYPE_F32>(t.state, dense, have) * factor;
+                const int64_t padded = int64_t(m) * t.ldx + n;
+                l.x = load4<D>(t.x, padded);
+                if constexpr (D != HBT_DTYPE_F32) l.x += load4<D>(t.low, padded);
                 if (p.last && p.update)
-                    l.w = by_dtype(p.out_dtype, [&](auto d) { return load_row<decltype(d)::value>(t.out, dense, have); });
+                    l.w = by_dtype(p.out_dtype, [&](auto d) {
+                        return load_row<decltype(d)::value>(t.out, int64_t(m) * t.cols + n, have);
+                    });
                 return l;
             },
             [&](int i, int j, f32x4 v, const Loaded& l) {
                 const int m = m0 + i, n = n0 + j, have = t.cols - n;
                 if (m >= t.rows || have <= 0) return v;
-                const int64_t dense = int64_t(m) * t.cols + n;
+                const int64_t padded = int64_t(m) * t.ldx + n;
                 v += l.x * p.a;
                 if (p.last) {
                     // w' = decay w - lr out_scale x, or the result out_scale x itself
                     v = p.update ? l.w * decay - v * (lr * t.out_scale) : v * t.out_scale;
-                    by_dtype(p.out_dtype, [&](auto d) { store_row<decltype(d)::value>(t.out, dense, have, v); });
+                    by_dtype(p.out_dtype, [&](auto d) {
+                        store_row<decltype(d)::value>(t.out, int64_t(m) * t.cols + n, have, v);
+                    });
+                } else if constexpr (D == HBT_DTYPE_F32) {
+                    store4<D>(t.x_next, padded, v);
                 } else {
-                    if constexpr (D != HBT_DTYPE_F32) store_row<HBT_DTYPE_F32>(t.state, dense, have, v);
-                    store4<D>(t.x_next, int64_t(m) * t.ldx + n, v);
+                    u32x2 high, low;
+                    split(v, high, low);
+                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(t.x_next) + padded) = high;
+                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(t.low) + padded) = low;
                 }
                 return v;
             });
@@ -427,7 +453,7 @@ using Tile128 = Tile<128, 128, 2, 2, 2>;
 using Tile64 = Tile<64, 64, 2, 2, 4>;
 
 struct Plan {
-    int64_t state, x0, x1, gram, poly, partial, factor, end;  // offsets of one matrix's storage
+    int64_t u, low, x0, x1, gram, poly, partial, factor, end;  // offsets of one matrix's storage
     int64_t chunks, ldx, ldg;
 };
 
@@ -441,8 +467,9 @@ Plan plan_of(int64_t rows, int64_t cols, int product, int64_t at) {
     Plan p{};
     p.ldx = (cols + 7) / 8 * 8;
     p.ldg = (side + 7) / 8 * 8;
-    p.chunks = (rows * cols + kChunk - 1) / kChunk;
-    p.state = take(rows * cols * 4);
+    p.chunks = (rows * p.ldx + kChunk - 1) / kChunk;
+    p.u = take(rows * p.ldx * 4);
+    p.low = product == HBT_DTYPE_F32 ? at : take(rows * p.ldx * 2);
     p.x0 = take(rows * p.ldx * size);
     p.x1 = take(rows * p.ldx * size);
     p.gram = take(side * p.ldg * size);
@@ -584,22 +611,23 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
         at = plan.end;
         if (kind != D) continue;
         const float scale = iterate_scale(rows, cols, D);
-        float* state = reinterpret_cast<float*>(workspace + plan.state);
+        float* u = reinterpret_cast<float*>(workspace + plan.u);
+        void* low = D == HBT_DTYPE_F32 ? nullptr : workspace + plan.low;
         float* factor = reinterpret_cast<float*>(workspace + plan.factor);
         double* partial = reinterpret_cast<double*>(workspace + plan.partial);
-        direction.entry[n] = {t.grads[i], t.momenta == nullptr ? nullptr : t.momenta[i], state, partial, rows * cols};
+        direction.entry[n] = {t.grads[i], t.momenta == nullptr ? nullptr : t.momenta[i], u, partial, rows, cols, plan.ldx};
         direction.blocks.first[n] = static_cast<int>(direction_blocks);
         direction_blocks += plan.chunks;
         norm.entry[n] = {partial, factor, plan.chunks, scale};
-        start.entry[n] = {state, workspace + plan.x0, factor, rows, cols, plan.ldx};
+        start.entry[n] = {u, workspace + plan.x0, low, factor, rows * (plan.ldx / 4)};
         start.blocks.first[n] = static_cast<int>(start_blocks);
-        start_blocks += (rows * (plan.ldx / 8) + 255) / 256;
+        start_blocks += (rows * (plan.ldx / 4) + 1023) / 1024;
         ++n;
         ProductArgs& group = rows <= cols ? wide : tall;
         group.problem[group.count++] = {workspace + plan.x0, workspace + plan.x1, workspace + plan.gram,
-                                        workspace + plan.poly, D == HBT_DTYPE_F32 ? nullptr : state, factor, t.outs[i],
-                                        static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(plan.ldx),
-                                        1.0f / (scale * scale), (t.scales == nullptr ? 1.0f : t.scales[i]) / scale};
+                                        workspace + plan.poly, low, t.outs[i], static_cast<int>(rows),
+                                        static_cast<int>(cols), static_cast<int>(plan.ldx), 1.0f / (scale * scale),
+                                        (t.scales == nullptr ? 1.0f : t.scales[i]) / scale};
     }
     if (n == 0) return HBT_OK;
     const dim3 direction_grid(static_cast<unsigned>(direction_blocks));
@@ -613,7 +641,7 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
     start_kernel<D><<<dim3(static_cast<unsigned>(start_blocks)), 256, 0, stream>>>(start);
     if ((status = check_launch(who)) != HBT_OK) return status;
     for (int s = 0; s < steps; ++s) {
-        for (ProductArgs* g : {&wide, &tall}) g->first = s == 0, g->last = s == steps - 1;
+        for (ProductArgs* g : {&wide, &tall}) g->last = s == steps - 1;
         if ((status = launch_phase<D, kGram, true>(who, wide, stream)) != HBT_OK ||
             (status = launch_phase<D, kGram, false>(who, tall, stream)) != HBT_OK ||
             (status = launch_phase<D, kSquare, true>(who, wide, stream)) != HBT_OK ||
