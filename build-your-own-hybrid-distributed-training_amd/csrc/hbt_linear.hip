@@ -65,26 +65,39 @@ struct ProductArgs {
     int tiles_m, tiles_n, act;
 };
 
-// The residual of four results of row i from column j.
+// What finishes results: bias, activation, residual, each store rounded once.  Offsets from a
+// tile's first element (m0, n0) fit 32 bits.
 template <int D>
-__device__ __forceinline__ f32x4 residual_of(const ProductArgs& p, int64_t i, int64_t j) {
-    if (p.residual == nullptr) return f32x4{0.f, 0.f, 0.f, 0.f};
-    return load_row<D>(p.residual, i * p.ldr + j, static_cast<int>(min<int64_t>(p.n - j, 4)));
-}
+struct TileEpilogue {
+    const char* bias;
+    const char* from;
+    char* y;
+    char* z;
+    int ldr, ldy, ldz, act;
 
-// Four results of row i from column j: bias, activation, residual, each store rounded once.
-template <int D>
-__device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_t j, f32x4 v, f32x4 residual) {
-    const int have = static_cast<int>(min<int64_t>(p.n - j, 4));
-    if (p.bias != nullptr) v += load_row<D>(p.bias, j, have);
-    if (p.z != nullptr) store_row<D>(p.z, i * p.ldz + j, have, v);
-    if (p.act != HBT_ACT_NONE) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = activate<D>(v[e], p.act);
+    __device__ __forceinline__ TileEpilogue(const ProductArgs& p, int64_t m0, int64_t n0) {
+        constexpr int B = elem_bytes<D>();
+        bias = p.bias == nullptr ? nullptr : static_cast<const char*>(p.bias) + n0 * B;
+        from = p.residual == nullptr ? nullptr : static_cast<const char*>(p.residual) + (m0 * p.ldr + n0) * B;
+        y = static_cast<char*>(p.y) + (m0 * p.ldy + n0) * B;
+        z = p.z == nullptr ? nullptr : static_cast<char*>(p.z) + (m0 * p.ldz + n0) * B;
+        ldr = static_cast<int>(p.ldr), ldy = static_cast<int>(p.ldy), ldz = static_cast<int>(p.ldz), act = p.act;
     }
-    if (p.residual != nullptr) v += residual;
-    store_row<D>(p.y, i * p.ldy + j, have, v);
-}
+    // `have`: results left in the row from column j, of which four are taken.
+    __device__ __forceinline__ f32x4 residual(int i, int j, int have) const {
+        return from == nullptr ? f32x4{0.f, 0.f, 0.f, 0.f} : load_row<D>(from, i * ldr + j, have);
+    }
+    __device__ __forceinline__ void store(int i, int j, int have, f32x4 v, f32x4 residual) const {
+        if (bias != nullptr) v += load_row<D>(bias, j, have);
+        if (z != nullptr) store_row<D>(z, i * ldz + j, have, v);
+        if (act != HBT_ACT_NONE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = activate<D>(v[e], act);
+        }
+        if (from != nullptr) v += residual;
+        store_row<D>(y, i * ldy + j, have, v);
+    }
+};
 
 template <int D, bool kA, bool kB, class T, bool kAsync>
 __global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs p) {
@@ -96,17 +109,19 @@ __global__ __launch_bounds__(T::kThreads, 2) void product_kernel(ProductArgs p) 
     const int64_t k0 = blockIdx.y * p.k_split, k1 = min(p.k, k0 + p.k_split);
     f32x4 acc[T::TM][T::TN];
     tile_product<D, kA, kB, T, kAsync>(p.a, p.lda, m0, p.m, p.b, p.ldb, n0, p.n, k0, k1, lds, acc);
+    const int rows = static_cast<int>(min<int64_t>(p.m - m0, T::BM)), cols = static_cast<int>(min<int64_t>(p.n - n0, T::BN));
+    const TileEpilogue<D> tile(p, m0, n0);
+    float* partial = p.partial == nullptr ? nullptr : p.partial + (blockIdx.y * p.m + m0) * p.ldp + n0;
+    const int ldp = static_cast<int>(p.ldp);
     finish_tile<T, kAsync, 2>(
         lds, acc,
         [&](int i, int j) {
-            const int64_t m = m0 + i, n = n0 + j;
-            return m < p.m && n < p.n && p.partial == nullptr ? residual_of<D>(p, m, n) : f32x4{0.f, 0.f, 0.f, 0.f};
+            return i < rows && j < cols && partial == nullptr ? tile.residual(i, j, cols - j) : f32x4{0.f, 0.f, 0.f, 0.f};
         },
         [&](int i, int j, f32x4 v, f32x4 residual) {
-            const int64_t m = m0 + i, n = n0 + j;
-            if (m >= p.m || n >= p.n) return v;
-            if (p.partial != nullptr) *reinterpret_cast<f32x4*>(p.partial + (blockIdx.y * p.m + m) * p.ldp + n) = v;
-            else epilogue<D>(p, m, n, v, residual);
+            if (i >= rows || j >= cols) return v;
+            if (partial != nullptr) *reinterpret_cast<f32x4*>(partial + i * ldp + j) = v;
+            else tile.store(i, j, cols - j, v, residual);
             return v;
         });
 }
@@ -120,7 +135,9 @@ __global__ __launch_bounds__(256) void join_kernel(ProductArgs p, int splits) {
         f32x4 v = *reinterpret_cast<const f32x4*>(p.partial + m * p.ldp + n);
         for (int s = 1; s < splits; ++s)
             v += *reinterpret_cast<const f32x4*>(p.partial + (s * p.m + m) * p.ldp + n);
-        epilogue<D>(p, m, n, v, residual_of<D>(p, m, n));
+        const TileEpilogue<D> tile(p, m, n);
+        const int have = static_cast<int>(min<int64_t>(p.n - n, 4));
+        tile.store(0, 0, have, v, tile.residual(0, 0, have));
     }
 }
 
@@ -181,7 +198,11 @@ __global__ __launch_bounds__(512) void thin_kernel(ProductArgs p) {
 #pragma unroll
         for (int i = 1; i < kWaves; ++i) acc += sums[i][lane];
         const int64_t n = n0 + 4 * q;
-        if (x_in && n < p.n) epilogue<D>(p, row, n, acc, residual_of<D>(p, row, n));
+        if (x_in && n < p.n) {
+            const TileEpilogue<D> tile(p, row, n);
+            const int have = static_cast<int>(min<int64_t>(p.n - n, 4));
+            tile.store(0, 0, have, acc, tile.residual(0, 0, have));
+        }
     }
 }
 

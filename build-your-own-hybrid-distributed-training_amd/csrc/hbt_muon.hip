@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) void start_kernel(StartArgs p) {
 }
 
 // ---- the products ----------------------------------------------------------------------
-enum Phase { kGram, kSquare, kIterate };
+enum Phase { kGram, kSquare, kIterate, kFinish };  // kFinish: the last iterate, into the result
 
 struct Problem {
     const void* x;        // the iterate in the product type, [rows][ldx]
@@ -210,7 +210,7 @@ struct ProductArgs {
     Problem problem[kMaxMatrices];
     const float* slot;    // null, or decay and learning rate are its first two floats
     float a, b, c, decay, lr;
-    int count, last, update, out_dtype;
+    int count, update, out_dtype;
 };
 
 template <typename F>
@@ -234,7 +234,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
     const int tile = global % run.tiles, side = kWide ? t.rows : t.cols;
     const int ldg = (side + 7) / 8 * 8;
     int tm, tn;
-    if constexpr (kPhase == kIterate) {
+    constexpr bool kProduct = kPhase == kIterate || kPhase == kFinish;
+    if constexpr (kProduct) {
         band_order<8>(tile, (t.rows + T::BM - 1) / T::BM, (t.cols + T::BN - 1) / T::BN, tm, tn);
     } else {  // the lower triangle of a symmetric result, row by row
         tm = static_cast<int>((sqrtf(8.0f * tile + 1.0f) - 1.0f) * 0.5f);
@@ -255,70 +256,75 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
     } else {
         tile_product<D, true, true, T, true>(t.x, t.ldx, m0, t.rows, t.poly, ldg, n0, side, 0, side, lds, acc);
     }
-    if constexpr (kPhase == kIterate) {
-        const float decay = p.slot != nullptr ? p.slot[0] : p.decay, lr = p.slot != nullptr ? p.slot[1] : p.lr;
-        struct Loaded {
-            f32x4 x, w;
+    // Offsets from the tile's first element fit 32 bits; loads past an edge repeat the last row or
+    // the last four columns, stores stop there.
+    if constexpr (kProduct) {
+        const int64_t at = int64_t(m0) * t.ldx + n0, dense = int64_t(m0) * t.cols + n0;
+        const int rows = t.rows - m0, cols = t.cols - n0, padded = t.ldx - n0, ldx = t.ldx, ldo = t.cols;
+        const char* x = static_cast<const char*>(t.x) + at * elem_bytes<D>();
+        const char* low = static_cast<const char*>(t.low) + at * 2;
+        const auto old = [&](int i, int j) {
+            const int from = min(i, rows - 1) * ldx + min(j, padded - 4);
+            f32x4 v = load4<D>(x, from);
+            if constexpr (D != HBT_DTYPE_F32) v += load4<D>(low, from);
+            return v;
         };
-        finish_tile<T, true, 8>(
-            lds, acc,
-            [&](int i, int j) {
-                Loaded l{};
-                const int m = m0 + i, n = n0 + j, have = t.cols - n;
-                if (m >= t.rows || have <= 0) return l;
-                const int64_t padded = int64_t(m) * t.ldx + n;
-                l.x = load4<D>(t.x, padded);
-                if constexpr (D != HBT_DTYPE_F32) l.x += load4<D>(t.low, padded);
-                if (p.last && p.update)
-                    l.w = by_dtype(p.out_dtype, [&](auto d) {
-                        return load_row<decltype(d)::value>(t.out, int64_t(m) * t.cols + n, have);
-                    });
-                return l;
-            },
-            [&](int i, int j, f32x4 v, const Loaded& l) {
-                const int m = m0 + i, n = n0 + j, have = t.cols - n;
-                if (m >= t.rows || have <= 0) return v;
-                const int64_t padded = int64_t(m) * t.ldx + n;
-                v += l.x * p.a;
-                if (p.last) {
-                    // w' = decay w - lr out_scale x, or the result out_scale x itself
-                    v = p.update ? l.w * decay - v * (lr * t.out_scale) : v * t.out_scale;
-                    by_dtype(p.out_dtype, [&](auto d) {
-                        store_row<decltype(d)::value>(t.out, int64_t(m) * t.cols + n, have, v);
-                    });
-                } else if constexpr (D == HBT_DTYPE_F32) {
-                    store4<D>(t.x_next, padded, v);
-                } else {
-                    u32x2 high, low;
-                    split(v, high, low);
-                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(t.x_next) + padded) = high;
-                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(t.low) + padded) = low;
+        if constexpr (kPhase == kIterate) {
+            char* to_x = static_cast<char*>(t.x_next) + at * elem_bytes<D>();
+            char* to_low = static_cast<char*>(t.low) + at * 2;
+            finish_tile<T, true, 8>(lds, acc, old, [&](int i, int j, f32x4 v, f32x4 l) {
+                v += l * p.a;
+                if (i < rows && j < padded) {
+                    const int to = i * ldx + j;
+                    if constexpr (D == HBT_DTYPE_F32) {
+                        store4<D>(to_x, to, v);
+                    } else {
+                        u32x2 high, rest;
+                        split(v, high, rest);
+                        *reinterpret_cast<u32x2*>(to_x + to * 2) = high;
+                        *reinterpret_cast<u32x2*>(to_low + to * 2) = rest;
+                    }
                 }
                 return v;
             });
+        } else {
+            const float decay = p.slot != nullptr ? p.slot[0] : p.decay, lr = p.slot != nullptr ? p.slot[1] : p.lr;
+            const float step = p.update ? -lr * t.out_scale : t.out_scale;
+            by_dtype(p.out_dtype, [&](auto d) {
+                constexpr int PD = decltype(d)::value;
+                char* out = static_cast<char*>(t.out) + dense * elem_bytes<PD>();
+                finish_tile<T, true, 2>(lds, acc, old, [&](int i, int j, f32x4 v, f32x4 l) {
+                    if (i >= rows || j >= cols) return v;
+                    const int to = i * ldo + j;
+                    // w' = decay w - lr out_scale x, or the result out_scale x itself
+                    v = (v + l * p.a) * step;
+                    if (p.update) v += load_row<PD>(out, to, cols - j) * decay;
+                    store_row<PD>(out, to, cols - j, v);
+                    return v;
+                });
+            });
+        }
     } else {
-        void* out = kPhase == kGram ? t.gram : t.poly;
+        const int rows = side - m0, cols = side - n0;
+        char* out = static_cast<char*>(kPhase == kGram ? t.gram : t.poly);
+        char* direct = out + (int64_t(m0) * ldg + n0) * elem_bytes<D>();
+        char* mirror = out + (int64_t(n0) * ldg + m0) * elem_bytes<D>();
+        const char* gram = static_cast<const char*>(t.gram) + (int64_t(m0) * ldg + n0) * elem_bytes<D>();
         // Off the diagonal the mirror image is stored too: the products are bitwise symmetric.
         finish_tile<T, true, 8>(
             lds, acc,
             [&](int i, int j) {
-                const int m = m0 + i, n = n0 + j;
-                f32x4 l = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (kPhase == kSquare) {
-                    if (m < side && n < side) l = load4<D>(t.gram, int64_t(m) * ldg + n);
-                }
-                return l;
+                if constexpr (kPhase == kGram) return f32x4{0.f, 0.f, 0.f, 0.f};
+                else return load4<D>(gram, min(i, rows - 1) * ldg + min(j, ldg - n0 - 4));
             },
             [&](int i, int j, f32x4 v, f32x4 l) {
-                const int m = m0 + i, n = n0 + j;
                 v = kPhase == kGram ? v * t.gram_scale : l * p.b + v * p.c;
-                if (m < side && n < side) store4<D>(out, int64_t(m) * ldg + n, v);
+                if (i < rows && j < cols) store4<D>(direct, i * ldg + j, v);
                 return v;
             },
             tm != tn,
             [&](int j, int i, f32x4 v) {
-                const int n = n0 + j, m = m0 + i;
-                if (n < side && m < side) store4<D>(out, int64_t(n) * ldg + m, v);
+                if (j < cols && i < rows) store4<D>(mirror, j * ldg + i, v);
             });
     }
 }
@@ -510,7 +516,7 @@ struct Matrices {
 
 int64_t tiles_of(const Problem& t, int size, Phase phase) {
     const auto n = [&](int64_t extent) { return (extent + size - 1) / size; };
-    if (phase == kIterate) return n(t.rows) * n(t.cols);
+    if (phase == kIterate || phase == kFinish) return n(t.rows) * n(t.cols);
     const int64_t s = n(std::min(t.rows, t.cols));
     return s * (s + 1) / 2;
 }
@@ -641,12 +647,16 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
     start_kernel<D><<<dim3(static_cast<unsigned>(start_blocks)), 256, 0, stream>>>(start);
     if ((status = check_launch(who)) != HBT_OK) return status;
     for (int s = 0; s < steps; ++s) {
-        for (ProductArgs* g : {&wide, &tall}) g->last = s == steps - 1;
         if ((status = launch_phase<D, kGram, true>(who, wide, stream)) != HBT_OK ||
             (status = launch_phase<D, kGram, false>(who, tall, stream)) != HBT_OK ||
             (status = launch_phase<D, kSquare, true>(who, wide, stream)) != HBT_OK ||
-            (status = launch_phase<D, kSquare, false>(who, tall, stream)) != HBT_OK ||
-            (status = launch_phase<D, kIterate, true>(who, wide, stream)) != HBT_OK ||
+            (status = launch_phase<D, kSquare, false>(who, tall, stream)) != HBT_OK)
+            return status;
+        if (s + 1 == steps) {
+            status = launch_phase<D, kFinish, true>(who, wide, stream);
+            return status != HBT_OK ? status : launch_phase<D, kFinish, false>(who, tall, stream);
+        }
+        if ((status = launch_phase<D, kIterate, true>(who, wide, stream)) != HBT_OK ||
             (status = launch_phase<D, kIterate, false>(who, tall, stream)) != HBT_OK)
             return status;
         for (ProductArgs* g : {&wide, &tall})
