@@ -274,34 +274,37 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* partial, int64_t
 }
 
 // ---- host ----------------------------------------------------------------------------
-using Tile256 = Tile<256, 256, 2, 4, 2>;
-using Tile128 = Tile<128, 128, 2, 2, 2>;
-using Tile64 = Tile<64, 64, 2, 2, 4>;
-
 struct Choice {
     int tile;    // 256, 128 or 64
     int splits;  // parts the sum over k is split into
 };
 
-constexpr int kMaxSplits = 16;
-
+// The cheapest tile and split by the estimate.  A split sum writes and reads its fp32 parts (about
+// 5 TB/s) in one more launch.  Tiles of 256 need operands that load straight into LDS.
 Choice choose(int64_t m, int64_t n, int64_t k, int dtype, bool aligned) {
-    const int bk = dtype == HBT_DTYPE_F32 ? 32 : 64;
-    const int64_t cus = 256;
-    const auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-    if (dtype != HBT_DTYPE_F32 && aligned && tiles(256) >= cus) return {256, 1};
-    const int tile = tiles(128) >= cus ? 128 : 64;
-    const int64_t count = tiles(tile), steps = (k + bk - 1) / bk;
-    int64_t splits = 1;
-    if (count < cus) splits = std::min<int64_t>({2 * cus / std::max<int64_t>(count, 1), steps / 8, kMaxSplits});
-    return {tile, static_cast<int>(std::max<int64_t>(splits, 1))};
+    const bool f32 = dtype == HBT_DTYPE_F32;
+    const int64_t steps = (k + (f32 ? 31 : 63)) / (f32 ? 32 : 64);
+    Choice best{64, 1};
+    double least = 0.0;
+    for (const int size : {64, 128, 256}) {
+        if (size == 256 && (f32 || !aligned)) continue;
+        const double fixed = size == 256 ? 9.0 : (size == 128 ? 6.0 : 3.5);
+        const int64_t tiles = ((m + size - 1) / size) * ((n + size - 1) / size);
+        for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            if (splits > 1 && (steps < 4 * splits || tiles * splits > 1024)) break;
+            double cost = round_cost(size, tiles * splits, static_cast<double>((steps + splits - 1) / splits), f32, fixed);
+            if (splits > 1) cost += 3.0 + 8.0 * m * n * splits / 5.0e6;
+            if (least == 0.0 || cost < least) least = cost, best = {size, splits};
+        }
+    }
+    return best;
 }
 
-// Whether an operand's 16-byte units can be loaded straight into LDS: rows on 16 bytes, and, where
-// it is not k-major, no unit across its last row.
-bool is_aligned(const void* p, int64_t ld, bool k_major, int64_t rows, int dtype) {
+// Whether an operand's 16-byte units can be loaded straight into LDS: rows on 16 bytes and no unit
+// across the last k (k-major) or the last row.
+bool is_aligned(const void* p, int64_t ld, int64_t extent, int dtype) {
     const int64_t unit = dtype == HBT_DTYPE_F32 ? 4 : 8;
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % unit == 0 && (k_major || rows % unit == 0);
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % unit == 0 && extent % unit == 0;
 }
 
 template <int D, bool kA, bool kB, class T, bool kAsync>
@@ -322,7 +325,7 @@ int32_t launch_tile(const char* who, ProductArgs& p, int splits, hipStream_t str
 template <int D, bool kA, bool kB>
 int32_t launch_product(const char* who, ProductArgs& p, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
     constexpr int BK = tile_k<D>();
-    const bool aligned = is_aligned(p.a, p.lda, kA, p.m, D) && is_aligned(p.b, p.ldb, kB, p.n, D);
+    const bool aligned = is_aligned(p.a, p.lda, kA ? p.k : p.m, D) && is_aligned(p.b, p.ldb, kB ? p.k : p.n, D);
     Choice c = choose(p.m, p.n, p.k, D, aligned);
     p.ldp = (p.n + 3) / 4 * 4;
     while (c.splits > 1 && 4 * c.splits * p.m * p.ldp > workspace_bytes) --c.splits;

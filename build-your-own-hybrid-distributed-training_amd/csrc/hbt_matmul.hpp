@@ -134,7 +134,7 @@ constexpr uint32_t kNowhere = 0xFFFFFF00u;
 // One operand's share of a tile: ROWS rows (m or n) by tile_k of k, moved by THREADS lanes.
 // kKMajor: element (row, k) at base[row * ld + k]; else at base[k * ld + row].
 // kAsync: rows and base on 16 bytes, and whole units (the rows of an operand that is not
-// k-major a multiple of a unit, or padded to one).
+// k-major, or the k of one that is, a multiple of a unit or padded to one, the k with zeros).
 template <int D, bool kKMajor, int ROWS, int THREADS, bool kAsync>
 struct Operand {
     static constexpr int E = unit_elems<D>(), BK = tile_k<D>(), B = elem_bytes<D>();
@@ -192,10 +192,12 @@ struct Operand {
         }
     }
 
-    // The whole k-tile at k0 into the LDS stage at byte address `lds`, without waiting: kUnits
-    // loads a wave.  They are written as assembly because the compiler makes every LDS read wait
-    // for all such loads; they have no register results, and wait_loads() below waits for them.
-    __device__ __forceinline__ void load_async(int64_t k0, uint32_t lds, int wave) const {
+    // The k-tile at k0 into the LDS stage at byte address `lds`, without waiting: kUnits loads a wave.
+    // Of the last k-tile only `left` values of k exist; other calls have kWhole.  The loads are
+    // written as assembly because the compiler makes every LDS read wait for all such loads; they
+    // have no register results, and wait_loads() below waits for them.
+    template <bool kWhole>
+    __device__ __forceinline__ void load_async(int64_t k0, int64_t left, uint32_t lds, int tid, int wave) const {
         const uint64_t at_k = reinterpret_cast<uint64_t>(base + (kKMajor ? k0 : k0 * ld) * B);
         const u32x4 buffer = {static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at_k))),
                               static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at_k >> 32))),
@@ -203,8 +205,13 @@ struct Operand {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (i * THREADS + wave * 64) * 16);
+            uint32_t from = offset[i];
+            if constexpr (!kWhole) {
+                const int u = i * THREADS + tid;
+                if (!(kKMajor ? column(u) * E < left : u / kUnitsPerLine < left)) from = kNowhere;
+            }
             asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :: "s"(to), "v"(offset[i]), "s"(buffer) : "memory");  // nothing else here uses m0
+                         :: "s"(to), "v"(from), "s"(buffer) : "memory");  // nothing else here uses m0
         }
     }
 
@@ -324,7 +331,8 @@ __device__ __forceinline__ void interleave() {
 
 // Forms the tile at rows m0 of A and n0 of B over k in [k0, k1) into acc: acc[i][j] holds, in
 // lane l, element m = 16 i + l % 16, n = 16 j + 4 (l / 16) + r (r = 0..3) of the wave's part.
-// A partial k-tile comes first and goes through registers, so that the loop moves whole ones.
+// A partial k-tile comes last among asynchronous loads, so that the others start on whole units,
+// and first among those through registers, whose loop then moves whole ones.
 template <int D, bool kA, bool kB, class T, bool kAsync>
 __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t m0, int64_t m_count, const void* b,
                                              int64_t ldb, int64_t n0, int64_t n_count, int64_t k0, int64_t k1,
@@ -344,26 +352,23 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
     oa.init(a, lda, m0, m_count, tid);
     ob.init(b, ldb, n0, n_count, tid);
     const int tiles = static_cast<int>((k1 - k0 + BK - 1) / BK);
-    const int part = static_cast<int>((k1 - k0) % BK);
     int64_t k = k0;  // the next k-tile to load
     if constexpr (kAsync) {
         constexpr int kLoads = OpA::kUnits + OpB::kUnits, kAhead = T::kStages - 1;
         const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
             (__attribute__((address_space(3))) char*)lds));
         const auto issue = [&](int stage) {
-            oa.load_async(k, at + stage * T::kStageBytes, wave);
-            ob.load_async(k, at + stage * T::kStageBytes + OpA::kBytes, wave);
+            const uint32_t to_a = at + stage * T::kStageBytes, to_b = to_a + OpA::kBytes;
+            if (k1 - k >= BK) {
+                oa.template load_async<true>(k, BK, to_a, tid, wave);
+                ob.template load_async<true>(k, BK, to_b, tid, wave);
+            } else {
+                oa.template load_async<false>(k, k1 - k, to_a, tid, wave);
+                ob.template load_async<false>(k, k1 - k, to_b, tid, wave);
+            }
             k += BK;
         };
-        if (part != 0) {
-            oa.load_part(k, part, tid);
-            ob.load_part(k, part, tid);
-            oa.store(lds, tid);
-            ob.store(lds + OpA::kBytes, tid);
-            k += part;
-        } else {
-            issue(0);
-        }
+        issue(0);
 #pragma unroll
         for (int s = 1; s <= kAhead; ++s)
             if (s < tiles) issue(s);
@@ -412,6 +417,7 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
             interleave<kReadsA + kReadsB, kMmas>();
         }
     } else {
+        const int part = static_cast<int>((k1 - k0) % BK);
         if (part != 0) {
             oa.load_part(k, part, tid);
             ob.load_part(k, part, tid);
@@ -538,6 +544,27 @@ __device__ __forceinline__ void band_order(int t, int tiles_m, int tiles_n, int&
     const int height = min(tiles_m - first, kBand), within = t - band * width;
     m = first + within % height;
     n = within / height;
+}
+
+// ---- the choice of a tile ---------------------------------------------------------------
+using Tile256 = Tile<256, 256, 2, 4, 2>;
+using Tile128 = Tile<128, 128, 2, 2, 2>;
+using Tile64 = Tile<64, 64, 2, 2, 4>;
+
+// An estimate, in microseconds, of `tiles` workgroups of `size` x `size` results with `steps`
+// k-tiles each: rounds of the device times a round's length.  Larger tiles read less per product
+// (bf16, 4096^3: 108 us in tiles of 256, 124 of 128, 206 of 64); smaller ones fill the device
+// with less, and a CU's two workgroups of 128 or 64 hide each other's first loads and stores
+// (2048 x 768 by 768: 27, 14 and 9 us).  `fixed`: what a round costs beside its k-tiles.
+// Round lengths are fitted to such measurements over 17 shapes (256 CUs, one workgroup of 256 or
+// two of the others a CU), within about a fifth.
+inline double round_cost(int size, int64_t tiles, double steps, bool f32, double fixed) {
+    constexpr int64_t kCus = 256;
+    if (size == 256) return static_cast<double>((tiles + kCus - 1) / kCus) * (steps * 1.5 + fixed);
+    const bool alone = tiles <= kCus;  // one workgroup a CU has the matrix cores for itself
+    const double step = size == 128 ? (f32 ? (alone ? 2.25 : 3.75) : (alone ? 0.7 : 0.98))
+                                    : (f32 ? (alone ? 0.7 : 1.1) : 0.41);
+    return static_cast<double>((tiles + 2 * kCus - 1) / (2 * kCus)) * (steps * step + fixed);
 }
 
 }  // namespace mm

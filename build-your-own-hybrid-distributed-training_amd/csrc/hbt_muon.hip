@@ -12,9 +12,9 @@
 // to 16 bits would be amplified by 3.4 a step in the directions that start small: on matrices with
 // a decaying spectrum fp16 products then end 6e-3 to 9e-3 off, and 3e-4 to 2e-3 with x in 32.
 //
-// Every phase takes all matrices of one orientation in one launch: the tiles of up to 32
+// Every phase takes all matrices in one launch: the tiles of up to 32
 // matrices of any sizes, found in a table in the launch's arguments.
-#include <numeric>
+#include <tuple>
 
 #include "hbt_matmul.hpp"
 
@@ -80,7 +80,8 @@ __global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
         const uint32_t local = unit0 + k * 256 + threadIdx.x, down = local / units;
         const int64_t row = row0 + down;
         const int col = static_cast<int>(local - down * units) * 4;
-        have[k] = row < t.rows ? static_cast<int>(min<int64_t>(t.cols - col, 4)) : 0;
+        // at most 0 in a row's padding, whose directions are zero; -8 past the last row
+        have[k] = row < t.rows ? static_cast<int>(min<int64_t>(t.cols - col, 4)) : -8;
         at[k] = row * t.cols + col;
         to[k] = row * t.ld + col;
         if (have[k] > 0) {
@@ -91,7 +92,10 @@ __global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-        if (have[k] <= 0) continue;
+        if (have[k] <= 0) {
+            if (have[k] > -8) *reinterpret_cast<f32x4*>(t.u + to[k]) = f32x4{0.f, 0.f, 0.f, 0.f};
+            continue;
+        }
         f32x4 u = g[k] * p.unscale * mul;
         if (t.v != nullptr) {
 #pragma unroll
@@ -101,10 +105,12 @@ __global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
             }
             store_row<HBT_DTYPE_F32>(t.v, at[k], have[k], v[k]);
         }
-        *reinterpret_cast<f32x4*>(t.u + to[k]) = u;  // past the last column: padding
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < have[k]) sum += double(u[e]) * double(u[e]);
+        for (int e = 0; e < 4; ++e) {
+            if (e >= have[k]) u[e] = 0.0f;
+            sum += double(u[e]) * double(u[e]);
+        }
+        *reinterpret_cast<f32x4*>(t.u + to[k]) = u;
     }
     const double total = block_sum<256>(sum);
     if (threadIdx.x == 0) t.partial[chunk] = total;
@@ -220,8 +226,10 @@ __device__ __forceinline__ auto by_dtype(int dtype, F&& f) {
     return f(std::integral_constant<int, HBT_DTYPE_F16>{});
 }
 
-// kWide: rows <= columns, so A = x x^T and x' = a x + B x; else A = x^T x and x' = a x + x B.
-template <int D, class T, Phase kPhase, bool kWide>
+// A wide matrix (rows <= columns) has A = x x^T and x' = a x + B x, a tall one A = x^T x and
+// x' = a x + x B.  Every array's rows are padded to 16 bytes with zeros: the products of zeros
+// keep the padding zero.
+template <int D, class T, Phase kPhase>
 __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductArgs p) {
     extern __shared__ __align__(16) char lds[];
     // Matrices of one shape share a run of workgroups, which starts at a multiple of 8: each XCD
@@ -231,7 +239,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
     if (local >= run.count * run.tiles) return;
     const int global = xcd_tile(local, run.count * run.tiles);
     const Problem& t = p.problem[run.first + global / run.tiles];
-    const int tile = global % run.tiles, side = kWide ? t.rows : t.cols;
+    const bool wide = t.rows <= t.cols;
+    const int tile = global % run.tiles, side = wide ? t.rows : t.cols;
     const int ldg = (side + 7) / 8 * 8;
     int tm, tn;
     constexpr bool kProduct = kPhase == kIterate || kPhase == kFinish;
@@ -246,12 +255,13 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
     const int m0 = tm * T::BM, n0 = tn * T::BN;
     f32x4 acc[T::TM][T::TN];
     if constexpr (kPhase == kGram) {
-        // Columns past the last one are padding of x's rows: read, never stored.
-        const int count = kWide ? side : t.ldx, k = kWide ? t.cols : t.rows;
-        tile_product<D, kWide, kWide, T, true>(t.x, t.ldx, m0, count, t.x, t.ldx, n0, count, 0, k, lds, acc);
+        if (wide)
+            tile_product<D, true, true, T, true>(t.x, t.ldx, m0, side, t.x, t.ldx, n0, side, 0, t.cols, lds, acc);
+        else
+            tile_product<D, false, false, T, true>(t.x, t.ldx, m0, t.ldx, t.x, t.ldx, n0, t.ldx, 0, t.rows, lds, acc);
     } else if constexpr (kPhase == kSquare) {
         tile_product<D, true, true, T, true>(t.gram, ldg, m0, side, t.gram, ldg, n0, side, 0, side, lds, acc);
-    } else if constexpr (kWide) {
+    } else if (wide) {
         tile_product<D, true, false, T, true>(t.poly, ldg, m0, side, t.x, t.ldx, n0, t.ldx, 0, side, lds, acc);
     } else {
         tile_product<D, true, true, T, true>(t.x, t.ldx, m0, t.rows, t.poly, ldg, n0, side, 0, side, lds, acc);
@@ -305,7 +315,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
             });
         }
     } else {
-        const int rows = side - m0, cols = side - n0;
+        const int rows = side - m0, cols = side - n0, padded_rows = ldg - m0, padded_cols = ldg - n0;
         char* out = static_cast<char*>(kPhase == kGram ? t.gram : t.poly);
         char* direct = out + (int64_t(m0) * ldg + n0) * elem_bytes<D>();
         char* mirror = out + (int64_t(n0) * ldg + m0) * elem_bytes<D>();
@@ -315,16 +325,17 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
             lds, acc,
             [&](int i, int j) {
                 if constexpr (kPhase == kGram) return f32x4{0.f, 0.f, 0.f, 0.f};
-                else return load4<D>(gram, min(i, rows - 1) * ldg + min(j, ldg - n0 - 4));
+                else return load4<D>(gram, min(i, rows - 1) * ldg + min(j, padded_cols - 4));
             },
             [&](int i, int j, f32x4 v, f32x4 l) {
                 v = kPhase == kGram ? v * t.gram_scale : l * p.b + v * p.c;
-                if (i < rows && j < cols) store4<D>(direct, i * ldg + j, v);
+                if (i >= rows) v = f32x4{0.f, 0.f, 0.f, 0.f};  // the mirror image's padding
+                if (i < rows && j < padded_cols) store4<D>(direct, i * ldg + j, v);
                 return v;
             },
             tm != tn,
             [&](int j, int i, f32x4 v) {
-                if (j < cols && i < rows) store4<D>(mirror, j * ldg + i, v);
+                if (j < cols && i < padded_rows) store4<D>(mirror, j * ldg + i, v);
             });
     }
 }
@@ -454,10 +465,6 @@ __global__ __launch_bounds__(512) void small_kernel(SmallArgs p) {
 }
 
 // ---- host ----------------------------------------------------------------------------
-using Tile256 = Tile<256, 256, 2, 4, 2>;
-using Tile128 = Tile<128, 128, 2, 2, 2>;
-using Tile64 = Tile<64, 64, 2, 2, 4>;
-
 struct Plan {
     int64_t u, low, x0, x1, gram, poly, partial, factor, end;  // offsets of one matrix's storage
     int64_t chunks, ldx, ldg;
@@ -521,7 +528,7 @@ int64_t tiles_of(const Problem& t, int size, Phase phase) {
     return s * (s + 1) / 2;
 }
 
-template <int D, class T, Phase kPhase, bool kWide>
+template <int D, class T, Phase kPhase>
 int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t stream) {
     constexpr int kLds = lds_bytes<T, true>();
     int64_t blocks = 0;
@@ -534,7 +541,7 @@ int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t
         p.blocks.first[r] = static_cast<int>(blocks);
         blocks += (int64_t(n) * p.run[r].tiles + 7) / 8 * 8;
     }
-    const auto kernel = newton_schulz_kernel<D, T, kPhase, kWide>;
+    const auto kernel = newton_schulz_kernel<D, T, kPhase>;
     if constexpr (kLds > 65536) {
         static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
@@ -544,19 +551,32 @@ int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t
     return check_launch(who);
 }
 
-template <int D, Phase kPhase, bool kWide>
+template <int D, Phase kPhase>
 int32_t launch_phase(const char* who, ProductArgs& p, hipStream_t stream) {
     if (p.count == 0) return HBT_OK;
-    int64_t tiles256 = 0, tiles128 = 0;
-    for (int i = 0; i < p.count; ++i) {
-        tiles256 += tiles_of(p.problem[i], 256, kPhase);
-        tiles128 += tiles_of(p.problem[i], 128, kPhase);
+    int best = 64;
+    double least = 0.0;
+    for (const int size : {64, 128, 256}) {
+        if (size == 256 && D == HBT_DTYPE_F32) continue;
+        int64_t tiles = 0;
+        double steps = 0.0;
+        for (int i = 0; i < p.count; ++i) {
+            const Problem& t = p.problem[i];
+            const int64_t count = tiles_of(t, size, kPhase);
+            const int k = kPhase == kGram ? std::max(t.rows, t.cols) : std::min(t.rows, t.cols);
+            tiles += count;
+            steps += static_cast<double>(count) * k / tile_k<D>();
+        }
+        // Mirror images, and the reads and writes of the iterate, make rounds longer than a layer's.
+        const double cost = round_cost(size, tiles, steps / tiles, D == HBT_DTYPE_F32,
+                                       size == 256 ? 20.0 : (size == 128 ? 13.0 : 4.0));
+        if (least == 0.0 || cost < least) least = cost, best = size;
     }
     if constexpr (D != HBT_DTYPE_F32) {
-        if (tiles256 >= 256) return launch_phase_tile<D, Tile256, kPhase, kWide>(who, p, 256, stream);
+        if (best == 256) return launch_phase_tile<D, Tile256, kPhase>(who, p, 256, stream);
     }
-    if (tiles128 >= 256) return launch_phase_tile<D, Tile128, kPhase, kWide>(who, p, 128, stream);
-    return launch_phase_tile<D, Tile64, kPhase, kWide>(who, p, 64, stream);
+    if (best == 128) return launch_phase_tile<D, Tile128, kPhase>(who, p, 128, stream);
+    return launch_phase_tile<D, Tile64, kPhase>(who, p, 64, stream);
 }
 
 // The small matrices of a call, all in one launch.
@@ -594,22 +614,16 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
             ProductArgs& common, int steps, double eps, char* workspace, hipStream_t stream) {
     NormArgs norm{};
     StartArgs start{};
-    ProductArgs wide = common, tall = common;
-    wide.count = tall.count = 0;
+    // Longest sums first, so that a launch's last workgroups are its shortest: over the longer
+    // sides for the Gram products, over the shorter ones for the others.
+    ProductArgs by_length = common, by_side = common;
+    by_length.count = by_side.count = 0;
     norm.eps = eps;
     direction.blocks.clear();
     start.blocks.clear();
-    // Longest sums first: a launch's last workgroups are then its shortest.
-    int order[kMaxMatrices];
-    std::iota(order, order + t.count, 0);
-    std::stable_sort(order, order + t.count, [&](int i, int j) {
-        const int64_t a = std::max(t.rows[i], t.cols[i]), b = std::max(t.rows[j], t.cols[j]);
-        return a != b ? a > b : t.rows[i] * t.cols[i] > t.rows[j] * t.cols[j];
-    });
     int64_t at = 0, direction_blocks = 0, start_blocks = 0;
     int n = 0;
-    for (int k = 0; k < t.count; ++k) {
-        const int i = order[k];
+    for (int i = 0; i < t.count; ++i) {
         const int64_t rows = t.rows[i], cols = t.cols[i];
         if (rows == 0 || cols == 0 || is_small(rows, cols)) continue;
         const int kind = product_of(rows, cols, product);
@@ -629,11 +643,10 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
         start.blocks.first[n] = static_cast<int>(start_blocks);
         start_blocks += (rows * (plan.ldx / 4) + 1023) / 1024;
         ++n;
-        ProductArgs& group = rows <= cols ? wide : tall;
-        group.problem[group.count++] = {workspace + plan.x0, workspace + plan.x1, workspace + plan.gram,
-                                        workspace + plan.poly, low, t.outs[i], static_cast<int>(rows),
-                                        static_cast<int>(cols), static_cast<int>(plan.ldx), 1.0f / (scale * scale),
-                                        (t.scales == nullptr ? 1.0f : t.scales[i]) / scale};
+        by_length.problem[by_length.count++] = {
+            workspace + plan.x0, workspace + plan.x1, workspace + plan.gram, workspace + plan.poly, low, t.outs[i],
+            static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(plan.ldx), 1.0f / (scale * scale),
+            (t.scales == nullptr ? 1.0f : t.scales[i]) / scale};
     }
     if (n == 0) return HBT_OK;
     const dim3 direction_grid(static_cast<unsigned>(direction_blocks));
@@ -646,24 +659,26 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
     if ((status = check_launch(who)) != HBT_OK) return status;
     start_kernel<D><<<dim3(static_cast<unsigned>(start_blocks)), 256, 0, stream>>>(start);
     if ((status = check_launch(who)) != HBT_OK) return status;
+    std::copy_n(by_length.problem, n, by_side.problem);
+    by_side.count = n;
+    const auto sort = [](ProductArgs& p, auto&& key) {
+        std::sort(p.problem, p.problem + p.count, [&](const Problem& a, const Problem& b) {
+            return std::make_tuple(-key(a), a.rows, a.cols, a.x) < std::make_tuple(-key(b), b.rows, b.cols, b.x);
+        });
+    };
+    sort(by_length, [](const Problem& t) { return std::max(t.rows, t.cols); });
+    sort(by_side, [](const Problem& t) { return std::min(t.rows, t.cols); });
     for (int s = 0; s < steps; ++s) {
-        if ((status = launch_phase<D, kGram, true>(who, wide, stream)) != HBT_OK ||
-            (status = launch_phase<D, kGram, false>(who, tall, stream)) != HBT_OK ||
-            (status = launch_phase<D, kSquare, true>(who, wide, stream)) != HBT_OK ||
-            (status = launch_phase<D, kSquare, false>(who, tall, stream)) != HBT_OK)
+        if ((status = launch_phase<D, kGram>(who, by_length, stream)) != HBT_OK ||
+            (status = launch_phase<D, kSquare>(who, by_side, stream)) != HBT_OK)
             return status;
-        if (s + 1 == steps) {
-            status = launch_phase<D, kFinish, true>(who, wide, stream);
-            return status != HBT_OK ? status : launch_phase<D, kFinish, false>(who, tall, stream);
-        }
-        if ((status = launch_phase<D, kIterate, true>(who, wide, stream)) != HBT_OK ||
-            (status = launch_phase<D, kIterate, false>(who, tall, stream)) != HBT_OK)
-            return status;
-        for (ProductArgs* g : {&wide, &tall})
-            for (int i = 0; i < g->count; ++i) {
-                const void* x = g->problem[i].x;
-                g->problem[i].x = g->problem[i].x_next;
-                g->problem[i].x_next = const_cast<void*>(x);
+        if (s + 1 == steps) return launch_phase<D, kFinish>(who, by_side, stream);
+        if ((status = launch_phase<D, kIterate>(who, by_side, stream)) != HBT_OK) return status;
+        for (ProductArgs* p : {&by_length, &by_side})
+            for (int i = 0; i < n; ++i) {
+                const void* x = p->problem[i].x;
+                p->problem[i].x = p->problem[i].x_next;
+                p->problem[i].x_next = const_cast<void*>(x);
             }
     }
     return HBT_OK;
