@@ -212,6 +212,7 @@ struct SlopeArgs {
     const void* z;
     void* dz;
     float* partial;  // [row blocks][ldp] column sums, or null
+    void* dbias;     // or the sums of the only block
     int64_t lddy, ldz, lddz, ldp, m, n;
     int rows_per_block, act;
 };
@@ -248,12 +249,13 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs p) {
             }
         }
     }
-    if (p.partial == nullptr) return;
+    if (p.partial == nullptr && p.dbias == nullptr) return;
     sums[wave][lane] = sum;
     __syncthreads();
     if (wave == 0 && j < p.n) {
         sum = ((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane];
-        *reinterpret_cast<f32x4*>(p.partial + blockIdx.y * p.ldp + j) = sum;  // ldp: a multiple of 4
+        if (p.dbias != nullptr) store_row<D>(p.dbias, j, static_cast<int>(min<int64_t>(p.n - j, 4)), sum);
+        else *reinterpret_cast<f32x4*>(p.partial + blockIdx.y * p.ldp + j) = sum;  // ldp: a multiple of 4
     }
 }
 
@@ -271,6 +273,59 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* partial, int64_t
     __syncthreads();
     if (wave == 0 && j < n)
         store_elem<D>(db, j, ((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]);
+}
+
+// ---- small layers ----------------------------------------------------------------------
+// A layer whose three sizes are at most 64 has its whole backward pass in one workgroup and one
+// launch (the parts above are four, and such a pass is launch latency): dz, x and W in LDS in
+// fp32, a lane per result.
+constexpr int kSmall = 64, kSmallLd = kSmall + 1;
+inline bool is_small(int64_t tokens, int64_t inner, int64_t outer) {
+    return tokens > 0 && inner > 0 && outer > 0 && tokens <= kSmall && inner <= kSmall && outer <= kSmall;
+}
+
+struct SmallArgs {
+    const void *dy, *x, *w, *z;
+    void *dx, *dw, *dbias;
+    int lddy, ldx, ldw, ldz, lddx, lddw, tokens, inner, outer, act;
+};
+
+template <int D>
+__global__ __launch_bounds__(512) void small_backward_kernel(SmallArgs p) {
+    __shared__ float dz[kSmall * kSmallLd], x[kSmall * kSmallLd], w[kSmall * kSmallLd];
+    const int tid = threadIdx.x;
+    for (int i = tid; i < p.tokens * p.outer; i += 512) {
+        const int t = i / p.outer, o = i % p.outer;
+        float g = load_elem<D>(p.dy, int64_t(t) * p.lddy + o);
+        if (p.act != HBT_ACT_NONE) g *= slope<D>(load_elem<D>(p.z, int64_t(t) * p.ldz + o), p.act);
+        dz[t * kSmallLd + o] = g;
+    }
+    if (p.dw != nullptr)
+        for (int i = tid; i < p.tokens * p.inner; i += 512)
+            x[i / p.inner * kSmallLd + i % p.inner] = load_elem<D>(p.x, int64_t(i / p.inner) * p.ldx + i % p.inner);
+    if (p.dx != nullptr)
+        for (int i = tid; i < p.outer * p.inner; i += 512)
+            w[i / p.inner * kSmallLd + i % p.inner] = load_elem<D>(p.w, int64_t(i / p.inner) * p.ldw + i % p.inner);
+    __syncthreads();
+    if (p.dx != nullptr)
+        for (int i = tid; i < p.tokens * p.inner; i += 512) {
+            const int t = i / p.inner, k = i % p.inner;
+            float sum = 0.0f;
+            for (int o = 0; o < p.outer; ++o) sum = fmaf(dz[t * kSmallLd + o], w[o * kSmallLd + k], sum);
+            store_elem<D>(p.dx, int64_t(t) * p.lddx + k, sum);
+        }
+    if (p.dw != nullptr)
+        for (int i = tid; i < p.outer * p.inner; i += 512) {
+            const int o = i / p.inner, k = i % p.inner;
+            float sum = 0.0f;
+            for (int t = 0; t < p.tokens; ++t) sum = fmaf(dz[t * kSmallLd + o], x[t * kSmallLd + k], sum);
+            store_elem<D>(p.dw, int64_t(o) * p.lddw + k, sum);
+        }
+    if (p.dbias != nullptr && tid < p.outer) {
+        float sum = 0.0f;
+        for (int t = 0; t < p.tokens; ++t) sum += dz[t * kSmallLd + tid];
+        store_elem<D>(p.dbias, tid, sum);
+    }
 }
 
 // ---- host ----------------------------------------------------------------------------
@@ -427,7 +482,8 @@ BackwardSpace backward_space(int64_t tokens, int64_t inner, int64_t outer, int32
         b.lddz = (outer + unit - 1) / unit * unit;
         b.dz_bytes = (tokens * b.lddz * size + 255) / 256 * 256;
     }
-    if (wants & HBT_LINEAR_DBIAS) {
+    if (is_small(tokens, inner, outer)) return BackwardSpace{};
+    if ((wants & HBT_LINEAR_DBIAS) && tokens > rows_per_block(tokens, outer)) {
         const int64_t rows = rows_per_block(tokens, outer);
         b.shared_bytes = 4 * ((tokens + rows - 1) / rows) * ((outer + 3) / 4 * 4);
     }
@@ -529,21 +585,29 @@ int32_t hbt_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t
     const hipStream_t s = as_stream(stream);
     return by_dtype(dtype, [&](auto d) -> int32_t {
         constexpr int D = decltype(d)::value;
+        if (is_small(tokens, inner, outer)) {
+            if (wants == 0) return HBT_OK;
+            const auto i = [](int64_t v) { return static_cast<int>(v); };
+            small_backward_kernel<D><<<dim3(1), 512, 0, s>>>({dy, x, w, z, dx, dw, dbias, i(lddy), i(ldx), i(ldw), i(ldz),
+                                                              i(lddx), i(lddw), i(tokens), i(inner), i(outer), activation});
+            return check_launch(who);
+        }
         SlopeArgs p{};
         p.dy = dy, p.z = z, p.dz = space.dz_bytes > 0 ? workspace : nullptr;
         p.lddy = lddy, p.ldz = ldz, p.lddz = space.lddz, p.ldp = (outer + 3) / 4 * 4;
-        p.partial = dbias != nullptr ? reinterpret_cast<float*>(shared) : nullptr;
         p.m = tokens, p.n = outer, p.act = activation;
         int64_t blocks = 0;
         if (tokens > 0 && outer > 0 && (p.dz != nullptr || dbias != nullptr)) {
             p.rows_per_block = rows_per_block(tokens, outer);
             blocks = (tokens + p.rows_per_block - 1) / p.rows_per_block;
+            if (dbias != nullptr && blocks > 1) p.partial = reinterpret_cast<float*>(shared);
+            else p.dbias = dbias;
             slope_kernel<D><<<dim3(static_cast<unsigned>((outer + 255) / 256), static_cast<unsigned>(blocks)), 256, 0,
                               s>>>(p);
             const int32_t launched = check_launch(who);
             if (launched != HBT_OK) return launched;
         }
-        if (dbias != nullptr && outer > 0) {
+        if (dbias != nullptr && outer > 0 && blocks != 1) {
             bias_kernel<D><<<dim3(static_cast<unsigned>((outer + 63) / 64)), 256, 0, s>>>(
                 p.partial, p.ldp, static_cast<int>(blocks), dbias, outer);
             const int32_t launched = check_launch(who);

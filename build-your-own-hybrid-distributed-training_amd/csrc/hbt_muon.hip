@@ -45,8 +45,10 @@ __device__ __forceinline__ int find_entry(const FirstBlocks& blocks, int block) 
 struct DirectionEntry {
     const void* g;
     float* v;        // null: u is the input itself
-    float* u;        // fp32, [rows][ld]
     double* partial;
+    void* x;         // the first iterate in the product type, [rows][ld]
+    void* low;       // the rest of it beside fp16 values
+    const float* factor;
     int64_t rows, cols, ld;
 };
 struct DirectionArgs {
@@ -58,10 +60,20 @@ struct DirectionArgs {
     int nesterov;
 };
 
-// One pass over the gradients: the momentum, the direction, and its squares summed in fp64.
-// A lane takes four columns of a row at a time; gradients and momenta lie dense, at any
-// alignment, the directions on rows of whole 16-byte units.
-template <int GD>
+// The fp16 value of x and what it leaves, itself in fp16.
+__device__ __forceinline__ void split(f32x4 x, u32x2& high, u32x2& low) {
+    high = u32x2{pack2_rounded<HBT_DTYPE_F16>(x[0], x[1]), pack2_rounded<HBT_DTYPE_F16>(x[2], x[3])};
+    f32x4 left;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) left[e] = x[e] - f16_to_f32((high[e / 2] >> (16 * (e % 2))) & 0xFFFFu);
+    low = u32x2{pack2_rounded<HBT_DTYPE_F16>(left[0], left[1]), pack2_rounded<HBT_DTYPE_F16>(left[2], left[3])};
+}
+
+// Two passes over the gradients and momenta, which lie dense, at any alignment; a lane takes four
+// columns of a row at a time.  kNorm: v' is stored and the squares of u are summed in fp64.
+// Otherwise u is formed again from v', by the same operations, and x = factor u is stored on
+// padded rows: reading g and v' twice moves no more than storing u between the passes would.
+template <int GD, int D, bool kNorm>
 __global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
     const int block = blockIdx.x, entry = find_entry(p.blocks, block);
     const DirectionEntry& t = p.entry[entry];
@@ -71,6 +83,7 @@ __global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
     const uint32_t unit0 = static_cast<uint32_t>(first - row0 * units);
     const float mul = p.grad_mul != nullptr ? *p.grad_mul : 1.0f;
     const float mu = p.slot != nullptr ? p.slot[2] : p.momentum, rest = p.slot != nullptr ? p.slot[3] : p.rest;
+    const float factor = kNorm ? 0.0f : *t.factor;
     constexpr int kUnits = kChunk / 1024;
     int64_t at[kUnits], to[kUnits];
     int have[kUnits];
@@ -80,10 +93,11 @@ __global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
         const uint32_t local = unit0 + k * 256 + threadIdx.x, down = local / units;
         const int64_t row = row0 + down;
         const int col = static_cast<int>(local - down * units) * 4;
-        // at most 0 in a row's padding, whose directions are zero; -8 past the last row
+        // at most 0 in a row's padding, whose x is zero; -8 past the last row
         have[k] = row < t.rows ? static_cast<int>(min<int64_t>(t.cols - col, 4)) : -8;
         at[k] = row * t.cols + col;
         to[k] = row * t.ld + col;
+        g[k] = v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (have[k] > 0) {
             g[k] = load_row<GD>(t.g, at[k], have[k]);
             if (t.v != nullptr) v[k] = load_row<HBT_DTYPE_F32>(t.v, at[k], have[k]);
@@ -92,28 +106,32 @@ __global__ __launch_bounds__(256) void direction_kernel(DirectionArgs p) {
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-        if (have[k] <= 0) {
-            if (have[k] > -8) *reinterpret_cast<f32x4*>(t.u + to[k]) = f32x4{0.f, 0.f, 0.f, 0.f};
-            continue;
-        }
+        if (have[k] <= (kNorm ? 0 : -8)) continue;
         f32x4 u = g[k] * p.unscale * mul;
         if (t.v != nullptr) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[k][e] = mu * v[k][e] + rest * u[e];
+                if constexpr (kNorm) v[k][e] = mu * v[k][e] + rest * u[e];
                 u[e] = p.nesterov ? mu * v[k][e] + rest * u[e] : v[k][e];
             }
-            store_row<HBT_DTYPE_F32>(t.v, at[k], have[k], v[k]);
+            if constexpr (kNorm) store_row<HBT_DTYPE_F32>(t.v, at[k], have[k], v[k]);
         }
+        if constexpr (kNorm) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (e >= have[k]) u[e] = 0.0f;
-            sum += double(u[e]) * double(u[e]);
+            for (int e = 0; e < 4; ++e) sum += double(u[e]) * double(u[e]);
+        } else if constexpr (D == HBT_DTYPE_F32) {
+            *reinterpret_cast<f32x4*>(static_cast<float*>(t.x) + to[k]) = u * factor;
+        } else {
+            u32x2 high, low;
+            split(u * factor, high, low);
+            *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(t.x) + to[k]) = high;
+            *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(t.low) + to[k]) = low;
         }
-        *reinterpret_cast<f32x4*>(t.u + to[k]) = u;
     }
-    const double total = block_sum<256>(sum);
-    if (threadIdx.x == 0) t.partial[chunk] = total;
+    if constexpr (kNorm) {
+        const double total = block_sum<256>(sum);
+        if (threadIdx.x == 0) t.partial[chunk] = total;
+    }
 }
 
 struct NormEntry {
@@ -143,53 +161,6 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
         const double norm = sqrt(total);
         const double floor = norm < p.eps ? p.eps : norm;  // a NaN norm stays one
         *t.factor = factor_of(t.scale, floor);
-    }
-}
-
-// The fp16 value of x and what it leaves, itself in fp16.
-__device__ __forceinline__ void split(f32x4 x, u32x2& high, u32x2& low) {
-    high = u32x2{pack2_rounded<HBT_DTYPE_F16>(x[0], x[1]), pack2_rounded<HBT_DTYPE_F16>(x[2], x[3])};
-    f32x4 left;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) left[e] = x[e] - f16_to_f32((high[e / 2] >> (16 * (e % 2))) & 0xFFFFu);
-    low = u32x2{pack2_rounded<HBT_DTYPE_F16>(left[0], left[1]), pack2_rounded<HBT_DTYPE_F16>(left[2], left[3])};
-}
-
-struct StartEntry {
-    const float* u;
-    void* x;
-    void* low;  // the rest of x beside fp16 values
-    const float* factor;
-    int64_t units;  // of four elements: whole rows with their padding
-};
-struct StartArgs {
-    FirstBlocks blocks;
-    StartEntry entry[kMaxMatrices];
-};
-
-// The first iterate in the product type.
-template <int D>
-__global__ __launch_bounds__(256) void start_kernel(StartArgs p) {
-    const int block = blockIdx.x, entry = find_entry(p.blocks, block);
-    const StartEntry& t = p.entry[entry];
-    const int64_t base = int64_t(block - p.blocks.first[entry]) * 1024 + threadIdx.x;
-    const float f = *t.factor;
-    f32x4 x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (base + k * 256 < t.units) x[k] = reinterpret_cast<const f32x4*>(t.u)[base + k * 256] * f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t i = base + k * 256;
-        if (i >= t.units) break;
-        if constexpr (D == HBT_DTYPE_F32) {
-            static_cast<f32x4*>(t.x)[i] = x[k];
-        } else {
-            u32x2 high, low;
-            split(x[k], high, low);
-            static_cast<u32x2*>(t.x)[i] = high;
-            static_cast<u32x2*>(t.low)[i] = low;
-        }
     }
 }
 
@@ -466,7 +437,7 @@ __global__ __launch_bounds__(512) void small_kernel(SmallArgs p) {
 
 // ---- host ----------------------------------------------------------------------------
 struct Plan {
-    int64_t u, low, x0, x1, gram, poly, partial, factor, end;  // offsets of one matrix's storage
+    int64_t low, x0, x1, gram, poly, partial, factor, end;  // offsets of one matrix's storage
     int64_t chunks, ldx, ldg;
 };
 
@@ -481,7 +452,6 @@ Plan plan_of(int64_t rows, int64_t cols, int product, int64_t at) {
     p.ldx = (cols + 7) / 8 * 8;
     p.ldg = (side + 7) / 8 * 8;
     p.chunks = (rows * p.ldx + kChunk - 1) / kChunk;
-    p.u = take(rows * p.ldx * 4);
     p.low = product == HBT_DTYPE_F32 ? at : take(rows * p.ldx * 2);
     p.x0 = take(rows * p.ldx * size);
     p.x1 = take(rows * p.ldx * size);
@@ -613,15 +583,13 @@ template <int D>
 int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t product, DirectionArgs& direction,
             ProductArgs& common, int steps, double eps, char* workspace, hipStream_t stream) {
     NormArgs norm{};
-    StartArgs start{};
     // Longest sums first, so that a launch's last workgroups are its shortest: over the longer
     // sides for the Gram products, over the shorter ones for the others.
     ProductArgs by_length = common, by_side = common;
     by_length.count = by_side.count = 0;
     norm.eps = eps;
     direction.blocks.clear();
-    start.blocks.clear();
-    int64_t at = 0, direction_blocks = 0, start_blocks = 0;
+    int64_t at = 0, direction_blocks = 0;
     int n = 0;
     for (int i = 0; i < t.count; ++i) {
         const int64_t rows = t.rows[i], cols = t.cols[i];
@@ -631,17 +599,14 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
         at = plan.end;
         if (kind != D) continue;
         const float scale = iterate_scale(rows, cols, D);
-        float* u = reinterpret_cast<float*>(workspace + plan.u);
         void* low = D == HBT_DTYPE_F32 ? nullptr : workspace + plan.low;
         float* factor = reinterpret_cast<float*>(workspace + plan.factor);
         double* partial = reinterpret_cast<double*>(workspace + plan.partial);
-        direction.entry[n] = {t.grads[i], t.momenta == nullptr ? nullptr : t.momenta[i], u, partial, rows, cols, plan.ldx};
+        direction.entry[n] = {t.grads[i], t.momenta == nullptr ? nullptr : t.momenta[i], partial, workspace + plan.x0, low,
+                              factor, rows, cols, plan.ldx};
         direction.blocks.first[n] = static_cast<int>(direction_blocks);
         direction_blocks += plan.chunks;
         norm.entry[n] = {partial, factor, plan.chunks, scale};
-        start.entry[n] = {u, workspace + plan.x0, low, factor, rows * (plan.ldx / 4)};
-        start.blocks.first[n] = static_cast<int>(start_blocks);
-        start_blocks += (rows * (plan.ldx / 4) + 1023) / 1024;
         ++n;
         by_length.problem[by_length.count++] = {
             workspace + plan.x0, workspace + plan.x1, workspace + plan.gram, workspace + plan.poly, low, t.outs[i],
@@ -649,16 +614,18 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
             (t.scales == nullptr ? 1.0f : t.scales[i]) / scale};
     }
     if (n == 0) return HBT_OK;
-    const dim3 direction_grid(static_cast<unsigned>(direction_blocks));
-    if (grad_dtype == HBT_DTYPE_F32) direction_kernel<HBT_DTYPE_F32><<<direction_grid, 256, 0, stream>>>(direction);
-    else if (grad_dtype == HBT_DTYPE_BF16) direction_kernel<HBT_DTYPE_BF16><<<direction_grid, 256, 0, stream>>>(direction);
-    else direction_kernel<HBT_DTYPE_F16><<<direction_grid, 256, 0, stream>>>(direction);
-    int32_t status = check_launch(who);
+    const dim3 grid(static_cast<unsigned>(direction_blocks));
+    const auto pass = [&](auto kNorm) {
+        constexpr bool norm_pass = decltype(kNorm)::value;
+        if (grad_dtype == HBT_DTYPE_F32) direction_kernel<HBT_DTYPE_F32, D, norm_pass><<<grid, 256, 0, stream>>>(direction);
+        else if (grad_dtype == HBT_DTYPE_BF16) direction_kernel<HBT_DTYPE_BF16, D, norm_pass><<<grid, 256, 0, stream>>>(direction);
+        else direction_kernel<HBT_DTYPE_F16, D, norm_pass><<<grid, 256, 0, stream>>>(direction);
+        return check_launch(who);
+    };
+    int32_t status = pass(std::true_type{});
     if (status != HBT_OK) return status;
     norm_kernel<<<dim3(n), 1024, 0, stream>>>(norm);
-    if ((status = check_launch(who)) != HBT_OK) return status;
-    start_kernel<D><<<dim3(static_cast<unsigned>(start_blocks)), 256, 0, stream>>>(start);
-    if ((status = check_launch(who)) != HBT_OK) return status;
+    if ((status = check_launch(who)) != HBT_OK || (status = pass(std::false_type{})) != HBT_OK) return status;
     std::copy_n(by_length.problem, n, by_side.problem);
     by_side.count = n;
     const auto sort = [](ProductArgs& p, auto&& key) {

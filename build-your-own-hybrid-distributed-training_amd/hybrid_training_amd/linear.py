@@ -127,42 +127,45 @@ class _FusedLinear(torch.autograd.Function):
         ctx.save_for_backward(x, weight, z)
         return y
 
+    # The backward pass runs on autograd's own thread, where host code is slower: it does as
+    # little as it can before its one call.
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
         want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if want_x or want_w or want_b:
-            outer, inner = weight.shape
-            device, dtype = x.device, x.dtype
-            g, ldg = _rows(dy, outer)
-            tokens = g.shape[0]
-            wants, xs, ws, ldx, ldw, across = 0, None, None, 0, 0, max(inner, 1)
-            if want_x:
-                wants |= _DX
-                ws, ldw = _rows(weight, inner)
-                dx = torch.empty(x.shape, dtype=dtype, device=device)
-            if want_w:
-                wants |= _DW
-                xs, ldx = _rows(x, inner)
-                dw = torch.empty((outer, inner), dtype=dtype, device=device)
-            if want_b:
-                wants |= _DBIAS
-                db = torch.empty(outer, dtype=dtype, device=device)
-            code, activation = _native.dtype_code(dtype), ACTIVATIONS[ctx.activation]
-            lib = _native.library()
-            with _native.device_guard(device):
-                nbytes = lib.hbt_linear_backward_workspace(tokens, inner, outer, code, activation, wants)
-                space, address = _workspace(nbytes, device)
-                status = lib.hbt_linear_backward(
-                    g.data_ptr(), ldg, None if xs is None else xs.data_ptr(), ldx,
-                    None if ws is None else ws.data_ptr(), ldw, None if z is None else z.data_ptr(), max(outer, 1),
-                    None if dx is None else dx.data_ptr(), across, None if dw is None else dw.data_ptr(), across,
-                    None if db is None else db.data_ptr(), tokens, inner, outer, code, activation, address, nbytes,
-                    _native.stream_of(device))
-            if status:
-                _native.check(status, "linear.hbt_linear_backward")
+        if not (want_x or want_w or want_b):
+            return None, None, None, dy if want_r else None, None
+        x, weight, z = ctx.saved_tensors
+        outer, inner = weight.shape
+        device, dtype, across = x.device, x.dtype, max(inner, 1)
+        g, ldg = _rows(dy, outer)
+        tokens = g.shape[0]
+        wants, ldx, ldw = 0, 0, 0
+        xs = ws = dx = dw = db = x_at = w_at = dx_at = dw_at = db_at = None
+        if want_x:
+            wants = _DX
+            ws, ldw = _rows(weight, inner)
+            dx = torch.empty(x.shape, dtype=dtype, device=device)
+            w_at, dx_at = ws.data_ptr(), dx.data_ptr()
+        if want_w:
+            wants |= _DW
+            xs, ldx = _rows(x, inner)
+            dw = torch.empty(weight.shape, dtype=dtype, device=device)
+            x_at, dw_at = xs.data_ptr(), dw.data_ptr()
+        if want_b:
+            wants |= _DBIAS
+            db = torch.empty(outer, dtype=dtype, device=device)
+            db_at = db.data_ptr()
+        code, activation = _native.dtype_code(dtype), ACTIVATIONS[ctx.activation]
+        lib = _native.library()
+        with _native.device_guard(device):
+            nbytes = lib.hbt_linear_backward_workspace(tokens, inner, outer, code, activation, wants)
+            space, address = _workspace(nbytes, device)
+            status = lib.hbt_linear_backward(
+                g.data_ptr(), ldg, x_at, ldx, w_at, ldw, None if z is None else z.data_ptr(), max(outer, 1), dx_at, across,
+                dw_at, across, db_at, tokens, inner, outer, code, activation, address, nbytes, _native.stream_of(device))
+        if status:
+            _native.check(status, "linear.hbt_linear_backward")
         return dx, dw, db, dy if want_r else None, None
 
 

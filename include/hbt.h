@@ -667,8 +667,9 @@ int32_t hbt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const
  *   whose weight and bias gradients FlatParamHandle.reduce_scatter_gradient
  *   (parallel/fsdp.py:704-769) and the DDP buckets (parallel/ddp.py:513) take.
  * dx, dw and dbias may each be NULL, which leaves it out; z is read only with an activation,
- * w only for dx and x only for dw.  dz is rounded once to the dtype for the products; dbias
- * sums the unrounded values in a fixed order.  With tokens = 0, dw and dbias are 0.
+ * w only for dx and x only for dw.  dz is rounded once to the dtype for the products
+ * (not where tokens, inner and outer are at most 64); dbias sums the unrounded values in a
+ * fixed order.  With tokens = 0, dw and dbias are 0.
  * `workspace` (256-byte aligned) holds at least hbt_linear_backward_workspace's bytes for
  * these sizes and `wants`, the HBT_LINEAR_* of the results asked for (-1 for bad arguments).
  * Layouts, dtypes and limits are hbt_linear's.  No atomics: results repeat bitwise.
