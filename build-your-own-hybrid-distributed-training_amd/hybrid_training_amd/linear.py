@@ -36,7 +36,6 @@ _DX, _DW, _DBIAS = 1, 2, 4
 def _rows(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
     """``t`` as rows of ``cols`` consecutive elements and the distance between them: a view
     where its strides allow one, else a dense copy."""
-    t = t.detach()
     if t.dim() != 2:
         t = t.reshape(-1, cols) if cols else t.reshape(math.prod(t.shape[:-1]), 0)
     rows = t.shape[0]
@@ -60,6 +59,18 @@ def _workspace(nbytes: int, device: torch.device) -> tuple[torch.Tensor | None, 
 
 def _check(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
            activation: str) -> None:
+    dtype, device = x.dtype, x.device
+    if (activation in ACTIVATIONS and dtype in _DTYPES and x.is_cuda and weight.dim() == 2 and x.dim() > 0
+            and x.shape[-1] == weight.shape[1] and weight.dtype == dtype and weight.device == device
+            and (bias is None or (bias.shape == weight.shape[:1] and bias.dtype == dtype and bias.device == device))
+            and (residual is None or (residual.shape == x.shape[:-1] + weight.shape[:1] and residual.dtype == dtype
+                                      and residual.device == device))):
+        return
+    _refuse(x, weight, bias, residual, activation)
+
+
+def _refuse(x, weight, bias, residual, activation) -> None:
+    """Name what :func:`_check` found wrong."""
     who = "linear.fused_linear"
     if activation not in ACTIVATIONS:
         raise UnsupportedFeatureError(format_error(who, "unknown activation", expected=sorted(ACTIVATIONS),
@@ -76,18 +87,15 @@ def _check(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, res
     if residual is not None and residual.shape != (*x.shape[:-1], outer):
         raise ShardingError(format_error(who, "the residual must have the result's shape",
                                          expected=(*x.shape[:-1], outer), observed=tuple(residual.shape)))
-    for t in (x, weight, bias, residual):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            _native.require_device_tensor(t, who)
-        if t.dtype != x.dtype or t.dtype not in _DTYPES:
-            raise UnsupportedFeatureError(
-                format_error(who, "x, weight, bias and residual share one dtype of bfloat16, float16 or float32",
-                             observed=[str(v.dtype) for v in (x, weight, bias, residual) if v is not None]))
-        if t.device != x.device:
-            raise ShardingError(format_error(who, "x, weight, bias and residual must be on one device",
-                                             expected=str(x.device), observed=str(t.device)))
+    given = [t for t in (x, weight, bias, residual) if t is not None]
+    for t in given:
+        _native.require_device_tensor(t, who)
+    if x.dtype not in _DTYPES or any(t.dtype != x.dtype for t in given):
+        raise UnsupportedFeatureError(
+            format_error(who, "x, weight, bias and residual share one dtype of bfloat16, float16 or float32",
+                         observed=[str(t.dtype) for t in given]))
+    raise ShardingError(format_error(who, "x, weight, bias and residual must be on one device",
+                                     expected=str(x.device), observed=[str(t.device) for t in given]))
 
 
 def _forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
@@ -102,13 +110,13 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, r
     z = torch.empty((tokens, outer), dtype=x.dtype, device=x.device) if keep else None
     if tokens == 0 or outer == 0:
         return y, z
-    b = None if bias is None else bias.detach().contiguous()
+    b = None if bias is None else bias.contiguous()
     r, ldr = (None, 0) if residual is None else _rows(residual, outer)
     code = _native.dtype_code(x.dtype)
     device = x.device
     with _native.device_guard(device):
         lib = _native.library()
-        nbytes = lib.hbt_linear_workspace(tokens, inner, outer, code)
+        nbytes = lib.hbt_linear_workspace(tokens, inner, outer, code) if tokens > 16 else 0
         space, address = _workspace(nbytes, device)
         status = lib.hbt_linear(
             rows.data_ptr(), ldx, w.data_ptr(), ldw, None if b is None else b.data_ptr(),
@@ -179,7 +187,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     layouts through a dense copy.  ``activation`` is one of :data:`ACTIVATIONS`.
     """
     _check(x, weight, bias, residual, activation)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         return _FusedLinear.apply(x, weight, bias, residual, activation)
     return _forward(x, weight, bias, residual, activation, keep=False)[0]
 
