@@ -353,108 +353,97 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
     ob.init(b, ldb, n0, n_count, tid);
     const int tiles = static_cast<int>((k1 - k0 + BK - 1) / BK);
     int64_t k = k0;  // the next k-tile to load
+    constexpr int kStages = kAsync ? T::kStages : 2, kLoads = OpA::kUnits + OpB::kUnits, kAhead = kStages - 1;
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+    const auto issue = [&](int stage) {  // asynchronous
+        const uint32_t to_a = at + stage * T::kStageBytes, to_b = to_a + OpA::kBytes;
+        if (k1 - k >= BK) {
+            oa.template load_async<true>(k, BK, to_a, tid, wave);
+            ob.template load_async<true>(k, BK, to_b, tid, wave);
+        } else {
+            oa.template load_async<false>(k, k1 - k, to_a, tid, wave);
+            ob.template load_async<false>(k, k1 - k, to_b, tid, wave);
+        }
+        k += BK;
+    };
+    const auto load = [&]() {  // into registers
+        oa.load(k, tid);
+        ob.load(k, tid);
+        k += BK;
+    };
+    const auto store = [&](int stage) {
+        oa.store(lds + stage * T::kStageBytes, tid);
+        ob.store(lds + stage * T::kStageBytes + OpA::kBytes, tid);
+    };
     if constexpr (kAsync) {
-        constexpr int kLoads = OpA::kUnits + OpB::kUnits, kAhead = T::kStages - 1;
-        const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-            (__attribute__((address_space(3))) char*)lds));
-        const auto issue = [&](int stage) {
-            const uint32_t to_a = at + stage * T::kStageBytes, to_b = to_a + OpA::kBytes;
-            if (k1 - k >= BK) {
-                oa.template load_async<true>(k, BK, to_a, tid, wave);
-                ob.template load_async<true>(k, BK, to_b, tid, wave);
-            } else {
-                oa.template load_async<false>(k, k1 - k, to_a, tid, wave);
-                ob.template load_async<false>(k, k1 - k, to_b, tid, wave);
-            }
-            k += BK;
-        };
         issue(0);
 #pragma unroll
         for (int s = 1; s <= kAhead; ++s)
             if (s < tiles) issue(s);
-        const auto landed = [&](int t) {  // tile t is in LDS for every wave
-            if (t + kAhead <= tiles) wait_loads<kLoads * (kAhead - 1)>();
-            else wait_loads<0>();
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-        };
         if (kAhead < tiles) wait_loads<kLoads * kAhead>();
         else wait_loads<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        // Each k-tile is two steps of two halves of the wave's rows.  While one half's matrix
-        // instructions run, the fragments of the next are read: two sets of each operand's are held.
-        constexpr int kHalf = T::TM / 2, kReadsA = OpA::kReads * kHalf, kReadsB = OpB::kReads * T::TN;
-        constexpr int kMmas = kHalf * T::TN * (B == 4 ? 4 : 1);
-        u32x4 a0[kHalf], a1[kHalf], b0[T::TN], b1[T::TN];
-        read<OpB>(b0, lds + OpA::kBytes, wn, 0, lane);
-        read<OpA>(a0, lds, wm, 0, lane);
-        int stage = 0;
-        for (int t = 0; t < tiles; ++t) {
-            const char* now = lds + stage * T::kStageBytes;
-            read<OpA>(a1, now, wm + 16 * kHalf, 0, lane);
-            multiply<D, T, 0>(a0, b0, acc);
-            interleave<kReadsA, kMmas>();
-            read<OpB>(b1, now + OpA::kBytes, wn, 1, lane);
-            read<OpA>(a0, now, wm, 1, lane);
-            multiply<D, T, kHalf>(a1, b0, acc);
-            interleave<kReadsA + kReadsB, kMmas>();
-            read<OpA>(a1, now, wm + 16 * kHalf, 1, lane);
-            multiply<D, T, 0>(a0, b1, acc);
-            interleave<kReadsA, kMmas>();
-            if (t + 1 < tiles) {
-                // At most the kAhead - 1 tiles after t + 1 are in flight, so it has landed; past the
-                // barrier it has for every wave, and every wave holds the last of tile t, whose
-                // stage the next load takes.
-                landed(t + 1);
-                if (t + 1 + kAhead < tiles) issue(stage);
-                stage = stage + 1 == T::kStages ? 0 : stage + 1;
-                const char* next = lds + stage * T::kStageBytes;
-                read<OpB>(b0, next + OpA::kBytes, wn, 0, lane);
-                read<OpA>(a0, next, wm, 0, lane);
-            }
-            multiply<D, T, kHalf>(a1, b1, acc);
-            interleave<kReadsA + kReadsB, kMmas>();
-        }
     } else {
         const int part = static_cast<int>((k1 - k0) % BK);
         if (part != 0) {
             oa.load_part(k, part, tid);
             ob.load_part(k, part, tid);
+            k += part;
         } else {
-            oa.load(k, tid);
-            ob.load(k, tid);
+            load();
         }
-        k += part != 0 ? part : BK;
-        oa.store(lds, tid);
-        ob.store(lds + OpA::kBytes, tid);
-        if (tiles > 1) {
-            oa.load(k, tid);
-            ob.load(k, tid);
-        }
+        store(0);
+        if (tiles > 1) load();
         __syncthreads();
-        for (int t = 0; t < tiles; ++t) {
-            const char* now = lds + (t & 1) * T::kStageBytes;
-            char* next = lds + ((t & 1) ^ 1) * T::kStageBytes;
-            u32x4 fa[T::TM], fb[T::TN];
-            read<OpB>(fb, now + OpA::kBytes, wn, 0, lane);
-            read<OpA>(fa, now, wm, 0, lane);
-            multiply<D, T, 0>(fa, fb, acc);
+    }
+    // Each k-tile is two steps of two halves of the wave's rows.  While one half's matrix
+    // instructions run, the fragments of the next are read: two sets of each operand's are held.
+    constexpr int kHalf = T::TM / 2, kReadsA = OpA::kReads * kHalf, kReadsB = OpB::kReads * T::TN;
+    constexpr int kMmas = kHalf * T::TN * (B == 4 ? 4 : 1);
+    u32x4 a0[kHalf], a1[kHalf], b0[T::TN], b1[T::TN];
+    read<OpB>(b0, lds + OpA::kBytes, wn, 0, lane);
+    read<OpA>(a0, lds, wm, 0, lane);
+    int stage = 0;
+    for (int t = 0; t < tiles; ++t) {
+        const char* now = lds + stage * T::kStageBytes;
+        read<OpA>(a1, now, wm + 16 * kHalf, 0, lane);
+        multiply<D, T, 0>(a0, b0, acc);
+        interleave<kReadsA, kMmas>();
+        if constexpr (!kAsync) {
+            // Every wave has passed the barrier that ended the reads of the other stage.
             if (t + 1 < tiles) {
-                // Every wave has passed the barrier that ended the reads of this stage.
-                oa.store(next, tid);
-                ob.store(next + OpA::kBytes, tid);
-                if (t + 2 < tiles) {
-                    k += BK;
-                    oa.load(k, tid);
-                    ob.load(k, tid);
-                }
+                store(stage ^ 1);
+                if (t + 2 < tiles) load();
             }
-            read<OpB>(fb, now + OpA::kBytes, wn, 1, lane);
-            read<OpA>(fa, now, wm, 1, lane);
-            multiply<D, T, 0>(fa, fb, acc);
-            if (t + 1 < tiles) __syncthreads();
         }
+        read<OpB>(b1, now + OpA::kBytes, wn, 1, lane);
+        read<OpA>(a0, now, wm, 1, lane);
+        multiply<D, T, kHalf>(a1, b0, acc);
+        interleave<kReadsA + kReadsB, kMmas>();
+        read<OpA>(a1, now, wm + 16 * kHalf, 1, lane);
+        multiply<D, T, 0>(a0, b1, acc);
+        interleave<kReadsA, kMmas>();
+        if (t + 1 < tiles) {
+            if constexpr (kAsync) {
+                // At most the kAhead - 1 tiles after t + 1 are in flight, so it has landed; past the
+                // barrier it has for every wave, and every wave holds the last of tile t, whose
+                // stage the next load takes.
+                if (t + 1 + kAhead <= tiles) wait_loads<kLoads * (kAhead - 1)>();
+                else wait_loads<0>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (t + 1 + kAhead < tiles) issue(stage);
+            } else {
+                __syncthreads();
+            }
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+            const char* next = lds + stage * T::kStageBytes;
+            read<OpB>(b0, next + OpA::kBytes, wn, 0, lane);
+            read<OpA>(a0, next, wm, 0, lane);
+        }
+        multiply<D, T, kHalf>(a1, b1, acc);
+        interleave<kReadsA + kReadsB, kMmas>();
     }
     __syncthreads();  // the LDS is free
 }
@@ -562,8 +551,11 @@ inline double round_cost(int size, int64_t tiles, double steps, bool f32, double
     constexpr int64_t kCus = 256;
     if (size == 256) return static_cast<double>((tiles + kCus - 1) / kCus) * (steps * 1.5 + fixed);
     const bool alone = tiles <= kCus;  // one workgroup a CU has the matrix cores for itself
-    const double step = size == 128 ? (f32 ? (alone ? 2.25 : 3.75) : (alone ? 0.7 : 0.98))
-                                    : (f32 ? (alone ? 0.7 : 1.1) : 0.41);
+    if (f32) {  // the matrix cores are the bound: workgroups of a CU take turns
+        const double step = size == 128 ? (alone ? 2.25 : 1.87) : (alone ? 0.7 : 0.52);
+        return static_cast<double>((tiles + kCus - 1) / kCus) * steps * step + fixed;
+    }
+    const double step = size == 128 ? (alone ? 0.7 : 0.98) : 0.41;
     return static_cast<double>((tiles + 2 * kCus - 1) / (2 * kCus)) * (steps * step + fixed);
 }
 

@@ -15,7 +15,7 @@ parameter written by the last product's epilogue.
 The iterate, every sum and the momentum are float32 (the norm float64).  ``product_dtype``
 says what the products read: ``float16``, whose 11 bits leave the result about 2e-3 off its
 exact value (relative, in the Frobenius norm), or ``float32``.  Matrices whose shorter side is at
-most 64 take ``float32`` products either way.
+most 128 take ``float32`` products either way.
 """
 
 from __future__ import annotations

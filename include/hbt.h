@@ -706,7 +706,7 @@ int32_t hbt_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t
  * into a HIP graph.
  * Dtypes: F32, BF16 or F16 each.  Sums are held in fp32 and the norm in fp64; x is carried in
  * fp32.  The products read x, A and B rounded to product_dtype: F16, or F32; a matrix whose
- * shorter side is at most 64 takes F32 either way.  A non-finite
+ * shorter side is at most 128 takes F32 either way.  A non-finite
  * gradient makes its whole matrix non-finite.  No atomics: results repeat bitwise.
  * `workspace` (256-byte aligned) holds at least hbt_orthogonal_workspace's bytes for these
  * matrices (-1 for bad arguments).
