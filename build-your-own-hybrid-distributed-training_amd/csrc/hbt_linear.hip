@@ -156,14 +156,13 @@ __global__ __launch_bounds__(512) void thin_kernel(ProductArgs p) {
     const char* x = static_cast<const char*>(p.a) + ((x_in ? row : 0) * p.lda + q * E) * B;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     const int64_t whole = p.k / kStep;
-    int64_t s = wave;
-    for (; s + (kUnroll - 1) * kWaves < whole; s += kUnroll * kWaves) {
+    int64_t s = wave * kUnroll;  // kUnroll consecutive steps a turn: 256 bytes of each row
+    for (; s + kUnroll <= whole; s += kUnroll * kWaves) {
         u32x4 fw[kUnroll], fx[kUnroll];
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i) {
-            const int64_t at = (s + i * kWaves) * kStep * B;
-            fw[i] = load16(w + at);
-            fx[i] = load16(x + at);
+            fw[i] = load16(w + (s + i) * kStep * B);
+            fx[i] = load16(x + (s + i) * kStep * B);
         }
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i) {
@@ -171,7 +170,7 @@ __global__ __launch_bounds__(512) void thin_kernel(ProductArgs p) {
             acc = mma<D>(fw[i], fx[i], acc);
         }
     }
-    for (; s < whole; s += kWaves) {
+    for (; s < whole; ++s) {  // the one wave whose turn is cut short
         const u32x4 fw = load16(w + s * kStep * B);
         u32x4 fx = load16(x + s * kStep * B);
         if (!x_in) fx = u32x4{0, 0, 0, 0};
