@@ -151,6 +151,7 @@ struct Operand {
     uint32_t offset[kUnits];
     u32x4 held[kUnits];
     bool straddles;        // some lane's unit crosses the last row (not k-major)
+    bool shifted;          // ... and is loaded back from that row, to be shifted down
 
     // LDS position of a unit: lines are XOR-swizzled in units so that the 16 rows of a
     // fragment read (k-major), or the four k of a transposing read, fall on distinct banks.
@@ -172,12 +173,41 @@ struct Operand {
         rows = static_cast<int>(row_count - row0 < ROWS ? row_count - row0 : ROWS);
         base = static_cast<const char*>(p) + (kKMajor ? row0 * ld_ : row0) * B;
         straddles = !kAsync && !kKMajor && rows < ROWS && rows % E != 0;
+        shifted = straddles && row_count >= E;
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = column(u);
             const bool in = kKMajor ? line < rows : (at + 1) * E <= rows;
             offset[i] = in ? static_cast<uint32_t>(line * ld * B) + at * 16 : kNowhere;
+            if constexpr (!kAsync && !kKMajor) {
+                if (shifted && at == rows / E) offset[i] = static_cast<uint32_t>(line * ld * B) + (rows - E) * B;
+            }
         }
+        if constexpr (!kAsync && !kKMajor) {
+            // A tile of fewer rows than a unit's reaches back before its own first one.
+            if (shifted && rows < E) {
+                base -= E * B;
+#pragma unroll
+                for (int i = 0; i < kUnits; ++i) offset[i] += offset[i] == kNowhere ? 0 : E * B;
+            }
+        }
+    }
+
+    // v moved down by `bytes`, 2 to 14, zeros following.
+    static __device__ __forceinline__ u32x4 shift_down(u32x4 v, int bytes) {
+        const int words = bytes >> 2, bits = (bytes & 3) * 8;
+        u32x4 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uint32_t low = 0, high = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                if (e + words == w) low = v[w];
+                if (e + words + 1 == w) high = v[w];
+            }
+            r[e] = __builtin_amdgcn_alignbit(high, low, bits);
+        }
+        return r;
     }
 
     // The lane's units of the whole k-tile at k0.
@@ -188,7 +218,7 @@ struct Operand {
         for (int i = 0; i < kUnits; ++i)
             held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset[i], 0, 0));
         if constexpr (!kAsync && !kKMajor) {
-            if (straddles) load_edge(at_k, BK, tid);
+            if (straddles && !shifted) load_edge(at_k, BK, tid);
         }
     }
 
@@ -222,11 +252,11 @@ struct Operand {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = column(u);
-            const bool in = kKMajor ? (at + 1) * E <= left : line < left;
+            const bool in = kKMajor ? (at + 1) * E <= left : line < left;  // out of the rows: already nowhere
             held[i] = __builtin_bit_cast(
                 u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, in ? offset[i] : kNowhere, 0, 0));
         }
-        if (straddles || (kKMajor && left % E != 0)) load_edge(at_k, left, tid);
+        if ((straddles && !shifted) || (kKMajor && left % E != 0)) load_edge(at_k, left, tid);
     }
 
     // Units that cross the last row or the last k, element by element.
@@ -252,7 +282,14 @@ struct Operand {
         }
     }
 
-    __device__ __forceinline__ void store(char* lds, int tid) const {
+    __device__ __forceinline__ void store(char* lds, int tid) {
+        if constexpr (!kAsync && !kKMajor) {
+            if (shifted) {
+#pragma unroll
+                for (int i = 0; i < kUnits; ++i)
+                    if (column(i * THREADS + tid) == rows / E) held[i] = shift_down(held[i], 16 - rows % E * B);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const int u = i * THREADS + tid, line = u / kUnitsPerLine, at = column(u) ^ swizzle(line);

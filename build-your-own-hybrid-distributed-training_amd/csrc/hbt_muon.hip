@@ -253,7 +253,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
         if constexpr (kPhase == kIterate) {
             char* to_x = static_cast<char*>(t.x_next) + at * elem_bytes<D>();
             char* to_low = static_cast<char*>(t.low) + at * 2;
-            finish_tile<T, true, 8>(lds, acc, old, [&](int i, int j, f32x4 v, f32x4 l) {
+            finish_tile<T, true, 16>(lds, acc, old, [&](int i, int j, f32x4 v, f32x4 l) {
                 v += l * p.a;
                 if (i < rows && j < padded) {
                     const int to = i * ldx + j;
