@@ -216,31 +216,44 @@ struct SlopeArgs {
     int rows_per_block, act;
 };
 
-// dz = dy act'(z) over a block of rows by 256 columns (four a lane), and the block's column
-// sums in row order: each of four waves adds every fourth row, and the four meet in LDS.
+// dz = dy act'(z) over a block of rows by 64 units of 16 bytes, one a lane, and the block's
+// column sums in row order: each of four waves adds every fourth row, and the four meet in LDS.
 template <int D>
 __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs p) {
-    __shared__ f32x4 sums[4][64];
+    constexpr int E = unit_elems<D>(), B = elem_bytes<D>();
+    __shared__ float sums[4][E][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t j = (int64_t(blockIdx.x) * 64 + lane) * 4;
+    const int64_t j = (int64_t(blockIdx.x) * 64 + lane) * E;
     const int64_t first = int64_t(blockIdx.y) * p.rows_per_block, last = min(p.m, first + p.rows_per_block);
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    if (j + 4 <= p.n) {
+    float sum[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = 0.0f;
+    if (j + E <= p.n) {
+        const char* dy = static_cast<const char*>(p.dy) + j * B;
+        const char* z = static_cast<const char*>(p.z) + j * B;
+        char* dz = static_cast<char*>(p.dz) + j * B;
 #pragma unroll 4
         for (int64_t i = first + wave; i < last; i += 4) {
-            f32x4 g = load4<D>(p.dy, i * p.lddy + j);
-            if (p.act != HBT_ACT_NONE) {
-                const f32x4 z = load4<D>(p.z, i * p.ldz + j);
+            const u32x4 gs = load16(dy + i * p.lddy * B);
+            const u32x4 zs = p.act == HBT_ACT_NONE ? gs : load16(z + i * p.ldz * B);
+            float g[E];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) g[e] *= slope<D>(z[e], p.act);
+            for (int e = 0; e < E; ++e) {
+                g[e] = element<D>(gs, e);
+                if (p.act != HBT_ACT_NONE) g[e] *= slope<D>(element<D>(zs, e), p.act);
+                sum[e] += g[e];
             }
-            if (p.dz != nullptr) store4<D>(p.dz, i * p.lddz + j, g);
-            sum += g;
+            if (p.dz != nullptr) {
+#pragma unroll
+                for (int e = 0; e < E; e += 4)
+                    store4<D>(dz + i * p.lddz * B, e, f32x4{g[e], g[e + 1], g[e + 2], g[e + 3]});
+            }
         }
     } else if (j < p.n) {
         for (int64_t i = first + wave; i < last; i += 4) {
-            for (int e = 0; e < 3; ++e) {
-                if (j + e >= p.n) break;
+#pragma unroll
+            for (int e = 0; e < E - 1; ++e) {
+                if (j + e >= p.n) continue;
                 float g = load_elem<D>(p.dy, i * p.lddy + j + e);
                 if (p.act != HBT_ACT_NONE) g *= slope<D>(load_elem<D>(p.z, i * p.ldz + j + e), p.act);
                 if (p.dz != nullptr) store_elem<D>(p.dz, i * p.lddz + j + e, g);
@@ -249,12 +262,16 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs p) {
         }
     }
     if (p.partial == nullptr && p.dbias == nullptr) return;
-    sums[wave][lane] = sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[wave][e][lane] = sum[e];
     __syncthreads();
-    if (wave == 0 && j < p.n) {
-        sum = ((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane];
-        if (p.dbias != nullptr) store_row<D>(p.dbias, j, static_cast<int>(min<int64_t>(p.n - j, 4)), sum);
-        else *reinterpret_cast<f32x4*>(p.partial + blockIdx.y * p.ldp + j) = sum;  // ldp: a multiple of 4
+    if (wave != 0 || j >= p.n) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (j + e >= p.n) break;
+        const float total = ((sums[0][e][lane] + sums[1][e][lane]) + sums[2][e][lane]) + sums[3][e][lane];
+        if (p.dbias != nullptr) store_elem<D>(p.dbias, j + e, total);
+        else p.partial[blockIdx.y * p.ldp + j + e] = total;
     }
 }
 
@@ -266,6 +283,7 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* partial, int64_t
     const int64_t j = int64_t(blockIdx.x) * 64 + lane;
     float sum = 0.0f;
     if (j < n) {
+#pragma unroll 8
         for (int b = wave; b < blocks; b += 4) sum += partial[b * ldp + j];
     }
     sums[wave][lane] = sum;
@@ -456,9 +474,11 @@ int64_t split_bytes(int64_t m, int64_t n, int64_t k, int32_t dtype) {
     return splits == 1 ? 0 : 4 * splits * m * ((n + 3) / 4 * 4);
 }
 
+int64_t columns_per_block(int dtype) { return dtype == HBT_DTYPE_F32 ? 256 : 512; }
+
 // Rows per block of the slope pass: enough blocks for the device, few enough partial sums.
-int rows_per_block(int64_t m, int64_t n) {
-    const int64_t columns = (n + 255) / 256;
+int rows_per_block(int64_t m, int64_t n, int dtype) {
+    const int64_t columns = (n + columns_per_block(dtype) - 1) / columns_per_block(dtype);
     int64_t rows = m * columns / 2048;
     rows = std::min<int64_t>(std::max<int64_t>(rows, 16), 256);
     while ((m + rows - 1) / rows > 65535) rows *= 2;
@@ -482,8 +502,8 @@ BackwardSpace backward_space(int64_t tokens, int64_t inner, int64_t outer, int32
         b.dz_bytes = (tokens * b.lddz * size + 255) / 256 * 256;
     }
     if (is_small(tokens, inner, outer)) return BackwardSpace{};
-    if ((wants & HBT_LINEAR_DBIAS) && tokens > rows_per_block(tokens, outer)) {
-        const int64_t rows = rows_per_block(tokens, outer);
+    if ((wants & HBT_LINEAR_DBIAS) && tokens > rows_per_block(tokens, outer, dtype)) {
+        const int64_t rows = rows_per_block(tokens, outer, dtype);
         b.shared_bytes = 4 * ((tokens + rows - 1) / rows) * ((outer + 3) / 4 * 4);
     }
     if (wants & HBT_LINEAR_DX)
@@ -597,11 +617,12 @@ int32_t hbt_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t
         p.m = tokens, p.n = outer, p.act = activation;
         int64_t blocks = 0;
         if (tokens > 0 && outer > 0 && (p.dz != nullptr || dbias != nullptr)) {
-            p.rows_per_block = rows_per_block(tokens, outer);
+            p.rows_per_block = rows_per_block(tokens, outer, dtype);
             blocks = (tokens + p.rows_per_block - 1) / p.rows_per_block;
             if (dbias != nullptr && blocks > 1) p.partial = reinterpret_cast<float*>(shared);
             else p.dbias = dbias;
-            slope_kernel<D><<<dim3(static_cast<unsigned>((outer + 255) / 256), static_cast<unsigned>(blocks)), 256, 0,
+            slope_kernel<D><<<dim3(static_cast<unsigned>((outer + columns_per_block(dtype) - 1) / columns_per_block(dtype)),
+                                   static_cast<unsigned>(blocks)), 256, 0,
                               s>>>(p);
             const int32_t launched = check_launch(who);
             if (launched != HBT_OK) return launched;

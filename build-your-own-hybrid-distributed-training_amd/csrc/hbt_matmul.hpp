@@ -84,6 +84,13 @@ __device__ __forceinline__ u32x4 load16(const char* at) {
     return u32x4{v[0], v[1], v[2], v[3]};
 }
 
+// Element e of a 16-byte unit.
+template <int D>
+__device__ __forceinline__ float element(const u32x4& unit, int e) {
+    if constexpr (D == HBT_DTYPE_F32) return __uint_as_float(unit[e]);
+    else return b16_to_f32<D == HBT_DTYPE_F16>((unit[e / 2] >> (16 * (e % 2))) & 0xFFFFu);
+}
+
 // Elements i .. i + 3, or as many of them as exist.
 template <int D>
 __device__ __forceinline__ f32x4 load_row(const void* p, int64_t i, int have) {
