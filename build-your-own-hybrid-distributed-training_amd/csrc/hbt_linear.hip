@@ -351,15 +351,20 @@ struct Choice {
     int splits;  // parts the sum over k is split into
 };
 
+// Work-items of a launch over every tile.
+int64_t tile_items(int64_t m, int64_t n, int size) {
+    return ((m + size - 1) / size) * ((n + size - 1) / size) * (size == 256 ? 512 : 256);
+}
+
 // The cheapest tile and split by the estimate.  A split sum writes and reads its fp32 parts (about
 // 5 TB/s) in one more launch.  Tiles of 256 need operands that load straight into LDS.
 Choice choose(int64_t m, int64_t n, int64_t k, int dtype, bool aligned) {
     const bool f32 = dtype == HBT_DTYPE_F32;
     const int64_t steps = (k + (f32 ? 31 : 63)) / (f32 ? 32 : 64);
-    Choice best{64, 1};
+    Choice best{128, 1};
     double least = 0.0;
     for (const int size : {64, 128, 256}) {
-        if (size == 256 && (f32 || !aligned)) continue;
+        if ((size == 256 && (f32 || !aligned)) || tile_items(m, n, size) > kGridMaxItems) continue;
         const double fixed = size == 256 ? 9.0 : (size == 128 ? 6.0 : 3.5);
         const int64_t tiles = ((m + size - 1) / size) * ((n + size - 1) / size);
         for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
@@ -386,9 +391,9 @@ int32_t launch_tile(const char* who, ProductArgs& p, int splits, hipStream_t str
     p.tiles_n = static_cast<int>((p.n + T::BN - 1) / T::BN);
     const auto kernel = product_kernel<D, kA, kB, T, kAsync>;
     if constexpr (kLds > 65536) {
-        static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-        if (set != hipSuccess) return check_hip(set, who);
+        static std::atomic<uint64_t> done{0};
+        const int32_t status = allow_lds(who, reinterpret_cast<const void*>(kernel), kLds, done);
+        if (status != HBT_OK) return status;
     }
     kernel<<<dim3(p.tiles_m * p.tiles_n, splits), T::kThreads, kLds, stream>>>(p);
     return check_launch(who);
@@ -431,8 +436,8 @@ int32_t fail(const char* who, const char* what) {
 
 // Rows of a tile are addressed by 31-bit byte offsets from its first one.
 constexpr int64_t kMaxLd = int64_t(1) << 20;
-// Tile and column-block counts stay far inside a grid's limits.
-constexpr int64_t kMaxSide = int64_t(1) << 27;
+// No launch over one side alone passes a grid's 2^32 - 1 work-items.
+constexpr int64_t kMaxSide = int64_t(1) << 26;
 
 int32_t check_matrix(const char* who, const void* p, int64_t rows, int64_t cols, int64_t ld, const char* name) {
     if (rows == 0 || cols == 0) return HBT_OK;
@@ -459,7 +464,8 @@ int32_t check_sizes(const char* who, int64_t m, int64_t n, int64_t k, int32_t dt
         set_error("%s: dtype %d is not F32, BF16 or F16", who, dtype);
         return HBT_ERR_INVALID_ARGUMENT;
     }
-    if (m > kMaxSide || n > kMaxSide || k > kMaxSide || ((m + 63) / 64) * ((n + 63) / 64) > 0x7FFFFFFF) {
+    if (m > kMaxSide || n > kMaxSide || k > kMaxSide || tile_items(m, n, 128) > kGridMaxItems ||
+        tile_items(n, k, 128) > kGridMaxItems || tile_items(m, k, 128) > kGridMaxItems) {
         set_error("%s: sizes %lld x %lld x %lld are past the launch limits", who, static_cast<long long>(m),
                   static_cast<long long>(n), static_cast<long long>(k));
         return HBT_ERR_UNSUPPORTED;

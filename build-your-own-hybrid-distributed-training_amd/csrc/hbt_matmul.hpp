@@ -15,6 +15,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "hbt_common.hpp"
@@ -577,6 +578,20 @@ __device__ __forceinline__ void band_order(int t, int tiles_m, int tiles_n, int&
     const int height = min(tiles_m - first, kBand), within = t - band * width;
     m = first + within % height;
     n = within / height;
+}
+
+// ---- launches ------------------------------------------------------------------------
+// Lets `kernel` use `bytes` of dynamic LDS on the current device, once for each device (`done`, a
+// bit a device, belongs to the kernel).
+inline int32_t allow_lds(const char* who, const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    const int32_t status = check_hip(hipGetDevice(&device), who);
+    if (status != HBT_OK) return status;
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_acquire) & bit) != 0) return HBT_OK;
+    const int32_t set = check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), who);
+    if (set == HBT_OK) done.fetch_or(bit, std::memory_order_release);
+    return set;
 }
 
 // ---- the choice of a tile ---------------------------------------------------------------

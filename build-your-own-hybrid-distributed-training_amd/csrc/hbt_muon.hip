@@ -514,9 +514,9 @@ int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t
     }
     const auto kernel = newton_schulz_kernel<D, T, kPhase>;
     if constexpr (kLds > 65536) {
-        static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-        if (set != hipSuccess) return check_hip(set, who);
+        static std::atomic<uint64_t> done{0};
+        const int32_t status = allow_lds(who, reinterpret_cast<const void*>(kernel), kLds, done);
+        if (status != HBT_OK) return status;
     }
     kernel<<<dim3(static_cast<unsigned>(blocks)), T::kThreads, kLds, stream>>>(p);
     return check_launch(who);
@@ -568,9 +568,9 @@ int32_t run_small(const char* who, const Matrices& t, int32_t grad_dtype, const 
     p.nesterov = direction.nesterov, p.steps = steps, p.update = common.update, p.out_dtype = common.out_dtype;
     const auto launch = [&](auto d) {
         const auto kernel = small_kernel<decltype(d)::value>;
-        static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds);
-        if (set != hipSuccess) return check_hip(set, who);
+        static std::atomic<uint64_t> done{0};
+        const int32_t status = allow_lds(who, reinterpret_cast<const void*>(kernel), kSmallLds, done);
+        if (status != HBT_OK) return status;
         kernel<<<dim3(n), 512, kSmallLds, stream>>>(p);
         return check_launch(who);
     };
