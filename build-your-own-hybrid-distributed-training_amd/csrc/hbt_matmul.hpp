@@ -113,6 +113,13 @@ __device__ __forceinline__ void store_row(void* p, int64_t i, int have, f32x4 v)
         if (e < have) store_elem<D>(p, i + e, v[e]);
 }
 
+// The same for data that is read once and does not fit the memory-side cache.
+__device__ __forceinline__ u32x4 stream16(const char* at) {
+    typedef uint32_t u __attribute__((ext_vector_type(4), aligned(2)));
+    const u v = __builtin_nontemporal_load(reinterpret_cast<const u*>(at));
+    return u32x4{v[0], v[1], v[2], v[3]};
+}
+
 // c += a b over one 16-byte fragment pair: 32 values of k in 2-byte types (one
 // instruction), 16 in fp32 (four).  Lane l holds row l % 16 of each operand and the unit of
 // k that its quarter l / 16 names; the order of k inside a fragment is the same in both.
