@@ -7,7 +7,7 @@ around it, with ``torch.nn.Linear``'s parameters and initialisation.
 
 Sums are held in float32; every stored value is rounded once to the tensors' dtype.  With an
 activation the backward pass keeps ``z = x W^T + bias`` in that dtype and forms ``act'`` from
-it.  No atomics run, so equal inputs give equal bits.
+it; a ReLU without a residual keeps its result, which has the same sign, in its place.  No atomics run, so equal inputs give equal bits.
 """
 
 from __future__ import annotations
@@ -106,8 +106,8 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, r
     rows, ldx = _rows(x, inner)
     tokens = rows.shape[0]
     w, ldw = _rows(weight, inner)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    z = torch.empty((tokens, outer), dtype=x.dtype, device=x.device) if keep else None
+    y = x.new_empty(shape)
+    z = x.new_empty((tokens, outer)) if keep else None
     if tokens == 0 or outer == 0:
         return y, z
     b = None if bias is None else bias.contiguous()
@@ -130,9 +130,10 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, r
 class _FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        y, z = _forward(x, weight, bias, residual, activation, keep=activation != "none")
+        from_result = activation == "relu" and residual is None
+        y, z = _forward(x, weight, bias, residual, activation, keep=activation != "none" and not from_result)
         ctx.activation = activation
-        ctx.save_for_backward(x, weight, z)
+        ctx.save_for_backward(x, weight, y if from_result else z)
         return y
 
     # The backward pass runs on autograd's own thread, where host code is slower: it does as
@@ -153,16 +154,16 @@ class _FusedLinear(torch.autograd.Function):
         if want_x:
             wants = _DX
             ws, ldw = _rows(weight, inner)
-            dx = torch.empty(x.shape, dtype=dtype, device=device)
+            dx = x.new_empty(x.shape)
             w_at, dx_at = ws.data_ptr(), dx.data_ptr()
         if want_w:
             wants |= _DW
             xs, ldx = _rows(x, inner)
-            dw = torch.empty(weight.shape, dtype=dtype, device=device)
+            dw = weight.new_empty(weight.shape)
             x_at, dw_at = xs.data_ptr(), dw.data_ptr()
         if want_b:
             wants |= _DBIAS
-            db = torch.empty(outer, dtype=dtype, device=device)
+            db = weight.new_empty(outer)
             db_at = db.data_ptr()
         code, activation = _native.dtype_code(dtype), ACTIVATIONS[ctx.activation]
         lib = _native.library()
