@@ -114,7 +114,8 @@ def orthogonalize(
     dtype; the results have their shapes, in ``dtype`` (default: theirs).  ``product_dtype``
     (default: float32 for float32 results, else float16) is what the matrix cores read; sums
     and the iterate are float32 either way.  A zero matrix gives zeros; one holding a
-    non-finite value comes out non-finite.  Layouts other than dense rows go through a copy.
+    non-finite value comes out non-finite.  Layouts other than dense rows go through a copy.  Not
+    differentiable.
     """
     who = "muon.orthogonalize"
     matrices = list(matrices)
