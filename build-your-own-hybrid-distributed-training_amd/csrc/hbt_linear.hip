@@ -413,6 +413,57 @@ int32_t launch_tile(const char* who, ProductArgs& p, int splits, hipStream_t str
     return check_launch(who);
 }
 
+// One product in tiles of 256, its last columns or rows in tiles of 128 where that is estimated
+// to be shorter: a round of 256 that is mostly empty takes as long as a full one.  896 tiles (the
+// weight gradient of 8192 x 4096 x 14336) are three rounds and a half, 850 us, and 797 cut; 788
+// (1024 x 768 x 50257) are three and 20 tiles, 113 us, and 102 cut.
+struct Cut {
+    int64_t m, n;  // the part in tiles of 256
+};
+Cut cut_of(int64_t m, int64_t n, int64_t k) {
+    const int64_t rows = (m + 255) / 256, cols = (n + 255) / 256;
+    const double steps = static_cast<double>((k + 63) / 64);
+    const auto rest = [&](int64_t r, int64_t c) {
+        return r <= 0 || c <= 0 ? 0.0 : round_cost(128, ((r + 127) / 128) * ((c + 127) / 128), steps, false, 6.0) + 3.0;
+    };
+    Cut best{m, n};
+    double least = 0.97 * round_cost(256, rows * cols, steps, false, 9.0);
+    for (int64_t less = 1; less < 256; ++less) {  // tile rows or columns left to the second launch
+        if (less < rows && less * cols < 256) {
+            const double cost = round_cost(256, (rows - less) * cols, steps, false, 9.0) + rest(m - (rows - less) * 256, n);
+            if (cost < least) least = cost, best = {(rows - less) * 256, n};
+        }
+        if (less < cols && less * rows < 256) {
+            const double cost = round_cost(256, rows * (cols - less), steps, false, 9.0) + rest(m, n - (cols - less) * 256);
+            if (cost < least) least = cost, best = {m, (cols - less) * 256};
+        }
+    }
+    return best;
+}
+
+template <int D, bool kA, bool kB>
+int32_t launch_large(const char* who, const ProductArgs& p, hipStream_t stream) {
+    constexpr int64_t B = elem_bytes<D>();
+    const Cut cut = cut_of(p.m, p.n, p.k);
+    ProductArgs first = p, last = p;
+    first.m = cut.m, first.n = cut.n;
+    const int32_t status = launch_tile<D, kA, kB, Tile256, true>(who, first, 1, stream);
+    if (status != HBT_OK || (cut.m == p.m && cut.n == p.n)) return status;
+    const int64_t m0 = cut.m < p.m ? cut.m : 0, n0 = cut.n < p.n ? cut.n : 0;
+    const auto moved = [](auto* at, int64_t elements) {
+        using Byte = std::conditional_t<std::is_const_v<std::remove_pointer_t<decltype(at)>>, const char, char>;
+        return at == nullptr ? at : static_cast<decltype(at)>(static_cast<Byte*>(at) + elements * B);
+    };
+    last.m = p.m - m0, last.n = p.n - n0;
+    last.a = moved(p.a, kA ? m0 * p.lda : m0);
+    last.b = moved(p.b, kB ? n0 * p.ldb : n0);
+    last.bias = moved(p.bias, n0);
+    last.residual = moved(p.residual, m0 * p.ldr + n0);
+    last.y = moved(p.y, m0 * p.ldy + n0);
+    last.z = moved(p.z, m0 * p.ldz + n0);
+    return launch_tile<D, kA, kB, Tile128, true>(who, last, 1, stream);
+}
+
 template <int D, bool kA, bool kB>
 int32_t launch_product(const char* who, ProductArgs& p, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
     constexpr int BK = tile_k<D>();
@@ -435,7 +486,8 @@ int32_t launch_product(const char* who, ProductArgs& p, void* workspace, int64_t
         status = aligned ? launch_tile<D, kA, kB, Tile128, true>(who, p, c.splits, stream)
                          : launch_tile<D, kA, kB, Tile128, false>(who, p, c.splits, stream);
     } else if constexpr (D != HBT_DTYPE_F32) {
-        status = launch_tile<D, kA, kB, Tile256, true>(who, p, c.splits, stream);
+        status = c.splits > 1 ? launch_tile<D, kA, kB, Tile256, true>(who, p, c.splits, stream)
+                              : launch_large<D, kA, kB>(who, p, stream);
     }
     if (status != HBT_OK || c.splits == 1) return status;
     const int64_t blocks = std::min<int64_t>((p.m * (p.ldp / 4) + 255) / 256, 4096);

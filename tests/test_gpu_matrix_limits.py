@@ -31,6 +31,14 @@ def test_aligned_sums_that_end_inside_a_tile(device, inner, dtype):
     check(*make(device, 136, 144, inner, dtype), "gelu_tanh")
 
 
+@pytest.mark.parametrize("shape", [(1000, 64, 50000), (8200, 64, 2100), (2048, 65536, 2048)], ids=str)
+def test_last_rounds_and_split_sums_of_large_tiles(device, shape):
+    """Results whose last columns or rows are formed in smaller tiles, and a long sum split over
+    large ones, with everything the epilogue does."""
+    print(shape, flush=True)
+    check(*make(device, *shape, torch.bfloat16), "relu")
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("shape", [(136, 72, 200), (520, 264, 312)], ids=str)
 def test_aligned_windows_of_nan(device, shape, dtype):
