@@ -416,7 +416,8 @@ int32_t launch_tile(const char* who, ProductArgs& p, int splits, hipStream_t str
 // One product in tiles of 256, its last columns or rows in tiles of 128 where that is estimated
 // to be shorter: a round of 256 that is mostly empty takes as long as a full one.  896 tiles (the
 // weight gradient of 8192 x 4096 x 14336) are three rounds and a half, 850 us, and 797 cut; 788
-// (1024 x 768 x 50257) are three and 20 tiles, 113 us, and 102 cut.
+// (1024 x 768 x 50257) are three and 20 tiles, 113 us, and 102 cut (one set of inputs, which the
+// memory-side cache holds; from memory 915 and 851, 124 and 119).
 struct Cut {
     int64_t m, n;  // the part in tiles of 256
 };
