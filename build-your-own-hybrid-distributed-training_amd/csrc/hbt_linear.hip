@@ -42,7 +42,8 @@ __device__ __forceinline__ float slope(float z, int act) {
             return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * expf(-0.5f * z * z) * 0.39894228f;
         case HBT_ACT_GELU_TANH: {
             const float s = sigmoid<D>(2.0f * kGeluC * (z + kGeluA * z * z * z));
-            return s + z * s * (1.0f - s) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * z * z);
+            // s (1 - s) is 0 long before z z overflows, which would leave 0 times infinity.
+            return s + z * s * (1.0f - s) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * fminf(z * z, 1e6f));
         }
         case HBT_ACT_SILU: {
             const float s = sigmoid<D>(z);

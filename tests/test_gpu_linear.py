@@ -185,6 +185,21 @@ def test_nonfinite_values_stay_in_their_rows(device, dtype):
     assert bool(fused_linear(x[7:8], w, b, activation="relu").isnan().all())
 
 
+@pytest.mark.parametrize("tokens", [40, 100])  # one workgroup's backward pass, and the slope pass
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_far_from_zero(device, name, dtype, tokens):
+    # z is the bias, whose square and cube pass float32: the slopes are 0 and 1, the sums whole numbers.
+    b = torch.tensor([1e25, -1e25, 100.0, -120.0], device=device, dtype=dtype).requires_grad_(True)
+    x = torch.zeros(tokens, 8, device=device, dtype=dtype)
+    w = torch.zeros(4, 8, device=device, dtype=dtype)
+    y = fused_linear(x, w, b, activation=name)
+    y.backward(torch.ones_like(y))
+    with torch.no_grad():
+        assert torch.equal(y, b.clamp_min(0).expand(tokens, 4))
+    assert b.grad.tolist() == [tokens, 0, tokens, 0]
+
+
 def test_gradients_match_differences(device):
     x, w, b, r, dy = make(device, 6, 9, 7, torch.float32)
     for name in ("gelu", "gelu_tanh", "silu"):
