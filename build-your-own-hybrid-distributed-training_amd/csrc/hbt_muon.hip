@@ -165,7 +165,9 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
 }
 
 // ---- the products ----------------------------------------------------------------------
-enum Phase { kGram, kSquare, kIterate, kFinish };  // kFinish: the last iterate, into the result
+// kFinish: the last iterate, into the result; kGramParts: a Gram product whose sum is split.
+enum Phase { kGram, kSquare, kIterate, kFinish, kGramParts };
+constexpr bool is_gram(Phase phase) { return phase == kGram || phase == kGramParts; }
 
 struct Problem {
     const void* x;        // the iterate in the product type, [rows][ldx]
@@ -173,13 +175,16 @@ struct Problem {
     void* gram;           // [side][ldg], side the shorter one
     void* poly;
     void* low;            // what x's fp16 values leave of it, [rows][ldx], or null
+    float* parts;         // [split][side][ldg]: the Gram product's sum in parts
     void* out;            // last step: the parameter or the result, [rows][cols]
     int rows, cols, ldx;
     float gram_scale;     // 1 / scale^2
     float out_scale;      // the step's multiple of x, over scale
+    int split;            // the number of parts
 };
 struct Run {
-    int first, count, tiles;  // its matrices, and the tiles of each
+    int first, count, tiles;  // its matrices, and the workgroups of each
+    int parts, part_k;        // a Gram product's sum in parts of part_k
 };
 struct ProductArgs {
     FirstBlocks blocks;
@@ -190,6 +195,7 @@ struct ProductArgs {
     int count, update, out_dtype;
     int stream;           // the iterates do not fit the memory-side cache
 };
+static_assert(sizeof(ProductArgs) <= 4096, "kernel arguments");
 
 template <typename F>
 __device__ __forceinline__ auto by_dtype(int dtype, F&& f) {
@@ -212,7 +218,12 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
     const int global = xcd_tile(local, run.count * run.tiles);
     const Problem& t = p.problem[run.first + global / run.tiles];
     const bool wide = t.rows <= t.cols;
-    const int tile = global % run.tiles, side = wide ? t.rows : t.cols;
+    const int side = wide ? t.rows : t.cols;
+    int tile = global % run.tiles, k0 = 0, k1 = wide ? t.cols : t.rows, part = 0;
+    if constexpr (kPhase == kGramParts) {  // the parts of one tile are neighbours
+        part = tile % run.parts, tile /= run.parts;
+        k0 = part * run.part_k, k1 = min(k1, k0 + run.part_k);
+    }
     const int ldg = (side + 7) / 8 * 8;
     int tm, tn;
     constexpr bool kProduct = kPhase == kIterate || kPhase == kFinish;
@@ -226,11 +237,11 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
     }
     const int m0 = tm * T::BM, n0 = tn * T::BN;
     f32x4 acc[T::TM][T::TN];
-    if constexpr (kPhase == kGram) {
+    if constexpr (is_gram(kPhase)) {
         if (wide)
-            tile_product<D, true, true, T, true>(t.x, t.ldx, m0, side, t.x, t.ldx, n0, side, 0, t.cols, lds, acc);
+            tile_product<D, true, true, T, true>(t.x, t.ldx, m0, side, t.x, t.ldx, n0, side, k0, k1, lds, acc);
         else
-            tile_product<D, false, false, T, true>(t.x, t.ldx, m0, t.ldx, t.x, t.ldx, n0, t.ldx, 0, t.rows, lds, acc);
+            tile_product<D, false, false, T, true>(t.x, t.ldx, m0, t.ldx, t.x, t.ldx, n0, t.ldx, k0, k1, lds, acc);
     } else if constexpr (kPhase == kSquare) {
         tile_product<D, true, true, T, true>(t.gram, ldg, m0, side, t.gram, ldg, n0, side, 0, side, lds, acc);
     } else if (wide) {
@@ -300,28 +311,63 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
         }
     } else {
         const int rows = side - m0, cols = side - n0, padded_rows = ldg - m0, padded_cols = ldg - n0;
-        char* out = static_cast<char*>(kPhase == kGram ? t.gram : t.poly);
+        char* out = static_cast<char*>(is_gram(kPhase) ? t.gram : t.poly);
         char* direct = out + (int64_t(m0) * ldg + n0) * elem_bytes<D>();
         char* mirror = out + (int64_t(n0) * ldg + m0) * elem_bytes<D>();
         const char* gram = static_cast<const char*>(t.gram) + (int64_t(m0) * ldg + n0) * elem_bytes<D>();
+        float* sums = kPhase == kGramParts && run.parts > 1 ? t.parts + (int64_t(part) * side + m0) * ldg + n0 : nullptr;
         // Off the diagonal the mirror image is stored too: the products are bitwise symmetric.
         finish_tile<T, true, 8>(
             lds, acc,
             [&](int i, int j) {
-                if constexpr (kPhase == kGram) return f32x4{0.f, 0.f, 0.f, 0.f};
+                if constexpr (is_gram(kPhase)) return f32x4{0.f, 0.f, 0.f, 0.f};
                 else return load4<D>(gram, min(i, rows - 1) * ldg + min(j, padded_cols - 4));
             },
             [&](int i, int j, f32x4 v, f32x4 l) {
-                v = kPhase == kGram ? v * t.gram_scale : l * p.b + v * p.c;
+                if constexpr (kPhase == kGramParts) {
+                    if (sums != nullptr) {
+                        if (i < rows && j < padded_cols) *reinterpret_cast<f32x4*>(sums + i * ldg + j) = v;
+                        return v;
+                    }
+                }
+                v = is_gram(kPhase) ? v * t.gram_scale : l * p.b + v * p.c;
                 if (i >= rows) v = f32x4{0.f, 0.f, 0.f, 0.f};  // the mirror image's padding
                 if (i < rows && j < padded_cols) store4<D>(direct, i * ldg + j, v);
                 return v;
             },
-            tm != tn,
+            tm != tn && sums == nullptr,
             [&](int j, int i, f32x4 v) {
                 if (j < cols && i < padded_rows) store4<D>(mirror, j * ldg + i, v);
             });
     }
+}
+
+// A Gram product from its parts, added in their order: four columns of a row a lane, read from the
+// lower triangle of tiles of `size` that the parts hold.
+template <int D>
+__global__ __launch_bounds__(256) void gram_join_kernel(ProductArgs p, int size) {
+    const int r = find_entry(p.blocks, blockIdx.x), local = blockIdx.x - p.blocks.first[r];
+    const Run& run = p.run[r];
+    const Problem& t = p.problem[run.first + local / run.tiles];
+    const int side = min(t.rows, t.cols), ldg = (side + 7) / 8 * 8, units = ldg / 4;
+    const int u = local % run.tiles * 256 + threadIdx.x, i = u / units, j = u % units * 4;
+    if (i >= side) return;
+    const int64_t part = int64_t(side) * ldg;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (i / size >= j / size) {
+        const float* at = t.parts + int64_t(i) * ldg + j;
+        for (int k = 0; k < run.parts; ++k) sum += *reinterpret_cast<const f32x4*>(at + k * part);
+    } else {
+        const float* at = t.parts + int64_t(j) * ldg + i;
+        for (int k = 0; k < run.parts; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += j + e < side ? at[k * part + e * ldg] : 0.0f;
+    }
+    sum *= t.gram_scale;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e >= side) sum[e] = 0.0f;
+    store4<D>(t.gram, int64_t(i) * ldg + j, sum);
 }
 
 // ---- small matrices --------------------------------------------------------------------
@@ -450,9 +496,22 @@ __global__ __launch_bounds__(512) void small_kernel(SmallArgs p) {
 
 // ---- host ----------------------------------------------------------------------------
 struct Plan {
-    int64_t low, x0, x1, gram, poly, partial, factor, end;  // offsets of one matrix's storage
+    int64_t low, x0, x1, gram, poly, parts, partial, factor, end;  // offsets of one matrix's storage
     int64_t chunks, ldx, ldg;
+    int split;
 };
+
+// The parts a Gram product's sum over the longer side is split into.  Long thin matrices have few
+// tiles, whose sums the parts spread over the device: up to 64 workgroups a matrix, eight k-tiles
+// or more each, where that is at least three parts (joining them is one more launch).  Five steps on
+// one 50257 x 64 matrix take 330 us, with whole sums 5490; on 24 of 4096 x 64 270 and 609.  The rule
+// sees one matrix, so that its bits do not depend on what shares its launches.
+int parts_of(int64_t rows, int64_t cols, int product) {
+    const int64_t n = (std::min(rows, cols) + 63) / 64, tiles = n * (n + 1) / 2;
+    const int64_t steps = std::max(rows, cols) / (product == HBT_DTYPE_F32 ? 32 : 64);
+    const int64_t parts = std::min(64 / tiles, steps / 8);
+    return parts < 3 ? 1 : static_cast<int>(parts);
+}
 
 Plan plan_of(int64_t rows, int64_t cols, int product, int64_t at) {
     const auto take = [&](int64_t bytes) {
@@ -470,6 +529,8 @@ Plan plan_of(int64_t rows, int64_t cols, int product, int64_t at) {
     p.x1 = take(rows * p.ldx * size);
     p.gram = take(side * p.ldg * size);
     p.poly = take(side * p.ldg * size);
+    p.split = parts_of(rows, cols, product);
+    p.parts = p.split == 1 ? at : take(p.split * side * p.ldg * 4);
     p.partial = take(p.chunks * 8);
     p.factor = take(4);
     p.end = at;
@@ -521,9 +582,16 @@ int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t
         const Problem& t = p.problem[i];
         int n = 1;
         while (i + n < p.count && p.problem[i + n].rows == t.rows && p.problem[i + n].cols == t.cols) ++n;
-        p.run[r] = {i, n, static_cast<int>(tiles_of(t, size, kPhase))};
+        Run& run = p.run[r];
+        run = {i, n, static_cast<int>(tiles_of(t, size, kPhase)), 1, 0};
+        if (kPhase == kGramParts) {
+            const int length = std::max(t.rows, t.cols);
+            run.part_k = ((length + t.split - 1) / t.split + tile_k<D>() - 1) / tile_k<D>() * tile_k<D>();
+            run.parts = (length + run.part_k - 1) / run.part_k;
+            run.tiles *= run.parts;
+        }
         p.blocks.first[r] = static_cast<int>(blocks);
-        blocks += (int64_t(n) * p.run[r].tiles + 7) / 8 * 8;
+        blocks += (int64_t(n) * run.tiles + 7) / 8 * 8;
     }
     const auto kernel = newton_schulz_kernel<D, T, kPhase>;
     if constexpr (kLds > 65536) {
@@ -532,6 +600,18 @@ int32_t launch_phase_tile(const char* who, ProductArgs& p, int size, hipStream_t
         if (status != HBT_OK) return status;
     }
     kernel<<<dim3(static_cast<unsigned>(blocks)), T::kThreads, kLds, stream>>>(p);
+    int32_t status = check_launch(who);
+    if (kPhase != kGramParts || status != HBT_OK) return status;
+    int64_t joins = 0;
+    for (int i = 0, r = 0; i < p.count; i += p.run[r++].count) {
+        const Problem& t = p.problem[i];
+        const int64_t side = std::min(t.rows, t.cols), units = (side + 7) / 8 * 2;
+        p.run[r].tiles = static_cast<int>((side * units + 255) / 256);
+        p.blocks.first[r] = static_cast<int>(joins);
+        if (p.run[r].parts > 1) joins += int64_t(p.run[r].count) * p.run[r].tiles;
+    }
+    if (joins == 0) return HBT_OK;
+    gram_join_kernel<D><<<dim3(static_cast<unsigned>(joins)), 256, 0, stream>>>(p, size);
     return check_launch(who);
 }
 
@@ -547,8 +627,8 @@ int32_t launch_phase(const char* who, ProductArgs& p, hipStream_t stream) {
         for (int i = 0; i < p.count; ++i) {
             const Problem& t = p.problem[i];
             const int64_t count = tiles_of(t, size, kPhase);
-            const int k = kPhase == kGram ? std::max(t.rows, t.cols) : std::min(t.rows, t.cols);
-            tiles += count;
+            const int k = is_gram(kPhase) ? std::max(t.rows, t.cols) : std::min(t.rows, t.cols);
+            tiles += count * (is_gram(kPhase) ? t.split : 1);
             steps += static_cast<double>(count) * k / tile_k<D>();
         }
         // Mirror images, and the reads and writes of the iterate, make rounds longer than a layer's.
@@ -605,6 +685,7 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
     direction.blocks.clear();
     int64_t at = 0, direction_blocks = 0, iterate_bytes = 0;
     int n = 0;
+    bool split = false;
     for (int i = 0; i < t.count; ++i) {
         const int64_t rows = t.rows[i], cols = t.cols[i];
         if (rows == 0 || cols == 0 || is_small(rows, cols)) continue;
@@ -621,12 +702,14 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
         direction.blocks.first[n] = static_cast<int>(direction_blocks);
         direction_blocks += plan.chunks;
         iterate_bytes += rows * plan.ldx * 4;
+        split |= plan.split > 1;
         norm.entry[n] = {partial, factor, plan.chunks, scale};
         ++n;
         by_length.problem[by_length.count++] = {
-            workspace + plan.x0, workspace + plan.x1, workspace + plan.gram, workspace + plan.poly, low, t.outs[i],
+            workspace + plan.x0, workspace + plan.x1, workspace + plan.gram, workspace + plan.poly, low,
+            reinterpret_cast<float*>(workspace + plan.parts), t.outs[i],
             static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(plan.ldx), 1.0f / (scale * scale),
-            (t.scales == nullptr ? 1.0f : t.scales[i]) / scale};
+            (t.scales == nullptr ? 1.0f : t.scales[i]) / scale, plan.split};
     }
     if (n == 0) return HBT_OK;
     const dim3 grid(static_cast<unsigned>(direction_blocks));
@@ -655,8 +738,8 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
     sort(by_length, [](const Problem& t) { return std::max(t.rows, t.cols); });
     sort(by_side, [](const Problem& t) { return std::min(t.rows, t.cols); });
     for (int s = 0; s < steps; ++s) {
-        if ((status = launch_phase<D, kGram>(who, by_length, stream)) != HBT_OK ||
-            (status = launch_phase<D, kSquare>(who, by_side, stream)) != HBT_OK)
+        status = split ? launch_phase<D, kGramParts>(who, by_length, stream) : launch_phase<D, kGram>(who, by_length, stream);
+        if (status != HBT_OK || (status = launch_phase<D, kSquare>(who, by_side, stream)) != HBT_OK)
             return status;
         if (s + 1 == steps) return launch_phase<D, kFinish>(who, by_side, stream);
         if ((status = launch_phase<D, kIterate>(who, by_side, stream)) != HBT_OK) return status;

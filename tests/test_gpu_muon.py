@@ -93,6 +93,20 @@ def test_a_list_of_mixed_sizes(device, dtype):
         assert torch.equal(orthogonalize([matrices[i]])[0], results[i])
 
 
+@pytest.mark.parametrize("shape", [(9001, 16), (16, 9001), (50257, 64), (70, 6000), (2600, 129), (129, 2600), (4100, 250),
+                                   (255, 7001)], ids=str)
+def test_long_thin_matrices(device, shape):
+    """Gram sums in parts, of odd lengths, beside matrices whose sums are whole; the bits stay a
+    matrix's own."""
+    shapes = [shape, (300, 300), shape, (40, 20)]
+    for dtype, product in ((torch.bfloat16, torch.float16), (torch.float32, torch.float32)):
+        matrices = [gradient(device, *s, dtype, seed=i) for i, s in enumerate(shapes)]
+        results = orthogonalize(matrices)
+        for m, r in zip(matrices, results):
+            assert off(r, exact(m)) < PRODUCT[product] + UNIT[dtype]
+            assert torch.equal(orthogonalize([m])[0], r)
+
+
 def test_large_matrices_take_the_large_tiles(device):
     for shape in ((4200, 4104), (4104, 4200)):
         g = gradient(device, *shape, torch.bfloat16)
