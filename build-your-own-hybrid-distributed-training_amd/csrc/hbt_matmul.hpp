@@ -241,22 +241,47 @@ struct Operand {
     // Of the last k-tile only `left` values of k exist; other calls have kWhole.  The loads are
     // written as assembly because the compiler makes every LDS read wait for all such loads; they
     // have no register results, and wait_loads() below waits for them.
+    //
+    // The hardware holds no load back for its scalar registers.  The compiler, which may form the
+    // descriptor by v_readfirstlane, does not see that a load reads it, so the wait states stand in
+    // the assembly: five between a vector instruction's scalar result and a load (the move to m0 and
+    // s_nop 3), one between a write of m0 and a load into LDS.  8192 x 8192 x 8192 in bf16 takes
+    // 817 us with them and 819 without.
     template <bool kWhole>
     __device__ __forceinline__ void load_async(int64_t k0, int64_t left, uint32_t lds, int tid, int wave) const {
+        static_assert(kUnits == 2 || kUnits == 4, "the assembly below");
         const uint64_t at_k = reinterpret_cast<uint64_t>(base + (kKMajor ? k0 : k0 * ld) * B);
         const u32x4 buffer = {static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at_k))),
                               static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at_k >> 32))),
                               0x7FFFFFFFu, 0x00020000u};
+        uint32_t from[kUnits];
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (i * THREADS + wave * 64) * 16);
-            uint32_t from = offset[i];
+            from[i] = offset[i];
             if constexpr (!kWhole) {
                 const int u = i * THREADS + tid;
-                if (!(kKMajor ? column(u) * E < left : u / kUnitsPerLine < left)) from = kNowhere;
+                if (!(kKMajor ? column(u) * E < left : u / kUnitsPerLine < left)) from[i] = kNowhere;
             }
-            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :: "s"(to), "v"(from), "s"(buffer) : "memory");  // nothing else here uses m0
+        }
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + wave * 64 * 16);
+        constexpr int kNext = THREADS * 16;  // bytes of LDS between a wave's units
+        if constexpr (kUnits == 2) {
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\t"
+                         "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+                         "s_add_u32 m0, m0, %4\n\ts_nop 0\n\t"
+                         "buffer_load_dwordx4 %2, %3, 0 offen lds"
+                         :: "s"(to), "v"(from[0]), "v"(from[1]), "s"(buffer), "n"(kNext) : "memory", "m0", "scc");
+        } else {
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\t"
+                         "buffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+                         "s_add_u32 m0, m0, %6\n\ts_nop 0\n\t"
+                         "buffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
+                         "s_add_u32 m0, m0, %6\n\ts_nop 0\n\t"
+                         "buffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
+                         "s_add_u32 m0, m0, %6\n\ts_nop 0\n\t"
+                         "buffer_load_dwordx4 %4, %5, 0 offen lds"
+                         :: "s"(to), "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "s"(buffer), "n"(kNext)
+                         : "memory", "m0", "scc");
         }
     }
 
