@@ -34,16 +34,20 @@ __device__ __forceinline__ float activate(float z, int act) {
         default: return z;
     }
 }
+// act'(z) of a stored z.  A z past its dtype's range is stored as an infinity, whose products
+// with the zeros around it would be NaN; the slopes have reached 0 and 1 long before kFar, which
+// stands in for everything past it (a NaN stays one), and whose square and cube stay finite.
+constexpr float kFar = 1e4f;
 template <int D>
 __device__ __forceinline__ float slope(float z, int act) {
+    z = z > kFar ? kFar : (z < -kFar ? -kFar : z);
     switch (act) {
         case HBT_ACT_RELU: return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
         case HBT_ACT_GELU:
             return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * expf(-0.5f * z * z) * 0.39894228f;
         case HBT_ACT_GELU_TANH: {
             const float s = sigmoid<D>(2.0f * kGeluC * (z + kGeluA * z * z * z));
-            // s (1 - s) is 0 long before z z overflows, which would leave 0 times infinity.
-            return s + z * s * (1.0f - s) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * fminf(z * z, 1e6f));
+            return s + z * s * (1.0f - s) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * z * z);
         }
         case HBT_ACT_SILU: {
             const float s = sigmoid<D>(z);

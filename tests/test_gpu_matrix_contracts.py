@@ -1,0 +1,41 @@
+"""What the matrix operators promise at their entry points beyond plain results: the gradients of a
+pre-activation past its dtype's range."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from hybrid_training_amd import fused_linear
+
+from .test_gpu_linear import DTYPES, make
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- values ----------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens", [40, 100])  # one workgroup's backward pass, and the slope pass
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_of_preactivations_past_float16(device, name, tokens):
+    """z = +-320000 is infinite as float16 keeps it; the slopes there are still 1 and 0."""
+    x = torch.full((tokens, 8), 200.0, dtype=torch.float16, device=device).requires_grad_(True)
+    w = torch.tensor([[200.0], [-200.0]], dtype=torch.float16, device=device).expand(2, 8).contiguous().requires_grad_(True)
+    b = torch.zeros(2, dtype=torch.float16, device=device).requires_grad_(True)
+    y = fused_linear(x, w, b, activation=name)
+    y.backward(torch.ones_like(y))
+    assert torch.equal(y, torch.tensor([float("inf"), 0.0], dtype=y.dtype, device=device).expand(tokens, 2))
+    assert b.grad.tolist() == [tokens, 0]
+    assert torch.equal(x.grad, torch.full_like(x, 200.0))
+    assert torch.equal(w.grad, torch.tensor([[200.0 * tokens], [0.0]], dtype=w.dtype, device=device).expand(2, 8))
+
+
+@pytest.mark.parametrize("tokens", [40, 100])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_a_nan_preactivation_has_nan_gradients(device, name, dtype, tokens):
+    x, w, b, _, dy = make(device, tokens, 24, 32, dtype, residual=False)
+    x[3, 5] = float("nan")
+    leaf = x.clone().requires_grad_(True)
+    fused_linear(leaf, w, b, activation=name).backward(dy)
+    rows = torch.arange(tokens, device=device) != 3
+    assert bool(leaf.grad[3].isnan().all()) and bool(leaf.grad[rows].isfinite().all())
