@@ -16,6 +16,7 @@ import math
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native
@@ -127,6 +128,13 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, r
     return y, z
 
 
+def _holds_tangent(*given: torch.Tensor | None) -> bool:
+    """Whether a tensor is dual: part of a forward-mode derivative."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in given)
+
+
 class _FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
@@ -180,7 +188,8 @@ class _FusedLinear(torch.autograd.Function):
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                  activation: str = "none", residual: torch.Tensor | None = None) -> torch.Tensor:
-    """``act(x weight^T + bias) + residual`` in one kernel, differentiable once.
+    """``act(x weight^T + bias) + residual`` in one kernel, differentiable once (backwards; a
+    forward-mode tangent is refused).
 
     ``x`` is ``[..., inner]``, ``weight`` ``[outer, inner]``, ``bias`` ``[outer]`` and
     ``residual`` ``[..., outer]``, all of one dtype: bfloat16, float16 or float32.  Any strides
@@ -188,6 +197,10 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     layouts through a dense copy.  ``activation`` is one of :data:`ACTIVATIONS`.
     """
     _check(x, weight, bias, residual, activation)
+    if _holds_tangent(x, weight, bias, residual):
+        raise UnsupportedFeatureError(
+            format_error("linear.fused_linear", "forward-mode derivatives have no kernel",
+                         resolution="differentiate backwards, or use torch.nn.functional.linear inside a dual level"))
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return _FusedLinear.apply(x, weight, bias, residual, activation)
