@@ -233,6 +233,9 @@ class MuonOptimizer(ShardedOptimizer):
         super().__init__([*rest, *chosen], others_config, norm_group=norm_group, device=device, recorder=recorder,
                          defer_clip=defer_clip, clip_in_step=clip_in_step)
         self._muon_config = config
+        self._due: list[_Batch] = []
+        self._space: torch.Tensor | None = None
+        self._recording: _native.GraphRecording | None = None
         self._matrices = {id(p) for p in chosen}
         options = dict(lr=config.learning_rate, weight_decay=config.weight_decay, momentum=config.momentum,
                        nesterov=config.nesterov, steps=config.steps, coefficients=config.coefficients,
@@ -247,71 +250,90 @@ class MuonOptimizer(ShardedOptimizer):
         return id(p) in self._matrices
 
     def _stepped_parameters(self):
-        """The others' share of the step, for the AdamW kernels, once every gradient, the
-        matrices' too, has been checked."""
+        """The others' share of the step, for the AdamW kernels.
+
+        By then the matrices' share, :attr:`_due`, is planned and its memory is allocated, so that
+        whatever it is refused for leaves every parameter, counter and state as it was."""
         self._due = []
-        others = []
+        others, batches = [], {}
+        recording = self._recording = self._recording_check()
         for item in super()._stepped_parameters():
-            (self._due if self._is_matrix(item[1]) else others).append(item)
-        for group, p, grad, state in self._due:
+            if not self._is_matrix(item[1]):
+                others.append(item)
+                continue
+            group, p, grad, state = item
             if torch.float64 in (p.dtype, grad.dtype):
                 raise UnsupportedFeatureError(format_error("muon.MuonOptimizer.step", "float64 matrices have no kernel",
                                                            observed=f"parameter {p.dtype}, gradient {grad.dtype}"))
             buffer = state.get("momentum_buffer") if state else None
-            if buffer is not None and (buffer.dtype != torch.float32 or buffer.shape != p.shape
-                                       or buffer.device != p.device or not buffer.is_contiguous()):
+            if buffer is None:
+                if recording is not None:
+                    raise _unrecordable("the first step creates the momentum buffer")
+            elif (buffer.dtype != torch.float32 or buffer.shape != p.shape or buffer.device != p.device
+                  or not buffer.is_contiguous()):
                 raise ShardingError(
                     format_error("muon.MuonOptimizer.step", "a momentum buffer must be a dense float32 tensor beside "
                                  "its parameter", expected=f"{tuple(p.shape)} on {p.device}",
                                  observed=f"{buffer.dtype} {tuple(buffer.shape)} on {buffer.device}"))
             check_newton_schulz("MuonOptimizer.step", group["steps"], group["coefficients"], group["norm_eps"])
+            unscale = _pending_unscale(grad)
+            key = (id(group), p.dtype, grad.dtype, unscale)
+            batch = batches.get(key)
+            if batch is None:
+                batch = batches[key] = _Batch(group, p.dtype, grad.dtype, unscale)
+            batch.params.append(p)
+            batch.grads.append(grad)
+            batch.buffers.append(buffer)
+            batch.fresh |= buffer is None
+        due = list(batches.values())
+        for batch in due:
+            batch.plan()
+        if due:
+            # One call's kernels follow another's on the stream, so all share the largest's storage.
+            self._space = torch.empty(max(n for batch in due for _, n in batch.calls), dtype=torch.uint8,
+                                      device=self._device)
+            for batch in due:
+                if batch.fresh:
+                    batch.buffers = [self._zero_state(p, "momentum_buffer") if v is None else v
+                                     for p, v in zip(batch.params, batch.buffers)]
+        self._due = due
         return others
 
     def _run_adamw_step(self, grad_mul: NormResult | None, write_back: bool) -> None:
-        super()._run_adamw_step(grad_mul, write_back)
-        due, self._due = self._due, []
-        recording = self._recording_check()
-        batches: dict[tuple, list[tuple]] = {}
-        for group, p, grad, _ in due:
-            state = self._optimizer.state[p]
-            if state.get("momentum_buffer") is None:
-                if recording is not None:
-                    raise _unrecordable("the first step creates the momentum buffer")
-                state["momentum_buffer"] = self._zero_state(p, "momentum_buffer")
-            key = (id(group), p.dtype, grad.dtype, _pending_unscale(grad))
-            batches.setdefault(key, []).append((group, p, grad, state["momentum_buffer"]))
-        with _native.device_guard(self._device):
-            for (_, pdtype, gdtype, unscale), batch in batches.items():
-                self._step_batch(batch, pdtype, gdtype, unscale, grad_mul, recording)
-                if _write_back_flag(write_back, grad_mul, unscale):
-                    # In-place semantics: .grad ends as the reference's multiplies leave it.
-                    scale_gradients([g for _, _, g, _ in batch], gdtype, unscale, _mul_ptr(grad_mul, gdtype),
-                                    self._device, "muon.hbt_scale_inplace")
+        try:
+            super()._run_adamw_step(grad_mul, write_back)
+            with _native.device_guard(self._device):
+                for batch in self._due:
+                    self._step_batch(batch, grad_mul)
+                    if _write_back_flag(write_back, grad_mul, batch.unscale):
+                        # In-place semantics: .grad ends as the reference's multiplies leave it.
+                        scale_gradients(batch.grads, batch.gdtype, batch.unscale, _mul_ptr(grad_mul, batch.gdtype),
+                                        self._device, "muon.hbt_scale_inplace")
+        finally:
+            self._due, self._space, self._recording = [], None, None
 
-    def _step_batch(self, batch, pdtype, gdtype, unscale, grad_mul, recording) -> None:
+    def _step_batch(self, batch: "_Batch", grad_mul: NormResult | None) -> None:
         """Matrices of one group and dtype pair, in calls of up to 32."""
         lib = _native.library()
         stream = _native.stream_of(self._device)
-        group = batch[0][0]
-        product = _product_code(group["product_dtype"], pdtype)
-        decay, lr, momentum, rest = _step_scalars(group)
+        space, recording = self._space, self._recording
+        decay, lr, momentum, rest = batch.scalars
+        if batch.fresh:
+            for p, buffer in zip(batch.params, batch.buffers):
+                self._optimizer.state[p]["momentum_buffer"] = buffer
         slot = None
         if recording is not None:
             slot = recording.new_slot()
             recording.steps.append(_RecordedMuon(self, recording.record_address(slot), batch))
-        for indices, nbytes in _call_groups([tuple(p.shape) for _, p, _, _ in batch], product):
-            items = [batch[i] for i in indices]
-            space = torch.empty(nbytes, dtype=torch.uint8, device=self._device)
-            params, buffers = [p for _, p, _, _ in items], [v for _, _, _, v in items]
-            scales = (ctypes.c_float * len(items))(*[_update_scale(group["scale"], p.shape) for p in params])
+        for indices, nbytes in batch.calls:
+            params, grads, buffers, scales = batch.of(indices)
             _native.check(lib.hbt_muon_step(
                 _native.pointer_array([p.data_ptr() for p in params]),
-                _native.pointer_array([g.data_ptr() for _, _, g, _ in items]),
+                _native.pointer_array([g.data_ptr() for g in grads]),
                 _native.pointer_array([v.data_ptr() for v in buffers]),
                 _native.int64_array([p.shape[0] for p in params]), _native.int64_array([p.shape[1] for p in params]),
-                scales, len(items), _native.dtype_code(pdtype), _native.dtype_code(gdtype), product, unscale,
-                _mul_ptr(grad_mul, gdtype), momentum, rest, int(bool(group["nesterov"])), int(group["steps"]),
-                *map(float, group["coefficients"]), float(group["norm_eps"]), decay, lr,
+                (ctypes.c_float * len(params))(*scales), len(params), _native.dtype_code(batch.pdtype), _native.dtype_code(batch.gdtype), batch.product,
+                batch.unscale, _mul_ptr(grad_mul, batch.gdtype), momentum, rest, *batch.options, decay, lr,
                 None if slot is None else slot.data_ptr(), space.data_ptr(), nbytes, stream), "muon.hbt_muon_step")
             increment_version(params + buffers)
 
@@ -358,17 +380,43 @@ def _update_scale(rule: str, shape: Sequence[int]) -> float:
                                                expected=["rms", "spectral"], observed=rule))
 
 
+class _Batch:
+    """The matrices of one group and dtype pair that a step moves, and the calls that do."""
+
+    def __init__(self, group: dict, pdtype: torch.dtype, gdtype: torch.dtype, unscale: float) -> None:
+        self.group, self.pdtype, self.gdtype, self.unscale = group, pdtype, gdtype, unscale
+        self.params: list[nn.Parameter] = []
+        self.grads: list[torch.Tensor] = []
+        self.buffers: list[torch.Tensor | None] = []
+        self.fresh = False  # some buffers are not in the optimizer's state yet
+
+    def plan(self) -> None:
+        """Everything the calls are formed from that can be refused."""
+        group = self.group
+        self.scalars = _step_scalars(group)
+        self.options = (int(bool(group["nesterov"])), int(group["steps"]), *map(float, group["coefficients"]),
+                        float(group["norm_eps"]))
+        self.product = _product_code(group["product_dtype"], self.pdtype)
+        self.scales = [_update_scale(group["scale"], p.shape) for p in self.params]
+        self.calls = _call_groups([p.shape for p in self.params], self.product)
+
+    def of(self, indices: list[int]) -> tuple[list, list, list, list]:
+        """Parameters, gradients, momenta and scales of one call."""
+        lists = (self.params, self.grads, self.buffers, self.scales)
+        return lists if len(self.calls) == 1 else tuple([values[i] for i in indices] for values in lists)
+
+
 class _RecordedMuon:
     """The matrices' share of a step recorded into a graph, whose kernels read decay, learning
     rate and momentum from a slot that each replay rewrites."""
 
-    def __init__(self, optimizer: MuonOptimizer, record: int, batch: list[tuple]) -> None:
+    def __init__(self, optimizer: MuonOptimizer, record: int, batch: _Batch) -> None:
         self._optimizer = optimizer
         self._record = record
-        self._params = [p for _, p, _, _ in batch]
-        self._grad_ptrs = [g.data_ptr() for _, _, g, _ in batch]
+        self._params = batch.params
+        self._grad_ptrs = [g.data_ptr() for g in batch.grads]
         self._operands = _RecordedOperands(optimizer, self._params, ("momentum_buffer",))
-        self._fixed = _fixed_options(batch[0][0])
+        self._fixed = _fixed_options(batch.group)
 
     @property
     def parameters(self) -> list[nn.Parameter]:
