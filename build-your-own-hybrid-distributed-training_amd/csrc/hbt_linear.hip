@@ -608,16 +608,18 @@ using namespace hbt::mm;
 extern "C" {
 
 int64_t hbt_linear_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype) {
-    if (tokens < 0 || inner < 0 || outer < 0) return -1;
-    if (dtype != HBT_DTYPE_F32 && dtype != HBT_DTYPE_BF16 && dtype != HBT_DTYPE_F16) return -1;
+    clear_error();
+    if (check_sizes("hbt_linear_workspace", tokens, outer, inner, dtype) != HBT_OK) return -1;
     return tokens <= 16 ? 0 : split_bytes(tokens, outer, inner, dtype);
 }
 
 int64_t hbt_linear_backward_workspace(int64_t tokens, int64_t inner, int64_t outer, int32_t dtype, int32_t activation,
                                       int32_t wants) {
-    if (tokens < 0 || inner < 0 || outer < 0 || wants < 0 || wants > 7) return -1;
-    if (dtype != HBT_DTYPE_F32 && dtype != HBT_DTYPE_BF16 && dtype != HBT_DTYPE_F16) return -1;
-    if (activation < HBT_ACT_NONE || activation > HBT_ACT_SILU) return -1;
+    clear_error();
+    const char* who = "hbt_linear_backward_workspace";
+    if (check_sizes(who, tokens, outer, inner, dtype) != HBT_OK) return -1;
+    if (activation < HBT_ACT_NONE || activation > HBT_ACT_SILU) return fail(who, "unknown activation");
+    if (wants < 0 || wants > 7) return fail(who, "unknown results are wanted");
     const BackwardSpace b = backward_space(tokens, inner, outer, dtype, activation, wants);
     return b.dz_bytes + b.shared_bytes;
 }

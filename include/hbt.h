@@ -645,7 +645,7 @@ int32_t hbt_exchange_capture_mode(int32_t mode, int32_t* previous);
  *
  * Small results of a long sum split it over workgroups: `workspace` (16-byte aligned) then
  * holds the fp32 parts.  hbt_linear_workspace gives the bytes that a call of these sizes can
- * use (-1 for bad arguments); with a smaller workspace, or NULL, the sum is split less or not
+ * use (-1 for arguments the call refuses); with a smaller workspace, or NULL, the sum is split less or not
  * at all, which is slower and rounds in another order.
  * ---------------------------------------------------------------------------- */
 #define HBT_ACT_NONE 0
@@ -671,7 +671,8 @@ int32_t hbt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const
  * (not where tokens, inner and outer are at most 64); dbias sums the unrounded values in a
  * fixed order.  With tokens = 0, dw and dbias are 0.
  * `workspace` (256-byte aligned) holds at least hbt_linear_backward_workspace's bytes for
- * these sizes and `wants`, the HBT_LINEAR_* of the results asked for (-1 for bad arguments).
+ * these sizes and `wants`, the HBT_LINEAR_* of the results asked for (-1 for arguments the call
+ * refuses).
  * Layouts, dtypes and limits are hbt_linear's.  No atomics: results repeat bitwise.
  * ---------------------------------------------------------------------------- */
 #define HBT_LINEAR_DX 1

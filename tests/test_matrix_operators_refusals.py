@@ -2,11 +2,16 @@
 
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from hybrid_training_amd import UnsupportedFeatureError, fused_linear, linear
+import hybrid_training_amd
+from hybrid_training_amd import UnsupportedFeatureError, _native, fused_linear, linear
 
 
 def test_forward_mode_derivatives_are_refused(monkeypatch):
@@ -27,3 +32,38 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
         # a level without a tangent is an ordinary call
         assert torch.equal(fused_linear(x, w, b, residual=r), x @ w.t())
     assert torch.equal(fused_linear(x, w, b, residual=r), x @ w.t())
+
+
+HUGE = [1 << 26, (1 << 26) + 1, 1 << 31, 1 << 48, 1 << 50, (1 << 63) - 1]
+
+
+def test_working_storage_of_sizes_past_the_limits():
+    """-1 wherever the call itself refuses, whatever the arithmetic on such sizes gives.  In a process
+    of its own: a division by zero ended it."""
+    code = f"""
+from hybrid_training_amd import _native
+lib = _native.library()
+for tokens in {HUGE}:
+    for wants in (1, 2, 4, 7):
+        print(lib.hbt_linear_backward_workspace(tokens, 8, 100, 0, 1, wants))
+    print(lib.hbt_linear_workspace(tokens, 8, 100, 1))
+    print(lib.hbt_linear_backward_workspace(8, tokens, tokens, 1, 1, 7), lib.hbt_linear_workspace(8, tokens, tokens, 1))
+"""
+    path = os.path.dirname(os.path.dirname(hybrid_training_amd.__file__))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          env={**os.environ, "PYTHONPATH": path})
+    assert done.returncode == 0, done.returncode
+    values = [int(v) for v in done.stdout.split()]
+    each = len(values) // len(HUGE)
+    assert each == 7 and all(v >= 0 for v in values[:5])  # 2^26 rows are within the limits
+    assert values[5:each] == [-1, -1]  # a product of 2^26 by 2^26 is not
+    assert values[each:] == [-1] * (len(values) - each)
+
+
+def test_working_storage_names_what_it_refuses():
+    lib = _native.library()
+    assert lib.hbt_linear_workspace(8, 8, -1, 0) == -1 and b"negative" in lib.hbt_last_error()
+    assert lib.hbt_linear_backward_workspace(8, 8, 8, 0, 9, 1) == -1 and b"activation" in lib.hbt_last_error()
+    assert lib.hbt_linear_backward_workspace(8, 8, 8, 0, 0, 8) == -1 and b"wanted" in lib.hbt_last_error()
+    assert lib.hbt_linear_workspace(1 << 27, 8, 8, 0) == -1 and b"launch limits" in lib.hbt_last_error()
+    assert lib.hbt_linear_workspace(8, 8, 8, 0) == 0 and lib.hbt_last_error() == b""
