@@ -54,13 +54,13 @@ _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 #: Working storage one call may ask for before a list of matrices is split (a single matrix may
 #: need more): 32 matrices of a few thousand squared fit.
 _WORKSPACE_CAP = 4 << 30
-#: Sides the kernels address (hbt_orthogonalize's limit).
-_MAX_SIDE = 1 << 20
+#: Sides the kernels address, and the elements of one call (hbt_orthogonalize's limits).
+_MAX_SIDE, _MAX_ELEMENTS = 1 << 20, 1 << 34
 
 
 def _call_groups(shapes: Sequence[tuple[int, int]], product: int) -> list[tuple[list[int], int]]:
     """(indices, workspace bytes) of the calls a list of matrices is split into, in order: at
-    most ``MAX_MATRICES`` matrices and ``_WORKSPACE_CAP`` bytes each."""
+    most ``MAX_MATRICES`` matrices, ``_MAX_ELEMENTS`` elements and ``_WORKSPACE_CAP`` bytes each."""
     lib = _native.library()
 
     def need(indices: list[int]) -> int:
@@ -74,18 +74,21 @@ def _call_groups(shapes: Sequence[tuple[int, int]], product: int) -> list[tuple[
     groups: list[tuple[list[int], int]] = []
     for first in range(0, len(shapes), _native.MAX_MATRICES):
         indices = list(range(first, min(first + _native.MAX_MATRICES, len(shapes))))
-        nbytes = need(indices)
-        if nbytes <= _WORKSPACE_CAP:
+        elements = [shapes[i][0] * shapes[i][1] for i in indices]
+        if sum(elements) <= _MAX_ELEMENTS and (nbytes := need(indices)) <= _WORKSPACE_CAP:
             groups.append((indices, nbytes))
             continue
-        sizes = [need([i]) for i in indices]  # whole 256-byte units: a call's need is their sum
         part: list[int] = []
-        for i, size in zip(indices, sizes):
-            if part and sum(sizes[j - first] for j in part) + size > _WORKSPACE_CAP:
-                groups.append((part, sum(sizes[j - first] for j in part)))
-                part = []
+        taken = held = 0
+        for i, count in zip(indices, elements):
+            size = need([i])  # whole 256-byte units: a call's need is their sum
+            if part and (taken + size > _WORKSPACE_CAP or held + count > _MAX_ELEMENTS):
+                groups.append((part, taken))
+                part, taken, held = [], 0, 0
             part.append(i)
-        groups.append((part, sum(sizes[j - first] for j in part)))
+            taken += size
+            held += count
+        groups.append((part, taken))
     return groups
 
 

@@ -11,7 +11,8 @@ import torch
 from torch.autograd import forward_ad
 
 import hybrid_training_amd
-from hybrid_training_amd import UnsupportedFeatureError, _native, fused_linear, linear
+from hybrid_training_amd import UnsupportedFeatureError, _native, fused_linear, linear, muon
+from hybrid_training_amd.errors import NativeKernelError
 
 
 def test_forward_mode_derivatives_are_refused(monkeypatch):
@@ -67,3 +68,22 @@ def test_working_storage_names_what_it_refuses():
     assert lib.hbt_linear_backward_workspace(8, 8, 8, 0, 0, 8) == -1 and b"wanted" in lib.hbt_last_error()
     assert lib.hbt_linear_workspace(1 << 27, 8, 8, 0) == -1 and b"launch limits" in lib.hbt_last_error()
     assert lib.hbt_linear_workspace(8, 8, 8, 0) == 0 and lib.hbt_last_error() == b""
+
+
+def test_lists_past_a_calls_elements_are_split(monkeypatch):
+    """A call takes 2^34 elements; a list of matrices that each fit takes as many calls as it needs."""
+    side = 1 << 16  # 2^32 elements a matrix
+    groups = muon._call_groups([(side, side)] * 9, _native.DTYPE_F16)
+    assert sum((indices for indices, _ in groups), []) == list(range(9))
+    monkeypatch.setattr(muon, "_WORKSPACE_CAP", 1 << 62)  # the elements alone
+    groups = muon._call_groups([(side, side)] * 9, _native.DTYPE_F16)
+    assert [indices for indices, _ in groups] == [[0, 1, 2, 3], [4, 5, 6, 7], [8]]
+    lib = _native.library()
+    for indices, nbytes in groups:
+        sides = _native.int64_array([side] * len(indices))
+        assert lib.hbt_orthogonal_workspace(sides, sides, len(indices), _native.DTYPE_F16) == nbytes > 0
+    # small matrices, which take no working storage, among them
+    assert [i for i, _ in muon._call_groups([(side, side)] * 4 + [(8, 8)], _native.DTYPE_F16)] == [[0, 1, 2, 3], [4]]
+    assert muon._call_groups([], _native.DTYPE_F16) == []
+    with pytest.raises(NativeKernelError, match="past the limits"):
+        muon._call_groups([(8, 8), (1 << 18, 1 << 18)], _native.DTYPE_F16)
