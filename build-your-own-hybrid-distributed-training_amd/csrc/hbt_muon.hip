@@ -5,10 +5,11 @@
 //   w' = decay w - lr scale x
 //
 // The iterate x is held in 32 bits: fp32, or, beside fp16 products, the fp16 value they read and
-// the fp16 rounding error of it (22 bits of mantissa).  The products read copies of x, A and B rounded to the product
-// type: fp16 (11 bits, and the values are bounded: singular values stay below 1.3, and x is
-// scaled by a power of two near the square root of its longer side, which puts its elements near
-// 1 and the first iterate's above fp16's subnormals) or, on request, fp32.  Rounding x itself
+// what it leaves of x, 2^11 times as large and in fp16 itself (22 bits of mantissa down to elements
+// of 2^-14, below them steps of 2^-36).  The products read copies of x, A and B rounded to the
+// product type: fp16 (11 bits, and the values are bounded: singular values stay below 1.3, and x
+// is scaled by a power of two near the square root of its longer side, which puts its elements
+// near 1 and the first iterate's above fp16's subnormals) or, on request, fp32.  Rounding x itself
 // to 16 bits would be amplified by 3.4 a step in the directions that start small: on matrices with
 // a decaying spectrum fp16 products then end 6e-3 to 9e-3 off, and 3e-4 to 2e-3 with x in 32.
 //
@@ -47,7 +48,7 @@ struct DirectionEntry {
     float* v;        // null: u is the input itself
     double* partial;
     void* x;         // the first iterate in the product type, [rows][ld]
-    void* low;       // the rest of it beside fp16 values
+    void* low;       // the rest of it beside fp16 values, times kLowScale
     const float* factor;
     int64_t rows, cols, ld;
 };
@@ -60,12 +61,14 @@ struct DirectionArgs {
     int nesterov;
 };
 
-// The fp16 value of x and what it leaves, itself in fp16.
+// The fp16 value of x and what it leaves, itself in fp16: at most 2^-11 of x, so 2^11 times that keeps
+// fp16's range and its 11 bits, where the remainder of an element below 1/4 is a subnormal.
+constexpr float kLowScale = 2048.0f;
 __device__ __forceinline__ void split(f32x4 x, u32x2& high, u32x2& low) {
     high = u32x2{pack2_rounded<HBT_DTYPE_F16>(x[0], x[1]), pack2_rounded<HBT_DTYPE_F16>(x[2], x[3])};
     f32x4 left;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) left[e] = x[e] - f16_to_f32((high[e / 2] >> (16 * (e % 2))) & 0xFFFFu);
+    for (int e = 0; e < 4; ++e) left[e] = (x[e] - f16_to_f32((high[e / 2] >> (16 * (e % 2))) & 0xFFFFu)) * kLowScale;
     low = u32x2{pack2_rounded<HBT_DTYPE_F16>(left[0], left[1]), pack2_rounded<HBT_DTYPE_F16>(left[2], left[3])};
 }
 
@@ -174,7 +177,7 @@ struct Problem {
     void* x_next;
     void* gram;           // [side][ldg], side the shorter one
     void* poly;
-    void* low;            // what x's fp16 values leave of it, [rows][ldx], or null
+    void* low;            // what x's fp16 values leave of it, times kLowScale, [rows][ldx], or null
     float* parts;         // [split][side][ldg]: the Gram product's sum in parts
     void* out;            // last step: the parameter or the result, [rows][cols]
     int rows, cols, ldx;
@@ -262,8 +265,9 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
             if constexpr (D != HBT_DTYPE_F32) {
                 const u32x2* rest = reinterpret_cast<const u32x2*>(low + int64_t(from) * 2);
                 const u32x2 r = p.stream ? __builtin_nontemporal_load(rest) : *rest;
-                v += f32x4{f16_to_f32(r[0] & 0xFFFFu), f16_to_f32(r[0] >> 16), f16_to_f32(r[1] & 0xFFFFu),
-                           f16_to_f32(r[1] >> 16)};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = fmaf(f16_to_f32((r[e / 2] >> (16 * (e % 2))) & 0xFFFFu), 1.0f / kLowScale, v[e]);
             }
             return v;
         };

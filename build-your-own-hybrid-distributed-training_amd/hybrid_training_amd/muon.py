@@ -12,10 +12,11 @@ and the parameter moves by ``-lr * scale * x`` after its weight decay.  One call
 gradients, the products on the matrix cores with every matrix of a phase in one launch, the
 parameter written by the last product's epilogue.
 
-The iterate, every sum and the momentum are float32 (the norm float64).  ``product_dtype``
-says what the products read: ``float16``, whose 11 bits leave the result about 2e-3 off its
-exact value (relative, in the Frobenius norm), or ``float32``.  Matrices whose shorter side is at
-most 128 take ``float32`` products either way.
+Every sum and the momentum are float32, the norm float64.  ``product_dtype`` says what the
+products read: ``float16``, whose 11 bits leave the result about 2e-3 off its exact value
+(relative, in the Frobenius norm), or ``float32``.  Matrices whose shorter side is at most 128 take
+``float32`` products either way.  The iterate takes 32 bits: float32, or beside ``float16``
+products their fp16 value and an fp16 remainder (22 bits of mantissa).
 """
 
 from __future__ import annotations
@@ -116,7 +117,7 @@ def orthogonalize(
     ``matrices`` are 2-D device tensors of any sizes, float32, bfloat16 or float16, of one
     dtype; the results have their shapes, in ``dtype`` (default: theirs).  ``product_dtype``
     (default: float32 for float32 results, else float16) is what the matrix cores read; sums
-    and the iterate are float32 either way.  A zero matrix gives zeros; one holding a
+    are float32 either way.  A zero matrix gives zeros; one holding a
     non-finite value comes out non-finite.  Layouts other than dense rows go through a copy.  Not
     differentiable.
     """

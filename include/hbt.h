@@ -705,10 +705,11 @@ int32_t hbt_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t
  * in fp32, each result rounded once.  `slot`: NULL, or device memory holding the fp32 decay,
  * lr, momentum and one_minus_momentum, read in place of the arguments when the kernels run, for a step recorded
  * into a HIP graph.
- * Dtypes: F32, BF16 or F16 each.  Sums are held in fp32 and the norm in fp64; x is carried in
- * fp32.  The products read x, A and B rounded to product_dtype: F16, or F32; a matrix whose
- * shorter side is at most 128 takes F32 either way.  A non-finite
- * gradient makes its whole matrix non-finite.  No atomics: results repeat bitwise.
+ * Dtypes: F32, BF16 or F16 each.  Sums are held in fp32 and the norm in fp64.  The products read
+ * x, A and B rounded to product_dtype: F16, or F32; a matrix whose shorter side is at most 128
+ * takes F32 either way.  x itself is carried in 32 bits: beside F32 products in fp32, beside F16
+ * ones as its fp16 value and an fp16 remainder (22 bits of mantissa).  A non-finite gradient makes
+ * its whole matrix non-finite.  No atomics: results repeat bitwise.
  * `workspace` (256-byte aligned) holds at least hbt_orthogonal_workspace's bytes for these
  * matrices (-1 for bad arguments).
  * ---------------------------------------------------------------------------- */
