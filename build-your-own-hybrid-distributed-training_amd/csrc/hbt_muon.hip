@@ -196,7 +196,6 @@ struct ProductArgs {
     const float* slot;    // null, or decay and learning rate are its first two floats
     float a, b, c, decay, lr;
     int count, update, out_dtype;
-    int stream;           // the iterates do not fit the memory-side cache
 };
 static_assert(sizeof(ProductArgs) <= 4096, "kernel arguments");
 
@@ -263,8 +262,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
             const int from = min(i, rows - 1) * ldx + min(j, padded - 4);
             f32x4 v = load4<D>(x, from);
             if constexpr (D != HBT_DTYPE_F32) {
-                const u32x2* rest = reinterpret_cast<const u32x2*>(low + int64_t(from) * 2);
-                const u32x2 r = p.stream ? __builtin_nontemporal_load(rest) : *rest;
+                const u32x2 r = *reinterpret_cast<const u32x2*>(low + int64_t(from) * 2);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     v[e] = fmaf(f16_to_f32((r[e / 2] >> (16 * (e % 2))) & 0xFFFFu), 1.0f / kLowScale, v[e]);
@@ -283,15 +281,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void newton_schulz_kernel(ProductAr
                     } else {
                         u32x2 high, rest;
                         split(v, high, rest);
-                        u32x2* at_x = reinterpret_cast<u32x2*>(to_x + int64_t(to) * 2);
-                        u32x2* at_low = reinterpret_cast<u32x2*>(to_low + int64_t(to) * 2);
-                        if (p.stream) {
-                            __builtin_nontemporal_store(high, at_x);
-                            __builtin_nontemporal_store(rest, at_low);
-                        } else {
-                            *at_x = high;
-                            *at_low = rest;
-                        }
+                        *reinterpret_cast<u32x2*>(to_x + int64_t(to) * 2) = high;
+                        *reinterpret_cast<u32x2*>(to_low + int64_t(to) * 2) = rest;
                     }
                 }
                 return v;
@@ -687,7 +678,7 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
     by_length.count = by_side.count = 0;
     norm.eps = eps;
     direction.blocks.clear();
-    int64_t at = 0, direction_blocks = 0, iterate_bytes = 0;
+    int64_t at = 0, direction_blocks = 0;
     int n = 0;
     bool split = false;
     for (int i = 0; i < t.count; ++i) {
@@ -705,7 +696,6 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
                               factor, rows, cols, plan.ldx};
         direction.blocks.first[n] = static_cast<int>(direction_blocks);
         direction_blocks += plan.chunks;
-        iterate_bytes += rows * plan.ldx * 4;
         split |= plan.split > 1;
         norm.entry[n] = {partial, factor, plan.chunks, scale};
         ++n;
@@ -728,10 +718,6 @@ int32_t run(const char* who, const Matrices& t, int32_t grad_dtype, int32_t prod
     if (status != HBT_OK) return status;
     norm_kernel<<<dim3(n), 1024, 0, stream>>>(norm);
     if ((status = check_launch(who)) != HBT_OK || (status = pass(std::false_type{})) != HBT_OK) return status;
-    // Iterates past the memory-side cache's 256 MB are written, and their rests read, past it: the
-    // iterate products of a Llama-3-8B layer 1690 against 1645 us, of GPT-2 small's attention
-    // matrices (113 MB) 91 and 88 us against 86.
-    by_length.stream = by_side.stream = iterate_bytes > (int64_t(256) << 20);
     std::copy_n(by_length.problem, n, by_side.problem);
     by_side.count = n;
     const auto sort = [](ProductArgs& p, auto&& key) {
