@@ -15,6 +15,13 @@ from hybrid_training_amd import UnsupportedFeatureError, _native, fused_linear, 
 from hybrid_training_amd.errors import NativeKernelError
 
 
+@pytest.fixture(autouse=True)
+def _no_error_is_left():
+    """The last refused call's message stays with the thread until a call succeeds."""
+    yield
+    assert _native.library().hbt_linear_workspace(8, 8, 8, 0) == 0
+
+
 def test_forward_mode_derivatives_are_refused(monkeypatch):
     """A tangent is not dropped: no kernel carries it, whichever argument holds it."""
     monkeypatch.setattr(linear, "_check", lambda *_: None)
