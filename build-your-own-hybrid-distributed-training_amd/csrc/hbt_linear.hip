@@ -223,7 +223,7 @@ struct SlopeArgs {
 
 // dz = dy act'(z) over a block of rows by 64 units of 16 bytes, one a lane, and the block's
 // column sums in row order: each of four waves adds every fourth row, and the four meet in LDS.
-// Bound by memory: 8192 x 14336 in bf16 takes 127 us (705 MB, 5.5 TB/s).  kStream, for dy and z
+// Bound by memory: 8192 x 14336 in bf16 takes 125 to 129 us (705 MB, 5.5 TB/s).  kStream, for dy and z
 // past the memory-side cache's 256 MB, reads them past it: 127 us against 146 there, but 11.8
 // against 10.1 on 1537 x 777, whose z the forward pass has left in it.
 template <int D, bool kStream>

@@ -221,7 +221,11 @@ class MuonConfig:
     ``scale`` says what multiplies the learning rate of a rows x cols matrix: ``"rms"``,
     ``0.2 sqrt(max(rows, cols))``, gives updates the size of AdamW's, so AdamW's learning rate
     and weight decay carry over; ``"spectral"`` is ``sqrt(max(1, rows / cols))``.
-    ``product_dtype`` is what the matrix cores read: ``"float16"`` or ``"float32"``.
+    ``product_dtype`` is what the matrix cores read.  ``"float16"`` leaves an update about 1e-3 off
+    its exact value (relative, in the Frobenius norm), where Newton-Schulz products themselves leave
+    singular values from 0.68 to 1.14; ``"float32"`` leaves it 4e-6 off and takes 3.6 times as
+    long on GPT-2 small's attention matrices (3.44 against 0.96 ms) and 7 times on a Llama-3-8B
+    layer (110 against 15.7 ms).
     """
 
     learning_rate: float = 1e-3

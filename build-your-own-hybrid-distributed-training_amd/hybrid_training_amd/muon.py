@@ -38,7 +38,6 @@ from .optim import (
     NormResult,
     ShardedOptimizer,
     _check_recorded_grad,
-    _device_state,
     _mul_ptr,
     _pending_unscale,
     _RecordedOperands,

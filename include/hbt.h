@@ -636,7 +636,7 @@ int32_t hbt_exchange_capture_mode(int32_t mode, int32_t* previous);
  * x is [tokens, inner], w [outer, inner], residual, y and z [tokens, outer], each of one
  * dtype (F32, BF16 or F16) with rows of consecutive elements, ld* elements apart (at least
  * the row's length, at most 2^20); bias holds `outer` elements of that dtype.  bias,
- * residual and z may be NULL.  z receives x W^T + bias, which hbt_linear_slope reads.  The
+ * residual and z may be NULL.  z receives x W^T + bias, which hbt_linear_backward reads.  The
  * sum over `inner` is held in fp32 and every stored value rounded once; inner = 0 gives a
  * zero product.  Activations: HBT_ACT_* below; HBT_ACT_GELU is z (1 + erf(z / sqrt 2)) / 2,
  * HBT_ACT_GELU_TANH z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2.
