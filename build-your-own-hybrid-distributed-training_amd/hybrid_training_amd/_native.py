@@ -53,6 +53,7 @@ __all__ = [
     "DTYPE_F64",
     "EXPORTED_SYMBOLS",
     "GraphRecording",
+    "MAX_ADAMW8_TENSORS",
     "MAX_LOCAL_RANKS",
     "MAX_MATRICES",
     "MAX_NORM_PARTS",
@@ -69,9 +70,10 @@ __all__ = [
     "stream_of",
 ]
 
-ABI_VERSION = 22
+ABI_VERSION = 23
 MAX_TENSORS_PER_LAUNCH = 16
 MAX_MATRICES = 32
+MAX_ADAMW8_TENSORS = 56
 MAX_LOCAL_RANKS = 64
 MAX_NORM_PARTS = 128
 CLIP_MAX_ELEMENTS = 1048576
@@ -309,6 +311,19 @@ EXPORTED_SYMBOLS: dict[str, tuple[object, tuple[object, ...]]] = {
          _c_i32, _c_f32, _c_void_p, _c_f32, _c_f32, _c_i32, _c_i32, _c_f32, _c_f32, _c_f32, _c_f64, _c_f32, _c_f32,
          _c_void_p,
          _c_void_p, _c_i64, _c_void_p),
+    ),
+    "hbt_adamw8_step": (
+        _c_i32,
+        (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_i32,
+         _c_f32, _c_void_p, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_void_p, _c_i32, _c_void_p),
+    ),
+    "hbt_moments8_encode": (
+        _c_i32,
+        (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_void_p),
+    ),
+    "hbt_moments8_decode": (
+        _c_i32,
+        (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_void_p),
     ),
 }
 

@@ -281,7 +281,7 @@ def collect_flat_shard_payload(
     hosts = [flat.detach().reshape(-1) if flat.device.type == "cpu" else _pinned_copy(flat)]
     add(hosts[0], key="{name}", category="model")
     if optimizer is not None:
-        state = optimizer.inner.state.get(_state_key(optimizer, handle.flat_param), {})
+        state = optimizer.exported_state(_state_key(optimizer, handle.flat_param))
         for state_name, value in state.items():
             if not torch.is_tensor(value) or value.dim() == 0 or value.numel() != handle.flat_param.numel():
                 scalar = value.item() if torch.is_tensor(value) else value
@@ -486,7 +486,7 @@ def load_flat_shard_checkpoint(
     index = next(i for i, p in enumerate(optimizer.parameters) if p is flat)
     entry: dict[str, Any] = {}
     for state_name in state_names:
-        buffer = torch.zeros(flat.numel(), dtype=flat.dtype, device=handle.device)
+        buffer = torch.zeros(flat.numel(), dtype=optimizer.state_dtype(flat), device=handle.device)
         found = load_flat_shard(buffer, layout, records, cache,
                                 key_of=lambda item, s=state_name: f"{item.name}::{s}", strict=False)
         if found or not layout:

@@ -178,7 +178,12 @@ class MixedPrecisionConfig:
 
 @dataclass(frozen=True)
 class OptimizerConfig:
-    """Optimizer hyper-parameters (``config.py:822-878``)."""
+    """Optimizer hyper-parameters (``config.py:822-878``).
+
+    ``state_format`` (no counterpart in the reference) says how AdamW's moments are held: ``"master"``
+    in the parameter's dtype, as the reference does, or ``"8bit"`` in two bytes an element
+    with float32 scales for each 256 (float32, bfloat16 or float16 masters in device memory).
+    """
 
     name: str = "adamw"
     learning_rate: float = 1e-3
@@ -187,8 +192,16 @@ class OptimizerConfig:
     eps: float = 1e-8
     momentum: float = 0.0
     cpu_offload_state: bool = False
+    state_format: str = "master"
 
     def __post_init__(self) -> None:
+        if self.state_format not in ("master", "8bit"):
+            _fail("OptimizerConfig", "unknown state format", ["master", "8bit"], self.state_format,
+                  "8bit holds AdamW's moments in two bytes an element")
+        if self.state_format == "8bit" and (self.name != "adamw" or self.cpu_offload_state):
+            _fail("OptimizerConfig", "8-bit moments are AdamW's, in device memory", "adamw without cpu_offload_state",
+                  {"name": self.name, "cpu_offload_state": self.cpu_offload_state},
+                  "hold the state in the master's dtype, or keep it on the device")
         if self.name not in {"adamw", "sgd"}:
             _fail("OptimizerConfig", "unknown optimizer", ["adamw", "sgd"], self.name,
                   "the step kernels implement AdamW and SGD")

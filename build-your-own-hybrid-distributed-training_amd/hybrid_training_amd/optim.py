@@ -37,10 +37,16 @@ and the HBM traffic of a clipped fp32 step:
   it in that window; a loss scaler that skips the step does so itself).  36 B/element;
 * ``defer_clip=True``: the update applies the multiplier and the gradients are never
   written; ``.grad`` keeps the unclipped values.  32 B/element.
+
+With ``OptimizerConfig(state_format="8bit")`` AdamW's moments are held in 8 bits each
+(``hbt_adamw8_step``, :mod:`~hybrid_training_amd.moments8`): 16 B/element instead of 28 for the
+update of fp32 masters.  The clip, its placements, the loss scaler and recorded steps work as above, and the
+state dict holds float32 moments, so a run can change between the formats.
 """
 
 from __future__ import annotations
 
+import ctypes
 from collections.abc import Callable, Iterable, Sequence
 from dataclasses import dataclass, field
 from typing import Any
@@ -50,7 +56,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.graph import increment_version
 
-from . import _native
+from . import _native, moments8
 from .config import OptimizerConfig
 from .errors import ConfigurationError, ShardingError, UnsupportedFeatureError, format_error
 from .groups import GroupHandle
@@ -759,6 +765,13 @@ def _adamw_scalars(group: dict, step: float) -> tuple[float, ...]:
     return (decay, 1 - beta1, beta2, 1 - beta2, bias_correction2_sqrt, float(group["eps"]), -step_size)
 
 
+def _adamw8_scalars(scalars: tuple[float, ...]) -> tuple[float, ...]:
+    """:func:`_adamw_scalars` as ``hbt_adamw8_step`` takes them: the second bias correction as a
+    factor."""
+    decay, lerp, beta2, one_minus_beta2, root, eps, neg_step = scalars
+    return decay, lerp, beta2, one_minus_beta2, 1.0 / root, eps, neg_step
+
+
 def _sgd_scalars(group: dict) -> tuple[tuple[float, ...], int]:
     """SGD's scalars (weight_decay, momentum, 1 - dampening, -lr; Python doubles, as torch
     forms them) and the flags they select, without the first-step and write-back flags."""
@@ -803,6 +816,8 @@ class _RecordedAdamW:
     slot with every other recorded step's), and returns the action that does what the
     eager step does to the host state: advance the parameters' step counters."""
 
+    _KEYS: tuple[str, ...] = ("exp_avg", "exp_avg_sq")
+
     def __init__(self, optimizer: "ShardedOptimizer", slot: torch.Tensor, record: int, params: list[nn.Parameter],
                  pdtype: torch.dtype, unscale: float, scalars: tuple[float, ...]) -> None:
         self._optimizer = optimizer
@@ -810,7 +825,7 @@ class _RecordedAdamW:
         self._record = record
         self._params = list(params)
         self._grad_ptrs = [p.grad.data_ptr() for p in params]
-        self._operands = _RecordedOperands(optimizer, self._params, ("exp_avg", "exp_avg_sq"))
+        self._operands = _RecordedOperands(optimizer, self._params, self._KEYS)
         self._pdtype = pdtype
         self._unscale = unscale
         self._lerp_small = abs(scalars[1]) < 0.5
@@ -831,6 +846,17 @@ class _RecordedAdamW:
         if len(found) != 1:
             raise _replay_error("the parameters recorded in one launch no longer share their step scalars")
         scalars = found.pop()
+        self._format(scalars)
+
+        def commit() -> None:
+            for s, value in zip(states, nexts):
+                s["step"].fill_(value)  # s["step"] += 1
+            self._operands.bump_versions()
+
+        return commit
+
+    def _format(self, scalars: tuple[float, ...]) -> None:
+        """Write the scalars into the slot's host record."""
         if (abs(scalars[1]) < 0.5) != self._lerp_small:
             raise _replay_error("beta1 crossed 0.5, which selects another recorded kernel")
         lib = _native.library()
@@ -841,12 +867,15 @@ class _RecordedAdamW:
                                                  *scalars)
         _native.check(status, "optim.hbt_adamw_scalar_record")
 
-        def commit() -> None:
-            for s, value in zip(states, nexts):
-                s["step"].fill_(value)  # s["step"] += 1
-            self._operands.bump_versions()
 
-        return commit
+class _RecordedAdamW8(_RecordedAdamW):
+    """The same over moments in 8 bits, whose slot holds the call's eight scalars in order."""
+
+    _KEYS = moments8.STATE_KEYS
+
+    def _format(self, scalars: tuple[float, ...]) -> None:
+        values = (self._unscale, *_adamw8_scalars(scalars))
+        ctypes.memmove(self._record, (ctypes.c_float * len(values))(*values), 4 * len(values))
 
 
 class _RecordedSgd:
@@ -1051,6 +1080,12 @@ class ShardedOptimizer:
                         observed=str(param.dtype),
                     )
                 )
+            if config.state_format == "8bit" and (is_host(param) or param.dtype == torch.float64):
+                raise UnsupportedFeatureError(
+                    format_error("optim.ShardedOptimizer", "8-bit moments belong to float32, bfloat16 or float16 "
+                                 "parameters in device memory", observed=f"{param.dtype} on {param.device}",
+                                 resolution='hold the state in the master\'s dtype (state_format="master")'))
+        self._eight_bit = config.state_format == "8bit"
         self._offload = bool(config.cpu_offload_state) and self._device.type != "cpu"
         if self._offload:
             # As in the reference, master copies live on the host and the inner
@@ -1286,7 +1321,9 @@ class ShardedOptimizer:
                 if grad is None:
                     continue
                 state = states.get(p)
-                if state:
+                if state and self._eight_bit and moments8.STATE_KEYS[0] in state:
+                    moments8.check_state(p, state, "optim.ShardedOptimizer.step")
+                elif state:
                     for key in read:
                         value = state.get(key)
                         if value is not None and not value.is_contiguous():
@@ -1306,8 +1343,11 @@ class ShardedOptimizer:
                     raise _unrecordable("the first step creates the optimizer state")
                 # Same initial state as torch.optim.Adam._init_group.
                 state["step"] = torch.tensor(0.0, dtype=torch.float32)
-                state["exp_avg"] = self._zero_state(p, "exp_avg")
-                state["exp_avg_sq"] = self._zero_state(p, "exp_avg_sq")
+                if self._eight_bit:
+                    state.update(moments8.zero_state(p))
+                else:
+                    state["exp_avg"] = self._zero_state(p, "exp_avg")
+                    state["exp_avg_sq"] = self._zero_state(p, "exp_avg_sq")
             step_t = state["step"]
             if recording is None:
                 step = _next_step(step_t)
@@ -1331,8 +1371,12 @@ class ShardedOptimizer:
                 slot = None
                 if recording is not None and resident:
                     slot = recording.new_slot()
-                    recording.steps.append(_RecordedAdamW(self, slot, recording.record_address(slot),
-                                                          [p for p, _, _ in resident], pdtype, unscale, scalars))
+                    recorded = _RecordedAdamW8 if self._eight_bit else _RecordedAdamW
+                    recording.steps.append(recorded(self, slot, recording.record_address(slot),
+                                                    [p for p, _, _ in resident], pdtype, unscale, scalars))
+                if self._eight_bit:
+                    self._launch_adamw8(resident, scalars, pdtype, gdtype, unscale, mul_ptr, flags, stream, slot)
+                    continue
                 for start in range(0, len(resident), _native.MAX_TENSORS_PER_LAUNCH):
                     chunk = resident[start : start + _native.MAX_TENSORS_PER_LAUNCH]
                     params = [p for p, _, _ in chunk]
@@ -1349,6 +1393,21 @@ class ShardedOptimizer:
                     )
                     _native.check(status, "optim.hbt_adamw_step")
                     increment_version(params + first + second)
+
+    def _launch_adamw8(self, batch, scalars, pdtype, gdtype, unscale, mul_ptr, flags, stream, slot) -> None:
+        """The update of ``(parameter, gradient, state)`` entries that share their scalars."""
+        lib = _native.library()
+        scalars = _adamw8_scalars(scalars)
+        for start in range(0, len(batch), _native.MAX_ADAMW8_TENSORS):
+            chunk = batch[start : start + _native.MAX_ADAMW8_TENSORS]
+            params, states = [p for p, _, _ in chunk], [s for _, _, s in chunk]
+            _native.check(lib.hbt_adamw8_step(
+                _native.pointer_array([p.data_ptr() for p in params]),
+                _native.pointer_array([g.data_ptr() for _, g, _ in chunk]), *moments8.tables(states),
+                _native.int64_array([p.numel() for p in params]), len(chunk), _native.dtype_code(pdtype),
+                _native.dtype_code(gdtype), unscale, mul_ptr, *scalars, None if slot is None else slot.data_ptr(),
+                flags, stream), "optim.hbt_adamw8_step")
+            increment_version(params + [s[key] for s in states for key in moments8.STATE_KEYS])
 
     def _recording_check(self) -> "_native.GraphRecording | None":
         """The graph recording this step joins, after refusing what a replay cannot repeat."""
@@ -1555,14 +1614,49 @@ class ShardedOptimizer:
                     total += value.numel() * value.element_size()
         return total
 
+    def moments(self, dtype: torch.dtype = torch.float32) -> list[tuple[torch.Tensor, torch.Tensor] | None]:
+        """AdamW's (first, second) moments of every parameter, in new tensors of ``dtype``; ``None``
+        where there are none (before the first step, SGD's, an orthogonalised matrix's).  8-bit
+        moments are the values that their codes stand for."""
+        if self._stream is not None:
+            self._stream.synchronize()
+        states = [self._optimizer.state.get(p) or {} for p in (self._cpu_parameters if self._offload
+                                                               else self._parameters)]
+        coded = [i for i, s in enumerate(states) if moments8.STATE_KEYS[0] in s]
+        found: list[tuple[torch.Tensor, torch.Tensor] | None] = [
+            (s["exp_avg"].to(dtype, copy=True), s["exp_avg_sq"].to(dtype, copy=True)) if "exp_avg_sq" in s else None
+            for s in states]
+        if coded:
+            for i, pair in zip(coded, moments8.decode([self._parameters[i] for i in coded], [states[i] for i in coded],
+                                                      self._device, dtype)):
+                found[i] = pair
+        return found
+
+    def exported_state(self, p: torch.Tensor) -> dict[str, Any]:
+        """The state of ``p`` (the tensor that keys the inner optimizer's state) as a checkpoint
+        holds it: an element of a state tensor for each of ``p``'s, 8-bit moments decoded to float32."""
+        state = dict(self._optimizer.state.get(p) or {})
+        if moments8.STATE_KEYS[0] in state:
+            pair = moments8.decode([p], [state], self._device)[0]
+            state = {k: v for k, v in state.items() if k not in moments8.STATE_KEYS}
+            state["exp_avg"], state["exp_avg_sq"] = pair
+        return state
+
+    def state_dtype(self, p: torch.Tensor) -> torch.dtype:
+        """The dtype of ``p``'s moments in :meth:`exported_state`."""
+        return torch.float32 if self._eight_bit else p.dtype
+
     # -- serialisation -------------------------------------------------------------------
     def state_dict(self) -> dict[str, Any]:
-        """Optimizer state keyed by parameter index (``sharded_optimizer.py:420-443``)."""
+        """Optimizer state keyed by parameter index (``sharded_optimizer.py:420-443``); moments
+        held in 8 bits as the float32 values that they stand for."""
         if self._stream is not None:
             self._stream.synchronize()
         inner = self._optimizer.state_dict()
         state: dict[int, dict[str, Any]] = {}
         for index, entry in inner["state"].items():
+            if self._eight_bit:
+                entry = self.exported_state(self._parameters[int(index)])
             state[int(index)] = {
                 key: (value.detach().cpu().clone() if torch.is_tensor(value) else value)
                 for key, value in entry.items()
@@ -1602,6 +1696,9 @@ class ShardedOptimizer:
             groups.append(merged)
         target = self._cpu_parameters if self._offload else self._parameters
         state: dict[int, dict[str, Any]] = {}
+        held: list[tuple[nn.Parameter, dict[str, torch.Tensor]]] = []
+        if self._eight_bit:
+            payload, held = self._encode_loaded(payload)
         for index, entry in payload["state"].items():
             reference = target[int(index)]
             state[int(index)] = {
@@ -1614,8 +1711,35 @@ class ShardedOptimizer:
                 for key, value in entry.items()
             }
         self._optimizer.load_state_dict({"state": state, "param_groups": groups})
+        for p, codes in held:
+            self._optimizer.state[p].update(codes)
         self._pending_mul = None
         self._pending_signature = None
+
+    def _encode_loaded(self, payload: dict[str, Any]) -> tuple[dict[str, Any], list]:
+        """``payload`` without AdamW's moments, and those in 8 bits beside their parameters."""
+        rest: dict[int, dict[str, Any]] = {}
+        params, pairs = [], []
+        for index, entry in payload["state"].items():
+            rest[index] = {k: v for k, v in entry.items() if k not in ("exp_avg", "exp_avg_sq")}
+            if "exp_avg" not in entry and "exp_avg_sq" not in entry:
+                continue
+            p = self._parameters[int(index)]
+            pair = []
+            for key in ("exp_avg", "exp_avg_sq"):
+                value = entry.get(key)
+                if not torch.is_tensor(value) or value.numel() != p.numel():
+                    raise ShardingError(
+                        format_error("optim.load_state_dict", f"the state {key!r} must hold one value per element",
+                                     expected=tuple(p.shape),
+                                     observed=tuple(value.shape) if torch.is_tensor(value) else type(value).__name__))
+                pair.append(value.detach().to(device=p.device, dtype=torch.float32).contiguous())
+            params.append(p)
+            pairs.append(tuple(pair))
+        states = [moments8.zero_state(p) for p in params]
+        if params:
+            moments8.encode(pairs, states, self._device)
+        return {**payload, "state": rest}, list(zip(params, states))
 
     def __repr__(self) -> str:
         return (

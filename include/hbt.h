@@ -38,6 +38,7 @@ extern "C" {
 /* ---- per-call limits ---------------------------------------------------------- */
 #define HBT_MAX_TENSORS_PER_LAUNCH 16 /* AdamW / norm tables; the host splits larger lists */
 #define HBT_MAX_MATRICES 32           /* orthogonalised matrices; the host splits larger lists */
+#define HBT_MAX_ADAMW8_TENSORS 56     /* 8-bit AdamW tables; the host splits larger lists */
 
 /* Message describing the last failed call on this thread ("" if none). */
 const char* hbt_last_error(void);
@@ -723,6 +724,47 @@ int32_t hbt_muon_step(void* const* params, const void* const* grads, float* cons
                       int32_t product_dtype, float unscale, const float* grad_mul, float momentum,
                       float one_minus_momentum, int32_t nesterov, int32_t steps, float a, float b, float c, double eps, float decay, float lr, const float* slot,
                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * AdamW with both moments held in 8 bits, over up to HBT_MAX_ADAMW8_TENSORS tensors.
+ *
+ * Replaces: ShardedOptimizer.step (optim/sharded_optimizer.py:340-355) where the state's
+ *   memory counts; the reference holds both moments in the parameter's dtype.
+ * Every 256 consecutive elements of a tensor are a block with two fp32 scales.  Element i of
+ * tensor t has codes m_codes[t][i] and v_codes[t][i] and scales m_scales[t][i / 256] and
+ * v_scales[t][i / 256]; codes are allocated in whole blocks (ceil(numel / 256) * 256 bytes, the
+ * ones past the end are written as zeros), codes and scales on 4 bytes.
+ *   m = e4m3(m_code) * (m_scale / 256)     (OCP e4m3, NaN included)
+ *   r = root(v_code) * v_scale             root(16 e + f) = (16 + f) 2^(e - 19), f 2^-18 for
+ *                                          e = 0; 255 is NaN;  v = r^2
+ * Encoding takes as scales the largest finite |m| and r of the block (a largest |m| under
+ * 2^-100 as 0) and rounds 256 m / m_scale and r / v_scale to the nearest code, ties to even, a positive
+ * r to a code of at least 1.  A value that is not finite is held as NaN, alone in its block.
+ * Zeroed codes and scales are zero moments.
+ * hbt_adamw8_step, per element, each operation in fp32 and rounded once (dtype pairs, R_G,
+ * unscale, grad_mul, decay, lerp_weight, eps, neg_step_size and flags as for hbt_adamw_step):
+ *   g = R_G(R_G(g_in * unscale) * (*grad_mul))
+ *   m = m + lerp_weight * (g - m)
+ *   r = sqrt(r * r * beta2 + (one_minus_beta2 * g) * g)
+ *   p = R_P(p * decay + (neg_step_size * m) / (r * inverse_bias_correction2_sqrt + eps))
+ * and m and r are encoded.  `slot`: NULL, or device memory holding the fp32 unscale, decay,
+ * lerp_weight, beta2, one_minus_beta2, inverse_bias_correction2_sqrt, eps and neg_step_size,
+ * read in place of the arguments when the kernels run, for a step recorded into a HIP graph.
+ * hbt_moments8_encode and hbt_moments8_decode convert fp32 moments to codes, and codes to
+ * moments of out_dtype (F32, or BF16).  Encoding what was decoded to F32 gives the same codes and scales,
+ * second moments under 2^-126 aside.
+ * ---------------------------------------------------------------------------- */
+int32_t hbt_adamw8_step(void* const* params, void* const* grads, void* const* m_codes, void* const* v_codes,
+                        float* const* m_scales, float* const* v_scales, const int64_t* numels, int32_t count,
+                        int32_t param_dtype, int32_t grad_dtype, float unscale, const float* grad_mul, float decay,
+                        float lerp_weight, float beta2, float one_minus_beta2, float inverse_bias_correction2_sqrt,
+                        float eps, float neg_step_size, const float* slot, int32_t flags, void* stream);
+int32_t hbt_moments8_encode(const float* const* firsts, const float* const* seconds, void* const* m_codes,
+                            void* const* v_codes, float* const* m_scales, float* const* v_scales,
+                            const int64_t* numels, int32_t count, void* stream);
+int32_t hbt_moments8_decode(const void* const* m_codes, const void* const* v_codes, const float* const* m_scales,
+                            const float* const* v_scales, void* const* firsts, void* const* seconds,
+                            const int64_t* numels, int32_t count, int32_t out_dtype, void* stream);
 
 #ifdef __cplusplus
 }
