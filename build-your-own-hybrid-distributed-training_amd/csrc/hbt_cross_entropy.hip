@@ -1,0 +1,977 @@
+// Softmax cross entropy over a large vocabulary from hidden states, with its gradients, without
+// the logits in memory.
+//
+//   z_iv = <x_i, W_v> + b_v;   lse_i = log sum_v exp z_iv
+//   loss_i = lse_i - (1 - s) z_i,t(i) - (s / V) sum_v z_iv
+//   dz_iv = c_i (exp(z_iv - lse_i) - (1 - s) [v = t(i)] - s / V);  dx = dz W;  dW = dz^T x
+//
+// The tokens that carry a loss are first gathered into consecutive rows: tokens without one cost
+// nothing after that, and whatever their hidden states hold reaches no sum.
+//
+// The logits of a tile never leave the workgroup that forms them: it takes each row's largest and
+// the sum of exp(z - largest) over its columns, and a row's tiles are joined afterwards.  For
+// gradients the tile also stores exp(z - largest), which needs only 16 bits (fp16: 2^-12 of a value
+// whose gradient is rounded to 2^-9 or 2^-12 next; fp32 for fp32 tensors), for a piece of the rows
+// at a time (at most kPieceBytes); one pass over a piece turns them into dz, rounded to the tensors' dtype
+// for the matrix cores, and the two products follow.  So the logits are formed once, 6 T V D operations in
+// all, where forming them again for the gradients would take 8.
+//
+// What a sum over pieces needs (dW, db) is carried in fp32.  A target's probability is not
+// taken from the stored values but from its fp32 logit: 1 - p would lose what fp16 rounds off p.
+#include "hbt_matmul.hpp"
+
+namespace hbt {
+namespace mm {
+namespace {
+
+constexpr int F32 = HBT_DTYPE_F32, BF16 = HBT_DTYPE_BF16, F16 = HBT_DTYPE_F16;
+constexpr int64_t kPieceBytes = int64_t(1) << 30;  // stored exponentials at a time
+constexpr int64_t kStatsBytes = int64_t(1) << 28;  // row statistics at a time, without gradients
+constexpr int kThin = 16;                          // rows of the kernel for few tokens
+constexpr int64_t kMostRows = int64_t(1) << 22;    // rows of a piece: a launch over them stays within a grid
+constexpr int64_t kMostTokens = int64_t(1) << 24;
+constexpr float kLog2e = 1.44269504f;
+
+// What the kernels of a call share.
+struct Control {
+    int32_t count;    // tokens that carry a loss
+    float scale_in;   // multiplies dz before it is rounded: keeps fp16 in range
+    float scale_out;  // multiplies the products
+};
+
+// A row's statistics: the largest logit, 1 / sum of exp(z - largest), log p of its target and what
+// multiplies its dz.  A target out of range makes the log p, and so the loss and the gradients, NaN.
+struct Row {
+    float top, inverse, log_p, weight;
+};
+
+// The rows of piece `piece` of `pieces`, of at most `most` rows each.
+struct Piece {
+    const Control* control;
+    int piece, pieces;
+};
+__device__ __forceinline__ void piece_rows(const Piece& p, int& first, int& rows) {
+    const int count = p.control->count;
+    const int each = ((count + p.pieces - 1) / p.pieces + 255) / 256 * 256;
+    first = min(p.piece * each, count);
+    rows = min(each, count - first);
+}
+
+template <int W>
+__device__ __forceinline__ float group_max(float x) {
+    if constexpr (W == 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    if constexpr (W >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    const auto move = [](float v, auto ctrl) {
+        return __uint_as_float(__builtin_amdgcn_mov_dpp(static_cast<int>(__float_as_uint(v)), decltype(ctrl)::value, 0xF,
+                                                        0xF, false));
+    };
+    x = fmaxf(x, move(x, std::integral_constant<int, 0x128>{}));
+    x = fmaxf(x, move(x, std::integral_constant<int, 0x124>{}));
+    x = fmaxf(x, move(x, std::integral_constant<int, 0x4E>{}));
+    return fmaxf(x, move(x, std::integral_constant<int, 0xB1>{}));
+}
+template <int W>
+__device__ __forceinline__ float group_sum(float x) {
+    if constexpr (W == 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (W >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    const auto move = [](float v, auto ctrl) {
+        return __uint_as_float(__builtin_amdgcn_mov_dpp(static_cast<int>(__float_as_uint(v)), decltype(ctrl)::value, 0xF,
+                                                        0xF, false));
+    };
+    x += move(x, std::integral_constant<int, 0x128>{});
+    x += move(x, std::integral_constant<int, 0x124>{});
+    x += move(x, std::integral_constant<int, 0x4E>{});
+    return x + move(x, std::integral_constant<int, 0xB1>{});
+}
+
+// exp(t) for t <= 0: the hardware's base-2 exponential where the result is rounded to 16 bits or
+// summed with others of its size, the accurate function for fp32 tensors.
+template <int D>
+__device__ __forceinline__ float exponential(float t) {
+    if constexpr (D == F32) return expf(t);
+    else return __builtin_amdgcn_exp2f(t * kLog2e);
+}
+
+// ---- the tokens that carry a loss ---------------------------------------------------------
+struct PrepareArgs {
+    const int64_t* target;
+    const float* token_grads;  // the loss's gradient for each token, or null for 1
+    Control* control;
+    int32_t* place;   // token -> row, -1 without a loss
+    int32_t* token;   // row -> token
+    int32_t* word;    // row -> target, -1 out of range
+    float* weight;    // row -> gradient
+    int64_t tokens, vocab, ignore;
+    int mean, half;
+};
+
+// One workgroup: rows in the order of the tokens.
+__global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
+    __shared__ int wave_count[16];
+    __shared__ float wave_top[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int count = 0;
+    float top = 0.0f;
+    for (int64_t base = 0; base < p.tokens; base += 1024) {
+        const int64_t i = base + threadIdx.x;
+        const int64_t t = i < p.tokens ? p.target[i] : p.ignore;
+        const bool valid = t != p.ignore;
+        const float g = valid && p.token_grads != nullptr ? p.token_grads[i] : 1.0f;
+        const uint64_t votes = __ballot(valid);
+        __syncthreads();
+        if (lane == 0) wave_count[wave] = __popcll(votes);
+        __syncthreads();
+        int row = count + __popcll(votes & ((uint64_t(1) << lane) - 1));
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) row += wave_count[w];
+            count += wave_count[w];
+        }
+        if (valid) {
+            p.token[row] = static_cast<int32_t>(i);
+            p.word[row] = t >= 0 && t < p.vocab ? static_cast<int32_t>(t) : -1;
+            p.weight[row] = g;
+            top = fmaxf(top, fabsf(g));
+        }
+        if (i < p.tokens) p.place[i] = valid ? row : -1;
+    }
+    top = group_max<64>(top);
+    if (lane == 0) wave_top[wave] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 0; w < 16; ++w) top = fmaxf(top, wave_top[w]);
+        // fp16 values of dz: the largest gradient comes to 2^13 to 2^14, far from both ends of the
+        // range; a power of two, so that nothing is rounded.
+        float in = 1.0f;
+        if (p.half && top > 0.0f && top < INFINITY) {
+            int e = 0;
+            frexpf(top, &e);
+            in = ldexpf(1.0f, max(-126, min(126, 14 - e)));
+        }
+        p.control->count = count;
+        p.control->scale_in = in;
+        // No token carries a loss: no gradient, where 1 / 0 times a sum of nothing would be NaN.
+        p.control->scale_out = count == 0 ? 0.0f : (p.mean ? 1.0f / static_cast<float>(count) : 1.0f) / in;
+    }
+}
+
+struct GatherArgs {
+    const void* x;
+    const int32_t* place;
+    void* rows;   // [count][ld], zeros behind the inner size
+    void* dx;     // zeros for the tokens without a loss, or null
+    float* loss;  // the same, or null
+    int64_t ldx, ld, lddx, tokens, inner;
+    int dx_wide;  // dx in fp32
+};
+
+// A wavefront a token.
+template <int D>
+__global__ __launch_bounds__(256) void gather_kernel(GatherArgs p) {
+    constexpr int E = unit_elems<D>(), B = elem_bytes<D>();
+    const int64_t token = blockIdx.x * int64_t(4) + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (token >= p.tokens) return;
+    const int row = p.place[token];
+    if (row >= 0) {
+        const char* from = static_cast<const char*>(p.x) + token * p.ldx * B;
+        char* to = static_cast<char*>(p.rows) + row * p.ld * B;
+        for (int64_t j = lane * E; j < p.ld; j += 64 * E) {
+            u32x4 v = {0, 0, 0, 0};
+            if (j + E <= p.inner) {
+                v = load16(from + j * B);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E - 1; ++e) {
+                    if (j + e >= p.inner) break;
+                    if constexpr (B == 4) v[e] = reinterpret_cast<const uint32_t*>(from)[j + e];
+                    else v[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[j + e]) << (16 * (e % 2));
+                }
+            }
+            *reinterpret_cast<u32x4*>(to + j * B) = v;
+        }
+        return;
+    }
+    if (p.loss != nullptr && lane == 0) p.loss[token] = 0.0f;
+    if (p.dx == nullptr) return;
+    if (p.dx_wide) {
+        for (int64_t j = lane; j < p.inner; j += 64) store_elem<F32>(p.dx, token * p.lddx + j, 0.0f);
+    } else {
+        for (int64_t j = lane; j < p.inner; j += 64) store_elem<D>(p.dx, token * p.lddx + j, 0.0f);
+    }
+}
+
+// ---- logits ---------------------------------------------------------------------------------
+struct LogitArgs {
+    const void* x;      // gathered rows
+    const void* w;
+    const void* bias;
+    const int32_t* word;
+    float2* stats;      // [row of the piece][tile]: largest, sum of exponentials
+    float* sums;        // the same: sum of the logits, or null without smoothing
+    float* target;      // row -> its target's logit
+    void* kept;         // [row of the piece][ldk] exponentials, or null
+    int64_t ldx, ldw, ldk, vocab, inner;
+    int tiles_n;
+    Piece piece;
+};
+
+// A tile's logits to statistics and exponentials.  A row's columns lie with BN / 4 lanes, so a row
+// is reduced within its wavefront.
+template <int D, class T, bool kAsync>
+__global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
+    extern __shared__ __align__(16) char lds[];
+    constexpr int kLanes = T::BN / 4;
+    int first, count;
+    piece_rows(p.piece, first, count);
+    const int tiles_m = (count + T::BM - 1) / T::BM, total = tiles_m * p.tiles_n;
+    if (static_cast<int>(blockIdx.x) >= total) return;
+    int tm, tn;
+    band_order<8>(xcd_tile(blockIdx.x, total), tiles_m, p.tiles_n, tm, tn);
+    const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
+    f32x4 acc[T::TM][T::TN];
+    const char* x = static_cast<const char*>(p.x) + first * p.ldx * elem_bytes<D>();
+    tile_product<D, true, true, T, kAsync>(x, p.ldx, m0, count, p.w, p.ldw, n0, p.vocab, 0, p.inner, lds, acc);
+    const int rows = static_cast<int>(min<int64_t>(count - m0, T::BM));
+    const int cols = static_cast<int>(min<int64_t>(p.vocab - n0, T::BN));
+    const int stored = static_cast<int>(min<int64_t>(p.ldk - n0, T::BN));
+    const int32_t* word = p.word + first + m0;
+    struct Loaded {
+        f32x4 bias;
+        int word;
+    };
+    finish_tile<T, kAsync, 2>(
+        lds, acc,
+        [&](int i, int j) {
+            Loaded l{{0.f, 0.f, 0.f, 0.f}, -1};
+            if (i < rows) l.word = word[i];
+            if (p.bias != nullptr && j < cols) l.bias = load_row<D>(p.bias, n0 + j, cols - j);
+            return l;
+        },
+        [&](int i, int j, f32x4 v, Loaded l) {
+            v += l.bias;
+            const int64_t at = l.word - n0 - j;  // the target's place among the four
+            const int64_t row = m0 + i;
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (at == e && i < rows) p.target[first + row] = v[e];
+                if (j + e < cols) sum += v[e];
+                else v[e] = -INFINITY;
+            }
+            const float top = group_max<kLanes>(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+            const float base = top == -INFINITY ? 0.0f : top;  // a tile of nothing but -inf
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = exponential<D>(v[e] - base);
+            const float part = group_sum<kLanes>((v[0] + v[1]) + (v[2] + v[3]));
+            if (p.sums != nullptr) sum = group_sum<kLanes>(sum);
+            if (i < rows) {
+                if (p.kept != nullptr && j < stored) store4<D == F32 ? F32 : F16>(p.kept, row * p.ldk + n0 + j, v);
+                if (j == 0) {
+                    p.stats[row * p.tiles_n + tn] = make_float2(top, part);
+                    if (p.sums != nullptr) p.sums[row * p.tiles_n + tn] = sum;
+                }
+            }
+            return v;
+        });
+}
+
+// At most 16 tokens, without gradients: the read of W.  A workgroup of 8 waves forms 16 logits of
+// every token as the linear layer's thin kernel does, and their statistics.
+template <int D>
+__global__ __launch_bounds__(512) void thin_logit_kernel(const void* x_, int64_t ldx, const void* w_, int64_t ldw,
+                                                         const void* bias, const int64_t* target, int tokens,
+                                                         int64_t vocab, int64_t inner, float2* stats, float* sums,
+                                                         float* target_logit) {
+    constexpr int E = unit_elems<D>(), kStep = 4 * E, kWaves = 8, kUnrolled = 4, B = elem_bytes<D>();
+    __shared__ f32x4 parts[kWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, q = lane >> 4;
+    const int64_t n0 = int64_t(blockIdx.x) * 16;
+    const bool w_in = n0 + row < vocab, x_in = row < tokens;
+    const char* w = static_cast<const char*>(w_) + ((n0 + (w_in ? row : 0)) * ldw + q * E) * B;
+    const char* x = static_cast<const char*>(x_) + ((x_in ? row : 0) * ldx + q * E) * B;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const int64_t whole = inner / kStep;
+    int64_t s = wave * kUnrolled;
+    for (; s + kUnrolled <= whole; s += kUnrolled * kWaves) {
+        u32x4 fw[kUnrolled], fx[kUnrolled];
+#pragma unroll
+        for (int i = 0; i < kUnrolled; ++i) {
+            fw[i] = load16(w + (s + i) * kStep * B);
+            fx[i] = load16(x + (s + i) * kStep * B);
+        }
+#pragma unroll
+        for (int i = 0; i < kUnrolled; ++i) acc = mma<D>(fw[i], fx[i], acc);
+    }
+    for (; s < whole; ++s) acc = mma<D>(load16(w + s * kStep * B), load16(x + s * kStep * B), acc);
+    if (wave == whole % kWaves && whole * kStep < inner) {  // the last, partial step
+        u32x4 fw = {0, 0, 0, 0}, fx = {0, 0, 0, 0};
+        const int64_t at = whole * kStep;
+        for (int e = 0; e < E; ++e) {
+            if (at + q * E + e >= inner) break;
+            if constexpr (B == 4) {
+                fw[e] = reinterpret_cast<const uint32_t*>(w)[at + e];
+                fx[e] = reinterpret_cast<const uint32_t*>(x)[at + e];
+            } else {
+                fw[e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(w)[at + e]) << (16 * (e % 2));
+                fx[e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(x)[at + e]) << (16 * (e % 2));
+            }
+        }
+        acc = mma<D>(fw, fx, acc);
+    }
+    parts[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) acc += parts[i][lane];
+    // The lane holds logits n0 + 4 q .. + 3 of token `row`.
+    const int64_t n = n0 + 4 * q;
+    const int have = static_cast<int>(min<int64_t>(vocab - n, 4));
+    if (bias != nullptr) acc += load_row<D>(bias, n, have);
+    const int64_t at = x_in ? target[row] - n : -1;
+    float sum = 0.0f, top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (e >= have) acc[e] = -INFINITY;
+        else sum += acc[e];
+        if (at == e && e < have) target_logit[row] = acc[e];
+        top = fmaxf(top, acc[e]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float part = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part += exponential<D>(acc[e] - base);
+    part += __shfl_xor(part, 16);
+    part += __shfl_xor(part, 32);
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (x_in && q == 0) {
+        stats[row * int64_t(gridDim.x) + blockIdx.x] = make_float2(top, part);
+        if (sums != nullptr) sums[row * int64_t(gridDim.x) + blockIdx.x] = sum;
+    }
+}
+
+// ---- a row's tiles joined ----------------------------------------------------------------
+struct JoinArgs {
+    const float2* stats;
+    const float* sums;
+    const float* target;       // row -> target's logit
+    const int32_t* word;       // row -> target, or null: `raw` names it
+    const int32_t* token;      // row -> token, or null: the same
+    const float* weight;       // row -> gradient, or null
+    const int64_t* raw;        // token -> target, without gathered rows
+    Row* row;                  // for the gradients, or null
+    float* loss;               // token -> loss, or null
+    double* row_loss;          // row -> loss, or null
+    int64_t ignore, vocab;
+    int tiles;
+    float smoothing;
+    Piece piece;               // control null: `rows` tokens
+    int rows;
+};
+
+// Sum over the 256 threads of a workgroup, in every thread, in a fixed order.
+__device__ __forceinline__ double join_sum(double x, double* shared) {
+    x = wave_sum(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return (shared[0] + shared[1]) + (shared[2] + shared[3]);
+}
+
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs p) {
+    __shared__ float tops[4];
+    __shared__ double shared[4];
+    int first = 0, count = p.rows;
+    if (p.piece.control != nullptr) piece_rows(p.piece, first, count);
+    const int i = blockIdx.x;
+    if (i >= count) return;
+    const float2* stats = p.stats + int64_t(i) * p.tiles;
+    float top = -INFINITY;
+    for (int t = threadIdx.x; t < p.tiles; t += 256) {
+        const float2 s = stats[t];
+        if (!(s.y <= 0.0f)) top = fmaxf(top, s.x);  // a NaN sum counts, an empty one does not
+    }
+    top = group_max<64>(top);
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    double total = 0.0, logits = 0.0;
+    for (int t = threadIdx.x; t < p.tiles; t += 256) {
+        const float2 s = stats[t];
+        if (!(s.y <= 0.0f)) total += s.y * expf(s.x - top);
+        if (p.sums != nullptr) logits += p.sums[int64_t(i) * p.tiles + t];
+    }
+    total = join_sum(total, shared);
+    if (p.sums != nullptr) logits = join_sum(logits, shared);
+    if (threadIdx.x != 0) return;
+    const int row = first + i;
+    const int64_t token = p.token != nullptr ? p.token[row] : row;
+    bool known;
+    if (p.word != nullptr) {
+        known = p.word[row] >= 0;
+    } else {
+        const int64_t t = p.raw[token];
+        if (t == p.ignore) {
+            if (p.loss != nullptr) p.loss[token] = 0.0f;
+            if (p.row_loss != nullptr) p.row_loss[row] = 0.0;
+            return;
+        }
+        known = t >= 0 && t < p.vocab;
+    }
+    // log p = (z_t - top) - log(sum): the two parts of a nearly certain target are both small
+    const double log_sum = log(total);
+    const double log_p = known ? (static_cast<double>(p.target[row]) - top) - log_sum : NAN;
+    double loss = -(1.0 - p.smoothing) * log_p;
+    if (p.smoothing != 0.0f) loss += p.smoothing * ((top + log_sum) - logits / static_cast<double>(p.vocab));
+    if (p.loss != nullptr) p.loss[token] = static_cast<float>(loss);
+    if (p.row_loss != nullptr) p.row_loss[row] = loss;
+    if (p.row != nullptr)
+        p.row[row] = Row{top, static_cast<float>(1.0 / total), static_cast<float>(log_p),
+                         p.weight[row] * p.piece.control->scale_in};
+}
+
+// The rows' losses added up in a fixed order; `divide`: their mean (0 / 0 without any).
+__global__ __launch_bounds__(1024) void total_kernel(const double* row_loss, const Control* control,
+                                                     const int64_t* raw, int64_t ignore, int64_t rows, int divide,
+                                                     float* loss) {
+    const int64_t count = control != nullptr ? control->count : rows;
+    double sum = 0.0, valid = 0.0;
+    for (int64_t i = threadIdx.x; i < count; i += 1024) {
+        sum += row_loss[i];
+        if (raw == nullptr || raw[i] != ignore) valid += 1.0;
+    }
+    sum = block_sum<1024>(sum);
+    __syncthreads();
+    valid = block_sum<1024>(valid);
+    if (threadIdx.x == 0) loss[0] = static_cast<float>(divide ? sum / valid : sum);
+}
+
+// ---- exponentials to dz, in place ----------------------------------------------------------
+struct SoftmaxArgs {
+    void* kept;
+    const float2* stats;
+    const Row* row;
+    const int32_t* word;
+    int64_t ldk, vocab;
+    int tiles, tile, segment;  // tiles of a row and their columns; columns a workgroup takes
+    float smoothing;
+    Piece piece;
+};
+
+// Bound by memory: a read and a write of 2 bytes (fp32: 4) an element.
+template <int D>
+__global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs p) {
+    constexpr int E = unit_elems<D>(), B = elem_bytes<D>(), S = D == F32 ? F32 : F16;
+    int first, count;
+    piece_rows(p.piece, first, count);
+    const int segments = static_cast<int>((p.ldk + p.segment - 1) / p.segment);
+    const int i = blockIdx.x / segments, part = blockIdx.x % segments;
+    if (i >= count) return;
+    const Row row = p.row[first + i];
+    const int word = p.word[first + i];
+    const float even = p.smoothing / static_cast<float>(p.vocab) * row.weight;
+    const float hit = (expm1f(row.log_p) + p.smoothing) * row.weight - even;
+    const bool known = word >= 0;
+    char* line = static_cast<char*>(p.kept) + int64_t(i) * p.ldk * B;
+    const float2* stats = p.stats + int64_t(i) * p.tiles;
+    const int64_t end = min<int64_t>(p.ldk, (part + 1) * int64_t(p.segment));
+    for (int64_t j = part * int64_t(p.segment) + threadIdx.x * E; j < end; j += 256 * E) {
+        const u32x4 unit = *reinterpret_cast<const u32x4*>(line + j * B);
+        const float factor = expf(stats[min<int64_t>(j, p.vocab - 1) / p.tile].x - row.top) * row.inverse * row.weight;
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            v[e] = element<S>(unit, e) * factor - even;
+            if (j + e == word) v[e] = hit;
+            if (!known) v[e] = NAN;
+            if (j + e >= p.vocab) v[e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e += 4) store4<D>(line, j + e, f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]});
+    }
+}
+
+// ---- the gradients' products ---------------------------------------------------------------
+struct GradArgs {
+    const void* a;
+    const void* b;
+    const float* before;   // sums of the earlier pieces, or null
+    void* y;
+    const int32_t* token;  // y's row for a row of the piece, or null: its own
+    float* partial;        // [splits][m][ldp]
+    int64_t lda, ldb, ldy, ldbefore, ldp, m, n, k, m_in, n_in;  // m_in, n_in: rows that the operands hold
+    int tiles_n, splits;
+    Piece piece;
+};
+
+// y = a b (dx: the rows of a are the piece's; dW: the sum runs over them), times the call's scale.
+template <int D, int OD, bool kRows>
+struct GradEpilogue {
+    const GradArgs& p;
+    float scale;
+    int first;
+    __device__ __forceinline__ f32x4 before(int64_t i, int64_t j, int have) const {
+        return p.before == nullptr ? f32x4{0.f, 0.f, 0.f, 0.f} : load_row<F32>(p.before, i * p.ldbefore + j, have);
+    }
+    __device__ __forceinline__ void store(int64_t i, int64_t j, int have, f32x4 v, f32x4 before) const {
+        v = v * scale + before;
+        const int64_t row = kRows ? p.token[first + i] : i;
+        store_row<OD>(p.y, row * p.ldy + j, have, v);
+    }
+};
+
+template <int D, int OD, bool kRows, class T, bool kAsync>
+__global__ __launch_bounds__(T::kThreads, 2) void grad_kernel(GradArgs p) {
+    extern __shared__ __align__(16) char lds[];
+    int first, count;
+    piece_rows(p.piece, first, count);
+    const int64_t m = kRows ? count : p.m, k = kRows ? p.k : count;
+    const int tiles_m = static_cast<int>((m + T::BM - 1) / T::BM), total = tiles_m * p.tiles_n;
+    if (static_cast<int>(blockIdx.x) >= total) return;
+    int tm, tn;
+    band_order<8>(xcd_tile(blockIdx.x, total), tiles_m, p.tiles_n, tm, tn);
+    const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
+    constexpr int BK = tile_k<D>();
+    const int64_t part = ((k + p.splits - 1) / p.splits + BK - 1) / BK * BK;
+    const int64_t k0 = min<int64_t>(k, blockIdx.y * part), k1 = min<int64_t>(k, k0 + part);
+    f32x4 acc[T::TM][T::TN];
+    const char* b = static_cast<const char*>(p.b) + (kRows ? 0 : first * p.ldb * elem_bytes<D>());
+    tile_product<D, kRows, false, T, kAsync>(p.a, p.lda, m0, kRows ? m : p.m_in, b, p.ldb, n0, p.n_in, k0, k1, lds, acc);
+    const int rows = static_cast<int>(min<int64_t>(m - m0, T::BM)), cols = static_cast<int>(min<int64_t>(p.n - n0, T::BN));
+    const GradEpilogue<D, OD, kRows> tile{p, p.piece.control->scale_out, first};
+    float* partial = p.partial == nullptr ? nullptr : p.partial + (blockIdx.y * p.m + m0) * p.ldp + n0;
+    finish_tile<T, kAsync, 2>(
+        lds, acc,
+        [&](int i, int j) {
+            return i < rows && j < cols && partial == nullptr ? tile.before(m0 + i, n0 + j, cols - j)
+                                                              : f32x4{0.f, 0.f, 0.f, 0.f};
+        },
+        [&](int i, int j, f32x4 v, f32x4 before) {
+            if (i >= rows || j >= cols) return v;
+            if (partial != nullptr) *reinterpret_cast<f32x4*>(partial + i * p.ldp + j) = v;
+            else tile.store(m0 + i, n0 + j, cols - j, v, before);
+            return v;
+        });
+}
+
+// Joins the parts of a split sum, in their order.
+template <int D, int OD, bool kRows>
+__global__ __launch_bounds__(256) void grad_join_kernel(GradArgs p) {
+    int first, count;
+    piece_rows(p.piece, first, count);
+    const int64_t m = kRows ? count : p.m, units = p.ldp / 4, total = m * units;
+    const GradEpilogue<D, OD, kRows> tile{p, p.piece.control->scale_out, first};
+    for (int64_t u = blockIdx.x * int64_t(256) + threadIdx.x; u < total; u += int64_t(gridDim.x) * 256) {
+        const int64_t i = u / units, j = u % units * 4;
+        f32x4 v = *reinterpret_cast<const f32x4*>(p.partial + i * p.ldp + j);
+        for (int s = 1; s < p.splits; ++s) v += *reinterpret_cast<const f32x4*>(p.partial + (s * p.m + i) * p.ldp + j);
+        const int have = static_cast<int>(min<int64_t>(p.n - j, 4));
+        tile.store(i, j, have, v, tile.before(i, j, have));
+    }
+}
+
+// ---- the bias gradient: column sums of dz ------------------------------------------------
+constexpr int kBiasBlocks = 64;  // parts that the rows of a piece are summed in
+template <int D>
+__global__ __launch_bounds__(256) void bias_part_kernel(const void* dz, int64_t ld, int64_t vocab, float* parts,
+                                                        Piece piece) {
+    int first, count;
+    piece_rows(piece, first, count);
+    const int64_t j = blockIdx.x * int64_t(256) + threadIdx.x;
+    if (j >= vocab) return;
+    const int each = (count + kBiasBlocks - 1) / kBiasBlocks, from = blockIdx.y * each, to = min(count, from + each);
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int i = from; i < to; ++i) sum += load_elem<D>(dz, i * ld + j);
+    parts[blockIdx.y * vocab + j] = sum;
+}
+// The parts in order, and the earlier pieces' sum; the last piece rounds it to `db`.
+template <int OD>
+__global__ __launch_bounds__(256) void bias_join_kernel(const float* parts, float* sums, void* db, int64_t vocab,
+                                                        Piece piece) {
+    const int64_t j = blockIdx.x * int64_t(256) + threadIdx.x;
+    if (j >= vocab) return;
+    float sum = 0.0f;
+    for (int b = 0; b < kBiasBlocks; ++b) sum += parts[b * vocab + j];
+    sum *= piece.control->scale_out;
+    if (piece.piece > 0) sum += sums[j];
+    if (piece.piece + 1 < piece.pieces) sums[j] = sum;
+    else store_elem<OD>(db, j, sum);
+}
+
+// ---- gradients held in fp32 until the loss's own gradient is known ---------------------------
+template <int OD>
+__global__ __launch_bounds__(256) void scale_round_kernel(const float* src, void* dst, int64_t n, const float* factor,
+                                                          int64_t block_base) {
+    const float f = *factor;
+    const int64_t i = ((block_base + blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (i < n) store_row<OD>(dst, i, static_cast<int>(min<int64_t>(n - i, 4)),
+                             load_row<F32>(src, i, static_cast<int>(min<int64_t>(n - i, 4))) * f);
+}
+
+// ---- host ------------------------------------------------------------------------------------
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Everything a call's launches and working storage follow from.
+struct Plan {
+    bool thin, grads, rows_only;
+    int size;               // logit tiles
+    int tiles, pieces;
+    int64_t most;           // rows of a piece, at most
+    int64_t ld, ldk;        // gathered rows; exponentials
+    int64_t control, place, token, word, weight, target, row, row_loss, rows, stats, sums, kept, dw_sums, db_sums,
+        parts, partial, bytes;
+};
+
+// `aligned`: W's rows load straight into LDS, which tiles of 256 need.
+Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants, int grad_dtype, bool smooth,
+             bool aligned) {
+    Plan p{};
+    const int64_t size = dtype == F32 ? 4 : 2;
+    p.grads = wants != 0;
+    p.thin = tokens <= kThin && !p.grads;
+    p.ld = up(std::max<int64_t>(inner, 1), 64);
+    p.ldk = up(vocab, 64);
+    int64_t at = 0;
+    const auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += up(bytes, 256);
+        return here;
+    };
+    if (p.thin) {
+        p.tiles = static_cast<int>((vocab + 15) / 16);
+        p.pieces = 1, p.most = tokens;
+    } else {
+        p.size = 0;
+        double least = 0.0;
+        const double steps = static_cast<double>((inner + (dtype == F32 ? 31 : 63)) / (dtype == F32 ? 32 : 64));
+        const int64_t rows = std::min<int64_t>(tokens, std::max<int64_t>(256, kPieceBytes / (p.ldk * size)));
+        for (const int s : {64, 128, 256}) {
+            if (s == 256 && (dtype == F32 || !aligned)) continue;
+            const double cost = round_cost(s, ((rows + s - 1) / s) * ((vocab + s - 1) / s), steps, dtype == F32,
+                                           s == 256 ? 9.0 : (s == 128 ? 6.0 : 3.5));
+            if (least == 0.0 || cost < least) least = cost, p.size = s;
+        }
+        p.tiles = static_cast<int>((vocab + p.size - 1) / p.size);
+        const int64_t row_bytes = p.grads ? p.ldk * size : 12 * p.tiles;
+        p.most = std::max<int64_t>(256, (p.grads ? kPieceBytes : kStatsBytes) / row_bytes / 256 * 256);
+        p.most = std::min(p.most, kMostRows);
+        p.pieces = static_cast<int>((tokens + p.most - 1) / p.most);
+        p.most = std::min(up(up(tokens, p.pieces) / p.pieces, 256), tokens);
+    }
+    p.target = take(4 * tokens);
+    p.row_loss = take(8 * tokens);
+    p.stats = take(8 * p.most * p.tiles);
+    p.sums = smooth ? take(4 * p.most * p.tiles) : 0;
+    if (!p.thin) {
+        p.control = take(sizeof(Control));
+        p.place = take(4 * tokens);
+        p.token = take(4 * tokens);
+        p.word = take(4 * tokens);
+        p.weight = take(4 * tokens);
+        p.rows = take(size * tokens * p.ld);
+    }
+    if (p.grads) {
+        p.row = take(sizeof(Row) * tokens);
+        p.kept = take(size * p.most * p.ldk);
+        const bool carried = p.pieces > 1;
+        if ((wants & HBT_LINEAR_DW) && carried && grad_dtype != F32) p.dw_sums = take(4 * vocab * inner);
+        if (wants & HBT_LINEAR_DBIAS) {
+            p.parts = take(4 * kBiasBlocks * vocab);
+            p.db_sums = take(4 * vocab);
+        }
+        int64_t partial = 0;
+        const auto split = [&](int64_t m, int64_t n, int64_t k) {
+            const int splits = std::max(choose(m, n, k, dtype, true).splits, choose(m, n, k, dtype, false).splits);
+            if (splits > 1) partial = std::max(partial, 4 * splits * m * up(n, 4));
+        };
+        if ((wants & HBT_LINEAR_DX) && inner > 0) split(p.most, inner, vocab);
+        if ((wants & HBT_LINEAR_DW) && inner > 0) split(vocab, inner, p.most);
+        p.partial = take(partial);
+    }
+    p.bytes = at;
+    return p;
+}
+
+template <class T, bool kAsync, class Kernel, class Args>
+int32_t launch(const char* who, Kernel kernel, const Args& args, int64_t tiles, int splits, std::atomic<uint64_t>& done,
+               hipStream_t s) {
+    constexpr int kLds = lds_bytes<T, kAsync>();
+    if constexpr (kLds > 65536) {
+        const int32_t status = allow_lds(who, reinterpret_cast<const void*>(kernel), kLds, done);
+        if (status != HBT_OK) return status;
+    }
+    kernel<<<dim3(static_cast<unsigned>(tiles), splits), T::kThreads, kLds, s>>>(args);
+    return check_launch(who);
+}
+
+template <int D, class T, bool kAsync>
+int32_t launch_logits(const char* who, const LogitArgs& p, int64_t rows, hipStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    return launch<T, kAsync>(who, logit_kernel<D, T, kAsync>, p, (rows + T::BM - 1) / T::BM * p.tiles_n, 1, done, s);
+}
+
+template <int D, int OD, bool kRows, class T, bool kAsync>
+int32_t launch_grad_tile(const char* who, GradArgs& p, hipStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    p.tiles_n = static_cast<int>((p.n + T::BN - 1) / T::BN);
+    return launch<T, kAsync>(who, grad_kernel<D, OD, kRows, T, kAsync>, p, (p.m + T::BM - 1) / T::BM * p.tiles_n,
+                             p.splits, done, s);
+}
+
+// p.m or p.k is the most that the piece's rows may be.
+template <int D, int OD, bool kRows>
+int32_t launch_grad(const char* who, GradArgs& p, bool aligned, void* space, hipStream_t s) {
+    const Choice c = choose(p.m, p.n, p.k, D, aligned);
+    p.splits = c.splits;
+    p.ldp = up(p.n, 4);
+    p.partial = c.splits > 1 ? static_cast<float*>(space) : nullptr;
+    int32_t status = HBT_OK;
+    if (c.tile == 64) {
+        status = aligned ? launch_grad_tile<D, OD, kRows, Tile64, true>(who, p, s)
+                         : launch_grad_tile<D, OD, kRows, Tile64, false>(who, p, s);
+    } else if (c.tile == 128) {
+        status = aligned ? launch_grad_tile<D, OD, kRows, Tile128, true>(who, p, s)
+                         : launch_grad_tile<D, OD, kRows, Tile128, false>(who, p, s);
+    } else if constexpr (D != F32) {
+        status = launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, s);
+    }
+    if (status != HBT_OK || c.splits == 1) return status;
+    const int64_t blocks = std::min<int64_t>((p.m * (p.ldp / 4) + 255) / 256, 4096);
+    grad_join_kernel<D, OD, kRows><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(p);
+    return check_launch(who);
+}
+
+int32_t refuse(const char* who, const char* what) {
+    set_error("%s: %s", who, what);
+    return HBT_ERR_INVALID_ARGUMENT;
+}
+
+int32_t check_sizes(const char* who, int64_t tokens, int64_t inner, int64_t vocab, int32_t dtype, int32_t wants,
+                    int32_t grad_dtype) {
+    if (tokens < 0 || inner < 0) return refuse(who, "a size is negative");
+    if (vocab < 1) return refuse(who, "the vocabulary is empty");
+    if (dtype != F32 && dtype != BF16 && dtype != F16) {
+        set_error("%s: dtype %d is not F32, BF16 or F16", who, dtype);
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    if (wants < 0 || wants > 7) return refuse(who, "unknown results are wanted");
+    if (wants != 0 && grad_dtype != dtype && grad_dtype != F32) return refuse(who, "gradients are of the tensors' dtype or F32");
+    if (vocab > kMaxLd - 64 || inner > kMaxLd - 64 || tokens > kMostTokens) {
+        set_error("%s: %lld tokens of %lld over %lld words are past the limits", who, static_cast<long long>(tokens),
+                  static_cast<long long>(inner), static_cast<long long>(vocab));
+        return HBT_ERR_UNSUPPORTED;
+    }
+    return HBT_OK;
+}
+
+int32_t check_rows(const char* who, const void* p, int64_t rows, int64_t cols, int64_t ld, const char* name) {
+    if (rows == 0 || cols == 0) return HBT_OK;
+    if (p == nullptr || ld < cols || ld > kMaxLd) {
+        set_error("%s: %s is null, or its rows are %lld elements apart (from %lld to %lld)", who, name,
+                  static_cast<long long>(ld), static_cast<long long>(cols), static_cast<long long>(kMaxLd));
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    return HBT_OK;
+}
+
+struct Call {
+    const void *x, *w, *bias;
+    const int64_t* target;
+    const float* token_grads;
+    float* loss;
+    void *dx, *dw, *db;
+    int64_t ldx, ldw, lddx, lddw, tokens, inner, vocab, ignore;
+    int reduction, wants;
+    float smoothing;
+};
+
+template <int D, int OD>
+int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipStream_t s) {
+    const auto at = [&](int64_t offset) { return static_cast<void*>(space + offset); };
+    float2* stats = static_cast<float2*>(at(plan.stats));
+    float* sums = c.smoothing != 0.0f ? static_cast<float*>(at(plan.sums)) : nullptr;
+    float* target = static_cast<float*>(at(plan.target));
+    double* row_loss = c.reduction == HBT_LOSS_NONE || c.loss == nullptr ? nullptr : static_cast<double*>(at(plan.row_loss));
+    float* token_loss = c.reduction == HBT_LOSS_NONE ? c.loss : nullptr;
+    const int mean = c.reduction == HBT_LOSS_MEAN;
+    int32_t status = HBT_OK;
+    JoinArgs join{};
+    join.stats = stats, join.sums = sums, join.target = target, join.loss = token_loss, join.row_loss = row_loss;
+    join.ignore = c.ignore, join.vocab = c.vocab, join.tiles = plan.tiles, join.smoothing = c.smoothing;
+    if (plan.thin) {
+        thin_logit_kernel<D><<<dim3(plan.tiles), 512, 0, s>>>(c.x, c.ldx, c.w, c.ldw, c.bias, c.target,
+                                                              static_cast<int>(c.tokens), c.vocab, c.inner, stats, sums, target);
+        if ((status = check_launch(who)) != HBT_OK) return status;
+        join.raw = c.target, join.rows = static_cast<int>(c.tokens);
+        join_kernel<<<dim3(static_cast<unsigned>(c.tokens)), 256, 0, s>>>(join);
+        if ((status = check_launch(who)) != HBT_OK || row_loss == nullptr) return status;
+        total_kernel<<<1, 1024, 0, s>>>(row_loss, nullptr, c.target, c.ignore, c.tokens, mean, c.loss);
+        return check_launch(who);
+    }
+    Control* control = static_cast<Control*>(at(plan.control));
+    int32_t* token = static_cast<int32_t*>(at(plan.token));
+    int32_t* word = static_cast<int32_t*>(at(plan.word));
+    int32_t* place = static_cast<int32_t*>(at(plan.place));
+    float* weight = static_cast<float*>(at(plan.weight));
+    void* rows = at(plan.rows);
+    prepare_kernel<<<1, 1024, 0, s>>>({c.target, c.token_grads, control, place, token, word, weight, c.tokens, c.vocab,
+                                       c.ignore, mean, D == F16 && plan.grads});
+    if ((status = check_launch(who)) != HBT_OK) return status;
+    gather_kernel<D><<<dim3(static_cast<unsigned>((c.tokens + 3) / 4)), 256, 0, s>>>(
+        {c.x, place, rows, c.dx, token_loss, c.ldx, plan.ld, c.lddx, c.tokens, c.inner, OD == F32});
+    if ((status = check_launch(who)) != HBT_OK) return status;
+    const bool aligned = is_aligned(c.w, c.ldw, c.inner, D);
+    void* kept = plan.grads ? at(plan.kept) : nullptr;
+    Row* row = plan.grads ? static_cast<Row*>(at(plan.row)) : nullptr;
+    for (int i = 0; i < plan.pieces; ++i) {
+        const Piece piece{control, i, plan.pieces};
+        LogitArgs l{};
+        l.x = rows, l.w = c.w, l.bias = c.bias, l.word = word, l.stats = stats, l.sums = sums, l.target = target;
+        l.kept = kept, l.ldx = plan.ld, l.ldw = c.ldw, l.ldk = plan.ldk, l.vocab = c.vocab, l.inner = c.inner;
+        l.tiles_n = plan.tiles, l.piece = piece;
+        if (plan.size == 64) {
+            status = aligned ? launch_logits<D, Tile64, true>(who, l, plan.most, s)
+                             : launch_logits<D, Tile64, false>(who, l, plan.most, s);
+        } else if (plan.size == 128) {
+            status = aligned ? launch_logits<D, Tile128, true>(who, l, plan.most, s)
+                             : launch_logits<D, Tile128, false>(who, l, plan.most, s);
+        } else if constexpr (D != F32) {
+            status = launch_logits<D, Tile256, true>(who, l, plan.most, s);
+        }
+        if (status != HBT_OK) return status;
+        join.word = word, join.token = token, join.weight = weight, join.row = row, join.piece = piece;
+        join_kernel<<<dim3(static_cast<unsigned>(plan.most)), 256, 0, s>>>(join);
+        if ((status = check_launch(who)) != HBT_OK) return status;
+        if (!plan.grads) continue;
+        const int segment = 256 * unit_elems<D>() * 4;
+        softmax_kernel<D><<<dim3(static_cast<unsigned>((plan.ldk + segment - 1) / segment * plan.most)), 256, 0, s>>>({kept, stats, row, word, plan.ldk,
+                                                                          c.vocab, plan.tiles, plan.size, segment,
+                                                                          c.smoothing, piece});
+        if ((status = check_launch(who)) != HBT_OK) return status;
+        const bool last = i + 1 == plan.pieces;
+        if ((c.wants & HBT_LINEAR_DX) && c.inner > 0) {
+            GradArgs g{};
+            g.a = kept, g.b = c.w, g.y = c.dx, g.token = token, g.lda = plan.ldk, g.ldb = c.ldw, g.ldy = c.lddx;
+            g.m = plan.most, g.n = c.inner, g.k = c.vocab, g.m_in = plan.most, g.n_in = c.inner, g.piece = piece;
+            if ((status = launch_grad<D, OD, true>(who, g, aligned, at(plan.partial), s)) != HBT_OK) return status;
+        }
+        if ((c.wants & HBT_LINEAR_DW) && c.inner > 0) {
+            GradArgs g{};
+            g.a = kept, g.b = rows, g.lda = plan.ldk, g.ldb = plan.ld;
+            g.m = c.vocab, g.n = c.inner, g.k = plan.most, g.m_in = up(c.vocab, 8), g.n_in = up(c.inner, 8), g.piece = piece;
+            // Between pieces the sums stand dense in fp32: in working storage, or in an fp32 result.
+            float* carried = OD == F32 ? static_cast<float*>(c.dw) : static_cast<float*>(at(plan.dw_sums));
+            const int64_t ldcarried = OD == F32 ? c.lddw : c.inner;
+            g.before = i > 0 ? carried : nullptr, g.ldbefore = ldcarried;
+            if (last) {
+                g.y = c.dw, g.ldy = c.lddw;
+                status = launch_grad<D, OD, false>(who, g, true, at(plan.partial), s);
+            } else {
+                g.y = carried, g.ldy = ldcarried;
+                status = launch_grad<D, F32, false>(who, g, true, at(plan.partial), s);
+            }
+            if (status != HBT_OK) return status;
+        }
+        if (c.wants & HBT_LINEAR_DBIAS) {
+            float* parts = static_cast<float*>(at(plan.parts));
+            const unsigned blocks = static_cast<unsigned>((c.vocab + 255) / 256);
+            bias_part_kernel<D><<<dim3(blocks, kBiasBlocks), 256, 0, s>>>(kept, plan.ldk, c.vocab, parts, piece);
+            if ((status = check_launch(who)) != HBT_OK) return status;
+            bias_join_kernel<OD><<<dim3(blocks), 256, 0, s>>>(parts, static_cast<float*>(at(plan.db_sums)), c.db, c.vocab, piece);
+            if ((status = check_launch(who)) != HBT_OK) return status;
+        }
+    }
+    if (row_loss == nullptr) return HBT_OK;
+    total_kernel<<<1, 1024, 0, s>>>(row_loss, control, nullptr, c.ignore, 0, mean, c.loss);
+    return check_launch(who);
+}
+
+}  // namespace
+}  // namespace mm
+}  // namespace hbt
+
+using namespace hbt;
+using namespace hbt::mm;
+
+extern "C" {
+
+int64_t hbt_linear_cross_entropy_workspace(int64_t tokens, int64_t inner, int64_t vocab, int32_t dtype, int32_t wants,
+                                           int32_t grad_dtype, float smoothing) {
+    clear_error();
+    const char* who = "hbt_linear_cross_entropy_workspace";
+    if (check_sizes(who, tokens, inner, vocab, dtype, wants, grad_dtype) != HBT_OK) return -1;
+    if (tokens == 0) return 0;
+    const bool smooth = smoothing != 0.0f;
+    return std::max(plan_of(tokens, inner, vocab, dtype, wants, grad_dtype, smooth, true).bytes,
+                    plan_of(tokens, inner, vocab, dtype, wants, grad_dtype, smooth, false).bytes);
+}
+
+int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                                 const int64_t* target, const float* token_grads, float* loss, void* dx, int64_t lddx,
+                                 void* dw, int64_t lddw, void* dbias, int64_t tokens, int64_t inner, int64_t vocab,
+                                 int32_t dtype, int32_t grad_dtype, int64_t ignore_index, float smoothing,
+                                 int32_t reduction, void* workspace, int64_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* who = "hbt_linear_cross_entropy";
+    const int32_t wants = (dx != nullptr ? HBT_LINEAR_DX : 0) | (dw != nullptr ? HBT_LINEAR_DW : 0) |
+                          (dbias != nullptr ? HBT_LINEAR_DBIAS : 0);
+    int32_t status = check_sizes(who, tokens, inner, vocab, dtype, wants, grad_dtype);
+    if (status != HBT_OK) return status;
+    if (!(smoothing >= 0.0f && smoothing <= 1.0f)) return refuse(who, "smoothing lies outside [0, 1]");
+    if (reduction < HBT_LOSS_NONE || reduction > HBT_LOSS_SUM) return refuse(who, "unknown reduction");
+    if (reduction != HBT_LOSS_NONE && token_grads != nullptr) return refuse(who, "token_grads belong to separate losses");
+    if (tokens == 0) return refuse(who, "there are no tokens");
+    if (loss == nullptr && wants == 0) return refuse(who, "nothing is wanted");
+    if (target == nullptr) return refuse(who, "target is null");
+    if ((status = check_rows(who, x, tokens, inner, ldx, "x")) != HBT_OK ||
+        (status = check_rows(who, w, vocab, inner, ldw, "w")) != HBT_OK ||
+        (dx != nullptr && (status = check_rows(who, dx, tokens, inner, lddx, "dx")) != HBT_OK) ||
+        (dw != nullptr && (status = check_rows(who, dw, vocab, inner, lddw, "dw")) != HBT_OK))
+        return status;
+    const Plan plan = plan_of(tokens, inner, vocab, dtype, wants, grad_dtype, smoothing != 0.0f,
+                              is_aligned(w, ldw, inner, dtype));
+    if (workspace == nullptr || workspace_bytes < plan.bytes || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+        return refuse(who, "the workspace is smaller than hbt_linear_cross_entropy_workspace's, or off 256 bytes");
+    const Call c{x, w, bias, target, token_grads, loss, dx, dw, dbias, ldx, ldw, lddx, lddw, tokens, inner, vocab,
+                 ignore_index, reduction, wants, smoothing};
+    char* space = static_cast<char*>(workspace);
+    const hipStream_t s = as_stream(stream);
+    const bool wide = wants != 0 && grad_dtype == F32;
+    if (dtype == F32) return run<F32, F32>(who, c, plan, space, s);
+    if (dtype == BF16) return wide ? run<BF16, F32>(who, c, plan, space, s) : run<BF16, BF16>(who, c, plan, space, s);
+    return wide ? run<F16, F32>(who, c, plan, space, s) : run<F16, F16>(who, c, plan, space, s);
+}
+
+int32_t hbt_scale_round(const float* src, void* dst, int64_t numel, int32_t dtype, const float* factor, void* stream) {
+    clear_error();
+    const char* who = "hbt_scale_round";
+    if (dtype != F32 && dtype != BF16 && dtype != F16) {
+        set_error("%s: dtype %d is not F32, BF16 or F16", who, dtype);
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    if (numel < 0) return refuse(who, "numel is negative");
+    if (numel > 0 && (src == nullptr || dst == nullptr || factor == nullptr)) return refuse(who, "a pointer is null");
+    return launch_sliced(who, (numel + 1023) / 1024, 256, [&](int64_t first, dim3 grid) {
+        const hipStream_t s = as_stream(stream);
+        if (dtype == F32) scale_round_kernel<F32><<<grid, 256, 0, s>>>(src, dst, numel, factor, first);
+        else if (dtype == BF16) scale_round_kernel<BF16><<<grid, 256, 0, s>>>(src, dst, numel, factor, first);
+        else scale_round_kernel<F16><<<grid, 256, 0, s>>>(src, dst, numel, factor, first);
+    });
+}
+
+}  // extern "C"

@@ -650,5 +650,77 @@ inline double round_cost(int size, int64_t tiles, double steps, bool f32, double
     return static_cast<double>((tiles + 2 * kCus - 1) / (2 * kCus)) * (steps * step + fixed);
 }
 
+struct Choice {
+    int tile;    // 256, 128 or 64
+    int splits;  // parts the sum over k is split into
+};
+
+// Work-items of a launch over every tile.
+inline int64_t tile_items(int64_t m, int64_t n, int size) {
+    return ((m + size - 1) / size) * ((n + size - 1) / size) * (size == 256 ? 512 : 256);
+}
+
+// The cheapest tile and split by the estimate.  A split sum writes and reads its fp32 parts (about
+// 5 TB/s) in one more launch.  Tiles of 256 need operands that load straight into LDS.
+inline Choice choose(int64_t m, int64_t n, int64_t k, int dtype, bool aligned) {
+    const bool f32 = dtype == HBT_DTYPE_F32;
+    const int64_t steps = (k + (f32 ? 31 : 63)) / (f32 ? 32 : 64);
+    Choice best{128, 1};
+    double least = 0.0;
+    for (const int size : {64, 128, 256}) {
+        if ((size == 256 && (f32 || !aligned)) || tile_items(m, n, size) > kGridMaxItems) continue;
+        const double fixed = size == 256 ? 9.0 : (size == 128 ? 6.0 : 3.5);
+        const int64_t tiles = ((m + size - 1) / size) * ((n + size - 1) / size);
+        for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            if (splits > 1 && (steps < 4 * splits || tiles * splits > 1024)) break;
+            double cost = round_cost(size, tiles * splits, static_cast<double>((steps + splits - 1) / splits), f32, fixed);
+            if (splits > 1) cost += 3.0 + 8.0 * m * n * splits / 5.0e6;
+            if (least == 0.0 || cost < least) least = cost, best = {size, splits};
+        }
+    }
+    return best;
+}
+
+// Whether an operand's 16-byte units can be loaded straight into LDS: rows on 16 bytes and no unit
+// across the last k (k-major) or the last row.
+inline bool is_aligned(const void* p, int64_t ld, int64_t extent, int dtype) {
+    const int64_t unit = dtype == HBT_DTYPE_F32 ? 4 : 8;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % unit == 0 && extent % unit == 0;
+}
+
+// One product in tiles of 256, its last columns or rows in tiles of 128 where that is estimated
+// to be shorter: a round of 256 that is mostly empty takes as long as a full one.  896 tiles (the
+// weight gradient of 8192 x 4096 x 14336) are three rounds and a half, 850 us, and 797 cut; 788
+// (1024 x 768 x 50257) are three and 20 tiles, 113 us, and 102 cut (one set of inputs, which the
+// memory-side cache holds; from memory 915 and 851, 124 and 119).
+struct Cut {
+    int64_t m, n;  // the part in tiles of 256
+};
+inline Cut cut_of(int64_t m, int64_t n, int64_t k) {
+    const int64_t rows = (m + 255) / 256, cols = (n + 255) / 256;
+    const double steps = static_cast<double>((k + 63) / 64);
+    const auto rest = [&](int64_t r, int64_t c) {
+        return r <= 0 || c <= 0 ? 0.0 : round_cost(128, ((r + 127) / 128) * ((c + 127) / 128), steps, false, 6.0) + 3.0;
+    };
+    Cut best{m, n};
+    double least = 0.97 * round_cost(256, rows * cols, steps, false, 9.0);
+    for (int64_t less = 1; less < 256; ++less) {  // tile rows or columns left to the second launch
+        if (less < rows && less * cols < 256) {
+            const double cost = round_cost(256, (rows - less) * cols, steps, false, 9.0) + rest(m - (rows - less) * 256, n);
+            if (cost < least) least = cost, best = {(rows - less) * 256, n};
+        }
+        if (less < cols && less * rows < 256) {
+            const double cost = round_cost(256, rows * (cols - less), steps, false, 9.0) + rest(m, n - (cols - less) * 256);
+            if (cost < least) least = cost, best = {m, (cols - less) * 256};
+        }
+    }
+    return best;
+}
+
+// Rows of a tile are addressed by 31-bit byte offsets from its first one.
+constexpr int64_t kMaxLd = int64_t(1) << 20;
+// No launch over one side alone passes a grid's 2^32 - 1 work-items.
+constexpr int64_t kMaxSide = int64_t(1) << 26;
+
 }  // namespace mm
 }  // namespace hbt

@@ -30,6 +30,7 @@ from .errors import (
     format_error,
 )
 from .buckets import BucketedGradients, BucketLayout, GradientBucket, build_buckets
+from .cross_entropy import LinearCrossEntropy, linear_cross_entropy
 from .flat_param import (FlatParameter, FlatParamHandle, PieceLayout, ShardedTensorPiece, optimizer_parameter_layout,
                          reshard_state_dict_pieces)
 from .grad_scaler import GradScaler, GradScalerState

@@ -70,7 +70,7 @@ __all__ = [
     "stream_of",
 ]
 
-ABI_VERSION = 23
+ABI_VERSION = 24
 MAX_TENSORS_PER_LAUNCH = 16
 MAX_MATRICES = 32
 MAX_ADAMW8_TENSORS = 56
@@ -312,6 +312,14 @@ EXPORTED_SYMBOLS: dict[str, tuple[object, tuple[object, ...]]] = {
          _c_void_p,
          _c_void_p, _c_i64, _c_void_p),
     ),
+    "hbt_linear_cross_entropy_workspace": (_c_i64, (_c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32)),
+    "hbt_linear_cross_entropy": (
+        _c_i32,
+        (_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p,
+         _c_i64, _c_void_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i64, _c_f32, _c_i32, _c_void_p, _c_i64,
+         _c_void_p),
+    ),
+    "hbt_scale_round": (_c_i32, (_c_void_p, _c_void_p, _c_i64, _c_i32, _c_void_p, _c_void_p)),
     "hbt_adamw8_step": (
         _c_i32,
         (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_i32,

@@ -766,6 +766,52 @@ int32_t hbt_moments8_decode(const void* const* m_codes, const void* const* v_cod
                             const float* const* v_scales, void* const* firsts, void* const* seconds,
                             const int64_t* numels, int32_t count, int32_t out_dtype, void* stream);
 
+/* ------------------------------------------------------------------------------
+ * Softmax cross entropy over a vocabulary from hidden states, with its gradients, the logits
+ * never in memory.
+ *
+ * Replaces: the output layer and the loss of TrainingEngine.train_step's forward and backward
+ *   passes (training/engine.py:352-422), which the reference leaves to torch.
+ * x is [tokens][ldx], w [vocab][ldw], both `inner` long, bias [vocab] or NULL, of one dtype (F32,
+ * BF16 or F16); target holds one class a token:
+ *   z = x w^T + bias;  loss_i = (1 - smoothing) (lse(z_i) - z_i,target) + smoothing (lse(z_i) - mean z_i)
+ *   dz_i = c_i (softmax(z_i) - (1 - smoothing) onehot - smoothing / vocab)
+ *   dx = dz w,  dw = dz^T x,  dbias = column sums of dz
+ * A token whose target is ignore_index has loss 0, a zero row of dx and no part in the rest,
+ * whatever its row of x holds.  Any other target outside [0, vocab) makes its loss, and every
+ * gradient that the token takes part in, NaN.
+ * reduction HBT_LOSS_NONE: loss is [tokens] fp32 (NULL for the gradients alone) and c_i =
+ * token_grads[i] (fp32; NULL = 1).  HBT_LOSS_SUM: loss is one fp32, c_i = 1.  HBT_LOSS_MEAN:
+ * its quotient by the number of tokens that are not ignored (0 / 0, NaN, without any), c_i one over that
+ * number (gradients are zeros without any).
+ * dx, dw and dbias may each be NULL; they are of grad_dtype: dtype, or F32.  Sums and statistics are
+ * fp32 or wider; dz is rounded to `dtype` once, for the matrix cores.  No atomics: results
+ * repeat bitwise.  Rows are at most 2^20 elements apart, vocab and inner at most 2^20 - 64, tokens
+ * from 1 to 2^24.
+ * `workspace` (256-byte aligned) holds at least hbt_linear_cross_entropy_workspace's bytes (-1
+ * for sizes that the call refuses; `wants`: HBT_LINEAR_DX / DW / DBIAS of the gradients given):
+ * at most 1 GiB of exponentials, the gathered rows, and an fp32 dw where there are more.
+ * ---------------------------------------------------------------------------- */
+#define HBT_LOSS_NONE 0
+#define HBT_LOSS_MEAN 1
+#define HBT_LOSS_SUM 2
+int64_t hbt_linear_cross_entropy_workspace(int64_t tokens, int64_t inner, int64_t vocab, int32_t dtype, int32_t wants,
+                                           int32_t grad_dtype, float smoothing);
+int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                                 const int64_t* target, const float* token_grads, float* loss, void* dx, int64_t lddx,
+                                 void* dw, int64_t lddw, void* dbias, int64_t tokens, int64_t inner, int64_t vocab,
+                                 int32_t dtype, int32_t grad_dtype, int64_t ignore_index, float smoothing,
+                                 int32_t reduction, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * dst[i] = src[i] * (*factor), an fp32 product rounded once to dst's dtype (F32, BF16 or F16).
+ *
+ * Replaces: the multiplication by the loss's own gradient that autograd's backward pass
+ *   (training/engine.py:352-422) starts with, for fp32 gradients held until then.
+ * `factor` is one fp32 in device memory.  dst may be src for F32 only.
+ * ---------------------------------------------------------------------------- */
+int32_t hbt_scale_round(const float* src, void* dst, int64_t numel, int32_t dtype, const float* factor, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,68 @@
+"""What the loss over a vocabulary refuses, and its working storage, without a device."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from hybrid_training_amd import LinearCrossEntropy, _native, linear_cross_entropy
+from hybrid_training_amd.errors import UnsupportedFeatureError
+
+GIB = 1 << 30
+
+
+def test_host_tensors_are_refused():
+    head = LinearCrossEntropy(8, 20)
+    assert [tuple(p.shape) for p in head.parameters()] == [(20, 8)]
+    assert "vocabulary=20" in repr(head)
+    with pytest.raises(UnsupportedFeatureError, match="HIP device"):
+        head(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(UnsupportedFeatureError, match="reduction"):
+        linear_cross_entropy(torch.zeros(3, 8), torch.zeros(20, 8), torch.zeros(3, dtype=torch.int64), reduction="avg")
+
+
+def test_working_storage():
+    size = _native.library().hbt_linear_cross_entropy_workspace
+    assert size(0, 64, 100, 1, 0, 1, 0.0) == 0
+    # one token over a large vocabulary: statistics alone
+    assert 0 < size(1, 4096, 128256, 1, 0, 1, 0.0) < 1 << 20
+    # evaluation never holds logits, training at most 1 GiB of exponentials beside rows and fp32 sums
+    assert size(8192, 4096, 128256, 1, 0, 1, 0.0) < 8192 * 4096 * 2 + (1 << 28) + (8 << 20)
+    one = size(4096, 4096, 128256, 1, 3, 1, 0.0)
+    assert one < GIB + 4096 * 4096 * 2 + (1 << 27)
+    more = size(8192, 4096, 128256, 1, 3, 1, 0.0)
+    assert more < GIB + 8192 * 4096 * 2 + 4 * 128256 * 4096 + (1 << 27)
+    assert size(16384, 4096, 128256, 1, 3, 1, 0.0) - more < 8192 * 4096 * 2 + (4 << 20)
+    # fp32 results carry the sums themselves
+    assert size(8192, 4096, 128256, 1, 3, 0, 0.0) < more - 4 * 128256 * 4096 + (1 << 20)
+    assert size(10, 64, 100, 1, 0, 1, 0.1) > size(10, 64, 100, 1, 0, 1, 0.0)
+    for bad in ((-1, 64, 100, 1, 0, 1), (1, -1, 100, 1, 0, 1), (1, 64, 0, 1, 0, 1), (1, 64, 100, 3, 0, 1),
+                (1, 64, 100, 1, 8, 1), (1, 64, 100, 1, 1, 2), (1, 64, (1 << 20), 1, 0, 1), (1, 1 << 20, 100, 1, 0, 1),
+                ((1 << 24) + 1, 64, 100, 1, 0, 1)):
+        assert size(*bad, 0.0) == -1 and _native.library().hbt_last_error()
+    assert size(0, 64, 100, 1, 0, 1, 0.0) == 0  # leaves no message behind
+
+
+def test_the_library_refuses_bad_calls_before_any_launch():
+    lib = _native.library()
+    p = ctypes.c_void_p(4096)
+
+    def call(x=p, ldx=64, w=p, ldw=64, target=p, token_grads=None, loss=p, dx=None, lddx=0, dw=None, lddw=0, tokens=4,
+             inner=64, vocab=100, dtype=1, grad_dtype=1, smoothing=0.0, reduction=0, space=p, nbytes=1 << 30):
+        return lib.hbt_linear_cross_entropy(x, ldx, w, ldw, None, target, token_grads, loss, dx, lddx, dw, lddw, None,
+                                            tokens, inner, vocab, dtype, grad_dtype, -100, smoothing, reduction, space,
+                                            nbytes, None)
+
+    for wrong in (dict(tokens=0), dict(tokens=-1), dict(vocab=0), dict(dtype=3), dict(x=None), dict(w=None),
+                  dict(ldx=63), dict(ldw=(1 << 20) + 1), dict(target=None), dict(loss=None), dict(smoothing=-0.1),
+                  dict(smoothing=float("nan")), dict(reduction=3), dict(reduction=1, token_grads=p),
+                  dict(dx=p, lddx=63), dict(dw=p, lddw=63), dict(dx=p, lddx=64, grad_dtype=2), dict(space=None),
+                  dict(nbytes=16), dict(space=ctypes.c_void_p(4100))):
+        assert call(**wrong) in (-1, -2), wrong
+        assert b"hbt_linear_cross_entropy" in lib.hbt_last_error()
+    assert lib.hbt_scale_round(None, None, 4, 1, None, None) == -1
+    assert lib.hbt_scale_round(p, p, 4, 3, p, None) == -1
+    assert lib.hbt_scale_round(p, p, -4, 1, p, None) == -1
+    assert lib.hbt_scale_round(None, None, 0, 1, None, None) == 0  # nothing to do, and no message left behind
