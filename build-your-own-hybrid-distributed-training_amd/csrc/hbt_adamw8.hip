@@ -25,21 +25,23 @@ using mm::f32x4;
 using mm::load_row;
 using mm::store_row;
 
-constexpr int kBlock = 256;    // elements that share scales: one wavefront's four a lane
-constexpr int kWaves = 4;      // wavefronts of a workgroup
-constexpr int kUnroll = 2;     // blocks a wavefront has in flight
+constexpr int kBlock = 256;  // elements that share scales: one wavefront's four a lane
+// Encoding and decoding: four wavefronts, each with two blocks in flight (decoding 1,003,782,656
+// elements to bf16: 949 us; single wavefronts 983, four blocks a wavefront 1051).  The step: single
+// wavefronts with a block each (fp32: 2683 us; four wavefronts 2822, two blocks a wavefront 3015).
+constexpr int kWaves = 4, kUnroll = 2;
 constexpr int64_t kTile = int64_t(kBlock) * kWaves * kUnroll;
 constexpr int kMaxTensors = HBT_MAX_ADAMW8_TENSORS;
 // First moments this far under 1 would overflow the scale's reciprocal; such a block is held as zeros.
 constexpr float kLeastScale = 7.8886090522101181e-31f;  // 2^-100
 
+// Codes of four consecutive elements stand together, those of their first moments and then those of
+// their roots, so a lane moves them by one 8-byte access; a block's are 512 consecutive bytes.
 struct Table {
     void* p[kMaxTensors];
     void* g[kMaxTensors];
-    uint8_t* mc[kMaxTensors];
-    uint8_t* vc[kMaxTensors];
-    float* ms[kMaxTensors];
-    float* vs[kMaxTensors];
+    uint2* codes[kMaxTensors];
+    float2* scales[kMaxTensors];  // a block's M and R
     int64_t n[kMaxTensors];
     int64_t first[kMaxTensors];  // the tensor's first tile
     int32_t count;
@@ -60,35 +62,36 @@ __device__ __forceinline__ int owner(const Table& tab, int64_t tile) {
     return low;
 }
 
+// Magnitudes are compared as the whole numbers that their bits are, which orders non-negative floats.
+constexpr uint32_t kInfinity = 0x7F800000u;
+// The bits of |x|, or of 0 for what is not finite.
+__device__ __forceinline__ uint32_t magnitude(float x) {
+    const uint32_t bits = __float_as_uint(x) & 0x7FFFFFFFu;
+    return bits < kInfinity ? bits : 0u;
+}
 template <int kCtrl>
-__device__ __forceinline__ float row_move(float x) {
-    return __uint_as_float(__builtin_amdgcn_mov_dpp(static_cast<int>(__float_as_uint(x)), kCtrl, 0xF, 0xF, false));
+__device__ __forceinline__ uint32_t row_move(uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), kCtrl, 0xF, 0xF, false));
 }
-// The largest of a non-negative value over the wavefront, in every lane.
-__device__ __forceinline__ float wave_max(float x) {
-    const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(half[0]), __uint_as_float(half[1]));
-    const auto row = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(row[0]), __uint_as_float(row[1]));
-    x = fmaxf(x, row_move<0x128>(x));  // row_ror:8
-    x = fmaxf(x, row_move<0x124>(x));  // row_ror:4
-    x = fmaxf(x, row_move<0x4E>(x));   // quad_perm [2, 3, 0, 1]
-    return fmaxf(x, row_move<0xB1>(x));  // quad_perm [1, 0, 3, 2]
+// The largest over the wavefront, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    const auto half = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = max(half[0], half[1]);
+    const auto row = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(row[0], row[1]);
+    x = max(x, row_move<0x128>(x));  // row_ror:8
+    x = max(x, row_move<0x124>(x));  // row_ror:4
+    x = max(x, row_move<0x4E>(x));   // quad_perm [2, 3, 0, 1]
+    return max(x, row_move<0xB1>(x));  // quad_perm [1, 0, 3, 2]
 }
-
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
-__device__ __forceinline__ float magnitude(float x) { return finite(x) ? fabsf(x) : 0.0f; }
 
 // ---- the codes -------------------------------------------------------------------------
-// Four first moments as e4m3 codes of 256 m / scale.  What is not finite becomes NaN, there
-// and nowhere else in its block.
+// Four first moments as e4m3 codes of 256 m / scale.  What is not finite becomes NaN (the format
+// has no infinity, and 0 times one is NaN where the scale is 0), there and nowhere else in its block.
 __device__ __forceinline__ uint32_t encode_first(f32x4 m, float scale) {
     const float inverse = scale > 0.0f ? 256.0f / scale : 0.0f;
-    float r[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = finite(m[e]) ? m[e] * inverse : NAN;
-    int code = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], code, true));
+    const int code = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] * inverse, m[1] * inverse, 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(m[2] * inverse, m[3] * inverse, code, true));
 }
 __device__ __forceinline__ f32x4 decode_first(uint32_t code, float scale) {
     const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code), false);
@@ -104,95 +107,92 @@ __device__ __forceinline__ f32x4 decode_first(uint32_t code, float scale) {
 constexpr float kDown = 1.92592994438723585e-34f, kUp = 5.19229685853482763e33f;  // 2^-112, 2^112
 constexpr uint32_t kNanCode = 255;
 __device__ __forceinline__ uint32_t encode_root(float r, float inverse) {
-    if (!finite(r)) return kNanCode;
     const uint32_t bits = __float_as_uint(r * inverse * kDown);
     const uint32_t code = (bits + 0x3FFFFu + ((bits >> 19) & 1u)) >> 19;
-    return code == 0u && r > 0.0f ? 1u : code;
+    // At least 1 for a positive root, at most the code of NaN, which the bits of infinity and NaN pass.
+    return max(min(code, kNanCode), min(__float_as_uint(r), 1u));
 }
 __device__ __forceinline__ uint32_t encode_roots(f32x4 r, float scale) {
     const float inverse = scale > 0.0f ? 1.0f / scale : 0.0f;
     return encode_root(r[0], inverse) | encode_root(r[1], inverse) << 8 | encode_root(r[2], inverse) << 16 |
            encode_root(r[3], inverse) << 24;
 }
-__device__ __forceinline__ float decode_root(uint32_t code, float scale) {
-    return code == kNanCode ? NAN : __uint_as_float(code << 19) * kUp * scale;
-}
 __device__ __forceinline__ f32x4 decode_roots(uint32_t code, float scale) {
-    return f32x4{decode_root(code & 255u, scale), decode_root((code >> 8) & 255u, scale),
-                 decode_root((code >> 16) & 255u, scale), decode_root(code >> 24, scale)};
+    f32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = __uint_as_float(((code >> (8 * e)) & 255u) << 19) * kUp * scale;
+    // Whether a byte is 255: a zero byte of the complement.
+    if (((~code - 0x01010101u) & code & 0x80808080u) != 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (((code >> (8 * e)) & 255u) == kNanCode) r[e] = NAN;
+    }
+    return r;
 }
 
 // Codes and scales of a block, of which the lane holds four moments and roots.
 __device__ __forceinline__ void store_block(const Table& tab, int t, int64_t block, int lane, f32x4 m, f32x4 r) {
-    float top_m = fmaxf(fmaxf(magnitude(m[0]), magnitude(m[1])), fmaxf(magnitude(m[2]), magnitude(m[3])));
-    float top_r = fmaxf(fmaxf(magnitude(r[0]), magnitude(r[1])), fmaxf(magnitude(r[2]), magnitude(r[3])));
-    top_m = wave_max(top_m), top_r = wave_max(top_r);
+    uint32_t m_bits = 0, r_bits = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m_bits = max(m_bits, magnitude(m[e])), r_bits = max(r_bits, magnitude(r[e]));
+    float top_m = __uint_as_float(wave_max(m_bits));
+    const float top_r = __uint_as_float(wave_max(r_bits));
     if (top_m < kLeastScale) top_m = 0.0f;
-    const int64_t at = block * 64 + lane;
-    reinterpret_cast<uint32_t*>(tab.mc[t])[at] = encode_first(m, top_m);
-    reinterpret_cast<uint32_t*>(tab.vc[t])[at] = encode_roots(r, top_r);
-    if (lane == 0) {
-        tab.ms[t][block] = top_m;
-        tab.vs[t][block] = top_r;
-    }
+    tab.codes[t][block * 64 + lane] = make_uint2(encode_first(m, top_m), encode_roots(r, top_r));
+    if (lane == 0) tab.scales[t][block] = make_float2(top_m, top_r);
 }
 
 // ---- kernels -----------------------------------------------------------------------------
+// Waits for the global loads issued so far, and keeps the next ones behind.
+__device__ __forceinline__ void wait_for_loads() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// A wavefront a block.  With fp32 gradients each stream is waited for before the next one is
+// asked for: 1,003,782,656 elements take 2647 us (6.1 TB/s), 2790 with all loads in flight together.
+// 2-byte gradients leave less to move for the same arithmetic (a correctly rounded root and division an
+// element), which the loads then have to hide behind: 2335 us together and the gradient last (bf16, 6.0 TB/s),
+// 2475 one after another.
 template <int PD, int GD, bool kWriteBack>
-__global__ __launch_bounds__(64 * kWaves) void adamw8_kernel(Table tab, Scalars s, const Scalars* __restrict__ slot,
-                                                             const float* __restrict__ grad_mul, int64_t tile_base) {
+__global__ __launch_bounds__(64) void adamw8_kernel(Table tab, Scalars s, const Scalars* __restrict__ slot,
+                                                    const float* __restrict__ grad_mul, int64_t tile_base) {
     if (slot != nullptr) s = *slot;
     const int64_t tile = tile_base + blockIdx.x;
-    const int t = owner(tab, tile), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t n = tab.n[t], first = (tile - tab.first[t]) * (kWaves * kUnroll) + wave;
+    const int t = owner(tab, tile), lane = threadIdx.x;
+    const int64_t n = tab.n[t], block = tile - tab.first[t], e = block * kBlock + lane * 4;
+    const int have = static_cast<int>(min<int64_t>(n - e, 4));
     const float mul = grad_mul != nullptr ? *grad_mul : 1.0f;
-    const bool scaled = mul != 1.0f || s.unscale != 1.0f;
-    f32x4 p[kUnroll], g[kUnroll];
-    uint32_t mc[kUnroll], vc[kUnroll];
-    float ms[kUnroll], vs[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const int64_t block = first + u * kWaves, e = block * kBlock + lane * 4;
-        const int have = static_cast<int>(min<int64_t>(n - e, 4));
-        mc[u] = vc[u] = 0;
-        ms[u] = vs[u] = 0.0f;
-        p[u] = g[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (block * kBlock < n) {
-            g[u] = load_row<GD>(tab.g[t], e, have);
-            p[u] = load_row<PD>(tab.p[t], e, have);
-            mc[u] = reinterpret_cast<const uint32_t*>(tab.mc[t])[block * 64 + lane];
-            vc[u] = reinterpret_cast<const uint32_t*>(tab.vc[t])[block * 64 + lane];
-            ms[u] = tab.ms[t][block];
-            vs[u] = tab.vs[t][block];
-        }
+    f32x4 g;
+    if constexpr (GD == HBT_DTYPE_F32) {
+        g = load_row<GD>(tab.g[t], e, have);
+        wait_for_loads();
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const int64_t block = first + u * kWaves, e = block * kBlock + lane * 4;
-        if (block * kBlock >= n) break;
-        const int have = static_cast<int>(min<int64_t>(n - e, 4));
-        if (scaled) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (s.unscale != 1.0f) g[u][c] = round_to<GD>(g[u][c] * s.unscale);
-                g[u][c] = round_to<GD>(g[u][c] * mul);
-            }
-            if constexpr (kWriteBack) store_row<GD>(tab.g[t], e, have, g[u]);
-        }
-        f32x4 m = decode_first(mc[u], ms[u]), r = decode_roots(vc[u], vs[u]);
+    const uint2 codes = tab.codes[t][block * 64 + lane];
+    const float2 scales = tab.scales[t][block];
+    if constexpr (GD == HBT_DTYPE_F32) wait_for_loads();
+    f32x4 p = load_row<PD>(tab.p[t], e, have);
+    if constexpr (GD == HBT_DTYPE_F32) wait_for_loads();
+    else g = load_row<GD>(tab.g[t], e, have);
+    if (mul != 1.0f || s.unscale != 1.0f) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            if (c >= have) {  // past the tensor's end: nothing that a scale could come from
-                m[c] = r[c] = 0.0f;
-                continue;
-            }
-            m[c] = m[c] + s.lerp * (g[u][c] - m[c]);
-            r[c] = __builtin_sqrtf(r[c] * r[c] * s.beta2 + (s.one_minus_beta2 * g[u][c]) * g[u][c]);
-            p[u][c] = p[u][c] * s.decay + (s.neg_step * m[c]) / (r[c] * s.inverse_root + s.eps);
+            if (s.unscale != 1.0f) g[c] = round_to<GD>(g[c] * s.unscale);
+            g[c] = round_to<GD>(g[c] * mul);
         }
-        store_row<PD>(tab.p[t], e, have, p[u]);
-        store_block(tab, t, block, lane, m, r);
+        if constexpr (kWriteBack) store_row<GD>(tab.g[t], e, have, g);
     }
+    f32x4 m = decode_first(codes.x, scales.x), r = decode_roots(codes.y, scales.y);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        m[c] = m[c] + s.lerp * (g[c] - m[c]);
+        r[c] = __builtin_sqrtf(r[c] * r[c] * s.beta2 + (s.one_minus_beta2 * g[c]) * g[c]);
+        p[c] = p[c] * s.decay + (s.neg_step * m[c]) / (r[c] * s.inverse_root + s.eps);
+        if (c >= have) m[c] = r[c] = 0.0f;  // past the tensor's end: nothing that a scale could come from
+    }
+    store_row<PD>(tab.p[t], e, have, p);
+    store_block(tab, t, block, lane, m, r);
 }
 
 // Moments in fp32 (tab.p, tab.g: first and second) to codes.
@@ -221,10 +221,10 @@ __global__ __launch_bounds__(64 * kWaves) void decode_kernel(Table tab, int64_t 
         const int64_t block = first + u * kWaves, e = block * kBlock + lane * 4;
         if (block * kBlock >= n) break;
         const int have = static_cast<int>(min<int64_t>(n - e, 4));
-        const uint32_t mc = reinterpret_cast<const uint32_t*>(tab.mc[t])[block * 64 + lane];
-        const uint32_t vc = reinterpret_cast<const uint32_t*>(tab.vc[t])[block * 64 + lane];
-        const f32x4 r = decode_roots(vc, tab.vs[t][block]);
-        store_row<OD>(tab.p[t], e, have, decode_first(mc, tab.ms[t][block]));
+        const uint2 codes = tab.codes[t][block * 64 + lane];
+        const float2 scales = tab.scales[t][block];
+        const f32x4 r = decode_roots(codes.y, scales.y);
+        store_row<OD>(tab.p[t], e, have, decode_first(codes.x, scales.x));
         store_row<OD>(tab.g[t], e, have, f32x4{r[0] * r[0], r[1] * r[1], r[2] * r[2], r[3] * r[3]});
     }
 }
@@ -232,14 +232,12 @@ __global__ __launch_bounds__(64 * kWaves) void decode_kernel(Table tab, int64_t 
 // ---- host ----------------------------------------------------------------------------
 // Fills the table and counts its tiles, or refuses it.
 int32_t fill(const char* who, Table& tab, int64_t& tiles, const void* const* p, const void* const* g,
-             void* const* m_codes, void* const* v_codes, float* const* m_scales, float* const* v_scales,
-             const int64_t* numels, int32_t count) {
+             void* const* codes, void* const* scales, const int64_t* numels, int32_t count, int64_t tile) {
     if (count < 0 || count > kMaxTensors) {
         set_error("%s: count must lie in [0, %d], got %d", who, kMaxTensors, count);
         return HBT_ERR_INVALID_ARGUMENT;
     }
-    if (count > 0 && (p == nullptr || g == nullptr || m_codes == nullptr || v_codes == nullptr ||
-                      m_scales == nullptr || v_scales == nullptr || numels == nullptr)) {
+    if (count > 0 && (p == nullptr || g == nullptr || codes == nullptr || scales == nullptr || numels == nullptr)) {
         set_error("%s: null table pointer", who);
         return HBT_ERR_INVALID_ARGUMENT;
     }
@@ -251,27 +249,22 @@ int32_t fill(const char* who, Table& tab, int64_t& tiles, const void* const* p, 
             return HBT_ERR_INVALID_ARGUMENT;
         }
         if (numels[i] == 0) continue;
-        const void* given[] = {p[i], g[i], m_codes[i], v_codes[i], m_scales[i], v_scales[i]};
-        for (const void* at : given)
-            if (at == nullptr) {
-                set_error("%s: tensor %d has a null data pointer", who, i);
-                return HBT_ERR_INVALID_ARGUMENT;
-            }
-        for (int k = 2; k < 6; ++k)
-            if (reinterpret_cast<uintptr_t>(given[k]) % 4 != 0) {
-                set_error("%s: tensor %d has codes or scales off 4 bytes", who, i);
-                return HBT_ERR_INVALID_ARGUMENT;
-            }
+        if (p[i] == nullptr || g[i] == nullptr || codes[i] == nullptr || scales[i] == nullptr) {
+            set_error("%s: tensor %d has a null data pointer", who, i);
+            return HBT_ERR_INVALID_ARGUMENT;
+        }
+        if ((reinterpret_cast<uintptr_t>(codes[i]) | reinterpret_cast<uintptr_t>(scales[i])) % 8 != 0) {
+            set_error("%s: tensor %d has codes or scales off 8 bytes", who, i);
+            return HBT_ERR_INVALID_ARGUMENT;
+        }
         const int at = tab.count++;
         tab.p[at] = const_cast<void*>(p[i]);
         tab.g[at] = const_cast<void*>(g[i]);
-        tab.mc[at] = static_cast<uint8_t*>(m_codes[i]);
-        tab.vc[at] = static_cast<uint8_t*>(v_codes[i]);
-        tab.ms[at] = m_scales[i];
-        tab.vs[at] = v_scales[i];
+        tab.codes[at] = static_cast<uint2*>(codes[i]);
+        tab.scales[at] = static_cast<float2*>(scales[i]);
         tab.n[at] = numels[i];
         tab.first[at] = tiles;
-        tiles += (numels[i] + kTile - 1) / kTile;
+        tiles += (numels[i] + tile - 1) / tile;
     }
     return HBT_OK;
 }
@@ -283,11 +276,11 @@ using namespace hbt;
 
 extern "C" {
 
-int32_t hbt_adamw8_step(void* const* params, void* const* grads, void* const* m_codes, void* const* v_codes,
-                        float* const* m_scales, float* const* v_scales, const int64_t* numels, int32_t count,
-                        int32_t param_dtype, int32_t grad_dtype, float unscale, const float* grad_mul, float decay,
-                        float lerp_weight, float beta2, float one_minus_beta2, float inverse_bias_correction2_sqrt,
-                        float eps, float neg_step_size, const float* slot, int32_t flags, void* stream) {
+int32_t hbt_adamw8_step(void* const* params, void* const* grads, void* const* codes, void* const* scales,
+                        const int64_t* numels, int32_t count, int32_t param_dtype, int32_t grad_dtype, float unscale,
+                        const float* grad_mul, float decay, float lerp_weight, float beta2, float one_minus_beta2,
+                        float inverse_bias_correction2_sqrt, float eps, float neg_step_size, const float* slot,
+                        int32_t flags, void* stream) {
     clear_error();
     const char* who = "hbt_adamw8_step";
     constexpr int F32 = HBT_DTYPE_F32, BF16 = HBT_DTYPE_BF16, F16 = HBT_DTYPE_F16;
@@ -308,18 +301,18 @@ int32_t hbt_adamw8_step(void* const* params, void* const* grads, void* const* m_
     }
     Table tab{};
     int64_t tiles = 0;
-    const int32_t status = fill(who, tab, tiles, params, grads, m_codes, v_codes, m_scales, v_scales, numels, count);
+    const int32_t status = fill(who, tab, tiles, params, grads, codes, scales, numels, count, kBlock);
     if (status != HBT_OK) return status;
     const Scalars s{unscale, decay, lerp_weight, beta2, one_minus_beta2, inverse_bias_correction2_sqrt, eps,
                     neg_step_size};
     const Scalars* from = reinterpret_cast<const Scalars*>(slot);
     const bool write_back = (flags & HBT_STEP_WRITE_GRAD) != 0;
     const hipStream_t st = as_stream(stream);
-    return launch_sliced(who, tiles, 64 * kWaves, [&](int64_t first, dim3 grid) {
+    return launch_sliced(who, tiles, 64, [&](int64_t first, dim3 grid) {
         const auto launch = [&](auto pd, auto gd) {
             constexpr int PD = decltype(pd)::value, GD = decltype(gd)::value;
-            if (write_back) adamw8_kernel<PD, GD, true><<<grid, 64 * kWaves, 0, st>>>(tab, s, from, grad_mul, first);
-            else adamw8_kernel<PD, GD, false><<<grid, 64 * kWaves, 0, st>>>(tab, s, from, grad_mul, first);
+            if (write_back) adamw8_kernel<PD, GD, true><<<grid, 64, 0, st>>>(tab, s, from, grad_mul, first);
+            else adamw8_kernel<PD, GD, false><<<grid, 64, 0, st>>>(tab, s, from, grad_mul, first);
         };
         const std::integral_constant<int, F32> f32{};
         const std::integral_constant<int, BF16> bf16{};
@@ -331,24 +324,20 @@ int32_t hbt_adamw8_step(void* const* params, void* const* grads, void* const* m_
     });
 }
 
-int32_t hbt_moments8_encode(const float* const* firsts, const float* const* seconds, void* const* m_codes,
-                            void* const* v_codes, float* const* m_scales, float* const* v_scales,
-                            const int64_t* numels, int32_t count, void* stream) {
+int32_t hbt_moments8_encode(const void* const* firsts, const void* const* seconds, void* const* codes,
+                            void* const* scales, const int64_t* numels, int32_t count, void* stream) {
     clear_error();
     const char* who = "hbt_moments8_encode";
     Table tab{};
     int64_t tiles = 0;
-    const int32_t status = fill(who, tab, tiles, reinterpret_cast<const void* const*>(firsts),
-                                reinterpret_cast<const void* const*>(seconds), m_codes, v_codes, m_scales, v_scales,
-                                numels, count);
+    const int32_t status = fill(who, tab, tiles, firsts, seconds, codes, scales, numels, count, kTile);
     if (status != HBT_OK) return status;
     return launch_sliced(who, tiles, 64 * kWaves, [&](int64_t first, dim3 grid) {
         encode_kernel<<<grid, 64 * kWaves, 0, as_stream(stream)>>>(tab, first);
     });
 }
 
-int32_t hbt_moments8_decode(const void* const* m_codes, const void* const* v_codes, const float* const* m_scales,
-                            const float* const* v_scales, void* const* firsts, void* const* seconds,
+int32_t hbt_moments8_decode(void* const* codes, void* const* scales, void* const* firsts, void* const* seconds,
                             const int64_t* numels, int32_t count, int32_t out_dtype, void* stream) {
     clear_error();
     const char* who = "hbt_moments8_decode";
@@ -358,9 +347,7 @@ int32_t hbt_moments8_decode(const void* const* m_codes, const void* const* v_cod
     }
     Table tab{};
     int64_t tiles = 0;
-    const int32_t status = fill(who, tab, tiles, firsts, seconds, const_cast<void* const*>(m_codes),
-                                const_cast<void* const*>(v_codes), const_cast<float* const*>(m_scales),
-                                const_cast<float* const*>(v_scales), numels, count);
+    const int32_t status = fill(who, tab, tiles, firsts, seconds, codes, scales, numels, count, kTile);
     if (status != HBT_OK) return status;
     return launch_sliced(who, tiles, 64 * kWaves, [&](int64_t first, dim3 grid) {
         if (out_dtype == HBT_DTYPE_F32) decode_kernel<HBT_DTYPE_F32><<<grid, 64 * kWaves, 0, as_stream(stream)>>>(tab, first);

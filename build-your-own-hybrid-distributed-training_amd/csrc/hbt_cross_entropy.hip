@@ -25,7 +25,7 @@ namespace mm {
 namespace {
 
 constexpr int F32 = HBT_DTYPE_F32, BF16 = HBT_DTYPE_BF16, F16 = HBT_DTYPE_F16;
-constexpr int64_t kPieceBytes = int64_t(1) << 30;  // stored exponentials at a time
+constexpr int64_t kPieceBytes = int64_t(2) << 30;  // stored exponentials at a time
 constexpr int64_t kStatsBytes = int64_t(1) << 28;  // row statistics at a time, without gradients
 constexpr int kThin = 16;                          // rows of the kernel for few tokens
 constexpr int64_t kMostRows = int64_t(1) << 22;    // rows of a piece: a launch over them stays within a grid
@@ -57,43 +57,11 @@ __device__ __forceinline__ void piece_rows(const Piece& p, int& first, int& rows
     rows = min(each, count - first);
 }
 
-template <int W>
-__device__ __forceinline__ float group_max(float x) {
-    if constexpr (W == 64) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    }
-    if constexpr (W >= 32) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    }
-    const auto move = [](float v, auto ctrl) {
-        return __uint_as_float(__builtin_amdgcn_mov_dpp(static_cast<int>(__float_as_uint(v)), decltype(ctrl)::value, 0xF,
-                                                        0xF, false));
-    };
-    x = fmaxf(x, move(x, std::integral_constant<int, 0x128>{}));
-    x = fmaxf(x, move(x, std::integral_constant<int, 0x124>{}));
-    x = fmaxf(x, move(x, std::integral_constant<int, 0x4E>{}));
-    return fmaxf(x, move(x, std::integral_constant<int, 0xB1>{}));
-}
-template <int W>
-__device__ __forceinline__ float group_sum(float x) {
-    if constexpr (W == 64) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    if constexpr (W >= 32) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    const auto move = [](float v, auto ctrl) {
-        return __uint_as_float(__builtin_amdgcn_mov_dpp(static_cast<int>(__float_as_uint(v)), decltype(ctrl)::value, 0xF,
-                                                        0xF, false));
-    };
-    x += move(x, std::integral_constant<int, 0x128>{});
-    x += move(x, std::integral_constant<int, 0x124>{});
-    x += move(x, std::integral_constant<int, 0x4E>{});
-    return x + move(x, std::integral_constant<int, 0xB1>{});
+// The largest over the wavefront, in every lane.
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
+    return x;
 }
 
 // exp(t) for t <= 0: the hardware's base-2 exponential where the result is rounded to 16 bits or
@@ -146,7 +114,7 @@ __global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
         }
         if (i < p.tokens) p.place[i] = valid ? row : -1;
     }
-    top = group_max<64>(top);
+    top = wave_max(top);
     if (lane == 0) wave_top[wave] = top;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -218,21 +186,45 @@ struct LogitArgs {
     const void* w;
     const void* bias;
     const int32_t* word;
-    float2* stats;      // [row of the piece][tile]: largest, sum of exponentials
+    float2* stats;      // [tile][row of the piece]: largest, sum of exponentials
     float* sums;        // the same: sum of the logits, or null without smoothing
     float* target;      // row -> its target's logit
     void* kept;         // [row of the piece][ldk] exponentials, or null
-    int64_t ldx, ldw, ldk, vocab, inner;
+    int64_t ldx, ldw, ldk, stride, vocab, inner;  // stride: rows of stats
     int tiles_n;
     Piece piece;
 };
 
-// A tile's logits to statistics and exponentials.  A row's columns lie with BN / 4 lanes, so a row
-// is reduced within its wavefront.
+// The larger, or the sum, of a value over the four quarters of a wavefront (lanes l % 16).
+__device__ __forceinline__ float quarters_max(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// A 4 x 4 transposition between four registers and the four quarters of a wavefront: afterwards
+// register c of quarter q holds what register q of quarter c held.
+__device__ __forceinline__ void transpose_quarters(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+    const auto ac = __builtin_amdgcn_permlane32_swap(a, c, false, false);
+    const auto bd = __builtin_amdgcn_permlane32_swap(b, d, false, false);
+    const auto low = __builtin_amdgcn_permlane16_swap(ac[0], bd[0], false, false);
+    const auto high = __builtin_amdgcn_permlane16_swap(ac[1], bd[1], false, false);
+    a = low[0], b = low[1], c = high[0], d = high[1];
+}
+
+// A tile's logits to statistics and exponentials, in the registers that the matrix cores leave
+// them in: lane l holds, of row l % 16 of each sixteen rows, four columns of each sixteen.  The
+// largest of a row is taken in the lane, over the quarters, and over the wavefronts through LDS.
 template <int D, class T, bool kAsync>
 __global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
     extern __shared__ __align__(16) char lds[];
-    constexpr int kLanes = T::BN / 4;
     int first, count;
     piece_rows(p.piece, first, count);
     const int tiles_m = (count + T::BM - 1) / T::BM, total = tiles_m * p.tiles_n;
@@ -244,47 +236,129 @@ __global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
     const char* x = static_cast<const char*>(p.x) + first * p.ldx * elem_bytes<D>();
     tile_product<D, true, true, T, kAsync>(x, p.ldx, m0, count, p.w, p.ldw, n0, p.vocab, 0, p.inner, lds, acc);
     const int rows = static_cast<int>(min<int64_t>(count - m0, T::BM));
-    const int cols = static_cast<int>(min<int64_t>(p.vocab - n0, T::BN));
-    const int stored = static_cast<int>(min<int64_t>(p.ldk - n0, T::BN));
-    const int32_t* word = p.word + first + m0;
-    struct Loaded {
-        f32x4 bias;
-        int word;
-    };
-    finish_tile<T, kAsync, 2>(
-        lds, acc,
-        [&](int i, int j) {
-            Loaded l{{0.f, 0.f, 0.f, 0.f}, -1};
-            if (i < rows) l.word = word[i];
-            if (p.bias != nullptr && j < cols) l.bias = load_row<D>(p.bias, n0 + j, cols - j);
-            return l;
-        },
-        [&](int i, int j, f32x4 v, Loaded l) {
-            v += l.bias;
-            const int64_t at = l.word - n0 - j;  // the target's place among the four
-            const int64_t row = m0 + i;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
+    const int wm = (wave / T::WN) * (T::BM / T::WM) + (lane & 15), wn = (wave % T::WN) * (T::BN / T::WN);
+    const int left = static_cast<int>(p.vocab - n0) - wn;  // columns from the wavefront's first one
+    if (p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j) {
+            const int have = left - 16 * j - 4 * q;
+            const f32x4 b = load_row<D>(p.bias, n0 + wn + 16 * j + 4 * q, have);
+#pragma unroll
+            for (int i = 0; i < T::TM; ++i) acc[i][j] += b;
+        }
+    }
+    const bool edge = left < 16 * T::TN;
+    float* line = reinterpret_cast<float*>(lds);  // [3][WN][BM]: largest, sums of exponentials and of logits
+    constexpr int kLine = T::WN * T::BM;
+    const int slot = (wave % T::WN) * T::BM + wm;
+    if (p.sums != nullptr) {
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
             float sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (at == e && i < rows) p.target[first + row] = v[e];
-                if (j + e < cols) sum += v[e];
-                else v[e] = -INFINITY;
-            }
-            const float top = group_max<kLanes>(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
-            const float base = top == -INFINITY ? 0.0f : top;  // a tile of nothing but -inf
+            for (int j = 0; j < T::TN; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = exponential<D>(v[e] - base);
-            const float part = group_sum<kLanes>((v[0] + v[1]) + (v[2] + v[3]));
-            if (p.sums != nullptr) sum = group_sum<kLanes>(sum);
-            if (i < rows) {
-                if (p.kept != nullptr && j < stored) store4<D == F32 ? F32 : F16>(p.kept, row * p.ldk + n0 + j, v);
-                if (j == 0) {
-                    p.stats[row * p.tiles_n + tn] = make_float2(top, part);
-                    if (p.sums != nullptr) p.sums[row * p.tiles_n + tn] = sum;
-                }
+                for (int e = 0; e < 4; ++e) sum += 16 * j + 4 * q + e < left ? acc[i][j][e] : 0.0f;
+            sum = quarters_sum(sum);
+            if (q == 0) line[2 * kLine + slot + 16 * i] = sum;
+        }
+    }
+    if (edge) {
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (16 * j + 4 * q + e >= left) acc[i][j][e] = -INFINITY;
+    }
+    const int32_t* word = p.word + first + m0;
+    int at[T::TM];  // the target's column from the wavefront's first one
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) at[i] = wm + 16 * i < rows ? word[wm + 16 * i] - static_cast<int>(n0) - wn : -1;
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j)
+            top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
+        top = quarters_max(top);
+        if (q == 0) line[slot + 16 * i] = top;
+    }
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) {
+        const bool here = at[i] >= 0 && at[i] < 16 * T::TN;
+        if (__any(here)) {  // seldom: a wavefront's columns are a small part of the vocabulary
+            float z = 0.0f;
+#pragma unroll
+            for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (at[i] == 16 * j + 4 * q + e) z = acc[i][j][e];
+            if (here && ((at[i] >> 2) & 3) == q) p.target[first + m0 + wm + 16 * i] = z;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) {
+        float top = line[wm + 16 * i];
+#pragma unroll
+        for (int w = 1; w < T::WN; ++w) top = fmaxf(top, line[w * T::BM + wm + 16 * i]);
+        if (top == -INFINITY) top = 0.0f;  // a tile of nothing but -inf
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = exponential<D>(acc[i][j][e] - top);
+            sum += (acc[i][j][0] + acc[i][j][1]) + (acc[i][j][2] + acc[i][j][3]);
+        }
+        sum = quarters_sum(sum);
+        if (q == 0) line[kLine + slot + 16 * i] = sum;
+        // Whole runs of the wavefront's columns lie inside a stored row, whose length is a multiple of 64.
+        if (p.kept == nullptr || n0 + wn >= p.ldk) continue;
+        const int64_t to = (m0 + wm + 16 * i) * p.ldk + n0 + wn;
+        const bool in = wm + 16 * i < rows;
+        if constexpr (D == F32) {
+#pragma unroll
+            for (int j = 0; j < T::TN; ++j)
+                if (in) *reinterpret_cast<f32x4*>(static_cast<float*>(p.kept) + to + 16 * j + 4 * q) = acc[i][j];
+        } else {
+            uint32_t h[T::TN][2];
+#pragma unroll
+            for (int j = 0; j < T::TN; ++j) {
+                h[j][0] = pack2_rounded<F16>(acc[i][j][0], acc[i][j][1]);
+                h[j][1] = pack2_rounded<F16>(acc[i][j][2], acc[i][j][3]);
             }
-            return v;
-        });
+            uint16_t* kept = static_cast<uint16_t*>(p.kept) + to;
+            if constexpr (T::TN == 4) {  // sixteen consecutive columns a lane, 128 bytes of a row a wavefront
+                transpose_quarters(h[0][0], h[1][0], h[2][0], h[3][0]);
+                transpose_quarters(h[0][1], h[1][1], h[2][1], h[3][1]);
+                if (in) {
+                    u32x4* out = reinterpret_cast<u32x4*>(kept + 16 * q);
+                    out[0] = u32x4{h[0][0], h[0][1], h[1][0], h[1][1]};
+                    out[1] = u32x4{h[2][0], h[2][1], h[3][0], h[3][1]};
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < T::TN; ++j)
+                    if (in) *reinterpret_cast<u32x2*>(kept + 16 * j + 4 * q) = u32x2{h[j][0], h[j][1]};
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows; i += T::kThreads) {
+        float top = line[i], sum = line[kLine + i];
+#pragma unroll
+        for (int w = 1; w < T::WN; ++w) top = fmaxf(top, line[w * T::BM + i]), sum += line[kLine + w * T::BM + i];
+        p.stats[tn * p.stride + m0 + i] = make_float2(top, sum);
+        if (p.sums != nullptr) {
+            float logits = line[2 * kLine + i];
+#pragma unroll
+            for (int w = 1; w < T::WN; ++w) logits += line[2 * kLine + w * T::BM + i];
+            p.sums[tn * p.stride + m0 + i] = logits;
+        }
+    }
 }
 
 // At most 16 tokens, without gradients: the read of W.  A workgroup of 8 waves forms 16 logits of
@@ -376,49 +450,26 @@ struct JoinArgs {
     Row* row;                  // for the gradients, or null
     float* loss;               // token -> loss, or null
     double* row_loss;          // row -> loss, or null
-    int64_t ignore, vocab;
+    int64_t ignore, vocab, stride;
     int tiles;
     float smoothing;
-    Piece piece;               // control null: `rows` tokens
-    int rows;
+    Piece piece;
 };
 
-// Sum over the 256 threads of a workgroup, in every thread, in a fixed order.
-__device__ __forceinline__ double join_sum(double x, double* shared) {
-    x = wave_sum(x);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
-    __syncthreads();
-    return (shared[0] + shared[1]) + (shared[2] + shared[3]);
-}
-
-__global__ __launch_bounds__(256) void join_kernel(JoinArgs p) {
-    __shared__ float tops[4];
-    __shared__ double shared[4];
-    int first = 0, count = p.rows;
-    if (p.piece.control != nullptr) piece_rows(p.piece, first, count);
-    const int i = blockIdx.x;
-    if (i >= count) return;
-    const float2* stats = p.stats + int64_t(i) * p.tiles;
+// A running log-sum: the largest so far and the sum of exponentials over it.  An empty tile (sum 0)
+// adds nothing, a NaN sum stays one.
+struct Running {
     float top = -INFINITY;
-    for (int t = threadIdx.x; t < p.tiles; t += 256) {
-        const float2 s = stats[t];
-        if (!(s.y <= 0.0f)) top = fmaxf(top, s.x);  // a NaN sum counts, an empty one does not
+    double sum = 0.0;
+    __device__ __forceinline__ void add(float t, double s) {
+        if (s == 0.0) return;
+        const float high = fmaxf(top, t);
+        sum = (sum == 0.0 ? 0.0 : sum * expf(top - high)) + s * (t == high ? 1.0 : static_cast<double>(expf(t - high)));
+        top = high;
     }
-    top = group_max<64>(top);
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    double total = 0.0, logits = 0.0;
-    for (int t = threadIdx.x; t < p.tiles; t += 256) {
-        const float2 s = stats[t];
-        if (!(s.y <= 0.0f)) total += s.y * expf(s.x - top);
-        if (p.sums != nullptr) logits += p.sums[int64_t(i) * p.tiles + t];
-    }
-    total = join_sum(total, shared);
-    if (p.sums != nullptr) logits = join_sum(logits, shared);
-    if (threadIdx.x != 0) return;
-    const int row = first + i;
+};
+
+__device__ __forceinline__ void finish_row(const JoinArgs& p, int row, const Running& r, double logits) {
     const int64_t token = p.token != nullptr ? p.token[row] : row;
     bool known;
     if (p.word != nullptr) {
@@ -433,15 +484,78 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs p) {
         known = t >= 0 && t < p.vocab;
     }
     // log p = (z_t - top) - log(sum): the two parts of a nearly certain target are both small
-    const double log_sum = log(total);
-    const double log_p = known ? (static_cast<double>(p.target[row]) - top) - log_sum : NAN;
+    const double log_sum = log(r.sum);
+    const double log_p = known ? (static_cast<double>(p.target[row]) - r.top) - log_sum : NAN;
     double loss = -(1.0 - p.smoothing) * log_p;
-    if (p.smoothing != 0.0f) loss += p.smoothing * ((top + log_sum) - logits / static_cast<double>(p.vocab));
+    if (p.smoothing != 0.0f) loss += p.smoothing * ((r.top + log_sum) - logits / static_cast<double>(p.vocab));
     if (p.loss != nullptr) p.loss[token] = static_cast<float>(loss);
     if (p.row_loss != nullptr) p.row_loss[row] = loss;
     if (p.row != nullptr)
-        p.row[row] = Row{top, static_cast<float>(1.0 / total), static_cast<float>(log_p),
+        p.row[row] = Row{r.top, static_cast<float>(1.0 / r.sum), static_cast<float>(log_p),
                          p.weight[row] * p.piece.control->scale_in};
+}
+
+// Statistics [tile][row]: a workgroup joins 64 rows, a lane each; its wavefronts take tiles in turn.
+constexpr int kJoinWaves = 8;
+__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(JoinArgs p) {
+    __shared__ float tops[kJoinWaves][64];
+    __shared__ double totals[kJoinWaves][64], logit_sums[kJoinWaves][64];
+    int first, count;
+    piece_rows(p.piece, first, count);
+    if (static_cast<int>(blockIdx.x) * 64 >= count) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane, at = min(i, count - 1);
+    Running r;
+    double logits = 0.0;
+    for (int t = wave; t < p.tiles; t += 4 * kJoinWaves) {
+        float2 s[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // four loads in flight
+            const int tile = t + k * kJoinWaves;
+            s[k] = tile < p.tiles ? p.stats[tile * p.stride + at] : make_float2(0.0f, 0.0f);
+            if (p.sums != nullptr && tile < p.tiles) logits += p.sums[tile * p.stride + at];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r.add(s[k].x, s[k].y);
+    }
+    tops[wave][lane] = r.top, totals[wave][lane] = r.sum, logit_sums[wave][lane] = logits;
+    __syncthreads();
+    if (wave != 0 || i >= count) return;
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w) {
+        r.add(tops[w][lane], totals[w][lane]);
+        logits += logit_sums[w][lane];
+    }
+    finish_row(p, first + i, r, logits);
+}
+
+// Statistics [row][tile], many tiles and few rows: a workgroup a row, its lanes' parts joined in a tree.
+__global__ __launch_bounds__(1024) void thin_join_kernel(JoinArgs p) {
+    __shared__ float tops[1024];
+    __shared__ double totals[1024], logit_sums[1024];
+    const int row = blockIdx.x, tid = threadIdx.x;
+    Running r;
+    double logits = 0.0;
+    for (int t = tid; t < p.tiles; t += 4096) {
+        float2 s[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int tile = t + k * 1024;
+            s[k] = tile < p.tiles ? p.stats[row * p.stride + tile] : make_float2(0.0f, 0.0f);
+            if (p.sums != nullptr && tile < p.tiles) logits += p.sums[row * p.stride + tile];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r.add(s[k].x, s[k].y);
+    }
+    tops[tid] = r.top, totals[tid] = r.sum, logit_sums[tid] = logits;
+    for (int half = 512; half > 0; half >>= 1) {
+        __syncthreads();
+        if (tid < half) {
+            r.add(tops[tid + half], totals[tid + half]);
+            logits += logit_sums[tid + half];
+            tops[tid] = r.top, totals[tid] = r.sum, logit_sums[tid] = logits;
+        }
+    }
+    if (tid == 0) finish_row(p, row, r, logits);
 }
 
 // The rows' losses added up in a fixed order; `divide`: their mean (0 / 0 without any).
@@ -466,8 +580,8 @@ struct SoftmaxArgs {
     const float2* stats;
     const Row* row;
     const int32_t* word;
-    int64_t ldk, vocab;
-    int tiles, tile, segment;  // tiles of a row and their columns; columns a workgroup takes
+    int64_t ldk, vocab, stride;
+    int tile, segment;  // columns of a tile, and those that a workgroup takes
     float smoothing;
     Piece piece;
 };
@@ -487,11 +601,11 @@ __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs p) {
     const float hit = (expm1f(row.log_p) + p.smoothing) * row.weight - even;
     const bool known = word >= 0;
     char* line = static_cast<char*>(p.kept) + int64_t(i) * p.ldk * B;
-    const float2* stats = p.stats + int64_t(i) * p.tiles;
+    const float2* stats = p.stats + i;
     const int64_t end = min<int64_t>(p.ldk, (part + 1) * int64_t(p.segment));
     for (int64_t j = part * int64_t(p.segment) + threadIdx.x * E; j < end; j += 256 * E) {
         const u32x4 unit = *reinterpret_cast<const u32x4*>(line + j * B);
-        const float factor = expf(stats[min<int64_t>(j, p.vocab - 1) / p.tile].x - row.top) * row.inverse * row.weight;
+        const float factor = expf(stats[min<int64_t>(j, p.vocab - 1) / p.tile * p.stride].x - row.top) * row.inverse * row.weight;
         float v[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -613,14 +727,30 @@ __global__ __launch_bounds__(256) void bias_join_kernel(const float* parts, floa
     else store_elem<OD>(db, j, sum);
 }
 
-// ---- gradients held in fp32 until the loss's own gradient is known ---------------------------
-template <int OD>
-__global__ __launch_bounds__(256) void scale_round_kernel(const float* src, void* dst, int64_t n, const float* factor,
-                                                          int64_t block_base) {
-    const float f = *factor;
-    const int64_t i = ((block_base + blockIdx.x) * 256 + threadIdx.x) * 4;
-    if (i < n) store_row<OD>(dst, i, static_cast<int>(min<int64_t>(n - i, 4)),
-                             load_row<F32>(src, i, static_cast<int>(min<int64_t>(n - i, 4))) * f);
+// ---- the loss's own gradient -----------------------------------------------------------------
+struct ScaleArgs {
+    const void* src[HBT_MAX_SCALED];
+    void* dst[HBT_MAX_SCALED];
+    int64_t n[HBT_MAX_SCALED];
+    int count;
+    const float* factor;
+};
+// In place (SD == OD) nothing is to be done for a factor of 1, which is known on the device alone:
+// the workgroups are few and walk the tensors, so that such a launch ends at once (525 million bf16
+// elements: 3 us, where a workgroup for each 1024 elements takes 230).
+template <int SD, int OD>
+__global__ __launch_bounds__(256) void scale_round_kernel(ScaleArgs p) {
+    const float f = *p.factor;
+    if (SD == OD && f == 1.0f && p.src[0] == p.dst[0]) return;
+    for (int t = 0; t < p.count; ++t) {
+        const int64_t n = p.n[t];
+        for (int64_t i = (blockIdx.x * int64_t(256) + threadIdx.x) * 8; i < n; i += int64_t(gridDim.x) * 2048) {
+            const int have = static_cast<int>(min<int64_t>(n - i, 8));
+            const f32x4 a = load_row<SD>(p.src[t], i, have), b = load_row<SD>(p.src[t], i + 4, have - 4);
+            store_row<OD>(p.dst[t], i, have, a * f);
+            store_row<OD>(p.dst[t], i + 4, have - 4, b * f);
+        }
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -817,8 +947,8 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
         thin_logit_kernel<D><<<dim3(plan.tiles), 512, 0, s>>>(c.x, c.ldx, c.w, c.ldw, c.bias, c.target,
                                                               static_cast<int>(c.tokens), c.vocab, c.inner, stats, sums, target);
         if ((status = check_launch(who)) != HBT_OK) return status;
-        join.raw = c.target, join.rows = static_cast<int>(c.tokens);
-        join_kernel<<<dim3(static_cast<unsigned>(c.tokens)), 256, 0, s>>>(join);
+        join.raw = c.target, join.stride = plan.tiles;
+        thin_join_kernel<<<dim3(static_cast<unsigned>(c.tokens)), 1024, 0, s>>>(join);
         if ((status = check_launch(who)) != HBT_OK || row_loss == nullptr) return status;
         total_kernel<<<1, 1024, 0, s>>>(row_loss, nullptr, c.target, c.ignore, c.tokens, mean, c.loss);
         return check_launch(who);
@@ -843,7 +973,7 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
         LogitArgs l{};
         l.x = rows, l.w = c.w, l.bias = c.bias, l.word = word, l.stats = stats, l.sums = sums, l.target = target;
         l.kept = kept, l.ldx = plan.ld, l.ldw = c.ldw, l.ldk = plan.ldk, l.vocab = c.vocab, l.inner = c.inner;
-        l.tiles_n = plan.tiles, l.piece = piece;
+        l.tiles_n = plan.tiles, l.stride = plan.most, l.piece = piece;
         if (plan.size == 64) {
             status = aligned ? launch_logits<D, Tile64, true>(who, l, plan.most, s)
                              : launch_logits<D, Tile64, false>(who, l, plan.most, s);
@@ -855,12 +985,13 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
         }
         if (status != HBT_OK) return status;
         join.word = word, join.token = token, join.weight = weight, join.row = row, join.piece = piece;
-        join_kernel<<<dim3(static_cast<unsigned>(plan.most)), 256, 0, s>>>(join);
+        join.stride = plan.most;
+        join_kernel<<<dim3(static_cast<unsigned>((plan.most + 63) / 64)), 64 * kJoinWaves, 0, s>>>(join);
         if ((status = check_launch(who)) != HBT_OK) return status;
         if (!plan.grads) continue;
         const int segment = 256 * unit_elems<D>() * 4;
         softmax_kernel<D><<<dim3(static_cast<unsigned>((plan.ldk + segment - 1) / segment * plan.most)), 256, 0, s>>>({kept, stats, row, word, plan.ldk,
-                                                                          c.vocab, plan.tiles, plan.size, segment,
+                                                                          c.vocab, plan.most, plan.size, segment,
                                                                           c.smoothing, piece});
         if ((status = check_launch(who)) != HBT_OK) return status;
         const bool last = i + 1 == plan.pieces;
@@ -957,21 +1088,46 @@ int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int6
     return wide ? run<F16, F32>(who, c, plan, space, s) : run<F16, F16>(who, c, plan, space, s);
 }
 
-int32_t hbt_scale_round(const float* src, void* dst, int64_t numel, int32_t dtype, const float* factor, void* stream) {
+int32_t hbt_scale_round(const void* const* srcs, void* const* dsts, const int64_t* numels, int32_t count,
+                        int32_t src_dtype, int32_t dst_dtype, const float* factor, void* stream) {
     clear_error();
     const char* who = "hbt_scale_round";
-    if (dtype != F32 && dtype != BF16 && dtype != F16) {
-        set_error("%s: dtype %d is not F32, BF16 or F16", who, dtype);
+    if (count < 0 || count > HBT_MAX_SCALED) {
+        set_error("%s: count must lie in [0, %d], got %d", who, HBT_MAX_SCALED, count);
         return HBT_ERR_INVALID_ARGUMENT;
     }
-    if (numel < 0) return refuse(who, "numel is negative");
-    if (numel > 0 && (src == nullptr || dst == nullptr || factor == nullptr)) return refuse(who, "a pointer is null");
-    return launch_sliced(who, (numel + 1023) / 1024, 256, [&](int64_t first, dim3 grid) {
-        const hipStream_t s = as_stream(stream);
-        if (dtype == F32) scale_round_kernel<F32><<<grid, 256, 0, s>>>(src, dst, numel, factor, first);
-        else if (dtype == BF16) scale_round_kernel<BF16><<<grid, 256, 0, s>>>(src, dst, numel, factor, first);
-        else scale_round_kernel<F16><<<grid, 256, 0, s>>>(src, dst, numel, factor, first);
-    });
+    const bool pair = (src_dtype == F32 && (dst_dtype == F32 || dst_dtype == BF16 || dst_dtype == F16)) ||
+                      (src_dtype == BF16 && dst_dtype == BF16) || (src_dtype == F16 && dst_dtype == F16);
+    if (!pair) {
+        set_error("%s: dtypes (%d, %d) are not of F32 to any, or of one 2-byte dtype", who, src_dtype, dst_dtype);
+        return HBT_ERR_INVALID_ARGUMENT;
+    }
+    if (count > 0 && (srcs == nullptr || dsts == nullptr || numels == nullptr || factor == nullptr))
+        return refuse(who, "a table or the factor is null");
+    ScaleArgs p{};
+    p.factor = factor;
+    int64_t longest = 0;
+    bool in_place = true;
+    for (int i = 0; i < count; ++i) {
+        if (numels[i] < 0) return refuse(who, "numel is negative");
+        if (numels[i] == 0) continue;
+        if (srcs[i] == nullptr || dsts[i] == nullptr) return refuse(who, "a data pointer is null");
+        if (srcs[i] == dsts[i] && src_dtype != dst_dtype) return refuse(who, "in place, both dtypes must be the same");
+        in_place = in_place && srcs[i] == dsts[i];
+        p.src[p.count] = srcs[i], p.dst[p.count] = dsts[i], p.n[p.count++] = numels[i];
+        longest = std::max(longest, numels[i]);
+    }
+    if (p.count == 0) return HBT_OK;
+    for (int i = 0; i < p.count; ++i)
+        if (!in_place && p.src[i] == p.dst[i]) return refuse(who, "either every tensor is scaled in place or none");
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((longest + 2047) / 2048, 4096)));
+    const hipStream_t s = as_stream(stream);
+    if (src_dtype == F32 && dst_dtype == F32) scale_round_kernel<F32, F32><<<grid, 256, 0, s>>>(p);
+    else if (src_dtype == F32 && dst_dtype == BF16) scale_round_kernel<F32, BF16><<<grid, 256, 0, s>>>(p);
+    else if (src_dtype == F32) scale_round_kernel<F32, F16><<<grid, 256, 0, s>>>(p);
+    else if (src_dtype == BF16) scale_round_kernel<BF16, BF16><<<grid, 256, 0, s>>>(p);
+    else scale_round_kernel<F16, F16><<<grid, 256, 0, s>>>(p);
+    return check_launch(who);
 }
 
 }  // extern "C"

@@ -70,10 +70,10 @@ __all__ = [
     "stream_of",
 ]
 
-ABI_VERSION = 24
+ABI_VERSION = 25
 MAX_TENSORS_PER_LAUNCH = 16
 MAX_MATRICES = 32
-MAX_ADAMW8_TENSORS = 56
+MAX_ADAMW8_TENSORS = 80
 MAX_LOCAL_RANKS = 64
 MAX_NORM_PARTS = 128
 CLIP_MAX_ELEMENTS = 1048576
@@ -319,20 +319,17 @@ EXPORTED_SYMBOLS: dict[str, tuple[object, tuple[object, ...]]] = {
          _c_i64, _c_void_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i64, _c_f32, _c_i32, _c_void_p, _c_i64,
          _c_void_p),
     ),
-    "hbt_scale_round": (_c_i32, (_c_void_p, _c_void_p, _c_i64, _c_i32, _c_void_p, _c_void_p)),
+    "hbt_scale_round": (
+        _c_i32, (_ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_i32, _c_void_p, _c_void_p)),
     "hbt_adamw8_step": (
         _c_i32,
-        (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_i32,
-         _c_f32, _c_void_p, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_void_p, _c_i32, _c_void_p),
+        (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_i32, _c_f32, _c_void_p, _c_f32,
+         _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_void_p, _c_i32, _c_void_p),
     ),
     "hbt_moments8_encode": (
-        _c_i32,
-        (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_void_p),
-    ),
+        _c_i32, (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_void_p)),
     "hbt_moments8_decode": (
-        _c_i32,
-        (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_void_p),
-    ),
+        _c_i32, (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_void_p)),
 }
 
 _LOCK = threading.Lock()

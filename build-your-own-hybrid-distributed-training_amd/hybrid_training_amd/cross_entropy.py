@@ -3,7 +3,7 @@
 :func:`linear_cross_entropy` is ``cross_entropy(x W^T + bias, target)`` without the logits in
 memory (``hbt_linear_cross_entropy``): a tile of logits becomes its rows' statistics in the
 workgroup that forms it.  With gradients wanted, the exponentials of a piece of the rows (at
-most 1 GiB in 16 bits; float32 tensors keep 32) stand in working storage until the two products that follow
+most 2 GiB in 16 bits; float32 tensors keep 32) stand in working storage until the two products that follow
 have read them, so nothing of that size outlives the call.
 
 A summed or averaged loss computes its gradients in the forward pass, where the exponentials are,
@@ -29,7 +29,6 @@ from torch.autograd.function import once_differentiable
 from . import _native
 from .errors import ShardingError, UnsupportedFeatureError, format_error
 from .linear import _holds_tangent, _rows
-from .optim import scale_gradients
 
 __all__ = ["LinearCrossEntropy", "REDUCTIONS", "linear_cross_entropy"]
 
@@ -134,21 +133,21 @@ def _compute(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, t
 def _scaled(grads: list[torch.Tensor | None], factor: torch.Tensor, dtype: torch.dtype) -> list[torch.Tensor | None]:
     """``grads`` times a device scalar, in ``dtype``: in place where they are in it already, which
     reads and writes nothing for a factor of 1."""
-    present = [g for g in grads if g is not None]
-    device = factor.device
-    factor = factor.to(torch.float32)
-    if all(g.dtype == dtype for g in present):
-        scale_gradients([g for g in present if g.numel()], dtype, 1.0, factor.data_ptr(), device,
-                        "cross_entropy.hbt_scale_inplace")
+    present = [i for i, g in enumerate(grads) if g is not None]
+    if not present:
         return grads
-    out = [None if g is None else torch.empty(g.shape, dtype=dtype, device=device) for g in grads]
-    lib = _native.library()
+    device, held = factor.device, grads[present[0]].dtype
+    out = list(grads)
+    if held != dtype:
+        for i in present:
+            out[i] = torch.empty(grads[i].shape, dtype=dtype, device=device)
     with _native.device_guard(device):
-        for g, o in zip(grads, out):
-            if g is not None and g.numel():
-                _native.check(lib.hbt_scale_round(g.data_ptr(), o.data_ptr(), g.numel(), _native.dtype_code(dtype),
-                                                  factor.data_ptr(), _native.stream_of(device)),
-                              "cross_entropy.hbt_scale_round")
+        _native.check(_native.library().hbt_scale_round(
+            _native.pointer_array([grads[i].data_ptr() for i in present]),
+            _native.pointer_array([out[i].data_ptr() for i in present]),
+            _native.int64_array([grads[i].numel() for i in present]), len(present), _native.dtype_code(held),
+            _native.dtype_code(dtype), factor.to(torch.float32).data_ptr(), _native.stream_of(device)),
+            "cross_entropy.hbt_scale_round")
     return out
 
 

@@ -21,8 +21,10 @@ __all__ = ["BLOCK", "STATE_KEYS", "check_state", "decode", "encode", "zero_state
 
 #: Consecutive elements that share their scales.
 BLOCK = 256
-#: A parameter's state: codes and scales of the first moment and of the second one's root.
-STATE_KEYS = ("exp_avg_codes", "exp_avg_sq_codes", "exp_avg_scales", "exp_avg_sq_scales")
+#: A parameter's state: codes, [blocks][groups of four][first moments and roots][four], and scales,
+#: [blocks][first moments and roots].
+STATE_KEYS = ("moment_codes", "moment_scales")
+_CODES, _SCALES = STATE_KEYS
 
 
 def _blocks(numel: int) -> int:
@@ -32,19 +34,23 @@ def _blocks(numel: int) -> int:
 def zero_state(p: torch.Tensor) -> dict[str, torch.Tensor]:
     """Zero moments beside ``p``."""
     blocks = _blocks(p.numel())
-    codes = torch.zeros(2, blocks * BLOCK, dtype=torch.uint8, device=p.device)
-    scales = torch.zeros(2, blocks, dtype=torch.float32, device=p.device)
-    return dict(zip(STATE_KEYS, (codes[0], codes[1], scales[0], scales[1])))
+    return {_CODES: torch.zeros(blocks, 2 * BLOCK, dtype=torch.uint8, device=p.device),
+            _SCALES: torch.zeros(blocks, 2, dtype=torch.float32, device=p.device)}
 
 
 def check_state(p: torch.Tensor, state: dict, operation: str) -> None:
     """Refuse codes or scales that are not the ones :func:`zero_state` lays out."""
-    blocks = _blocks(p.numel())
-    for key, count, dtype in zip(STATE_KEYS, (blocks * BLOCK, blocks * BLOCK, blocks, blocks),
-                                 (torch.uint8, torch.uint8, torch.float32, torch.float32)):
-        value = state.get(key)
+    blocks = (p.numel() + 255) >> 8
+    codes, scales = state.get(_CODES), state.get(_SCALES)
+    if (codes is not None and scales is not None and codes.dtype is torch.uint8 and scales.dtype is torch.float32
+            and codes.numel() == blocks << 9 and scales.numel() == blocks << 1 and codes.is_contiguous()
+            and scales.is_contiguous() and codes.is_cuda and scales.is_cuda
+            and codes.get_device() == scales.get_device() == p.get_device()
+            and not (codes.data_ptr() | scales.data_ptr()) & 7):
+        return
+    for key, value, count, dtype in ((_CODES, codes, blocks << 9, torch.uint8), (_SCALES, scales, blocks << 1, torch.float32)):
         if (value is None or value.dtype != dtype or value.numel() != count or value.device != p.device
-                or not value.is_contiguous() or (count and value.data_ptr() % 4)):
+                or not value.is_contiguous() or value.data_ptr() % 8):
             raise ShardingError(
                 format_error(operation, f"the state {key!r} must lie dense beside its parameter",
                              expected=f"{count} of {dtype} on {p.device}",
@@ -53,8 +59,9 @@ def check_state(p: torch.Tensor, state: dict, operation: str) -> None:
 
 
 def tables(states: Sequence[dict]) -> tuple:
-    """The four pointer tables of a call over ``states``."""
-    return tuple(_native.pointer_array([s[key].data_ptr() for s in states]) for key in STATE_KEYS)
+    """The pointer tables of a call over ``states``."""
+    return (_native.pointer_array([s[_CODES].data_ptr() for s in states]),
+            _native.pointer_array([s[_SCALES].data_ptr() for s in states]))
 
 
 def _chunks(items: Sequence) -> list:
@@ -75,6 +82,29 @@ def encode(pairs: Sequence[tuple[torch.Tensor, torch.Tensor]], states: Sequence[
                 "optim.hbt_moments8_encode")
 
 
+#: Smaller results share one allocation: a tensor costs more to allocate than to decode.
+_SHARED_MAX = 1 << 18
+
+
+def _results(params: Sequence[torch.Tensor], dtype: torch.dtype, device: torch.device) -> list:
+    """Uninitialised (first, second) tensors shaped like ``params``."""
+    small = [i for i, p in enumerate(params) if p.numel() <= _SHARED_MAX]
+    out: list = [None] * len(params)
+    if len(small) > 1:
+        sizes = []
+        for i in small:
+            n = params[i].numel()
+            sizes += (n, -n % 64, n, -n % 64)  # each starts on a 128-byte line
+        parts = torch.empty(sum(sizes), dtype=dtype, device=device).split(sizes)
+        for k, i in enumerate(small):
+            m, v, shape = parts[4 * k], parts[4 * k + 2], params[i].shape
+            out[i] = (m, v) if len(shape) == 1 else (m.view(shape), v.view(shape))
+    for i, p in enumerate(params):
+        if out[i] is None:
+            out[i] = (torch.empty(p.shape, dtype=dtype, device=device), torch.empty(p.shape, dtype=dtype, device=device))
+    return out
+
+
 def decode(params: Sequence[torch.Tensor], states: Sequence[dict], device: torch.device,
            dtype: torch.dtype = torch.float32) -> list[tuple[torch.Tensor, torch.Tensor]]:
     """The (first, second) moments that ``states`` stand for, shaped like ``params``."""
@@ -82,8 +112,7 @@ def decode(params: Sequence[torch.Tensor], states: Sequence[dict], device: torch
         raise UnsupportedFeatureError(format_error("optim.moments", "moments are decoded to float32 or bfloat16",
                                                    observed=str(dtype)))
     lib = _native.library()
-    out = [(torch.empty(p.shape, dtype=dtype, device=p.device), torch.empty(p.shape, dtype=dtype, device=p.device))
-           for p in params]
+    out = _results(params, dtype, device)
     with _native.device_guard(device):
         stream = _native.stream_of(device)
         for chunk in _chunks(list(zip(out, states))):

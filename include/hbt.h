@@ -38,7 +38,7 @@ extern "C" {
 /* ---- per-call limits ---------------------------------------------------------- */
 #define HBT_MAX_TENSORS_PER_LAUNCH 16 /* AdamW / norm tables; the host splits larger lists */
 #define HBT_MAX_MATRICES 32           /* orthogonalised matrices; the host splits larger lists */
-#define HBT_MAX_ADAMW8_TENSORS 56     /* 8-bit AdamW tables; the host splits larger lists */
+#define HBT_MAX_ADAMW8_TENSORS 80     /* 8-bit AdamW tables; the host splits larger lists */
 
 /* Message describing the last failed call on this thread ("" if none). */
 const char* hbt_last_error(void);
@@ -730,15 +730,16 @@ int32_t hbt_muon_step(void* const* params, const void* const* grads, float* cons
  *
  * Replaces: ShardedOptimizer.step (optim/sharded_optimizer.py:340-355) where the state's
  *   memory counts; the reference holds both moments in the parameter's dtype.
- * Every 256 consecutive elements of a tensor are a block with two fp32 scales.  Element i of
- * tensor t has codes m_codes[t][i] and v_codes[t][i] and scales m_scales[t][i / 256] and
- * v_scales[t][i / 256]; codes are allocated in whole blocks (ceil(numel / 256) * 256 bytes, the
- * ones past the end are written as zeros), codes and scales on 4 bytes.
- *   m = e4m3(m_code) * (m_scale / 256)     (OCP e4m3, NaN included)
- *   r = root(v_code) * v_scale             root(16 e + f) = (16 + f) 2^(e - 19), f 2^-18 for
- *                                          e = 0; 255 is NaN;  v = r^2
+ * Every 256 consecutive elements of a tensor are a block.  Block b of tensor t has two fp32 scales,
+ * scales[t][2 b] (first moments) and scales[t][2 b + 1] (roots of second ones), and 512 bytes of
+ * codes from codes[t][512 b]: for each four consecutive elements the four codes of their first
+ * moments, then the four of their roots.  Both are allocated for whole blocks, ceil(numel / 256) of
+ * them, on 8 bytes; codes past the end are written as zeros.
+ *   m = e4m3(code) * (scale / 256)     (OCP e4m3, NaN included)
+ *   r = root(code) * scale             root(16 e + f) = (16 + f) 2^(e - 19), f 2^-18 for e = 0; 255
+ *                                      is NaN;  v = r^2
  * Encoding takes as scales the largest finite |m| and r of the block (a largest |m| under
- * 2^-100 as 0) and rounds 256 m / m_scale and r / v_scale to the nearest code, ties to even, a positive
+ * 2^-100 as 0) and rounds 256 m / scale and r / scale to the nearest code, ties to even, a positive
  * r to a code of at least 1.  A value that is not finite is held as NaN, alone in its block.
  * Zeroed codes and scales are zero moments.
  * hbt_adamw8_step, per element, each operation in fp32 and rounded once (dtype pairs, R_G,
@@ -754,16 +755,14 @@ int32_t hbt_muon_step(void* const* params, const void* const* grads, float* cons
  * moments of out_dtype (F32, or BF16).  Encoding what was decoded to F32 gives the same codes and scales,
  * second moments under 2^-126 aside.
  * ---------------------------------------------------------------------------- */
-int32_t hbt_adamw8_step(void* const* params, void* const* grads, void* const* m_codes, void* const* v_codes,
-                        float* const* m_scales, float* const* v_scales, const int64_t* numels, int32_t count,
-                        int32_t param_dtype, int32_t grad_dtype, float unscale, const float* grad_mul, float decay,
-                        float lerp_weight, float beta2, float one_minus_beta2, float inverse_bias_correction2_sqrt,
-                        float eps, float neg_step_size, const float* slot, int32_t flags, void* stream);
-int32_t hbt_moments8_encode(const float* const* firsts, const float* const* seconds, void* const* m_codes,
-                            void* const* v_codes, float* const* m_scales, float* const* v_scales,
-                            const int64_t* numels, int32_t count, void* stream);
-int32_t hbt_moments8_decode(const void* const* m_codes, const void* const* v_codes, const float* const* m_scales,
-                            const float* const* v_scales, void* const* firsts, void* const* seconds,
+int32_t hbt_adamw8_step(void* const* params, void* const* grads, void* const* codes, void* const* scales,
+                        const int64_t* numels, int32_t count, int32_t param_dtype, int32_t grad_dtype, float unscale,
+                        const float* grad_mul, float decay, float lerp_weight, float beta2, float one_minus_beta2,
+                        float inverse_bias_correction2_sqrt, float eps, float neg_step_size, const float* slot,
+                        int32_t flags, void* stream);
+int32_t hbt_moments8_encode(const void* const* firsts, const void* const* seconds, void* const* codes,
+                            void* const* scales, const int64_t* numels, int32_t count, void* stream);
+int32_t hbt_moments8_decode(void* const* codes, void* const* scales, void* const* firsts, void* const* seconds,
                             const int64_t* numels, int32_t count, int32_t out_dtype, void* stream);
 
 /* ------------------------------------------------------------------------------
@@ -790,7 +789,7 @@ int32_t hbt_moments8_decode(const void* const* m_codes, const void* const* v_cod
  * from 1 to 2^24.
  * `workspace` (256-byte aligned) holds at least hbt_linear_cross_entropy_workspace's bytes (-1
  * for sizes that the call refuses; `wants`: HBT_LINEAR_DX / DW / DBIAS of the gradients given):
- * at most 1 GiB of exponentials, the gathered rows, and an fp32 dw where there are more.
+ * at most 2 GiB of exponentials, the gathered rows, and an fp32 dw where there are more.
  * ---------------------------------------------------------------------------- */
 #define HBT_LOSS_NONE 0
 #define HBT_LOSS_MEAN 1
@@ -804,13 +803,17 @@ int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int6
                                  int32_t reduction, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------
- * dst[i] = src[i] * (*factor), an fp32 product rounded once to dst's dtype (F32, BF16 or F16).
+ * dst = src * (*factor) over up to HBT_MAX_SCALED tensors, each fp32 product rounded once.
  *
  * Replaces: the multiplication by the loss's own gradient that autograd's backward pass
- *   (training/engine.py:352-422) starts with, for fp32 gradients held until then.
- * `factor` is one fp32 in device memory.  dst may be src for F32 only.
+ *   (training/engine.py:352-422) starts with, for gradients computed before it is known.
+ * src_dtype F32 to dst_dtype F32, BF16 or F16, or one 2-byte dtype to itself; `factor` is one fp32
+ * in device memory.  Every tensor is scaled in place (dst = src, dtypes the same; a factor of 1
+ * then reads and writes nothing) or none is.
  * ---------------------------------------------------------------------------- */
-int32_t hbt_scale_round(const float* src, void* dst, int64_t numel, int32_t dtype, const float* factor, void* stream);
+#define HBT_MAX_SCALED 4
+int32_t hbt_scale_round(const void* const* srcs, void* const* dsts, const int64_t* numels, int32_t count,
+                        int32_t src_dtype, int32_t dst_dtype, const float* factor, void* stream);
 
 #ifdef __cplusplus
 }

@@ -27,15 +27,15 @@ def test_state_is_laid_out_in_whole_blocks(numel):
     state = moments8.zero_state(torch.empty(numel))
     blocks = -(-numel // 256)
     assert tuple(state) == moments8.STATE_KEYS
-    assert [state[k].numel() for k in moments8.STATE_KEYS] == [blocks * 256, blocks * 256, blocks, blocks]
-    assert all(state[k].data_ptr() % 4 == 0 for k in moments8.STATE_KEYS if numel)
+    assert [state[k].numel() for k in moments8.STATE_KEYS] == [blocks * 512, blocks * 2]
+    assert all(state[k].data_ptr() % 8 == 0 for k in moments8.STATE_KEYS if numel)
 
 
 def test_the_library_refuses_bad_tables_before_any_launch():
     lib = _native.library()
     scalars = (1.0, None, 1.0, 0.1, 0.9, 0.1, 1.0, 1e-8, -1e-3, None, 0, None)
-    none = (None,) * 7
-    assert lib.hbt_adamw8_step(*none, 57, 0, 0, *scalars) == -1
+    none = (None,) * 5
+    assert lib.hbt_adamw8_step(*none, 81, 0, 0, *scalars) == -1
     assert b"hbt_adamw8_step: count" in lib.hbt_last_error()
     assert lib.hbt_adamw8_step(*none, 1, 0, 0, *scalars) == -1
     assert lib.hbt_adamw8_step(*none, 0, 0, 2, *scalars) == -1
@@ -44,13 +44,13 @@ def test_the_library_refuses_bad_tables_before_any_launch():
     assert lib.hbt_adamw8_step(*none, 0, 0, 0, *scalars[:-2], 1, None) == -1
     assert lib.hbt_adamw8_step(*none, 0, 0, 0, *scalars[:-3], ctypes.c_void_p(4098), 0, None) == -1
     assert lib.hbt_adamw8_step(*none, 0, 0, 0, *scalars) == 0
-    one, odd, n = _native.pointer_array([4096]), _native.pointer_array([4097]), _native.int64_array([1])
-    assert lib.hbt_adamw8_step(one, one, odd, one, one, one, n, 1, 0, 0, *scalars) == -1
-    assert b"off 4 bytes" in lib.hbt_last_error()
-    assert lib.hbt_adamw8_step(one, one, one, one, one, one, _native.int64_array([-1]), 1, 0, 0, *scalars) == -1
+    one, odd, n = _native.pointer_array([4096]), _native.pointer_array([4100]), _native.int64_array([1])
+    assert lib.hbt_adamw8_step(one, one, odd, one, n, 1, 0, 0, *scalars) == -1
+    assert b"off 8 bytes" in lib.hbt_last_error()
+    assert lib.hbt_adamw8_step(one, one, one, one, _native.int64_array([-1]), 1, 0, 0, *scalars) == -1
     zero = _native.pointer_array([0])
-    assert lib.hbt_adamw8_step(zero, one, one, one, one, one, n, 1, 0, 0, *scalars) == -1
-    assert lib.hbt_moments8_encode(*none, 57, None) == -1
+    assert lib.hbt_adamw8_step(zero, one, one, one, n, 1, 0, 0, *scalars) == -1
+    assert lib.hbt_moments8_encode(*none, 81, None) == -1
     assert lib.hbt_moments8_decode(*none, 0, 2, None) == -1
     assert b"out_dtype 2" in lib.hbt_last_error()
     assert lib.hbt_moments8_decode(*none, 0, 1, None) == 0

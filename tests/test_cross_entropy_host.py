@@ -28,15 +28,15 @@ def test_working_storage():
     assert size(0, 64, 100, 1, 0, 1, 0.0) == 0
     # one token over a large vocabulary: statistics alone
     assert 0 < size(1, 4096, 128256, 1, 0, 1, 0.0) < 1 << 20
-    # evaluation never holds logits, training at most 1 GiB of exponentials beside rows and fp32 sums
+    # evaluation never holds logits, training at most 2 GiB of exponentials beside rows and fp32 sums
     assert size(8192, 4096, 128256, 1, 0, 1, 0.0) < 8192 * 4096 * 2 + (1 << 28) + (8 << 20)
-    one = size(4096, 4096, 128256, 1, 3, 1, 0.0)
-    assert one < GIB + 4096 * 4096 * 2 + (1 << 27)
-    more = size(8192, 4096, 128256, 1, 3, 1, 0.0)
-    assert more < GIB + 8192 * 4096 * 2 + 4 * 128256 * 4096 + (1 << 27)
-    assert size(16384, 4096, 128256, 1, 3, 1, 0.0) - more < 8192 * 4096 * 2 + (4 << 20)
+    one = size(8192, 4096, 128256, 1, 3, 1, 0.0)
+    assert one < 2 * GIB + 8192 * 4096 * 2 + (1 << 27)
+    more = size(16384, 4096, 128256, 1, 3, 1, 0.0)
+    assert more < 2 * GIB + 16384 * 4096 * 2 + 4 * 128256 * 4096 + (1 << 27)
+    assert size(32768, 4096, 128256, 1, 3, 1, 0.0) - more < 16384 * 4096 * 2 + (4 << 20)
     # fp32 results carry the sums themselves
-    assert size(8192, 4096, 128256, 1, 3, 0, 0.0) < more - 4 * 128256 * 4096 + (1 << 20)
+    assert size(16384, 4096, 128256, 1, 3, 0, 0.0) < more - 4 * 128256 * 4096 + (1 << 20)
     assert size(10, 64, 100, 1, 0, 1, 0.1) > size(10, 64, 100, 1, 0, 1, 0.0)
     for bad in ((-1, 64, 100, 1, 0, 1), (1, -1, 100, 1, 0, 1), (1, 64, 0, 1, 0, 1), (1, 64, 100, 3, 0, 1),
                 (1, 64, 100, 1, 8, 1), (1, 64, 100, 1, 1, 2), (1, 64, (1 << 20), 1, 0, 1), (1, 1 << 20, 100, 1, 0, 1),
@@ -62,7 +62,13 @@ def test_the_library_refuses_bad_calls_before_any_launch():
                   dict(nbytes=16), dict(space=ctypes.c_void_p(4100))):
         assert call(**wrong) in (-1, -2), wrong
         assert b"hbt_linear_cross_entropy" in lib.hbt_last_error()
-    assert lib.hbt_scale_round(None, None, 4, 1, None, None) == -1
-    assert lib.hbt_scale_round(p, p, 4, 3, p, None) == -1
-    assert lib.hbt_scale_round(p, p, -4, 1, p, None) == -1
-    assert lib.hbt_scale_round(None, None, 0, 1, None, None) == 0  # nothing to do, and no message left behind
+    one, four = _native.pointer_array([4096]), _native.int64_array([4])
+    assert lib.hbt_scale_round(None, None, None, 1, 0, 1, p, None) == -1
+    assert lib.hbt_scale_round(one, one, four, 5, 0, 0, p, None) == -1
+    assert lib.hbt_scale_round(one, one, four, 1, 0, 1, p, None) == -1  # in place with two dtypes
+    assert lib.hbt_scale_round(one, one, four, 1, 1, 0, p, None) == -1
+    assert lib.hbt_scale_round(one, one, four, 1, 0, 0, None, None) == -1
+    assert lib.hbt_scale_round(_native.pointer_array([4096, 8192]), _native.pointer_array([4096, 12288]),
+                               _native.int64_array([4, 4]), 2, 0, 0, p, None) == -1
+    assert lib.hbt_scale_round(one, one, _native.int64_array([-4]), 1, 0, 0, p, None) == -1
+    assert lib.hbt_scale_round(None, None, None, 0, 0, 1, None, None) == 0  # nothing to do, and no message left behind

@@ -125,10 +125,8 @@ def test_every_code_stands_for_its_value():
     p = torch.empty(256, device=DEV)
     state = moments8.zero_state(p)
     every = torch.arange(256, device=DEV).to(torch.uint8)
-    state["exp_avg_codes"].copy_(every)
-    state["exp_avg_sq_codes"].copy_(every)
-    state["exp_avg_scales"].fill_(3.0)
-    state["exp_avg_sq_scales"].fill_(0.75)
+    state["moment_codes"].view(64, 2, 4).copy_(every.view(64, 1, 4).expand(64, 2, 4))
+    state["moment_scales"].copy_(torch.tensor([[3.0, 0.75]]))
     (m, v), = moments8.decode([p], [state], DEV)
     first = every.view(torch.float8_e4m3fn).float() * (3.0 / 256)
     assert torch.equal(torch.isnan(m), torch.isnan(first)) and torch.equal(m.nan_to_num(0), first.nan_to_num(0))
@@ -201,6 +199,13 @@ def test_zeros_tiny_and_non_finite_gradients():
     assert torch.isfinite(m[514:]).all() and torch.isfinite(v[514:]).all() and torch.isfinite(p[514:].detach()).all()
     assert (m[514:768] == m[514]).all() and m[514] > 0
     assert v[769] > 0 and v[769] <= (2.0**-18 * 1.0001) ** 2 * v[768]
+    # a block of nothing finite has zero scales and keeps NaN everywhere
+    state = moments8.zero_state(torch.empty(256))
+    state = {k: v.to(DEV) for k, v in state.items()}
+    wild = torch.tensor([math.inf, -math.inf, math.nan, math.inf] * 64, device=DEV)
+    moments8.encode([(wild, wild.abs())], [state], DEV)
+    (wm, wv), = moments8.decode([wild], [state], DEV)
+    assert (state["moment_scales"] == 0).all() and torch.isnan(wm).all() and torch.isnan(wv).all()
     # the next step starts from them: the element that was not finite stays so, alone
     p.grad.copy_(torch.full((1024,), 0.1, device=DEV))
     optimizer.step()
@@ -366,12 +371,12 @@ def test_state_that_does_not_fit_is_refused():
     optimizer = _optimizer(params)
     optimizer.step()
     before = [p.detach().clone(), *_codes(optimizer, p)]
-    kept = optimizer.inner.state[p]["exp_avg_codes"]
-    for wrong in (kept[:300], kept.float(), kept.cpu()):
-        optimizer.inner.state[p]["exp_avg_codes"] = wrong
-        with pytest.raises(ShardingError, match="exp_avg_codes"):
+    kept = optimizer.inner.state[p]["moment_codes"]
+    for wrong in (kept[:1], kept.float(), kept.cpu()):
+        optimizer.inner.state[p]["moment_codes"] = wrong
+        with pytest.raises(ShardingError, match="moment_codes"):
             optimizer.step()
-    optimizer.inner.state[p]["exp_avg_codes"] = kept
+    optimizer.inner.state[p]["moment_codes"] = kept
     assert optimizer.inner.state[p]["step"] == 1
     assert all(torch.equal(x, y) for x, y in zip(before, [p.detach(), *_codes(optimizer, p)]))
     payload = optimizer.state_dict()

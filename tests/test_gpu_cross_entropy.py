@@ -310,8 +310,8 @@ def test_some_gradients_alone(which):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_more_rows_than_one_piece_holds(dtype):
-    """9000 x 65537 exponentials pass 1 GiB: the sums over rows are carried from piece to piece."""
-    tokens, inner, vocab = 9000, 24, 65537
+    """18000 x 65537 exponentials pass 2 GiB: the sums over rows are carried from piece to piece."""
+    tokens, inner, vocab = 18000, 24, 65537
     x, w, b, target = _inputs(tokens, inner, vocab, dtype, bias=True, ignored=0.05)
     leaves = [t.requires_grad_(True) for t in (x, w, b)]
     loss = linear_cross_entropy(x, w, target, b, reduction="sum")
