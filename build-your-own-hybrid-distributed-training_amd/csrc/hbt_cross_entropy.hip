@@ -64,13 +64,21 @@ __device__ __forceinline__ float wave_max(float x) {
     return x;
 }
 
-// exp(t) for t <= 0: the hardware's base-2 exponential where the result is rounded to 16 bits or
-// summed with others of its size, the accurate function for fp32 tensors.
+// Statistics, and the exponentials under them, are in units of log(2) for 2-byte tensors: their
+// logits are multiplied by log2(e) once and the hardware's base-2 exponential takes them (2^-23 or so
+// off, far below what 16 bits keep).  fp32 tensors keep the natural unit and the accurate function.
+template <int D>
+__device__ __forceinline__ float in_units(float z) {
+    if constexpr (D == F32) return z;
+    else return z * kLog2e;
+}
 template <int D>
 __device__ __forceinline__ float exponential(float t) {
     if constexpr (D == F32) return expf(t);
-    else return __builtin_amdgcn_exp2f(t * kLog2e);
+    else return __builtin_amdgcn_exp2f(t);
 }
+template <int D>
+constexpr double unit() { return D == F32 ? 1.0 : 0.69314718055994531; }
 
 // ---- the tokens that carry a loss ---------------------------------------------------------
 struct PrepareArgs {
@@ -190,8 +198,9 @@ struct LogitArgs {
     float* sums;        // the same: sum of the logits, or null without smoothing
     float* target;      // row -> its target's logit
     void* kept;         // [row of the piece][ldk] exponentials, or null
-    int64_t ldx, ldw, ldk, stride, vocab, inner;  // stride: rows of stats
-    int tiles_n;
+    int64_t ldx, ldw, ldk, stride, inner;  // stride: rows of stats
+    int64_t column, end;     // the words [column, end) of this launch, whose tiles are first_tile and on
+    int tiles_n, first_tile;
     Piece piece;
 };
 
@@ -209,155 +218,205 @@ __device__ __forceinline__ float quarters_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// A 4 x 4 transposition between four registers and the four quarters of a wavefront: afterwards
-// register c of quarter q holds what register q of quarter c held.
-__device__ __forceinline__ void transpose_quarters(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
-    const auto ac = __builtin_amdgcn_permlane32_swap(a, c, false, false);
-    const auto bd = __builtin_amdgcn_permlane32_swap(b, d, false, false);
-    const auto low = __builtin_amdgcn_permlane16_swap(ac[0], bd[0], false, false);
-    const auto high = __builtin_amdgcn_permlane16_swap(ac[1], bd[1], false, false);
-    a = low[0], b = low[1], c = high[0], d = high[1];
+// Two registers of sixteen columns' neighbours: quarter q of a wavefront holds columns 4 q .. + 3 of the
+// first sixteen in `a` and of the next sixteen in `b`; afterwards it holds columns 8 q .. + 3 of the
+// thirty-two in `a` and 8 q + 4 .. + 7 in `b`.
+__device__ __forceinline__ void pair_columns(uint32_t& a, uint32_t& b) {
+    const auto half = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    const auto row = __builtin_amdgcn_permlane16_swap(half[0], half[1], false, false);
+    a = row[0], b = row[1];
 }
 
-// A tile's logits to statistics and exponentials, in the registers that the matrix cores leave
+// Tiles' logits to statistics and exponentials, in the registers that the matrix cores leave
 // them in: lane l holds, of row l % 16 of each sixteen rows, four columns of each sixteen.  The
 // largest of a row is taken in the lane, over the quarters, and over the wavefronts through LDS.
+//
+// A workgroup takes every gridDim.x-th tile.  With tiles of 256, of which a CU holds one, the grid is
+// one workgroup a CU, and the first loads of its next tile are in flight while it reduces this one's logits.
 template <int D, class T, bool kAsync>
 __global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
     extern __shared__ __align__(16) char lds[];
     int first, count;
     piece_rows(p.piece, first, count);
     const int tiles_m = (count + T::BM - 1) / T::BM, total = tiles_m * p.tiles_n;
-    if (static_cast<int>(blockIdx.x) >= total) return;
-    int tm, tn;
-    band_order<8>(xcd_tile(blockIdx.x, total), tiles_m, p.tiles_n, tm, tn);
-    const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
-    f32x4 acc[T::TM][T::TN];
+    int t = blockIdx.x;
+    if (t >= total) return;
+    // A thread's places are worked out anew for each tile: kept through the products, they would take
+    // registers that those need.
+    const auto thread = []() {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        return tid;
+    };
+    const auto row_of = [](int tid) { return (tid >> 6) / T::WN * (T::BM / T::WM) + (tid & 15); };
+    const auto column_of = [](int tid) { return __builtin_amdgcn_readfirstlane(tid >> 6) % T::WN * (T::BN / T::WN); };
+    const int32_t* words = p.word + first;
     const char* x = static_cast<const char*>(p.x) + first * p.ldx * elem_bytes<D>();
-    tile_product<D, true, true, T, kAsync>(x, p.ldx, m0, count, p.w, p.ldw, n0, p.vocab, 0, p.inner, lds, acc);
-    const int rows = static_cast<int>(min<int64_t>(count - m0, T::BM));
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
-    const int wm = (wave / T::WN) * (T::BM / T::WM) + (lane & 15), wn = (wave % T::WN) * (T::BN / T::WN);
-    const int left = static_cast<int>(p.vocab - n0) - wn;  // columns from the wavefront's first one
-    if (p.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j) {
-            const int have = left - 16 * j - 4 * q;
-            const f32x4 b = load_row<D>(p.bias, n0 + wn + 16 * j + 4 * q, have);
-#pragma unroll
-            for (int i = 0; i < T::TM; ++i) acc[i][j] += b;
-        }
-    }
-    const bool edge = left < 16 * T::TN;
-    float* line = reinterpret_cast<float*>(lds);  // [3][WN][BM]: largest, sums of exponentials and of logits
+    float* line = reinterpret_cast<float*>(lds + lds_bytes<T, kAsync>());  // [3][WN][BM]: largest, two sums
     constexpr int kLine = T::WN * T::BM;
-    const int slot = (wave % T::WN) * T::BM + wm;
-    if (p.sums != nullptr) {
+    TileProduct<D, true, true, T, kAsync> tile;
+    int64_t m0, n0;
+    int tn;
+    int word[T::TM];        // the rows' targets, and once they have arrived a byte for each: the
+    uint32_t places[2];     // target's column from the wavefront's first one, 255 outside of its columns
+    static_assert(T::TM <= 8 && 16 * T::TN <= 255, "a byte a row");
+    const auto begin = [&]() {
+        int tm;
+        band_order<8>(xcd_tile(t, total), tiles_m, p.tiles_n, tm, tn);
+        m0 = int64_t(tm) * T::BM, n0 = p.column + int64_t(tn) * T::BN;
+        const int tid = thread();
+        if (p.inner > 0) {
+            tile.init(x, p.ldx, m0, count, p.w, p.ldw, n0, p.end, 0, p.inner, tid);
+            tile.begin(lds);
+        }
+        const int wm = row_of(tid);
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) word[i] = words[min(static_cast<int>(m0) + wm + 16 * i, count - 1)];
+    };
+    const auto place = [&]() {
+        const int wn = column_of(thread());
+        places[0] = places[1] = 0;
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum += 16 * j + 4 * q + e < left ? acc[i][j][e] : 0.0f;
-            sum = quarters_sum(sum);
-            if (q == 0) line[2 * kLine + slot + 16 * i] = sum;
+            const int at = word[i] - static_cast<int>(n0) - wn;
+            places[i / 4] |= (at >= 0 && at < 16 * T::TN ? static_cast<uint32_t>(at) : 255u) << (8 * (i % 4));
         }
-    }
-    if (edge) {
+    };
+    f32x4 acc[T::TM][T::TN];
+    begin();
+    for (;;) {
+        place();
+        if (p.inner > 0) {
+            tile.run(lds, acc);
+        } else {
+#pragma unroll
+            for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+                for (int j = 0; j < T::TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            __syncthreads();
+        }
+        const int64_t m = m0, n = n0;
+        const int tid = thread(), q = (tid >> 4) & 3, wm = row_of(tid), wn = column_of(tid), slot = wn / (T::BN / T::WN) * T::BM + wm;
+        const int rows = static_cast<int>(min<int64_t>(count - m, T::BM));
+        const int left = static_cast<int>(p.end - n) - wn;  // columns from the wavefront's first one
+        const int column = tn + p.first_tile;
+        const uint32_t targets[2] = {places[0], places[1]};
+        if (p.bias != nullptr) {
+#pragma unroll
+            for (int j = 0; j < T::TN; ++j) {
+                const f32x4 b = load_row<D>(p.bias, n + wn + 16 * j + 4 * q, left - 16 * j - 4 * q);
+#pragma unroll
+                for (int i = 0; i < T::TM; ++i) acc[i][j] += b;
+            }
+        }
+        t += gridDim.x;
+        const bool more = T::BM == 256 && t < total;
+        if (more) begin();
+        if (p.sums != nullptr) {
+#pragma unroll
+            for (int i = 0; i < T::TM; ++i) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum += 16 * j + 4 * q + e < left ? acc[i][j][e] : 0.0f;
+                sum = quarters_sum(sum);
+                if (q == 0) line[2 * kLine + slot + 16 * i] = sum;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < T::TM; ++i)
 #pragma unroll
             for (int j = 0; j < T::TN; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (16 * j + 4 * q + e >= left) acc[i][j][e] = -INFINITY;
-    }
-    const int32_t* word = p.word + first + m0;
-    int at[T::TM];  // the target's column from the wavefront's first one
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = in_units<D>(acc[i][j][e]);
+        if (left < 16 * T::TN) {  // past the last column
 #pragma unroll
-    for (int i = 0; i < T::TM; ++i) at[i] = wm + 16 * i < rows ? word[wm + 16 * i] - static_cast<int>(n0) - wn : -1;
-#pragma unroll
-    for (int i = 0; i < T::TM; ++i) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j)
-            top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
-        top = quarters_max(top);
-        if (q == 0) line[slot + 16 * i] = top;
-    }
-#pragma unroll
-    for (int i = 0; i < T::TM; ++i) {
-        const bool here = at[i] >= 0 && at[i] < 16 * T::TN;
-        if (__any(here)) {  // seldom: a wavefront's columns are a small part of the vocabulary
-            float z = 0.0f;
-#pragma unroll
-            for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (at[i] == 16 * j + 4 * q + e) z = acc[i][j][e];
-            if (here && ((at[i] >> 2) & 3) == q) p.target[first + m0 + wm + 16 * i] = z;
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < T::TM; ++i) {
-        float top = line[wm + 16 * i];
-#pragma unroll
-        for (int w = 1; w < T::WN; ++w) top = fmaxf(top, line[w * T::BM + wm + 16 * i]);
-        if (top == -INFINITY) top = 0.0f;  // a tile of nothing but -inf
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] = exponential<D>(acc[i][j][e] - top);
-            sum += (acc[i][j][0] + acc[i][j][1]) + (acc[i][j][2] + acc[i][j][3]);
-        }
-        sum = quarters_sum(sum);
-        if (q == 0) line[kLine + slot + 16 * i] = sum;
-        // Whole runs of the wavefront's columns lie inside a stored row, whose length is a multiple of 64.
-        if (p.kept == nullptr || n0 + wn >= p.ldk) continue;
-        const int64_t to = (m0 + wm + 16 * i) * p.ldk + n0 + wn;
-        const bool in = wm + 16 * i < rows;
-        if constexpr (D == F32) {
-#pragma unroll
-            for (int j = 0; j < T::TN; ++j)
-                if (in) *reinterpret_cast<f32x4*>(static_cast<float*>(p.kept) + to + 16 * j + 4 * q) = acc[i][j];
-        } else {
-            uint32_t h[T::TN][2];
-#pragma unroll
-            for (int j = 0; j < T::TN; ++j) {
-                h[j][0] = pack2_rounded<F16>(acc[i][j][0], acc[i][j][1]);
-                h[j][1] = pack2_rounded<F16>(acc[i][j][2], acc[i][j][3]);
-            }
-            uint16_t* kept = static_cast<uint16_t*>(p.kept) + to;
-            if constexpr (T::TN == 4) {  // sixteen consecutive columns a lane, 128 bytes of a row a wavefront
-                transpose_quarters(h[0][0], h[1][0], h[2][0], h[3][0]);
-                transpose_quarters(h[0][1], h[1][1], h[2][1], h[3][1]);
-                if (in) {
-                    u32x4* out = reinterpret_cast<u32x4*>(kept + 16 * q);
-                    out[0] = u32x4{h[0][0], h[0][1], h[1][0], h[1][1]};
-                    out[1] = u32x4{h[2][0], h[2][1], h[3][0], h[3][1]};
-                }
-            } else {
+            for (int i = 0; i < T::TM; ++i)
 #pragma unroll
                 for (int j = 0; j < T::TN; ++j)
-                    if (in) *reinterpret_cast<u32x2*>(kept + 16 * j + 4 * q) = u32x2{h[j][0], h[j][1]};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (16 * j + 4 * q + e >= left) acc[i][j][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
+            float top = fmaxf(fmaxf(acc[i][0][0], acc[i][0][1]), fmaxf(acc[i][0][2], acc[i][0][3]));
+#pragma unroll
+            for (int j = 1; j < T::TN; ++j)
+                top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
+            top = quarters_max(top);
+            if (q == 0) line[slot + 16 * i] = top;
+        }
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
+            const int at = (targets[i / 4] >> (8 * (i % 4))) & 255;
+            if (__any(at != 255)) {  // seldom: a wavefront's columns are a small part of the vocabulary
+                float z = 0.0f;
+#pragma unroll
+                for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (at == 16 * j + 4 * q + e) z = acc[i][j][e];
+                if (at != 255 && ((at >> 2) & 3) == q && wm + 16 * i < rows) p.target[first + m + wm + 16 * i] = z;
             }
         }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows; i += T::kThreads) {
-        float top = line[i], sum = line[kLine + i];
+        __syncthreads();
 #pragma unroll
-        for (int w = 1; w < T::WN; ++w) top = fmaxf(top, line[w * T::BM + i]), sum += line[kLine + w * T::BM + i];
-        p.stats[tn * p.stride + m0 + i] = make_float2(top, sum);
-        if (p.sums != nullptr) {
-            float logits = line[2 * kLine + i];
+        for (int i = 0; i < T::TM; ++i) {
+            float top = line[wm + 16 * i];
 #pragma unroll
-            for (int w = 1; w < T::WN; ++w) logits += line[2 * kLine + w * T::BM + i];
-            p.sums[tn * p.stride + m0 + i] = logits;
+            for (int w = 1; w < T::WN; ++w) top = fmaxf(top, line[w * T::BM + wm + 16 * i]);
+            if (top == -INFINITY) top = 0.0f;  // a tile of nothing but -inf
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < T::TN; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = exponential<D>(acc[i][j][e] - top);
+                sum += (acc[i][j][0] + acc[i][j][1]) + (acc[i][j][2] + acc[i][j][3]);
+            }
+            sum = quarters_sum(sum);
+            if (q == 0) line[kLine + slot + 16 * i] = sum;
+            // Whole runs of the wavefront's columns lie inside a stored row, whose length is a multiple of 64.
+            if (p.kept == nullptr || n + wn >= p.ldk) continue;
+            const int64_t to = (m + wm + 16 * i) * p.ldk + n + wn;
+            const bool in = wm + 16 * i < rows;
+            if constexpr (D == F32) {
+#pragma unroll
+                for (int j = 0; j < T::TN; ++j)
+                    if (in) *reinterpret_cast<f32x4*>(static_cast<float*>(p.kept) + to + 16 * j + 4 * q) = acc[i][j];
+            } else {
+                uint32_t h[T::TN][2];
+#pragma unroll
+                for (int j = 0; j < T::TN; ++j) {
+                    h[j][0] = pack2_rounded<F16>(acc[i][j][0], acc[i][j][1]);
+                    h[j][1] = pack2_rounded<F16>(acc[i][j][2], acc[i][j][3]);
+                }
+                uint16_t* kept = static_cast<uint16_t*>(p.kept) + to;
+#pragma unroll
+                for (int j = 0; j < T::TN; j += 2) {  // 64 bytes of a row a quarter: eight columns a lane
+                    pair_columns(h[j][0], h[j + 1][0]);
+                    pair_columns(h[j][1], h[j + 1][1]);
+                    if (in) *reinterpret_cast<u32x4*>(kept + 16 * j + 8 * q) = u32x4{h[j][0], h[j][1], h[j + 1][0], h[j + 1][1]};
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);  // a row at a time: mixed, they do not fit the registers
         }
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows; i += T::kThreads) {
+            float top = line[i], sum = line[kLine + i];
+#pragma unroll
+            for (int w = 1; w < T::WN; ++w) top = fmaxf(top, line[w * T::BM + i]), sum += line[kLine + w * T::BM + i];
+            p.stats[column * p.stride + m + i] = make_float2(top, sum);
+            if (p.sums != nullptr) {
+                float logits = line[2 * kLine + i];
+#pragma unroll
+                for (int w = 1; w < T::WN; ++w) logits += line[2 * kLine + w * T::BM + i];
+                p.sums[column * p.stride + m + i] = logits;
+            }
+        }
+        if (!more) return;
+        // A barrier above lies between this and the next tile's writes of the lines.
     }
 }
 
@@ -417,8 +476,8 @@ __global__ __launch_bounds__(512) void thin_logit_kernel(const void* x_, int64_t
     float sum = 0.0f, top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        if (e >= have) acc[e] = -INFINITY;
-        else sum += acc[e];
+        if (e < have) sum += acc[e];
+        acc[e] = e < have ? in_units<D>(acc[e]) : -INFINITY;
         if (at == e && e < have) target_logit[row] = acc[e];
         top = fmaxf(top, acc[e]);
     }
@@ -451,6 +510,7 @@ struct JoinArgs {
     float* loss;               // token -> loss, or null
     double* row_loss;          // row -> loss, or null
     int64_t ignore, vocab, stride;
+    double unit;               // of the largest and the targets' logits
     int tiles;
     float smoothing;
     Piece piece;
@@ -461,10 +521,10 @@ struct JoinArgs {
 struct Running {
     float top = -INFINITY;
     double sum = 0.0;
-    __device__ __forceinline__ void add(float t, double s) {
+    __device__ __forceinline__ void add(float t, double s, float unit) {
         if (s == 0.0) return;
         const float high = fmaxf(top, t);
-        sum = (sum == 0.0 ? 0.0 : sum * expf(top - high)) + s * (t == high ? 1.0 : static_cast<double>(expf(t - high)));
+        sum = (sum == 0.0 ? 0.0 : sum * expf((top - high) * unit)) + s * expf((t - high) * unit);
         top = high;
     }
 };
@@ -485,9 +545,9 @@ __device__ __forceinline__ void finish_row(const JoinArgs& p, int row, const Run
     }
     // log p = (z_t - top) - log(sum): the two parts of a nearly certain target are both small
     const double log_sum = log(r.sum);
-    const double log_p = known ? (static_cast<double>(p.target[row]) - r.top) - log_sum : NAN;
+    const double log_p = known ? (static_cast<double>(p.target[row]) - r.top) * p.unit - log_sum : NAN;
     double loss = -(1.0 - p.smoothing) * log_p;
-    if (p.smoothing != 0.0f) loss += p.smoothing * ((r.top + log_sum) - logits / static_cast<double>(p.vocab));
+    if (p.smoothing != 0.0f) loss += p.smoothing * ((r.top * p.unit + log_sum) - logits / static_cast<double>(p.vocab));
     if (p.loss != nullptr) p.loss[token] = static_cast<float>(loss);
     if (p.row_loss != nullptr) p.row_loss[row] = loss;
     if (p.row != nullptr)
@@ -495,37 +555,41 @@ __device__ __forceinline__ void finish_row(const JoinArgs& p, int row, const Run
                          p.weight[row] * p.piece.control->scale_in};
 }
 
-// Statistics [tile][row]: a workgroup joins 64 rows, a lane each; its wavefronts take tiles in turn.
-constexpr int kJoinWaves = 8;
-__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(JoinArgs p) {
-    __shared__ float tops[kJoinWaves][64];
-    __shared__ double totals[kJoinWaves][64], logit_sums[kJoinWaves][64];
+// Statistics [tile][row]: a workgroup joins 16 rows, 128 bytes of a tile's; its 32 groups of 16 lanes
+// take tiles in turn.
+constexpr int kJoinRows = 16, kJoinGroups = 32;
+__global__ __launch_bounds__(kJoinRows * kJoinGroups) void join_kernel(JoinArgs p) {
+    __shared__ float tops[kJoinGroups][kJoinRows];
+    __shared__ double totals[kJoinGroups][kJoinRows], logit_sums[kJoinGroups][kJoinRows];
     int first, count;
     piece_rows(p.piece, first, count);
-    if (static_cast<int>(blockIdx.x) * 64 >= count) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane, at = min(i, count - 1);
+    if (static_cast<int>(blockIdx.x) * kJoinRows >= count) return;
+    const int lane = threadIdx.x % kJoinRows, group = threadIdx.x / kJoinRows;
+    const int i = blockIdx.x * kJoinRows + lane, at = min(i, count - 1);
+    const float unit = static_cast<float>(p.unit);
     Running r;
     double logits = 0.0;
-    for (int t = wave; t < p.tiles; t += 4 * kJoinWaves) {
+    for (int t = group; t < p.tiles; t += 4 * kJoinGroups) {
         float2 s[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {  // four loads in flight
-            const int tile = t + k * kJoinWaves;
+            const int tile = t + k * kJoinGroups;
             s[k] = tile < p.tiles ? p.stats[tile * p.stride + at] : make_float2(0.0f, 0.0f);
             if (p.sums != nullptr && tile < p.tiles) logits += p.sums[tile * p.stride + at];
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) r.add(s[k].x, s[k].y);
+        for (int k = 0; k < 4; ++k) r.add(s[k].x, s[k].y, unit);
     }
-    tops[wave][lane] = r.top, totals[wave][lane] = r.sum, logit_sums[wave][lane] = logits;
-    __syncthreads();
-    if (wave != 0 || i >= count) return;
-#pragma unroll
-    for (int w = 1; w < kJoinWaves; ++w) {
-        r.add(tops[w][lane], totals[w][lane]);
-        logits += logit_sums[w][lane];
+    for (int half = kJoinGroups / 2; half > 0; half >>= 1) {
+        tops[group][lane] = r.top, totals[group][lane] = r.sum, logit_sums[group][lane] = logits;
+        __syncthreads();
+        if (group < half) {
+            r.add(tops[group + half][lane], totals[group + half][lane], unit);
+            logits += logit_sums[group + half][lane];
+        }
+        __syncthreads();
     }
-    finish_row(p, first + i, r, logits);
+    if (group == 0 && i < count) finish_row(p, first + i, r, logits);
 }
 
 // Statistics [row][tile], many tiles and few rows: a workgroup a row, its lanes' parts joined in a tree.
@@ -533,6 +597,7 @@ __global__ __launch_bounds__(1024) void thin_join_kernel(JoinArgs p) {
     __shared__ float tops[1024];
     __shared__ double totals[1024], logit_sums[1024];
     const int row = blockIdx.x, tid = threadIdx.x;
+    const float unit = static_cast<float>(p.unit);
     Running r;
     double logits = 0.0;
     for (int t = tid; t < p.tiles; t += 4096) {
@@ -544,13 +609,13 @@ __global__ __launch_bounds__(1024) void thin_join_kernel(JoinArgs p) {
             if (p.sums != nullptr && tile < p.tiles) logits += p.sums[row * p.stride + tile];
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) r.add(s[k].x, s[k].y);
+        for (int k = 0; k < 4; ++k) r.add(s[k].x, s[k].y, unit);
     }
     tops[tid] = r.top, totals[tid] = r.sum, logit_sums[tid] = logits;
     for (int half = 512; half > 0; half >>= 1) {
         __syncthreads();
         if (tid < half) {
-            r.add(tops[tid + half], totals[tid + half]);
+            r.add(tops[tid + half], totals[tid + half], unit);
             logits += logit_sums[tid + half];
             tops[tid] = r.top, totals[tid] = r.sum, logit_sums[tid] = logits;
         }
@@ -581,7 +646,8 @@ struct SoftmaxArgs {
     const Row* row;
     const int32_t* word;
     int64_t ldk, vocab, stride;
-    int tile, segment;  // columns of a tile, and those that a workgroup takes
+    int64_t cut;  // the words before it are in tiles of `tile` columns, the others in tiles of `last`
+    int tile, last, segment;  // segment: columns that a workgroup takes
     float smoothing;
     Piece piece;
 };
@@ -605,7 +671,9 @@ __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs p) {
     const int64_t end = min<int64_t>(p.ldk, (part + 1) * int64_t(p.segment));
     for (int64_t j = part * int64_t(p.segment) + threadIdx.x * E; j < end; j += 256 * E) {
         const u32x4 unit = *reinterpret_cast<const u32x4*>(line + j * B);
-        const float factor = expf(stats[min<int64_t>(j, p.vocab - 1) / p.tile * p.stride].x - row.top) * row.inverse * row.weight;
+        const int64_t word_at = min<int64_t>(j, p.vocab - 1);
+        const int64_t at = word_at < p.cut ? word_at / p.tile : p.cut / p.tile + (word_at - p.cut) / p.last;
+        const float factor = exponential<D>(stats[at * p.stride].x - row.top) * row.inverse * row.weight;
         float v[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -628,9 +696,19 @@ struct GradArgs {
     const int32_t* token;  // y's row for a row of the piece, or null: its own
     float* partial;        // [splits][m][ldp]
     int64_t lda, ldb, ldy, ldbefore, ldp, m, n, k, m_in, n_in;  // m_in, n_in: rows that the operands hold
-    int tiles_n, splits;
+    int tile, tiles_n, blocks, splits;
     Piece piece;
 };
+
+// The tiles of a product over `m` rows and the parts of each one's sum.  The grid is made for as
+// many rows as there may be; where fewer carry a loss, a split sum takes the workgroups that they leave:
+// 1801 rows of 3001, 1000 x 32003: 6 parts of 32 tiles instead of 4, 135 us where 4 take 198.
+template <bool kRows>
+__device__ __forceinline__ void tiles_and_splits(const GradArgs& p, int64_t m, int& tiles_m, int& splits) {
+    tiles_m = static_cast<int>((m + p.tile - 1) / p.tile);
+    splits = p.splits;
+    if (kRows && splits > 1 && tiles_m > 0) splits = max(splits, min(p.blocks / (tiles_m * p.tiles_n), 16));
+}
 
 // y = a b (dx: the rows of a are the piece's; dW: the sum runs over them), times the call's scale.
 template <int D, int OD, bool kRows>
@@ -654,20 +732,21 @@ __global__ __launch_bounds__(T::kThreads, 2) void grad_kernel(GradArgs p) {
     int first, count;
     piece_rows(p.piece, first, count);
     const int64_t m = kRows ? count : p.m, k = kRows ? p.k : count;
-    const int tiles_m = static_cast<int>((m + T::BM - 1) / T::BM), total = tiles_m * p.tiles_n;
-    if (static_cast<int>(blockIdx.x) >= total) return;
-    int tm, tn;
-    band_order<8>(xcd_tile(blockIdx.x, total), tiles_m, p.tiles_n, tm, tn);
+    int tiles_m, splits, tm, tn;
+    tiles_and_splits<kRows>(p, m, tiles_m, splits);
+    const int total = tiles_m * p.tiles_n, split = total > 0 ? static_cast<int>(blockIdx.x) / total : splits;
+    if (split >= splits) return;
+    band_order<8>(xcd_tile(static_cast<int>(blockIdx.x) - split * total, total), tiles_m, p.tiles_n, tm, tn);
     const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
     constexpr int BK = tile_k<D>();
-    const int64_t part = ((k + p.splits - 1) / p.splits + BK - 1) / BK * BK;
-    const int64_t k0 = min<int64_t>(k, blockIdx.y * part), k1 = min<int64_t>(k, k0 + part);
+    const int64_t part = ((k + splits - 1) / splits + BK - 1) / BK * BK;
+    const int64_t k0 = min<int64_t>(k, split * part), k1 = min<int64_t>(k, k0 + part);
     f32x4 acc[T::TM][T::TN];
     const char* b = static_cast<const char*>(p.b) + (kRows ? 0 : first * p.ldb * elem_bytes<D>());
     tile_product<D, kRows, false, T, kAsync>(p.a, p.lda, m0, kRows ? m : p.m_in, b, p.ldb, n0, p.n_in, k0, k1, lds, acc);
     const int rows = static_cast<int>(min<int64_t>(m - m0, T::BM)), cols = static_cast<int>(min<int64_t>(p.n - n0, T::BN));
     const GradEpilogue<D, OD, kRows> tile{p, p.piece.control->scale_out, first};
-    float* partial = p.partial == nullptr ? nullptr : p.partial + (blockIdx.y * p.m + m0) * p.ldp + n0;
+    float* partial = p.partial == nullptr ? nullptr : p.partial + (split * m + m0) * p.ldp + n0;
     finish_tile<T, kAsync, 2>(
         lds, acc,
         [&](int i, int j) {
@@ -688,11 +767,13 @@ __global__ __launch_bounds__(256) void grad_join_kernel(GradArgs p) {
     int first, count;
     piece_rows(p.piece, first, count);
     const int64_t m = kRows ? count : p.m, units = p.ldp / 4, total = m * units;
+    int tiles_m, splits;
+    tiles_and_splits<kRows>(p, m, tiles_m, splits);
     const GradEpilogue<D, OD, kRows> tile{p, p.piece.control->scale_out, first};
     for (int64_t u = blockIdx.x * int64_t(256) + threadIdx.x; u < total; u += int64_t(gridDim.x) * 256) {
         const int64_t i = u / units, j = u % units * 4;
         f32x4 v = *reinterpret_cast<const f32x4*>(p.partial + i * p.ldp + j);
-        for (int s = 1; s < p.splits; ++s) v += *reinterpret_cast<const f32x4*>(p.partial + (s * p.m + i) * p.ldp + j);
+        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(p.partial + (s * m + i) * p.ldp + j);
         const int have = static_cast<int>(min<int64_t>(p.n - j, 4));
         tile.store(i, j, have, v, tile.before(i, j, have));
     }
@@ -760,12 +841,28 @@ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 struct Plan {
     bool thin, grads, rows_only;
     int size;               // logit tiles
+    int64_t cut;            // the words from here on are in tiles of 128 instead
     int tiles, pieces;
     int64_t most;           // rows of a piece, at most
     int64_t ld, ldk;        // gathered rows; exponentials
     int64_t control, place, token, word, weight, target, row, row_loss, rows, stats, sums, kept, dw_sums, db_sums,
         parts, partial, bytes;
 };
+
+// Where the last, mostly empty round of tiles of 256 is better formed in tiles of 128: the words from
+// which on they are.  788 tiles (1024 tokens over 50257 words) are three rounds and 20 tiles.
+int64_t column_cut(int64_t rows, int64_t vocab, double steps) {
+    const int64_t high = (rows + 255) / 256, wide = (vocab + 255) / 256, high128 = (rows + 127) / 128;
+    int64_t best = vocab;
+    double least = 0.97 * round_cost(256, high * wide, steps, false, 9.0);
+    for (int64_t less = 1; less < std::min<int64_t>(wide, 256) && less * high < 256; ++less) {
+        const int64_t cut = (wide - less) * 256;
+        const double cost = round_cost(256, high * (wide - less), steps, false, 9.0) +
+                            round_cost(128, high128 * ((vocab - cut + 127) / 128), steps, false, 6.0) + 3.0;
+        if (cost < least) least = cost, best = cut;
+    }
+    return best;
+}
 
 // `aligned`: W's rows load straight into LDS, which tiles of 256 need.
 Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants, int grad_dtype, bool smooth,
@@ -796,7 +893,8 @@ Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants,
                                            s == 256 ? 9.0 : (s == 128 ? 6.0 : 3.5));
             if (least == 0.0 || cost < least) least = cost, p.size = s;
         }
-        p.tiles = static_cast<int>((vocab + p.size - 1) / p.size);
+        p.cut = p.size == 256 ? column_cut(rows, vocab, steps) : vocab;
+        p.tiles = static_cast<int>((p.cut + p.size - 1) / p.size + (vocab - p.cut + 127) / 128);
         const int64_t row_bytes = p.grads ? p.ldk * size : 12 * p.tiles;
         p.most = std::max<int64_t>(256, (p.grads ? kPieceBytes : kStatsBytes) / row_bytes / 256 * 256);
         p.most = std::min(p.most, kMostRows);
@@ -827,7 +925,7 @@ Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants,
         int64_t partial = 0;
         const auto split = [&](int64_t m, int64_t n, int64_t k) {
             const int splits = std::max(choose(m, n, k, dtype, true).splits, choose(m, n, k, dtype, false).splits);
-            if (splits > 1) partial = std::max(partial, 4 * splits * m * up(n, 4));
+            if (splits > 1) partial = std::max(partial, 4 * splits * up(m, 256) * up(n, 4));
         };
         if ((wants & HBT_LINEAR_DX) && inner > 0) split(p.most, inner, vocab);
         if ((wants & HBT_LINEAR_DW) && inner > 0) split(vocab, inner, p.most);
@@ -837,30 +935,54 @@ Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants,
     return p;
 }
 
-template <class T, bool kAsync, class Kernel, class Args>
-int32_t launch(const char* who, Kernel kernel, const Args& args, int64_t tiles, int splits, std::atomic<uint64_t>& done,
-               hipStream_t s) {
-    constexpr int kLds = lds_bytes<T, kAsync>();
+template <class T, bool kAsync, int kLds = lds_bytes<T, kAsync>(), class Kernel, class Args>
+int32_t launch(const char* who, Kernel kernel, const Args& args, int64_t blocks, std::atomic<uint64_t>& done, hipStream_t s) {
     if constexpr (kLds > 65536) {
         const int32_t status = allow_lds(who, reinterpret_cast<const void*>(kernel), kLds, done);
         if (status != HBT_OK) return status;
     }
-    kernel<<<dim3(static_cast<unsigned>(tiles), splits), T::kThreads, kLds, s>>>(args);
+    kernel<<<dim3(static_cast<unsigned>(blocks)), T::kThreads, kLds, s>>>(args);
     return check_launch(who);
 }
 
+// The words [column, end), whose statistics are tiles first_tile and on.
 template <int D, class T, bool kAsync>
-int32_t launch_logits(const char* who, const LogitArgs& p, int64_t rows, hipStream_t s) {
+int32_t launch_logits(const char* who, LogitArgs p, int64_t rows, int64_t column, int64_t end, int first_tile,
+                      hipStream_t s) {
     static std::atomic<uint64_t> done{0};
-    return launch<T, kAsync>(who, logit_kernel<D, T, kAsync>, p, (rows + T::BM - 1) / T::BM * p.tiles_n, 1, done, s);
+    constexpr int kLds = lds_bytes<T, kAsync>() + 3 * 4 * T::WN * T::BM;
+    p.column = column, p.end = end, p.first_tile = first_tile;
+    p.tiles_n = static_cast<int>((end - column + T::BN - 1) / T::BN);
+    int64_t tiles = (rows + T::BM - 1) / T::BM * p.tiles_n;
+    if (T::BM == 256) tiles = std::min<int64_t>(tiles, device_cu_count());
+    return launch<T, kAsync, kLds>(who, logit_kernel<D, T, kAsync>, p, tiles, done, s);
 }
 
 template <int D, int OD, bool kRows, class T, bool kAsync>
 int32_t launch_grad_tile(const char* who, GradArgs& p, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
+    p.tile = T::BM;
     p.tiles_n = static_cast<int>((p.n + T::BN - 1) / T::BN);
-    return launch<T, kAsync>(who, grad_kernel<D, OD, kRows, T, kAsync>, p, (p.m + T::BM - 1) / T::BM * p.tiles_n,
-                             p.splits, done, s);
+    p.blocks = static_cast<int>((p.m + T::BM - 1) / T::BM * p.tiles_n * p.splits);
+    return launch<T, kAsync>(who, grad_kernel<D, OD, kRows, T, kAsync>, p, p.blocks, done, s);
+}
+
+// dW in tiles of 256, its last rows or columns in tiles of 128 where that is estimated to be shorter
+// (cut_of, which has the measurements).
+template <int D, int OD>
+int32_t launch_cut(const char* who, const GradArgs& p, hipStream_t s) {
+    const Cut cut = cut_of(p.m, p.n, p.k);
+    GradArgs first = p, last = p;
+    first.m = cut.m, first.n = cut.n;
+    const int32_t status = launch_grad_tile<D, OD, false, Tile256, true>(who, first, s);
+    if (status != HBT_OK || (cut.m == p.m && cut.n == p.n)) return status;
+    const int64_t m0 = cut.m < p.m ? cut.m : 0, n0 = cut.n < p.n ? cut.n : 0;
+    last.m -= m0, last.m_in -= m0, last.n -= n0, last.n_in -= n0;
+    last.a = static_cast<const char*>(p.a) + m0 * elem_bytes<D>();
+    last.b = static_cast<const char*>(p.b) + n0 * elem_bytes<D>();
+    last.y = static_cast<char*>(p.y) + (m0 * p.ldy + n0) * elem_bytes<OD>();
+    if (p.before != nullptr) last.before = p.before + m0 * p.ldbefore + n0;
+    return launch_grad_tile<D, OD, false, Tile128, true>(who, last, s);
 }
 
 // p.m or p.k is the most that the piece's rows may be.
@@ -878,7 +1000,11 @@ int32_t launch_grad(const char* who, GradArgs& p, bool aligned, void* space, hip
         status = aligned ? launch_grad_tile<D, OD, kRows, Tile128, true>(who, p, s)
                          : launch_grad_tile<D, OD, kRows, Tile128, false>(who, p, s);
     } else if constexpr (D != F32) {
-        status = launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, s);
+        if constexpr (!kRows) {
+            status = c.splits == 1 ? launch_cut<D, OD>(who, p, s) : launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, s);
+        } else {
+            status = launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, s);
+        }
     }
     if (status != HBT_OK || c.splits == 1) return status;
     const int64_t blocks = std::min<int64_t>((p.m * (p.ldp / 4) + 255) / 256, 4096);
@@ -943,6 +1069,7 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
     JoinArgs join{};
     join.stats = stats, join.sums = sums, join.target = target, join.loss = token_loss, join.row_loss = row_loss;
     join.ignore = c.ignore, join.vocab = c.vocab, join.tiles = plan.tiles, join.smoothing = c.smoothing;
+    join.unit = unit<D>();
     if (plan.thin) {
         thin_logit_kernel<D><<<dim3(plan.tiles), 512, 0, s>>>(c.x, c.ldx, c.w, c.ldw, c.bias, c.target,
                                                               static_cast<int>(c.tokens), c.vocab, c.inner, stats, sums, target);
@@ -972,26 +1099,29 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
         const Piece piece{control, i, plan.pieces};
         LogitArgs l{};
         l.x = rows, l.w = c.w, l.bias = c.bias, l.word = word, l.stats = stats, l.sums = sums, l.target = target;
-        l.kept = kept, l.ldx = plan.ld, l.ldw = c.ldw, l.ldk = plan.ldk, l.vocab = c.vocab, l.inner = c.inner;
-        l.tiles_n = plan.tiles, l.stride = plan.most, l.piece = piece;
+        l.kept = kept, l.ldx = plan.ld, l.ldw = c.ldw, l.ldk = plan.ldk, l.inner = c.inner, l.stride = plan.most;
+        l.piece = piece;
+        const int64_t most = plan.most, vocab = c.vocab;
         if (plan.size == 64) {
-            status = aligned ? launch_logits<D, Tile64, true>(who, l, plan.most, s)
-                             : launch_logits<D, Tile64, false>(who, l, plan.most, s);
+            status = aligned ? launch_logits<D, Tile64, true>(who, l, most, 0, vocab, 0, s)
+                             : launch_logits<D, Tile64, false>(who, l, most, 0, vocab, 0, s);
         } else if (plan.size == 128) {
-            status = aligned ? launch_logits<D, Tile128, true>(who, l, plan.most, s)
-                             : launch_logits<D, Tile128, false>(who, l, plan.most, s);
+            status = aligned ? launch_logits<D, Tile128, true>(who, l, most, 0, vocab, 0, s)
+                             : launch_logits<D, Tile128, false>(who, l, most, 0, vocab, 0, s);
         } else if constexpr (D != F32) {
-            status = launch_logits<D, Tile256, true>(who, l, plan.most, s);
+            status = launch_logits<D, Tile256, true>(who, l, most, 0, plan.cut, 0, s);
+            if (status == HBT_OK && plan.cut < vocab)
+                status = launch_logits<D, Tile128, true>(who, l, most, plan.cut, vocab, static_cast<int>(plan.cut / 256), s);
         }
         if (status != HBT_OK) return status;
         join.word = word, join.token = token, join.weight = weight, join.row = row, join.piece = piece;
         join.stride = plan.most;
-        join_kernel<<<dim3(static_cast<unsigned>((plan.most + 63) / 64)), 64 * kJoinWaves, 0, s>>>(join);
+        join_kernel<<<dim3(static_cast<unsigned>((plan.most + kJoinRows - 1) / kJoinRows)), kJoinRows * kJoinGroups, 0, s>>>(join);
         if ((status = check_launch(who)) != HBT_OK) return status;
         if (!plan.grads) continue;
         const int segment = 256 * unit_elems<D>() * 4;
         softmax_kernel<D><<<dim3(static_cast<unsigned>((plan.ldk + segment - 1) / segment * plan.most)), 256, 0, s>>>({kept, stats, row, word, plan.ldk,
-                                                                          c.vocab, plan.most, plan.size, segment,
+                                                                          c.vocab, plan.most, plan.cut, plan.size, 128, segment,
                                                                           c.smoothing, piece});
         if ((status = check_launch(who)) != HBT_OK) return status;
         const bool last = i + 1 == plan.pieces;

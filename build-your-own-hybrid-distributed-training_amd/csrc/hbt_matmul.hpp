@@ -406,33 +406,35 @@ __device__ __forceinline__ void interleave() {
     }
 }
 
-// Forms the tile at rows m0 of A and n0 of B over k in [k0, k1) into acc: acc[i][j] holds, in
-// lane l, element m = 16 i + l % 16, n = 16 j + 4 (l / 16) + r (r = 0..3) of the wave's part.
+// Forms the tile at rows m0 of A and n0 of B over k in [k0, k1), k0 < k1, into acc: acc[i][j] holds,
+// in lane l, element m = 16 i + l % 16, n = 16 j + 4 (l / 16) + r (r = 0..3) of the wave's part.
 // A partial k-tile comes last among asynchronous loads, so that the others start on whole units,
 // and first among those through registers, whose loop then moves whole ones.
+//
+// init() takes the operands, begin() issues the first loads and run() does the rest.  Between begin()
+// and run() the LDS stages may not be touched; global loads and stores may be issued.
 template <int D, bool kA, bool kB, class T, bool kAsync>
-__device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t m0, int64_t m_count, const void* b,
-                                             int64_t ldb, int64_t n0, int64_t n_count, int64_t k0, int64_t k1,
-                                             char* lds, f32x4 (&acc)[T::TM][T::TN]) {
-    constexpr int BK = tile_k<D>(), B = elem_bytes<D>(), kThreads = T::kThreads;
+struct TileProduct {
+    static constexpr int BK = tile_k<D>(), B = elem_bytes<D>(), kThreads = T::kThreads;
     using OpA = Operand<D, kA, T::BM, kThreads, kAsync>;
     using OpB = Operand<D, kB, T::BN, kThreads, kAsync>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = (wave / T::WN) * (T::BM / T::WM), wn = (wave % T::WN) * (T::BN / T::WN);
-#pragma unroll
-    for (int i = 0; i < T::TM; ++i)
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (k0 >= k1) return;
+    static constexpr int kStages = kAsync ? T::kStages : 2, kLoads = OpA::kUnits + OpB::kUnits, kAhead = kStages - 1;
     OpA oa;
     OpB ob;
-    oa.init(a, lda, m0, m_count, tid);
-    ob.init(b, ldb, n0, n_count, tid);
-    const int tiles = static_cast<int>((k1 - k0 + BK - 1) / BK);
-    int64_t k = k0;  // the next k-tile to load
-    constexpr int kStages = kAsync ? T::kStages : 2, kLoads = OpA::kUnits + OpB::kUnits, kAhead = kStages - 1;
-    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-    const auto issue = [&](int stage) {  // asynchronous
+    int64_t k, k1;  // the next k-tile to load, and the end
+    int tiles;
+
+    __device__ __forceinline__ void init(const void* a, int64_t lda, int64_t m0, int64_t m_count, const void* b,
+                                         int64_t ldb, int64_t n0, int64_t n_count, int64_t k0, int64_t k1_,
+                                         int tid = threadIdx.x) {
+        oa.init(a, lda, m0, m_count, tid);
+        ob.init(b, ldb, n0, n_count, tid);
+        tiles = static_cast<int>((k1_ - k0 + BK - 1) / BK);
+        k = k0, k1 = k1_;
+    }
+    __device__ __forceinline__ void issue(char* lds, int stage) {  // asynchronous
+        const int tid = threadIdx.x, wave = tid >> 6;
+        const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
         const uint32_t to_a = at + stage * T::kStageBytes, to_b = to_a + OpA::kBytes;
         if (k1 - k >= BK) {
             oa.template load_async<true>(k, BK, to_a, tid, wave);
@@ -442,87 +444,119 @@ __device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t
             ob.template load_async<false>(k, k1 - k, to_b, tid, wave);
         }
         k += BK;
-    };
-    const auto load = [&]() {  // into registers
-        oa.load(k, tid);
-        ob.load(k, tid);
+    }
+    __device__ __forceinline__ void load() {  // into registers
+        oa.load(k, threadIdx.x);
+        ob.load(k, threadIdx.x);
         k += BK;
-    };
-    const auto store = [&](int stage) {
-        oa.store(lds + stage * T::kStageBytes, tid);
-        ob.store(lds + stage * T::kStageBytes + OpA::kBytes, tid);
-    };
-    if constexpr (kAsync) {
-        issue(0);
+    }
+    __device__ __forceinline__ void store(char* lds, int stage) {
+        oa.store(lds + stage * T::kStageBytes, threadIdx.x);
+        ob.store(lds + stage * T::kStageBytes + OpA::kBytes, threadIdx.x);
+    }
+    __device__ __forceinline__ void begin(char* lds) {
+        if constexpr (kAsync) {
+            issue(lds, 0);
 #pragma unroll
-        for (int s = 1; s <= kAhead; ++s)
-            if (s < tiles) issue(s);
-        if (kAhead < tiles) wait_loads<kLoads * kAhead>();
-        else wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    } else {
-        const int part = static_cast<int>((k1 - k0) % BK);
-        if (part != 0) {
-            oa.load_part(k, part, tid);
-            ob.load_part(k, part, tid);
-            k += part;
+            for (int s = 1; s <= kAhead; ++s)
+                if (s < tiles) issue(lds, s);
         } else {
-            load();
-        }
-        store(0);
-        if (tiles > 1) load();
-        __syncthreads();
-    }
-    // Each k-tile is two steps of two halves of the wave's rows.  While one half's matrix
-    // instructions run, the fragments of the next are read: two sets of each operand's are held.
-    constexpr int kHalf = T::TM / 2, kReadsA = OpA::kReads * kHalf, kReadsB = OpB::kReads * T::TN;
-    constexpr int kMmas = kHalf * T::TN * (B == 4 ? 4 : 1);
-    u32x4 a0[kHalf], a1[kHalf], b0[T::TN], b1[T::TN];
-    read<OpB>(b0, lds + OpA::kBytes, wn, 0, lane);
-    read<OpA>(a0, lds, wm, 0, lane);
-    int stage = 0;
-    for (int t = 0; t < tiles; ++t) {
-        const char* now = lds + stage * T::kStageBytes;
-        read<OpA>(a1, now, wm + 16 * kHalf, 0, lane);
-        multiply<D, T, 0>(a0, b0, acc);
-        interleave<kReadsA, kMmas>();
-        if constexpr (!kAsync) {
-            // Every wave has passed the barrier that ended the reads of the other stage.
-            if (t + 1 < tiles) {
-                store(stage ^ 1);
-                if (t + 2 < tiles) load();
-            }
-        }
-        read<OpB>(b1, now + OpA::kBytes, wn, 1, lane);
-        read<OpA>(a0, now, wm, 1, lane);
-        multiply<D, T, kHalf>(a1, b0, acc);
-        interleave<kReadsA + kReadsB, kMmas>();
-        read<OpA>(a1, now, wm + 16 * kHalf, 1, lane);
-        multiply<D, T, 0>(a0, b1, acc);
-        interleave<kReadsA, kMmas>();
-        if (t + 1 < tiles) {
-            if constexpr (kAsync) {
-                // At most the kAhead - 1 tiles after t + 1 are in flight, so it has landed; past the
-                // barrier it has for every wave, and every wave holds the last of tile t, whose
-                // stage the next load takes.
-                if (t + 1 + kAhead <= tiles) wait_loads<kLoads * (kAhead - 1)>();
-                else wait_loads<0>();
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                if (t + 1 + kAhead < tiles) issue(stage);
+            const int part = static_cast<int>((k1 - k) % BK);
+            if (part != 0) {
+                oa.load_part(k, part, threadIdx.x);
+                ob.load_part(k, part, threadIdx.x);
+                k += part;
             } else {
-                __syncthreads();
+                load();
             }
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-            const char* next = lds + stage * T::kStageBytes;
-            read<OpB>(b0, next + OpA::kBytes, wn, 0, lane);
-            read<OpA>(a0, next, wm, 0, lane);
         }
-        multiply<D, T, kHalf>(a1, b1, acc);
-        interleave<kReadsA + kReadsB, kMmas>();
     }
-    __syncthreads();  // the LDS is free
+    __device__ __forceinline__ void run(char* lds, f32x4 (&acc)[T::TM][T::TN]) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        const int wm = (wave / T::WN) * (T::BM / T::WM), wn = (wave % T::WN) * (T::BN / T::WN);
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < T::TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (kAsync) {
+            // Whatever was issued since begin() counts too, so this waits for the first stage at least.
+            if (kAhead < tiles) wait_loads<kLoads * kAhead>();
+            else wait_loads<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        } else {
+            store(lds, 0);
+            if (tiles > 1) load();
+            __syncthreads();
+        }
+        // Each k-tile is two steps of two halves of the wave's rows.  While one half's matrix
+        // instructions run, the fragments of the next are read: two sets of each operand's are held.
+        constexpr int kHalf = T::TM / 2, kReadsA = OpA::kReads * kHalf, kReadsB = OpB::kReads * T::TN;
+        constexpr int kMmas = kHalf * T::TN * (B == 4 ? 4 : 1);
+        u32x4 a0[kHalf], a1[kHalf], b0[T::TN], b1[T::TN];
+        read<OpB>(b0, lds + OpA::kBytes, wn, 0, lane);
+        read<OpA>(a0, lds, wm, 0, lane);
+        int stage = 0;
+        for (int t = 0; t < tiles; ++t) {
+            const char* now = lds + stage * T::kStageBytes;
+            read<OpA>(a1, now, wm + 16 * kHalf, 0, lane);
+            multiply<D, T, 0>(a0, b0, acc);
+            interleave<kReadsA, kMmas>();
+            if constexpr (!kAsync) {
+                // Every wave has passed the barrier that ended the reads of the other stage.
+                if (t + 1 < tiles) {
+                    store(lds, stage ^ 1);
+                    if (t + 2 < tiles) load();
+                }
+            }
+            read<OpB>(b1, now + OpA::kBytes, wn, 1, lane);
+            read<OpA>(a0, now, wm, 1, lane);
+            multiply<D, T, kHalf>(a1, b0, acc);
+            interleave<kReadsA + kReadsB, kMmas>();
+            read<OpA>(a1, now, wm + 16 * kHalf, 1, lane);
+            multiply<D, T, 0>(a0, b1, acc);
+            interleave<kReadsA, kMmas>();
+            if (t + 1 < tiles) {
+                if constexpr (kAsync) {
+                    // At most the kAhead - 1 tiles after t + 1 are in flight, so it has landed; past the
+                    // barrier it has for every wave, and every wave holds the last of tile t, whose
+                    // stage the next load takes.
+                    if (t + 1 + kAhead <= tiles) wait_loads<kLoads * (kAhead - 1)>();
+                    else wait_loads<0>();
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                    if (t + 1 + kAhead < tiles) issue(lds, stage);
+                } else {
+                    __syncthreads();
+                }
+                stage = stage + 1 == kStages ? 0 : stage + 1;
+                const char* next = lds + stage * T::kStageBytes;
+                read<OpB>(b0, next + OpA::kBytes, wn, 0, lane);
+                read<OpA>(a0, next, wm, 0, lane);
+            }
+            multiply<D, T, kHalf>(a1, b1, acc);
+            interleave<kReadsA + kReadsB, kMmas>();
+        }
+        __syncthreads();  // the LDS is free
+    }
+};
+
+// One tile from its first load to its last product; zeros where there is no k.
+template <int D, bool kA, bool kB, class T, bool kAsync>
+__device__ __forceinline__ void tile_product(const void* a, int64_t lda, int64_t m0, int64_t m_count, const void* b,
+                                             int64_t ldb, int64_t n0, int64_t n_count, int64_t k0, int64_t k1,
+                                             char* lds, f32x4 (&acc)[T::TM][T::TN]) {
+    if (k0 >= k1) {
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < T::TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        return;
+    }
+    TileProduct<D, kA, kB, T, kAsync> tile;
+    tile.init(a, lda, m0, m_count, b, ldb, n0, n_count, k0, k1);
+    tile.begin(lds);
+    tile.run(lds, acc);
 }
 
 // Finishes the tile, four consecutive n of a row at a time: `load(m, n)` fetches what the result
