@@ -28,6 +28,11 @@ constexpr int F32 = HBT_DTYPE_F32, BF16 = HBT_DTYPE_BF16, F16 = HBT_DTYPE_F16;
 constexpr int64_t kPieceBytes = int64_t(2) << 30;  // stored exponentials at a time
 constexpr int64_t kStatsBytes = int64_t(1) << 28;  // row statistics at a time, without gradients
 constexpr int kThin = 16;                          // rows of the kernel for few tokens
+// Tokens from which on a 2-byte W with rows off 16 bytes is copied to rows on them first: its
+// products then load straight into LDS, in tiles of 256.  50257 x 765 in bf16: 8192 tokens, evaluated,
+// 1324 us without the copy and 641 with it, all gradients 3884 and 2291; 200 tokens 73 either way.  In
+// fp32 the matrix cores are the bound and a copy gains nothing (2048 x 1001 x 32003: 3265 and 3185 us).
+constexpr int64_t kPadTokens = 256;
 constexpr int64_t kMostRows = int64_t(1) << 22;    // rows of a piece: a launch over them stays within a grid
 constexpr int64_t kMostTokens = int64_t(1) << 24;
 constexpr float kLog2e = 1.44269504f;
@@ -142,6 +147,37 @@ __global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
     }
 }
 
+// `cols` elements from any boundary to a row of `ld`, zeros behind them; a wavefront.
+template <int D>
+__device__ __forceinline__ void copy_row(const char* from, char* to, int64_t cols, int64_t ld, int lane) {
+    constexpr int E = unit_elems<D>(), B = elem_bytes<D>();
+    for (int64_t j = lane * E; j < ld; j += 64 * E) {
+        u32x4 v = {0, 0, 0, 0};
+        if (j + E <= cols) {
+            v = load16(from + j * B);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E - 1; ++e) {
+                if (j + e >= cols) break;
+                if constexpr (B == 4) v[e] = reinterpret_cast<const uint32_t*>(from)[j + e];
+                else v[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[j + e]) << (16 * (e % 2));
+            }
+        }
+        *reinterpret_cast<u32x4*>(to + j * B) = v;
+    }
+}
+
+// A matrix whose rows are off 16 bytes, copied to rows that are not.
+template <int D>
+__global__ __launch_bounds__(256) void pad_kernel(const void* from, int64_t ld_from, void* to, int64_t ld, int64_t rows,
+                                                  int64_t cols) {
+    constexpr int B = elem_bytes<D>();
+    const int64_t row = blockIdx.x * int64_t(4) + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    copy_row<D>(static_cast<const char*>(from) + row * ld_from * B, static_cast<char*>(to) + row * ld * B, cols, ld,
+                threadIdx.x & 63);
+}
+
 struct GatherArgs {
     const void* x;
     const int32_t* place;
@@ -155,28 +191,14 @@ struct GatherArgs {
 // A wavefront a token.
 template <int D>
 __global__ __launch_bounds__(256) void gather_kernel(GatherArgs p) {
-    constexpr int E = unit_elems<D>(), B = elem_bytes<D>();
+    constexpr int B = elem_bytes<D>();
     const int64_t token = blockIdx.x * int64_t(4) + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (token >= p.tokens) return;
     const int row = p.place[token];
     if (row >= 0) {
-        const char* from = static_cast<const char*>(p.x) + token * p.ldx * B;
-        char* to = static_cast<char*>(p.rows) + row * p.ld * B;
-        for (int64_t j = lane * E; j < p.ld; j += 64 * E) {
-            u32x4 v = {0, 0, 0, 0};
-            if (j + E <= p.inner) {
-                v = load16(from + j * B);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E - 1; ++e) {
-                    if (j + e >= p.inner) break;
-                    if constexpr (B == 4) v[e] = reinterpret_cast<const uint32_t*>(from)[j + e];
-                    else v[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[j + e]) << (16 * (e % 2));
-                }
-            }
-            *reinterpret_cast<u32x4*>(to + j * B) = v;
-        }
+        copy_row<D>(static_cast<const char*>(p.x) + token * p.ldx * B, static_cast<char*>(p.rows) + row * p.ld * B, p.inner,
+                    p.ld, lane);
         return;
     }
     if (p.loss != nullptr && lane == 0) p.loss[token] = 0.0f;
@@ -808,6 +830,119 @@ __global__ __launch_bounds__(256) void bias_join_kernel(const float* parts, floa
     else store_elem<OD>(db, j, sum);
 }
 
+// ---- small calls --------------------------------------------------------------------------
+// Few tokens of a small model over a small vocabulary are launch latency: one workgroup does all of
+// a call in LDS, in fp32, where the kernels above are eleven launches.
+constexpr int kSmallTokens = 64, kSmallLds = 128 << 10;
+constexpr int64_t kSmallProduct = int64_t(1) << 17;  // multiplications of each product
+int64_t small_lds(int64_t tokens, int64_t inner, int64_t vocab) {
+    return 4 * (tokens * (inner + 1) + vocab * (inner + 1) + tokens * (vocab + 1));
+}
+bool is_small(int64_t tokens, int64_t inner, int64_t vocab) {
+    return tokens <= kSmallTokens && tokens * inner * vocab <= kSmallProduct && small_lds(tokens, inner, vocab) <= kSmallLds;
+}
+
+struct SmallArgs {
+    const void *x, *w, *bias;
+    const int64_t* target;
+    const float* token_grads;
+    float* loss;
+    void *dx, *dw, *db;
+    int64_t ldx, ldw, lddx, lddw, ignore;
+    int tokens, inner, vocab, reduction;
+    float smoothing;
+};
+
+template <int D, int OD>
+__global__ __launch_bounds__(1024) void small_kernel(SmallArgs p) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ double losses[kSmallTokens];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, across = p.inner + 1, wide = p.vocab + 1;
+    float* x = reinterpret_cast<float*>(lds);   // [tokens][across], zeros for a token without a loss
+    float* w = x + p.tokens * across;           // [vocab][across]
+    float* z = w + p.vocab * across;            // [tokens][wide]: logits, then dz
+    const int64_t mine = lane < p.tokens ? p.target[lane] : p.ignore;  // every wavefront has all targets
+    const uint64_t valid = __ballot(mine != p.ignore);
+    const int count = __popcll(valid);
+    for (int i = tid; i < p.tokens * p.inner; i += 1024) {
+        const int t = i / p.inner, k = i % p.inner;
+        x[t * across + k] = (valid >> t) & 1 ? load_elem<D>(p.x, t * p.ldx + k) : 0.0f;
+    }
+    for (int i = tid; i < p.vocab * p.inner; i += 1024) {
+        const int v = i / p.inner, k = i % p.inner;
+        w[v * across + k] = load_elem<D>(p.w, v * p.ldw + k);
+    }
+    __syncthreads();
+    for (int i = tid; i < p.tokens * p.vocab; i += 1024) {
+        const int t = i / p.vocab, v = i % p.vocab;
+        float sum = 0.0f;
+        for (int k = 0; k < p.inner; ++k) sum = fmaf(x[t * across + k], w[v * across + k], sum);
+        z[t * wide + v] = p.bias != nullptr ? sum + load_elem<D>(p.bias, v) : sum;
+    }
+    __syncthreads();
+    const float even = p.smoothing / static_cast<float>(p.vocab);
+    for (int t = wave; t < p.tokens; t += 16) {  // a wavefront a row
+        float* row = z + t * wide;
+        if (((valid >> t) & 1) == 0) {
+            if (lane == 0) losses[t] = 0.0;
+            for (int v = lane; v < p.vocab; v += 64) row[v] = 0.0f;
+            continue;
+        }
+        const int64_t word = __shfl(mine, t);
+        const bool known = word >= 0 && word < p.vocab;
+        float top = -INFINITY;
+        for (int v = lane; v < p.vocab; v += 64) top = fmaxf(top, row[v]);
+        top = wave_max(top);
+        if (top == -INFINITY) top = 0.0f;
+        double sum = 0.0, logits = 0.0;
+        for (int v = lane; v < p.vocab; v += 64) sum += expf(row[v] - top), logits += row[v];
+        sum = wave_sum(sum), logits = wave_sum(logits);
+        const double log_sum = log(sum), log_p = known ? (static_cast<double>(row[word]) - top) - log_sum : NAN;
+        if (lane == 0) {
+            losses[t] = -(1.0 - p.smoothing) * log_p;
+            if (p.smoothing != 0.0f) losses[t] += p.smoothing * ((top + log_sum) - logits / p.vocab);
+        }
+        const float weight = p.token_grads != nullptr ? p.token_grads[t] : 1.0f, inverse = static_cast<float>(1.0 / sum);
+        const float missing = expm1f(static_cast<float>(log_p)) + p.smoothing;
+        for (int v = lane; v < p.vocab; v += 64) {
+            const float part = v == word ? missing : expf(row[v] - top) * inverse;
+            row[v] = known ? (part - even) * weight : NAN;
+        }
+    }
+    __syncthreads();
+    const bool mean = p.reduction == HBT_LOSS_MEAN;
+    if (p.loss != nullptr) {
+        if (p.reduction == HBT_LOSS_NONE) {
+            if (tid < p.tokens) p.loss[tid] = static_cast<float>(losses[tid]);
+        } else if (wave == 0) {
+            const double sum = wave_sum(lane < p.tokens ? losses[lane] : 0.0);
+            if (lane == 0) p.loss[0] = static_cast<float>(mean ? sum / count : sum);
+        }
+    }
+    const float scale = count == 0 ? 0.0f : (mean ? 1.0f / static_cast<float>(count) : 1.0f);
+    if (p.dx != nullptr)
+        for (int i = tid; i < p.tokens * p.inner; i += 1024) {
+            const int t = i / p.inner, k = i % p.inner;
+            float sum = 0.0f;
+            if ((valid >> t) & 1)
+                for (int v = 0; v < p.vocab; ++v) sum = fmaf(z[t * wide + v], w[v * across + k], sum);
+            store_elem<OD>(p.dx, t * p.lddx + k, sum * scale);
+        }
+    if (p.dw != nullptr)
+        for (int i = tid; i < p.vocab * p.inner; i += 1024) {
+            const int v = i / p.inner, k = i % p.inner;
+            float sum = 0.0f;
+            for (int t = 0; t < p.tokens; ++t) sum = fmaf(z[t * wide + v], x[t * across + k], sum);
+            store_elem<OD>(p.dw, v * p.lddw + k, sum * scale);
+        }
+    if (p.db != nullptr)
+        for (int v = tid; v < p.vocab; v += 1024) {
+            float sum = 0.0f;
+            for (int t = 0; t < p.tokens; ++t) sum += z[t * wide + v];
+            store_elem<OD>(p.db, v, sum * scale);
+        }
+}
+
 // ---- the loss's own gradient -----------------------------------------------------------------
 struct ScaleArgs {
     const void* src[HBT_MAX_SCALED];
@@ -839,13 +974,13 @@ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // Everything a call's launches and working storage follow from.
 struct Plan {
-    bool thin, grads, rows_only;
+    bool thin, grads, pad;  // pad: W is copied to rows on 16 bytes first
     int size;               // logit tiles
     int64_t cut;            // the words from here on are in tiles of 128 instead
     int tiles, pieces;
     int64_t most;           // rows of a piece, at most
     int64_t ld, ldk;        // gathered rows; exponentials
-    int64_t control, place, token, word, weight, target, row, row_loss, rows, stats, sums, kept, dw_sums, db_sums,
+    int64_t control, place, token, word, weight, target, row, row_loss, rows, padded, stats, sums, kept, dw_sums, db_sums,
         parts, partial, bytes;
 };
 
@@ -868,9 +1003,12 @@ int64_t column_cut(int64_t rows, int64_t vocab, double steps) {
 Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants, int grad_dtype, bool smooth,
              bool aligned) {
     Plan p{};
+    if (is_small(tokens, inner, vocab)) return p;
     const int64_t size = dtype == F32 ? 4 : 2;
     p.grads = wants != 0;
     p.thin = tokens <= kThin && !p.grads;
+    p.pad = !aligned && dtype != F32 && tokens >= kPadTokens;
+    aligned = aligned || p.pad;
     p.ld = up(std::max<int64_t>(inner, 1), 64);
     p.ldk = up(vocab, 64);
     int64_t at = 0;
@@ -912,6 +1050,7 @@ Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants,
         p.word = take(4 * tokens);
         p.weight = take(4 * tokens);
         p.rows = take(size * tokens * p.ld);
+        if (p.pad) p.padded = take(size * vocab * p.ld);
     }
     if (p.grads) {
         p.row = take(sizeof(Row) * tokens);
@@ -1066,6 +1205,18 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
     float* token_loss = c.reduction == HBT_LOSS_NONE ? c.loss : nullptr;
     const int mean = c.reduction == HBT_LOSS_MEAN;
     int32_t status = HBT_OK;
+    if (is_small(c.tokens, c.inner, c.vocab)) {
+        static std::atomic<uint64_t> done{0};
+        const int bytes = static_cast<int>(small_lds(c.tokens, c.inner, c.vocab));
+        if (bytes > 65536 &&
+            (status = allow_lds(who, reinterpret_cast<const void*>(small_kernel<D, OD>), kSmallLds, done)) != HBT_OK)
+            return status;
+        small_kernel<D, OD><<<1, 1024, bytes, s>>>({c.x, c.w, c.bias, c.target, c.token_grads, c.loss, c.dx, c.dw, c.db, c.ldx,
+                                                    c.ldw, c.lddx, c.lddw, c.ignore, static_cast<int>(c.tokens),
+                                                    static_cast<int>(c.inner), static_cast<int>(c.vocab), c.reduction,
+                                                    c.smoothing});
+        return check_launch(who);
+    }
     JoinArgs join{};
     join.stats = stats, join.sums = sums, join.target = target, join.loss = token_loss, join.row_loss = row_loss;
     join.ignore = c.ignore, join.vocab = c.vocab, join.tiles = plan.tiles, join.smoothing = c.smoothing;
@@ -1092,14 +1243,21 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
     gather_kernel<D><<<dim3(static_cast<unsigned>((c.tokens + 3) / 4)), 256, 0, s>>>(
         {c.x, place, rows, c.dx, token_loss, c.ldx, plan.ld, c.lddx, c.tokens, c.inner, OD == F32});
     if ((status = check_launch(who)) != HBT_OK) return status;
-    const bool aligned = is_aligned(c.w, c.ldw, c.inner, D);
+    const bool aligned = plan.pad || is_aligned(c.w, c.ldw, c.inner, D);
+    const void* w = plan.pad ? at(plan.padded) : c.w;
+    const int64_t ldw = plan.pad ? plan.ld : c.ldw;
+    if (plan.pad) {
+        pad_kernel<D><<<dim3(static_cast<unsigned>((c.vocab + 3) / 4)), 256, 0, s>>>(c.w, c.ldw, at(plan.padded), plan.ld,
+                                                                                   c.vocab, c.inner);
+        if ((status = check_launch(who)) != HBT_OK) return status;
+    }
     void* kept = plan.grads ? at(plan.kept) : nullptr;
     Row* row = plan.grads ? static_cast<Row*>(at(plan.row)) : nullptr;
     for (int i = 0; i < plan.pieces; ++i) {
         const Piece piece{control, i, plan.pieces};
         LogitArgs l{};
-        l.x = rows, l.w = c.w, l.bias = c.bias, l.word = word, l.stats = stats, l.sums = sums, l.target = target;
-        l.kept = kept, l.ldx = plan.ld, l.ldw = c.ldw, l.ldk = plan.ldk, l.inner = c.inner, l.stride = plan.most;
+        l.x = rows, l.w = w, l.bias = c.bias, l.word = word, l.stats = stats, l.sums = sums, l.target = target;
+        l.kept = kept, l.ldx = plan.ld, l.ldw = ldw, l.ldk = plan.ldk, l.inner = c.inner, l.stride = plan.most;
         l.piece = piece;
         const int64_t most = plan.most, vocab = c.vocab;
         if (plan.size == 64) {
@@ -1127,8 +1285,8 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
         const bool last = i + 1 == plan.pieces;
         if ((c.wants & HBT_LINEAR_DX) && c.inner > 0) {
             GradArgs g{};
-            g.a = kept, g.b = c.w, g.y = c.dx, g.token = token, g.lda = plan.ldk, g.ldb = c.ldw, g.ldy = c.lddx;
-            g.m = plan.most, g.n = c.inner, g.k = c.vocab, g.m_in = plan.most, g.n_in = c.inner, g.piece = piece;
+            g.a = kept, g.b = w, g.y = c.dx, g.token = token, g.lda = plan.ldk, g.ldb = ldw, g.ldy = c.lddx;
+            g.m = plan.most, g.n = c.inner, g.k = c.vocab, g.m_in = plan.most, g.n_in = plan.pad ? up(c.inner, 8) : c.inner, g.piece = piece;
             if ((status = launch_grad<D, OD, true>(who, g, aligned, at(plan.partial), s)) != HBT_OK) return status;
         }
         if ((c.wants & HBT_LINEAR_DW) && c.inner > 0) {
@@ -1172,14 +1330,13 @@ using namespace hbt::mm;
 extern "C" {
 
 int64_t hbt_linear_cross_entropy_workspace(int64_t tokens, int64_t inner, int64_t vocab, int32_t dtype, int32_t wants,
-                                           int32_t grad_dtype, float smoothing) {
+                                           int32_t grad_dtype, float smoothing, int32_t aligned) {
     clear_error();
     const char* who = "hbt_linear_cross_entropy_workspace";
     if (check_sizes(who, tokens, inner, vocab, dtype, wants, grad_dtype) != HBT_OK) return -1;
     if (tokens == 0) return 0;
     const bool smooth = smoothing != 0.0f;
-    return std::max(plan_of(tokens, inner, vocab, dtype, wants, grad_dtype, smooth, true).bytes,
-                    plan_of(tokens, inner, vocab, dtype, wants, grad_dtype, smooth, false).bytes);
+    return plan_of(tokens, inner, vocab, dtype, wants, grad_dtype, smooth, aligned != 0).bytes;
 }
 
 int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -1206,7 +1363,8 @@ int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int6
         return status;
     const Plan plan = plan_of(tokens, inner, vocab, dtype, wants, grad_dtype, smoothing != 0.0f,
                               is_aligned(w, ldw, inner, dtype));
-    if (workspace == nullptr || workspace_bytes < plan.bytes || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    if (plan.bytes > 0 &&
+        (workspace == nullptr || workspace_bytes < plan.bytes || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return refuse(who, "the workspace is smaller than hbt_linear_cross_entropy_workspace's, or off 256 bytes");
     const Call c{x, w, bias, target, token_grads, loss, dx, dw, dbias, ldx, ldw, lddx, lddw, tokens, inner, vocab,
                  ignore_index, reduction, wants, smoothing};

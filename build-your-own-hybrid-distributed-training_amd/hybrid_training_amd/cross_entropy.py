@@ -115,69 +115,83 @@ def _compute(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, t
     with _native.device_guard(device):
         lib = _native.library()
         mask = sum(bit for bit, g in zip((1, 2, 4), grads) if g is not None)
-        nbytes = lib.hbt_linear_cross_entropy_workspace(tokens, inner, vocab, code, mask, held_code, smoothing)
+        size = x.element_size()
+        aligned = (w.data_ptr() | ldw * size | inner * size) & 15 == 0
+        nbytes = lib.hbt_linear_cross_entropy_workspace(tokens, inner, vocab, code, mask, held_code, smoothing, aligned)
         if nbytes < 0:
             _native.check(int(nbytes), "cross_entropy.hbt_linear_cross_entropy_workspace")
-        space = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        space = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         at = [None if g is None else g.data_ptr() for g in grads]
         across = max(inner, 1)
         _native.check(lib.hbt_linear_cross_entropy(
             rows.data_ptr(), ldx, w.data_ptr(), ldw, None if b is None else b.data_ptr(), words.data_ptr(),
             None if token_grads is None else token_grads.data_ptr(), None if loss is None else loss.data_ptr(), at[0],
             across, at[1], across, at[2], tokens, inner, vocab, code, held_code, ignore_index, smoothing,
-            REDUCTIONS[reduction], space.data_ptr(), nbytes, _native.stream_of(device)),
+            REDUCTIONS[reduction], None if space is None else space.data_ptr(), nbytes, _native.stream_of(device)),
             "cross_entropy.hbt_linear_cross_entropy")
     return loss, grads
 
 
-def _scaled(grads: list[torch.Tensor | None], factor: torch.Tensor, dtype: torch.dtype) -> list[torch.Tensor | None]:
-    """``grads`` times a device scalar, in ``dtype``: in place where they are in it already, which
-    reads and writes nothing for a factor of 1."""
-    present = [i for i, g in enumerate(grads) if g is not None]
-    if not present:
-        return grads
-    device, held = factor.device, grads[present[0]].dtype
-    out = list(grads)
-    if held != dtype:
-        for i in present:
-            out[i] = torch.empty(grads[i].shape, dtype=dtype, device=device)
-    with _native.device_guard(device):
-        _native.check(_native.library().hbt_scale_round(
-            _native.pointer_array([grads[i].data_ptr() for i in present]),
-            _native.pointer_array([out[i].data_ptr() for i in present]),
-            _native.int64_array([grads[i].numel() for i in present]), len(present), _native.dtype_code(held),
-            _native.dtype_code(dtype), factor.to(torch.float32).data_ptr(), _native.stream_of(device)),
-            "cross_entropy.hbt_scale_round")
-    return out
+class _Scaling:
+    """The call that multiplies ``grads`` by the loss's own gradient, a device scalar, into ``dtype``:
+    in place where they are in it already, which reads and writes nothing for a factor of 1.
+
+    Laid out in the forward pass: the backward one runs on autograd's own thread, where host
+    code is slower."""
+
+    def __init__(self, grads: list[torch.Tensor | None], dtype: torch.dtype) -> None:
+        present = [g for g in grads if g is not None]
+        self.device, held = present[0].device, present[0].dtype
+        self.results = grads
+        if held != dtype:
+            self.results = [None if g is None else torch.empty(g.shape, dtype=dtype, device=g.device) for g in grads]
+        self._held = grads
+        self._tables = (
+            _native.pointer_array([g.data_ptr() for g in present]),
+            _native.pointer_array([r.data_ptr() for r in self.results if r is not None]),
+            _native.int64_array([g.numel() for g in present]), len(present), _native.dtype_code(held),
+            _native.dtype_code(dtype))
+
+    def run(self, factor: torch.Tensor) -> list[torch.Tensor | None]:
+        if factor.dtype != torch.float32:
+            factor = factor.to(torch.float32)
+        with _native.device_guard(self.device):
+            _native.check(_native.library().hbt_scale_round(*self._tables, factor.data_ptr(),
+                                                            _native.stream_of(self.device)),
+                          "cross_entropy.hbt_scale_round")
+        return self.results
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, options):
-        ctx.options, ctx.dtype, ctx.grads = options, x.dtype, None
-        wants = (x.requires_grad, weight.requires_grad, bias is not None and bias.requires_grad)
+        ctx.options, ctx.scaling = options, None
         if options[1] == "none":
             loss, _ = _compute(x, weight, bias, target, options, (False, False, False))
         else:
-            loss, ctx.grads = _compute(x, weight, bias, target, options, wants)
+            wants = (x.requires_grad, weight.requires_grad, bias is not None and bias.requires_grad)
+            loss, grads = _compute(x, weight, bias, target, options, wants)
+            ctx.scaling = _Scaling(grads, x.dtype)
         ctx.save_for_backward(x, weight, bias, target)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        options = ctx.options
+        scaling, ctx.scaling = ctx.scaling, None  # its gradients become the leaves' own
+        if scaling is not None:
+            dx, dw, db = scaling.run(dloss)
+            return dx, dw, db, None, None
+        # Separate losses, or a second backward pass: from the beginning.
+        x, weight, bias, target = ctx.saved_tensors
         wants = ctx.needs_input_grad[:3]
-        if options[1] == "none":
-            x, weight, bias, target = ctx.saved_tensors
+        if ctx.options[1] == "none":
             token_grads = dloss.reshape(-1).to(torch.float32).contiguous()
-            _, grads = _compute(x, weight, bias, target, options, wants, token_grads, with_loss=False)
-            return *grads, None, None
-        grads, ctx.grads = ctx.grads, None  # they become the leaves' own
-        if grads is None:  # a second backward pass
-            x, weight, bias, target = ctx.saved_tensors
-            _, grads = _compute(x, weight, bias, target, options, wants, with_loss=False)
-        return *_scaled(grads, dloss, ctx.dtype), None, None
+            _, grads = _compute(x, weight, bias, target, ctx.options, wants, token_grads, with_loss=False)
+        else:
+            _, grads = _compute(x, weight, bias, target, ctx.options, wants, with_loss=False)
+            grads = _Scaling(grads, x.dtype).run(dloss)
+        return *grads, None, None
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None = None,

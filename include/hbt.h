@@ -788,14 +788,15 @@ int32_t hbt_moments8_decode(void* const* codes, void* const* scales, void* const
  * repeat bitwise.  Rows are at most 2^20 elements apart, vocab and inner at most 2^20 - 64, tokens
  * from 1 to 2^24.
  * `workspace` (256-byte aligned) holds at least hbt_linear_cross_entropy_workspace's bytes (-1
- * for sizes that the call refuses; `wants`: HBT_LINEAR_DX / DW / DBIAS of the gradients given):
- * at most 2 GiB of exponentials, the gathered rows, and an fp32 dw where there are more.
+ * for sizes that the call refuses; `wants`: HBT_LINEAR_DX / DW / DBIAS of the gradients given;
+ * `aligned`: whether w, ldw and inner are multiples of 16 bytes): at most 2 GiB of exponentials, the gathered
+ * rows, an fp32 dw where there are more, and a copy of a 2-byte w that is not aligned.
  * ---------------------------------------------------------------------------- */
 #define HBT_LOSS_NONE 0
 #define HBT_LOSS_MEAN 1
 #define HBT_LOSS_SUM 2
 int64_t hbt_linear_cross_entropy_workspace(int64_t tokens, int64_t inner, int64_t vocab, int32_t dtype, int32_t wants,
-                                           int32_t grad_dtype, float smoothing);
+                                           int32_t grad_dtype, float smoothing, int32_t aligned);
 int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                                  const int64_t* target, const float* token_grads, float* loss, void* dx, int64_t lddx,
                                  void* dw, int64_t lddw, void* dbias, int64_t tokens, int64_t inner, int64_t vocab,

@@ -25,24 +25,28 @@ def test_host_tensors_are_refused():
 
 def test_working_storage():
     size = _native.library().hbt_linear_cross_entropy_workspace
-    assert size(0, 64, 100, 1, 0, 1, 0.0) == 0
+    assert size(0, 64, 100, 1, 0, 1, 0.0, 1) == 0
+    assert size(16, 32, 97, 0, 7, 0, 0.0, 1) == 0  # a small call's stands in LDS
     # one token over a large vocabulary: statistics alone
-    assert 0 < size(1, 4096, 128256, 1, 0, 1, 0.0) < 1 << 20
+    assert 0 < size(1, 4096, 128256, 1, 0, 1, 0.0, 1) < 1 << 20
     # evaluation never holds logits, training at most 2 GiB of exponentials beside rows and fp32 sums
-    assert size(8192, 4096, 128256, 1, 0, 1, 0.0) < 8192 * 4096 * 2 + (1 << 28) + (8 << 20)
-    one = size(8192, 4096, 128256, 1, 3, 1, 0.0)
+    assert size(8192, 4096, 128256, 1, 0, 1, 0.0, 1) < 8192 * 4096 * 2 + (1 << 28) + (8 << 20)
+    one = size(8192, 4096, 128256, 1, 3, 1, 0.0, 1)
     assert one < 2 * GIB + 8192 * 4096 * 2 + (1 << 27)
-    more = size(16384, 4096, 128256, 1, 3, 1, 0.0)
+    more = size(16384, 4096, 128256, 1, 3, 1, 0.0, 1)
     assert more < 2 * GIB + 16384 * 4096 * 2 + 4 * 128256 * 4096 + (1 << 27)
-    assert size(32768, 4096, 128256, 1, 3, 1, 0.0) - more < 16384 * 4096 * 2 + (4 << 20)
+    assert size(32768, 4096, 128256, 1, 3, 1, 0.0, 1) - more < 16384 * 4096 * 2 + (4 << 20)
+    # a 2-byte weight off 16 bytes is copied for many tokens, an fp32 one is not
+    assert size(8192, 64, 50257, 1, 0, 1, 0.0, 0) - size(8192, 64, 50257, 1, 0, 1, 0.0, 1) > 50257 * 64 * 2 - (1 << 20)
+    assert size(8192, 64, 50257, 0, 0, 0, 0.0, 0) == size(8192, 64, 50257, 0, 0, 0, 0.0, 1)
     # fp32 results carry the sums themselves
-    assert size(16384, 4096, 128256, 1, 3, 0, 0.0) < more - 4 * 128256 * 4096 + (1 << 20)
-    assert size(10, 64, 100, 1, 0, 1, 0.1) > size(10, 64, 100, 1, 0, 1, 0.0)
+    assert size(16384, 4096, 128256, 1, 3, 0, 0.0, 1) < more - 4 * 128256 * 4096 + (1 << 20)
+    assert size(10, 64, 10000, 1, 0, 1, 0.1, 1) > size(10, 64, 10000, 1, 0, 1, 0.0, 1)
     for bad in ((-1, 64, 100, 1, 0, 1), (1, -1, 100, 1, 0, 1), (1, 64, 0, 1, 0, 1), (1, 64, 100, 3, 0, 1),
                 (1, 64, 100, 1, 8, 1), (1, 64, 100, 1, 1, 2), (1, 64, (1 << 20), 1, 0, 1), (1, 1 << 20, 100, 1, 0, 1),
                 ((1 << 24) + 1, 64, 100, 1, 0, 1)):
-        assert size(*bad, 0.0) == -1 and _native.library().hbt_last_error()
-    assert size(0, 64, 100, 1, 0, 1, 0.0) == 0  # leaves no message behind
+        assert size(*bad, 0.0, 1) == -1 and _native.library().hbt_last_error()
+    assert size(0, 64, 100, 1, 0, 1, 0.0, 1) == 0  # leaves no message behind
 
 
 def test_the_library_refuses_bad_calls_before_any_launch():
@@ -50,7 +54,7 @@ def test_the_library_refuses_bad_calls_before_any_launch():
     p = ctypes.c_void_p(4096)
 
     def call(x=p, ldx=64, w=p, ldw=64, target=p, token_grads=None, loss=p, dx=None, lddx=0, dw=None, lddw=0, tokens=4,
-             inner=64, vocab=100, dtype=1, grad_dtype=1, smoothing=0.0, reduction=0, space=p, nbytes=1 << 30):
+             inner=64, vocab=10000, dtype=1, grad_dtype=1, smoothing=0.0, reduction=0, space=p, nbytes=1 << 30):
         return lib.hbt_linear_cross_entropy(x, ldx, w, ldw, None, target, token_grads, loss, dx, lddx, dw, lddw, None,
                                             tokens, inner, vocab, dtype, grad_dtype, -100, smoothing, reduction, space,
                                             nbytes, None)

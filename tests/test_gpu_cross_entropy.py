@@ -261,7 +261,7 @@ def test_a_nearly_certain_target_keeps_its_gradient():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("tokens", [9, 150])
+@pytest.mark.parametrize("tokens", [9, 150, 390])
 def test_layouts(dtype, tokens):
     """Strides, offsets and shapes other than dense ones give the dense ones' bits."""
     x, w, b, target = _inputs(tokens, 64, 333, dtype, bias=True)
