@@ -98,6 +98,27 @@ struct PrepareArgs {
     int mean, half;
 };
 
+// `top`: the largest magnitude of a token's gradient.
+__device__ __forceinline__ void write_control(const PrepareArgs& p, int count, float top) {
+    // fp16 values of dz: the largest gradient comes to 2^13 to 2^14, far from both ends of the
+    // range; a power of two, so that nothing is rounded.
+    float in = 1.0f;
+    if (p.half && top > 0.0f && top < INFINITY) {
+        int e = 0;
+        frexpf(top, &e);
+        in = ldexpf(1.0f, max(-126, min(126, 14 - e)));
+    }
+    p.control->count = count;
+    p.control->scale_in = in;
+    // No token carries a loss: no gradient, where 1 / 0 times a sum of nothing would be NaN.
+    p.control->scale_out = count == 0 ? 0.0f : (p.mean ? 1.0f / static_cast<float>(count) : 1.0f) / in;
+}
+__device__ __forceinline__ void write_row(const PrepareArgs& p, int row, int64_t i, int64_t t, float weight) {
+    p.token[row] = static_cast<int32_t>(i);
+    p.word[row] = t >= 0 && t < p.vocab ? static_cast<int32_t>(t) : -1;
+    p.weight[row] = weight;
+}
+
 // One workgroup: rows in the order of the tokens.
 __global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
     __shared__ int wave_count[16];
@@ -120,9 +141,7 @@ __global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
             count += wave_count[w];
         }
         if (valid) {
-            p.token[row] = static_cast<int32_t>(i);
-            p.word[row] = t >= 0 && t < p.vocab ? static_cast<int32_t>(t) : -1;
-            p.weight[row] = g;
+            write_row(p, row, i, t, g);
             top = fmaxf(top, fabsf(g));
         }
         if (i < p.tokens) p.place[i] = valid ? row : -1;
@@ -132,18 +151,7 @@ __global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 0; w < 16; ++w) top = fmaxf(top, wave_top[w]);
-        // fp16 values of dz: the largest gradient comes to 2^13 to 2^14, far from both ends of the
-        // range; a power of two, so that nothing is rounded.
-        float in = 1.0f;
-        if (p.half && top > 0.0f && top < INFINITY) {
-            int e = 0;
-            frexpf(top, &e);
-            in = ldexpf(1.0f, max(-126, min(126, 14 - e)));
-        }
-        p.control->count = count;
-        p.control->scale_in = in;
-        // No token carries a loss: no gradient, where 1 / 0 times a sum of nothing would be NaN.
-        p.control->scale_out = count == 0 ? 0.0f : (p.mean ? 1.0f / static_cast<float>(count) : 1.0f) / in;
+        write_control(p, count, top);
     }
 }
 
@@ -188,14 +196,10 @@ struct GatherArgs {
     int dx_wide;  // dx in fp32
 };
 
-// A wavefront a token.
+// The token's row of x to its place, or zeros where it carries no loss; a wavefront.
 template <int D>
-__global__ __launch_bounds__(256) void gather_kernel(GatherArgs p) {
+__device__ __forceinline__ void gather_token(const GatherArgs& p, int64_t token, int row, int lane) {
     constexpr int B = elem_bytes<D>();
-    const int64_t token = blockIdx.x * int64_t(4) + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (token >= p.tokens) return;
-    const int row = p.place[token];
     if (row >= 0) {
         copy_row<D>(static_cast<const char*>(p.x) + token * p.ldx * B, static_cast<char*>(p.rows) + row * p.ld * B, p.inner,
                     p.ld, lane);
@@ -208,6 +212,45 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherArgs p) {
     } else {
         for (int64_t j = lane; j < p.inner; j += 64) store_elem<D>(p.dx, token * p.lddx + j, 0.0f);
     }
+}
+// A wavefront a token.
+template <int D>
+__global__ __launch_bounds__(256) void gather_kernel(GatherArgs p) {
+    const int64_t token = blockIdx.x * int64_t(4) + (threadIdx.x >> 6);
+    if (token < p.tokens) gather_token<D>(p, token, p.place[token], threadIdx.x & 63);
+}
+
+// Both of the above for at most kFewTokens tokens: a launch less, since every workgroup counts the
+// rows before its own tokens from the targets.
+constexpr int64_t kFewTokens = 2048;
+template <int D>
+__global__ __launch_bounds__(256) void prepare_few_kernel(PrepareArgs p, GatherArgs g) {
+    __shared__ int wave_before[4], wave_count[4];
+    __shared__ float wave_top[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.x * 4, tokens = static_cast<int>(p.tokens);
+    int before = 0, count = 0;  // of the wavefront's share: valid tokens before `first`, and all
+    float top = 0.0f;
+    for (int base = 0; base < tokens; base += 256) {
+        const int i = base + static_cast<int>(threadIdx.x);
+        const bool valid = i < tokens && p.target[i] != p.ignore;
+        before += __popcll(__ballot(valid && i < first));
+        count += __popcll(__ballot(valid));
+        if (blockIdx.x == 0 && valid) top = fmaxf(top, p.token_grads != nullptr ? fabsf(p.token_grads[i]) : 1.0f);
+    }
+    if (blockIdx.x == 0) top = wave_max(top);
+    if (lane == 0) wave_before[wave] = before, wave_count[wave] = count, wave_top[wave] = top;
+    __syncthreads();
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        write_control(p, (wave_count[0] + wave_count[1]) + (wave_count[2] + wave_count[3]),
+                      fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3])));
+    const int token = first + wave;
+    if (token >= tokens) return;
+    int row = (wave_before[0] + wave_before[1]) + (wave_before[2] + wave_before[3]);
+    for (int i = first; i < token; ++i) row += p.target[i] != p.ignore;
+    const int64_t t = p.target[token];
+    if (t == p.ignore) row = -1;
+    if (row >= 0 && lane == 0) write_row(p, row, token, t, p.token_grads != nullptr ? p.token_grads[token] : 1.0f);
+    gather_token<D>(g, token, row, lane);
 }
 
 // ---- logits ---------------------------------------------------------------------------------
@@ -1237,11 +1280,17 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
     int32_t* place = static_cast<int32_t*>(at(plan.place));
     float* weight = static_cast<float*>(at(plan.weight));
     void* rows = at(plan.rows);
-    prepare_kernel<<<1, 1024, 0, s>>>({c.target, c.token_grads, control, place, token, word, weight, c.tokens, c.vocab,
-                                       c.ignore, mean, D == F16 && plan.grads});
-    if ((status = check_launch(who)) != HBT_OK) return status;
-    gather_kernel<D><<<dim3(static_cast<unsigned>((c.tokens + 3) / 4)), 256, 0, s>>>(
-        {c.x, place, rows, c.dx, token_loss, c.ldx, plan.ld, c.lddx, c.tokens, c.inner, OD == F32});
+    const PrepareArgs prepare{c.target, c.token_grads, control, place, token, word, weight, c.tokens, c.vocab, c.ignore, mean,
+                              D == F16 && plan.grads};
+    const GatherArgs gather{c.x, place, rows, c.dx, token_loss, c.ldx, plan.ld, c.lddx, c.tokens, c.inner, OD == F32};
+    const dim3 gathers(static_cast<unsigned>((c.tokens + 3) / 4));
+    if (c.tokens <= kFewTokens) {
+        prepare_few_kernel<D><<<gathers, 256, 0, s>>>(prepare, gather);
+    } else {
+        prepare_kernel<<<1, 1024, 0, s>>>(prepare);
+        if ((status = check_launch(who)) != HBT_OK) return status;
+        gather_kernel<D><<<gathers, 256, 0, s>>>(gather);
+    }
     if ((status = check_launch(who)) != HBT_OK) return status;
     const bool aligned = plan.pad || is_aligned(c.w, c.ldw, c.inner, D);
     const void* w = plan.pad ? at(plan.padded) : c.w;
