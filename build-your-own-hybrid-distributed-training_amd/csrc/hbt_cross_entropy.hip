@@ -712,18 +712,22 @@ struct SoftmaxArgs {
     const int32_t* word;
     int64_t ldk, vocab, stride;
     int64_t cut;  // the words before it are in tiles of `tile` columns, the others in tiles of `last`
-    int tile, last, segment;  // segment: columns that a workgroup takes
+    int tile, last;
     float smoothing;
     Piece piece;
 };
 
-// Bound by memory: a read and a write of 2 bytes (fp32: 4) an element.
+constexpr int kSoftmaxUnits = 2;  // 16-byte units a lane
+// Bound by memory: a read and a write of 2 bytes (fp32: 4) an element, 8192 x 128256 in bf16 in 745 us
+// (5.6 TB/s), 8192 x 50257 in 297.  Two units a lane, read past the caches: as they are written 780 and 307;
+// four in a loop 815 and 317; one 710 and 315, but 52 for 44 where two fifths of the rows are none.
 template <int D>
 __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs p) {
     constexpr int E = unit_elems<D>(), B = elem_bytes<D>(), S = D == F32 ? F32 : F16;
     int first, count;
     piece_rows(p.piece, first, count);
-    const int segments = static_cast<int>((p.ldk + p.segment - 1) / p.segment);
+    constexpr int kSegment = 256 * kSoftmaxUnits * E;  // words a workgroup takes
+    const int segments = static_cast<int>((p.ldk + kSegment - 1) / kSegment);
     const int i = blockIdx.x / segments, part = blockIdx.x % segments;
     if (i >= count) return;
     const Row row = p.row[first + i];
@@ -733,16 +737,24 @@ __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs p) {
     const bool known = word >= 0;
     char* line = static_cast<char*>(p.kept) + int64_t(i) * p.ldk * B;
     const float2* stats = p.stats + i;
-    const int64_t end = min<int64_t>(p.ldk, (part + 1) * int64_t(p.segment));
-    for (int64_t j = part * int64_t(p.segment) + threadIdx.x * E; j < end; j += 256 * E) {
-        const u32x4 unit = *reinterpret_cast<const u32x4*>(line + j * B);
+    const int64_t first_word = (int64_t(part) * 256 * kSoftmaxUnits + threadIdx.x) * E;
+    u32x4 units[kSoftmaxUnits];
+#pragma unroll
+    for (int u = 0; u < kSoftmaxUnits; ++u) {
+        const int64_t j = first_word + u * 256 * E;
+        if (j < p.ldk) units[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(line + j * B));
+    }
+#pragma unroll
+    for (int u = 0; u < kSoftmaxUnits; ++u) {
+        const int64_t j = first_word + u * 256 * E;
+        if (j >= p.ldk) break;
         const int64_t word_at = min<int64_t>(j, p.vocab - 1);
         const int64_t at = word_at < p.cut ? word_at / p.tile : p.cut / p.tile + (word_at - p.cut) / p.last;
         const float factor = exponential<D>(stats[at * p.stride].x - row.top) * row.inverse * row.weight;
         float v[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            v[e] = element<S>(unit, e) * factor - even;
+            v[e] = element<S>(units[u], e) * factor - even;
             if (j + e == word) v[e] = hit;
             if (!known) v[e] = NAN;
             if (j + e >= p.vocab) v[e] = 0.0f;
@@ -1326,9 +1338,9 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
         join_kernel<<<dim3(static_cast<unsigned>((plan.most + kJoinRows - 1) / kJoinRows)), kJoinRows * kJoinGroups, 0, s>>>(join);
         if ((status = check_launch(who)) != HBT_OK) return status;
         if (!plan.grads) continue;
-        const int segment = 256 * unit_elems<D>() * 4;
+        const int64_t segment = 256 * kSoftmaxUnits * unit_elems<D>();
         softmax_kernel<D><<<dim3(static_cast<unsigned>((plan.ldk + segment - 1) / segment * plan.most)), 256, 0, s>>>({kept, stats, row, word, plan.ldk,
-                                                                          c.vocab, plan.most, plan.cut, plan.size, 128, segment,
+                                                                          c.vocab, plan.most, plan.cut, plan.size, 128,
                                                                           c.smoothing, piece});
         if ((status = check_launch(who)) != HBT_OK) return status;
         const bool last = i + 1 == plan.pieces;
