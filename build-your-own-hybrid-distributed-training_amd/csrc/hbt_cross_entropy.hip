@@ -27,7 +27,11 @@ namespace {
 constexpr int F32 = HBT_DTYPE_F32, BF16 = HBT_DTYPE_BF16, F16 = HBT_DTYPE_F16;
 constexpr int64_t kPieceBytes = int64_t(2) << 30;  // stored exponentials at a time
 constexpr int64_t kStatsBytes = int64_t(1) << 28;  // row statistics at a time, without gradients
-constexpr int kThin = 16;                          // rows of the kernel for few tokens
+// The kernel for few tokens takes up to 16; each of its workgroups reads all of them, which tells past
+// so many products: 4 x 4096 x 128256 take 199 us and in tiles 196, 2 tokens 191 and 198, 16 tokens 282 and
+// 198, but 16 x 768 x 50257 (0.6e9) 26.5 and 30.7.
+constexpr int kThin = 16;
+constexpr int64_t kThinProducts = int64_t(1) << 31;
 // Tokens from which on a 2-byte W with rows off 16 bytes is copied to rows on them first: its
 // products then load straight into LDS, in tiles of 256.  50257 x 765 in bf16: 8192 tokens, evaluated,
 // 1324 us without the copy and 641 with it, all gradients 3884 and 2291; 200 tokens 73 either way.  In
@@ -1061,7 +1065,7 @@ Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants,
     if (is_small(tokens, inner, vocab)) return p;
     const int64_t size = dtype == F32 ? 4 : 2;
     p.grads = wants != 0;
-    p.thin = tokens <= kThin && !p.grads;
+    p.thin = tokens <= kThin && tokens * inner * vocab <= kThinProducts && !p.grads;
     p.pad = !aligned && dtype != F32 && tokens >= kPadTokens;
     aligned = aligned || p.pad;
     p.ld = up(std::max<int64_t>(inner, 1), 64);

@@ -209,7 +209,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     loss and the gradients NaN.  Any strides are accepted, as by :func:`fused_linear`.
 
     With gradients wanted, a summed or averaged loss computes them here (see the module), so call
-    it under ``torch.no_grad()`` to evaluate; up to 16 tokens then take one read of the weight.
+    it under ``torch.no_grad()`` to evaluate.
     """
     _check(x, weight, target, bias, reduction, label_smoothing)
     if _holds_tangent(x, weight, bias):
