@@ -93,6 +93,7 @@ constexpr double unit() { return D == F32 ? 1.0 : 0.69314718055994531; }
 struct PrepareArgs {
     const int64_t* target;
     const float* token_grads;  // the loss's gradient for each token, or null for 1
+    const float* factor;       // the loss's own gradient, or null for 1
     Control* control;
     int32_t* place;   // token -> row, -1 without a loss
     int32_t* token;   // row -> token
@@ -115,7 +116,8 @@ __device__ __forceinline__ void write_control(const PrepareArgs& p, int count, f
     p.control->count = count;
     p.control->scale_in = in;
     // No token carries a loss: no gradient, where 1 / 0 times a sum of nothing would be NaN.
-    p.control->scale_out = count == 0 ? 0.0f : (p.mean ? 1.0f / static_cast<float>(count) : 1.0f) / in;
+    const float factor = p.factor != nullptr ? *p.factor : 1.0f;
+    p.control->scale_out = count == 0 ? 0.0f : (p.mean ? factor / static_cast<float>(count) : factor) / in;
 }
 __device__ __forceinline__ void write_row(const PrepareArgs& p, int row, int64_t i, int64_t t, float weight) {
     p.token[row] = static_cast<int32_t>(i);
@@ -904,7 +906,7 @@ bool is_small(int64_t tokens, int64_t inner, int64_t vocab) {
 struct SmallArgs {
     const void *x, *w, *bias;
     const int64_t* target;
-    const float* token_grads;
+    const float *token_grads, *factor;
     float* loss;
     void *dx, *dw, *db;
     int64_t ldx, ldw, lddx, lddw, ignore;
@@ -978,7 +980,8 @@ __global__ __launch_bounds__(1024) void small_kernel(SmallArgs p) {
             if (lane == 0) p.loss[0] = static_cast<float>(mean ? sum / count : sum);
         }
     }
-    const float scale = count == 0 ? 0.0f : (mean ? 1.0f / static_cast<float>(count) : 1.0f);
+    const float factor = p.factor != nullptr ? *p.factor : 1.0f;
+    const float scale = count == 0 ? 0.0f : (mean ? factor / static_cast<float>(count) : factor);
     if (p.dx != nullptr)
         for (int i = tid; i < p.tokens * p.inner; i += 1024) {
             const int t = i / p.inner, k = i % p.inner;
@@ -1246,7 +1249,7 @@ int32_t check_rows(const char* who, const void* p, int64_t rows, int64_t cols, i
 struct Call {
     const void *x, *w, *bias;
     const int64_t* target;
-    const float* token_grads;
+    const float *token_grads, *factor;
     float* loss;
     void *dx, *dw, *db;
     int64_t ldx, ldw, lddx, lddw, tokens, inner, vocab, ignore;
@@ -1270,7 +1273,7 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
         if (bytes > 65536 &&
             (status = allow_lds(who, reinterpret_cast<const void*>(small_kernel<D, OD>), kSmallLds, done)) != HBT_OK)
             return status;
-        small_kernel<D, OD><<<1, 1024, bytes, s>>>({c.x, c.w, c.bias, c.target, c.token_grads, c.loss, c.dx, c.dw, c.db, c.ldx,
+        small_kernel<D, OD><<<1, 1024, bytes, s>>>({c.x, c.w, c.bias, c.target, c.token_grads, c.factor, c.loss, c.dx, c.dw, c.db, c.ldx,
                                                     c.ldw, c.lddx, c.lddw, c.ignore, static_cast<int>(c.tokens),
                                                     static_cast<int>(c.inner), static_cast<int>(c.vocab), c.reduction,
                                                     c.smoothing});
@@ -1296,7 +1299,7 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
     int32_t* place = static_cast<int32_t*>(at(plan.place));
     float* weight = static_cast<float*>(at(plan.weight));
     void* rows = at(plan.rows);
-    const PrepareArgs prepare{c.target, c.token_grads, control, place, token, word, weight, c.tokens, c.vocab, c.ignore, mean,
+    const PrepareArgs prepare{c.target, c.token_grads, c.factor, control, place, token, word, weight, c.tokens, c.vocab, c.ignore, mean,
                               D == F16 && plan.grads};
     const GatherArgs gather{c.x, place, rows, c.dx, token_loss, c.ldx, plan.ld, c.lddx, c.tokens, c.inner, OD == F32};
     const dim3 gathers(static_cast<unsigned>((c.tokens + 3) / 4));
@@ -1405,8 +1408,8 @@ int64_t hbt_linear_cross_entropy_workspace(int64_t tokens, int64_t inner, int64_
 }
 
 int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
-                                 const int64_t* target, const float* token_grads, float* loss, void* dx, int64_t lddx,
-                                 void* dw, int64_t lddw, void* dbias, int64_t tokens, int64_t inner, int64_t vocab,
+                                 const int64_t* target, const float* token_grads, const float* factor, float* loss,
+                                 void* dx, int64_t lddx, void* dw, int64_t lddw, void* dbias, int64_t tokens, int64_t inner, int64_t vocab,
                                  int32_t dtype, int32_t grad_dtype, int64_t ignore_index, float smoothing,
                                  int32_t reduction, void* workspace, int64_t workspace_bytes, void* stream) {
     clear_error();
@@ -1431,7 +1434,7 @@ int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int6
     if (plan.bytes > 0 &&
         (workspace == nullptr || workspace_bytes < plan.bytes || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return refuse(who, "the workspace is smaller than hbt_linear_cross_entropy_workspace's, or off 256 bytes");
-    const Call c{x, w, bias, target, token_grads, loss, dx, dw, dbias, ldx, ldw, lddx, lddw, tokens, inner, vocab,
+    const Call c{x, w, bias, target, token_grads, factor, loss, dx, dw, dbias, ldx, ldw, lddx, lddw, tokens, inner, vocab,
                  ignore_index, reduction, wants, smoothing};
     char* space = static_cast<char*>(workspace);
     const hipStream_t s = as_stream(stream);

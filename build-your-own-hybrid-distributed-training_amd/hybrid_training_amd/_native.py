@@ -316,8 +316,8 @@ EXPORTED_SYMBOLS: dict[str, tuple[object, tuple[object, ...]]] = {
         _c_i64, (_c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32)),
     "hbt_linear_cross_entropy": (
         _c_i32,
-        (_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p,
-         _c_i64, _c_void_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i64, _c_f32, _c_i32, _c_void_p, _c_i64,
+        (_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64,
+         _c_void_p, _c_i64, _c_void_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i64, _c_f32, _c_i32, _c_void_p, _c_i64,
          _c_void_p),
     ),
     "hbt_scale_round": (

@@ -8,8 +8,8 @@ have read them, so nothing of that size outlives the call.
 
 A summed or averaged loss computes its gradients in the forward pass, where the exponentials are,
 and the backward pass multiplies them by the loss's own gradient: 6 operations for each token,
-word and hidden value instead of 8.  Separate losses (``reduction="none"``) form the logits
-again in the backward pass, which knows each token's gradient only then.
+word and hidden value instead of 8.  Separate losses (``reduction="none"``), whose gradients are
+known only then, and few float16 tokens of a large weight form the logits again in the backward pass.
 
 Sums and statistics are float32 or wider, and so is the loss.  The gradient of the logits is rounded once to the
 tensors' dtype, for the matrix cores.  Gradients of bfloat16 tensors are held rounded between
@@ -40,6 +40,11 @@ _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8)
 #: Sizes that the kernels address (hbt_linear_cross_entropy's limits).
 _MAX_SIDE, _MAX_TOKENS = (1 << 20) - 64, 1 << 24
 _WHO = "cross_entropy.linear_cross_entropy"
+#: Gradients of float16 tensors are computed in the forward pass and held in float32 from so many tokens
+#: on, or for weights of fewer elements.  For few tokens of a large weight, writing and reading its
+#: gradient costs more than forming the logits again: 64 x 4096 x 128256 take 1732 us held and 1204 us
+#: not, 1024 tokens 3999 and 4171; 500 x 1000 x 5000 take 146 and 161.
+_HOLD_TOKENS, _HOLD_ELEMENTS = 768, 1 << 24
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None, reduction: str,
@@ -86,21 +91,25 @@ def _check(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: to
 
 
 def _compute(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, target: torch.Tensor, options: tuple,
-             wants: tuple[bool, bool, bool], token_grads: torch.Tensor | None = None, with_loss: bool = True):
-    """(loss or None, [dx, dw, dbias], None where not wanted).  Gradients of a summed or averaged
-    loss of float16 tensors are float32."""
+             wants: tuple[bool, bool, bool], dloss: torch.Tensor | None = None):
+    """(loss, [dx, dw, dbias], None where not wanted); with the loss's own gradient ``dloss`` (None, [...]).
+    Without it, gradients of float16 tensors are float32."""
     ignore_index, reduction, smoothing = options
     vocab, inner = weight.shape
     device, dtype = x.device, x.dtype
     separate = reduction == "none"
-    held = torch.float32 if dtype == torch.float16 and not separate else dtype
-    loss = torch.empty(target.shape if separate else (), dtype=torch.float32, device=device) if with_loss else None
+    held = torch.float32 if dtype == torch.float16 and dloss is None else dtype
+    loss = torch.empty(target.shape if separate else (), dtype=torch.float32, device=device) if dloss is None else None
+    if dloss is not None:
+        dloss = dloss.to(torch.float32).contiguous()
     grads = [torch.empty(t.shape, dtype=held, device=device) if want else None
              for t, want in zip((x, weight, bias), wants)]
     words = target.reshape(-1)
     if words.dtype != torch.int64 or not words.is_contiguous():
         words = words.to(torch.int64).contiguous()
     tokens = words.numel()
+    if loss is None and not any(g is not None and g.numel() for g in grads):
+        return loss, grads  # of an inner size of 0
     if tokens == 0:
         if loss is not None and not separate:
             loss.fill_(math.nan if reduction == "mean" else 0.0)
@@ -125,9 +134,11 @@ def _compute(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, t
         across = max(inner, 1)
         _native.check(lib.hbt_linear_cross_entropy(
             rows.data_ptr(), ldx, w.data_ptr(), ldw, None if b is None else b.data_ptr(), words.data_ptr(),
-            None if token_grads is None else token_grads.data_ptr(), None if loss is None else loss.data_ptr(), at[0],
-            across, at[1], across, at[2], tokens, inner, vocab, code, held_code, ignore_index, smoothing,
-            REDUCTIONS[reduction], None if space is None else space.data_ptr(), nbytes, _native.stream_of(device)),
+            dloss.data_ptr() if dloss is not None and separate else None,
+            dloss.data_ptr() if dloss is not None and not separate else None,
+            None if loss is None else loss.data_ptr(), at[0], across, at[1], across, at[2], tokens, inner, vocab, code,
+            held_code, ignore_index, smoothing, REDUCTIONS[reduction], None if space is None else space.data_ptr(), nbytes,
+            _native.stream_of(device)),
             "cross_entropy.hbt_linear_cross_entropy")
     return loss, grads
 
@@ -166,7 +177,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, options):
         ctx.options, ctx.scaling = options, None
-        if options[1] == "none":
+        ctx.holds = options[1] != "none" and (x.dtype != torch.float16 or target.numel() >= _HOLD_TOKENS
+                                              or weight.numel() < _HOLD_ELEMENTS)
+        if not ctx.holds:
             loss, _ = _compute(x, weight, bias, target, options, (False, False, False))
         else:
             wants = (x.requires_grad, weight.requires_grad, bias is not None and bias.requires_grad)
@@ -182,15 +195,13 @@ class _LinearCrossEntropy(torch.autograd.Function):
         if scaling is not None:
             dx, dw, db = scaling.run(dloss)
             return dx, dw, db, None, None
-        # Separate losses, or a second backward pass: from the beginning.
         x, weight, bias, target = ctx.saved_tensors
         wants = ctx.needs_input_grad[:3]
-        if ctx.options[1] == "none":
-            token_grads = dloss.reshape(-1).to(torch.float32).contiguous()
-            _, grads = _compute(x, weight, bias, target, ctx.options, wants, token_grads, with_loss=False)
-        else:
-            _, grads = _compute(x, weight, bias, target, ctx.options, wants, with_loss=False)
+        if ctx.holds:  # a second backward pass, with the first one's bits
+            _, grads = _compute(x, weight, bias, target, ctx.options, wants)
             grads = _Scaling(grads, x.dtype).run(dloss)
+        else:
+            _, grads = _compute(x, weight, bias, target, ctx.options, wants, dloss)
         return *grads, None, None
 
 

@@ -782,7 +782,8 @@ int32_t hbt_moments8_decode(void* const* codes, void* const* scales, void* const
  * reduction HBT_LOSS_NONE: loss is [tokens] fp32 (NULL for the gradients alone) and c_i =
  * token_grads[i] (fp32; NULL = 1).  HBT_LOSS_SUM: loss is one fp32, c_i = 1.  HBT_LOSS_MEAN:
  * its quotient by the number of tokens that are not ignored (0 / 0, NaN, without any), c_i one over that
- * number (gradients are zeros without any).
+ * number (gradients are zeros without any).  `factor`: NULL for 1, or one fp32 in device memory that
+ * multiplies every c_i (the loss's own gradient).
  * dx, dw and dbias may each be NULL; they are of grad_dtype: dtype, or F32.  Sums and statistics are
  * fp32 or wider; dz is rounded to `dtype` once, for the matrix cores.  No atomics: results
  * repeat bitwise.  Rows are at most 2^20 elements apart, vocab and inner at most 2^20 - 64, tokens
@@ -798,8 +799,8 @@ int32_t hbt_moments8_decode(void* const* codes, void* const* scales, void* const
 int64_t hbt_linear_cross_entropy_workspace(int64_t tokens, int64_t inner, int64_t vocab, int32_t dtype, int32_t wants,
                                            int32_t grad_dtype, float smoothing, int32_t aligned);
 int32_t hbt_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
-                                 const int64_t* target, const float* token_grads, float* loss, void* dx, int64_t lddx,
-                                 void* dw, int64_t lddw, void* dbias, int64_t tokens, int64_t inner, int64_t vocab,
+                                 const int64_t* target, const float* token_grads, const float* factor, float* loss,
+                                 void* dx, int64_t lddx, void* dw, int64_t lddw, void* dbias, int64_t tokens, int64_t inner, int64_t vocab,
                                  int32_t dtype, int32_t grad_dtype, int64_t ignore_index, float smoothing,
                                  int32_t reduction, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -55,7 +55,7 @@ def test_the_library_refuses_bad_calls_before_any_launch():
 
     def call(x=p, ldx=64, w=p, ldw=64, target=p, token_grads=None, loss=p, dx=None, lddx=0, dw=None, lddw=0, tokens=4,
              inner=64, vocab=10000, dtype=1, grad_dtype=1, smoothing=0.0, reduction=0, space=p, nbytes=1 << 30):
-        return lib.hbt_linear_cross_entropy(x, ldx, w, ldw, None, target, token_grads, loss, dx, lddx, dw, lddw, None,
+        return lib.hbt_linear_cross_entropy(x, ldx, w, ldw, None, target, token_grads, None, loss, dx, lddx, dw, lddw, None,
                                             tokens, inner, vocab, dtype, grad_dtype, -100, smoothing, reduction, space,
                                             nbytes, None)
 

@@ -15,7 +15,7 @@ import math
 import pytest
 import torch
 
-from hybrid_training_amd import LinearCrossEntropy, StepGraph, linear_cross_entropy
+from hybrid_training_amd import LinearCrossEntropy, StepGraph, cross_entropy, linear_cross_entropy
 from hybrid_training_amd.errors import ShardingError, UnsupportedFeatureError
 
 pytestmark = pytest.mark.gpu
@@ -136,11 +136,14 @@ def test_separate_losses_take_each_tokens_gradient(dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [1.0, 1024.0, 0.3])
-def test_the_losss_own_gradient(dtype, scale):
-    x, w, b, target = _inputs(100, 40, 300, dtype, bias=True)
+@pytest.mark.parametrize("tokens, held", [(20, None), (20, 0), (100, None), (100, 0), (900, None)])
+def test_the_losss_own_gradient(dtype, scale, tokens, held, monkeypatch):
+    x, w, b, target = _inputs(tokens, 40, 300, dtype, bias=True)
     leaves = [t.requires_grad_(True) for t in (x, w, b)]
     _, _, grads, offs = _exact(x.detach(), w.detach(), b.detach(), target,
-                               grads=torch.full((100,), 0.01 * scale, device=DEV))
+                               grads=torch.full((tokens,), scale / tokens, device=DEV))
+    if held is not None:  # as for a large weight
+        monkeypatch.setattr(cross_entropy, "_HOLD_ELEMENTS", held)
     loss = linear_cross_entropy(x, w, target, b)
     first = torch.autograd.grad(loss, leaves, torch.tensor(scale, device=DEV), retain_graph=True)
     kept = [g.clone() for g in first]
