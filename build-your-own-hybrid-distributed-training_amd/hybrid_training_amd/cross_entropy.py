@@ -173,9 +173,25 @@ class _Scaling:
         return self.results
 
 
+def _refuse_eager_nodes(ctx, device: torch.device) -> None:
+    """Refuse to record a step whose tensors still hang on an eager step's autograd nodes.
+
+    Autograd runs a leaf's node on the stream that first used it, for as long as any loss keeps the node
+    alive.  Where that was the default stream, which cannot join a recording, the recorded backward pass
+    would end the process.  Each node notes its stream."""
+    stream = _native.stream_of(device)
+    for node, _ in ctx.next_functions:
+        if node is not None and node.metadata.setdefault("linear_cross_entropy_stream", stream) != stream:
+            if not node.metadata["linear_cross_entropy_stream"] and _native.capturing():
+                raise UnsupportedFeatureError(
+                    format_error(_WHO, "a loss of an eager step is still alive, and its parameters' autograd nodes with it",
+                                 resolution="delete it, or keep loss.detach(), before recording a step"))
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, options):
+        _refuse_eager_nodes(ctx, x.device)
         ctx.options, ctx.scaling = options, None
         ctx.holds = options[1] != "none" and (x.dtype != torch.float16 or target.numel() >= _HOLD_TOKENS
                                               or weight.numel() < _HOLD_ELEMENTS)
@@ -220,7 +236,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     loss and the gradients NaN.  Any strides are accepted, as by :func:`fused_linear`.
 
     With gradients wanted, a summed or averaged loss computes them here (see the module), so call
-    it under ``torch.no_grad()`` to evaluate.
+    it under ``torch.no_grad()`` to evaluate.  Before a step is recorded (:class:`StepGraph`), let go of the
+    losses of eager steps over the same tensors, or keep ``loss.detach()``: recording beside them is refused.
     """
     _check(x, weight, target, bias, reduction, label_smoothing)
     if _holds_tangent(x, weight, bias):

@@ -179,6 +179,27 @@ def test_a_list_longer_than_a_launch_steps_as_each_alone():
         assert all(torch.equal(a, b) for a, b in zip(_codes(one, p), _codes(o, q)))
 
 
+def test_elements_past_32_bits():
+    """A parameter of 2^31 + 300 elements: its last blocks step and decode as they do alone."""
+    numel, last = (1 << 31) + 300, (1 << 16) + 300
+    whole = torch.nn.Parameter(torch.zeros(numel, dtype=torch.bfloat16, device=DEV))
+    whole.grad = torch.zeros_like(whole)
+    alone, = _params([last], torch.bfloat16)
+    with torch.no_grad():
+        whole[-last:] = alone
+    optimizers = [_optimizer([whole]), _optimizer([alone])]
+    for step in (1, 2):
+        _new_grads([alone], step)
+        whole.grad[-last:] = alone.grad
+        for optimizer in optimizers:
+            optimizer.step()
+    assert torch.equal(whole.detach()[-last:], alone.detach())
+    assert not whole.detach()[: numel - last].any()
+    (far, near), (other, beside) = (o.moments(torch.bfloat16)[0] for o in optimizers)
+    assert torch.equal(far[-last:], other) and torch.equal(near[-last:], beside)
+    assert not far[: numel - last].any() and not near[: numel - last].any()
+
+
 def test_zeros_tiny_and_non_finite_gradients():
     params = _params([1024])
     p = params[0]

@@ -336,6 +336,74 @@ def test_more_rows_than_one_piece_holds(dtype):
         _close(g, t, off)
 
 
+def test_rows_far_apart():
+    """Rows 2^20 elements apart, past 4 GiB, are read where they lie and give the dense ones' bits."""
+    x, w, _, target = _inputs(2500, 64, 3000, torch.bfloat16)
+    dense = [t.clone().requires_grad_(True) for t in (x, w)]
+    loss = linear_cross_entropy(*dense, target)
+    want = [loss.detach(), *torch.autograd.grad(loss, dense)]
+    far = []
+    for t in (x, w):
+        room = torch.empty(t.shape[0], 1 << 20, dtype=t.dtype, device=DEV)
+        room[:, :64] = t
+        far.append(room[:, :64].requires_grad_(True))
+    loss = linear_cross_entropy(*far, target)
+    for a, c in zip(want, [loss.detach(), *torch.autograd.grad(loss, far)]):
+        assert torch.equal(a, c)
+
+
+def test_hidden_states_past_32_bits():
+    """1.1e6 x 2048 hidden states.  All but the last 1000 tokens' are zero, so the weight's gradient is a
+    sum of 1000 terms, whose bound holds, from the end of the tensor."""
+    tokens, inner, vocab, last = 1_100_000, 2048, 64, 1000
+    some, w, _, words = _inputs(last, inner, vocab, torch.bfloat16)
+    x = torch.zeros(tokens, inner, dtype=torch.bfloat16, device=DEV)
+    x[-last:] = some
+    target = torch.arange(tokens, device=DEV) % vocab
+    target[-last:] = words
+    dx, dw = torch.autograd.grad(
+        linear_cross_entropy(x.requires_grad_(True), w.requires_grad_(True), target, reduction="sum"), [x, w])
+    x, w = x.detach(), w.detach()
+    ones = torch.ones(tokens, device=DEV)
+    _, _, grads, offs = _exact(x[-last:], w, None, target[-last:], grads=ones[-last:])
+    _close(dw, grads[1], offs[1])
+    for at in range(0, tokens, 50_000):
+        part = slice(at, at + 50_000)
+        _, _, grads, offs = _exact(x[part], w, None, target[part], grads=ones[part])
+        _close(dx[part], grads[0], offs[0])
+
+
+def test_a_weight_past_32_bits():
+    """33 tokens over the largest vocabulary, a weight of 2.2e9 elements."""
+    tokens, inner, vocab = 33, 2112, (1 << 20) - 64
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    w = torch.empty(vocab, inner, dtype=torch.bfloat16, device=DEV).normal_(0, inner**-0.5, generator=gen)
+    target = torch.randint(vocab, (tokens,), device=DEV, generator=gen)
+    target[0], target[1] = vocab - 1, 0
+    x = (torch.randn(tokens, inner, device=DEV, generator=gen) + 12 * w[target].float()).bfloat16()
+    loss = linear_cross_entropy(x.requires_grad_(True), w.requires_grad_(True), target, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, [x, w])
+    x, w = x.detach(), w.detach()
+    chunks = [slice(i, min(i + 65536, vocab)) for i in range(0, vocab, 65536)]
+    x64 = x.double()
+    z = torch.cat([x64 @ w[c].double().t() for c in chunks], 1)
+    e = torch.stack([(x64.abs() @ w[c].double().abs().t()).amax(1, keepdim=True) for c in chunks]).amax(0)
+    e = e * (inner + 2) * 2.0**-24
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    p, one = torch.exp(z - lse), torch.zeros_like(z).scatter_(1, target[:, None], 1.0)
+    exact = (lse.squeeze(1) - z.gather(1, target[:, None]).squeeze(1)).sum()
+    assert abs(float(loss.detach()) - float(exact)) <= float((2 * e + 2.0**-21 * (1 + 2 * z.abs().amax(1, keepdim=True) + lse)).sum())
+    dz = p - one
+    off = dz.abs() * (2.0**-8 + 2.0**-11 + 2.0**-20) + 4 * e * p + 2.0**-23
+    want, near = torch.zeros_like(x64), torch.zeros_like(x64)
+    for c in chunks:
+        w64 = w[c].double()
+        want += dz[:, c] @ w64
+        near += off[:, c] @ w64.abs() + vocab * 2.0**-24 * (dz[:, c].abs() @ w64.abs())
+        _close(dw[c], dz[:, c].t() @ x64, off[:, c].t() @ x64.abs() + tokens * 2.0**-24 * (dz[:, c].abs().t() @ x64.abs()))
+    _close(dx, want, near)
+
+
 def test_gradients_against_differences():
     x, w, b, target = _inputs(6, 8, 40, torch.float32, bias=True)
     x64, w64, b64 = x.double(), w.double(), b.double()
@@ -416,6 +484,34 @@ def test_recorded_and_replayed():
         taped = [t.clone() for t in graph.output]
         for a, c in zip(taped, fixed()):
             assert torch.equal(a, c)
+
+
+def test_recording_beside_a_living_eager_loss():
+    """Its nodes belong to the default stream, which cannot join the recording: refused, until it is gone."""
+    x, w, _, target = _inputs(100, 32, 300, torch.bfloat16)
+    w.requires_grad_(True)
+    w.grad = torch.zeros_like(w)
+
+    def step():
+        loss = linear_cross_entropy(x, w, target)
+        loss.backward()
+        return loss.detach()
+
+    want = step()
+    alive = linear_cross_entropy(x, w, target)
+    with pytest.raises(UnsupportedFeatureError, match="still alive"):
+        StepGraph(step)
+    alive.backward()
+    kept = alive.detach()
+    del alive
+    graph = StepGraph(step)
+    w.grad.zero_()
+    once = torch.autograd.grad(linear_cross_entropy(x, w, target), [w])[0]
+    for count in (1, 2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(graph.output, want) and torch.equal(kept, want)
+        assert torch.equal(w.grad, once * count)
 
 
 def test_refusals():
