@@ -10,14 +10,15 @@
 //
 // The logits of a tile never leave the workgroup that forms them: it takes each row's largest and
 // the sum of exp(z - largest) over its columns, and a row's tiles are joined afterwards.  For
-// gradients the tile also stores exp(z - largest), which needs only 16 bits (fp16: 2^-12 of a value
-// whose gradient is rounded to 2^-9 or 2^-12 next; fp32 for fp32 tensors), for a piece of the rows
+// gradients the tile also stores exp(z - largest), which needs only 16 bits (fp16: 2^-11 of a value
+// whose gradient is rounded by 2^-8 or 2^-11 next; fp32 for fp32 tensors), for a piece of the rows
 // at a time (at most kPieceBytes); one pass over a piece turns them into dz, rounded to the tensors' dtype
 // for the matrix cores, and the two products follow.  So the logits are formed once, 6 T V D operations in
 // all, where forming them again for the gradients would take 8.
 //
-// What a sum over pieces needs (dW, db) is carried in fp32.  A target's probability is not
-// taken from the stored values but from its fp32 logit: 1 - p would lose what fp16 rounds off p.
+// What a sum over pieces needs (dW, db) is carried in fp32.  A target's exponential is left out of its
+// tile's sum and joins the others' in fp64, from its fp32 logit: both the loss and the gradient 1 - p of a
+// nearly certain target are the others' sum, which fp32 or fp16 would round off beside a 1.
 #include "hbt_matmul.hpp"
 
 namespace hbt {
@@ -39,6 +40,7 @@ constexpr int64_t kThinProducts = int64_t(1) << 31;
 constexpr int64_t kPadTokens = 256;
 constexpr int64_t kMostRows = int64_t(1) << 22;    // rows of a piece: a launch over them stays within a grid
 constexpr int64_t kMostTokens = int64_t(1) << 24;
+constexpr int64_t kMostParts = 1024;               // tiles' sums of dx that a call has room for
 constexpr float kLog2e = 1.44269504f;
 
 // What the kernels of a call share.
@@ -46,6 +48,7 @@ struct Control {
     int32_t count;    // tokens that carry a loss
     float scale_in;   // multiplies dz before it is rounded: keeps fp16 in range
     float scale_out;  // multiplies the products
+    int32_t splits;   // parts that the sums of dx are split into
 };
 
 // A row's statistics: the largest logit, 1 / sum of exp(z - largest), log p of its target and what
@@ -59,9 +62,11 @@ struct Piece {
     const Control* control;
     int piece, pieces;
 };
+__device__ __forceinline__ int rows_of_a_piece(int count, int pieces) {
+    return ((count + pieces - 1) / pieces + 255) / 256 * 256;
+}
 __device__ __forceinline__ void piece_rows(const Piece& p, int& first, int& rows) {
-    const int count = p.control->count;
-    const int each = ((count + p.pieces - 1) / p.pieces + 255) / 256 * 256;
+    const int count = p.control->count, each = rows_of_a_piece(count, p.pieces);
     first = min(p.piece * each, count);
     rows = min(each, count - first);
 }
@@ -90,6 +95,13 @@ template <int D>
 constexpr double unit() { return D == F32 ? 1.0 : 0.69314718055994531; }
 
 // ---- the tokens that carry a loss ---------------------------------------------------------
+// How the sums of dx may be split: tiles of `tile`, tiles_n across, and `steps` k-tiles each; a launch has
+// workgroups and room for `most` parts, 0 if none is to be split.
+struct SplitArgs {
+    int64_t inner;
+    int tile, tiles_n, steps, most, f32;
+};
+
 struct PrepareArgs {
     const int64_t* target;
     const float* token_grads;  // the loss's gradient for each token, or null for 1
@@ -100,11 +112,32 @@ struct PrepareArgs {
     int32_t* word;    // row -> target, -1 out of range
     float* weight;    // row -> gradient
     int64_t tokens, vocab, ignore;
-    int mean, half;
+    int mean, half, pieces;
+    SplitArgs split;
 };
 
-// `top`: the largest magnitude of a token's gradient.
-__device__ __forceinline__ void write_control(const PrepareArgs& p, int count, float top) {
+// The split of dx's sums, by the estimate that chose its tile: only here is it known how many rows
+// there are.  Lane s of a wavefront looks at s + 1 parts.  3001 tokens of which 1801 carry a loss, 1000 x 32003
+// in fp16: 8 parts and 145 us with their join, where the 4 of 3001 tokens, and 6, take 215 and 172.
+__device__ __forceinline__ int pick_splits(const SplitArgs& p, int rows, int lane) {
+    if (p.most == 0) return 1;
+    int splits = lane % 16 + 1;
+    const int tiles = (rows + p.tile - 1) / p.tile * p.tiles_n;
+    double cost = INFINITY;
+    if (splits == 1 || (p.steps >= 4 * splits && tiles * splits <= p.most))
+        cost = split_cost(p.tile, rows, p.inner, tiles, p.steps, splits, p.f32 != 0);
+    for (int m = 1; m < 16; m <<= 1) {
+        const double other = __shfl_xor(cost, m);
+        const int others = __shfl_xor(splits, m);
+        if (other < cost || (other == cost && others < splits)) cost = other, splits = others;
+    }
+    return splits;
+}
+
+// `top`: the largest magnitude of a token's gradient.  A wavefront.
+__device__ __forceinline__ void write_control(const PrepareArgs& p, int count, float top, int lane) {
+    const int splits = pick_splits(p.split, min(count, rows_of_a_piece(count, p.pieces)), lane);
+    if (lane != 0) return;
     // fp16 values of dz: the largest gradient comes to 2^13 to 2^14, far from both ends of the
     // range; a power of two, so that nothing is rounded.
     float in = 1.0f;
@@ -114,6 +147,7 @@ __device__ __forceinline__ void write_control(const PrepareArgs& p, int count, f
         in = ldexpf(1.0f, max(-126, min(126, 14 - e)));
     }
     p.control->count = count;
+    p.control->splits = splits;
     p.control->scale_in = in;
     // No token carries a loss: no gradient, where 1 / 0 times a sum of nothing would be NaN.
     const float factor = p.factor != nullptr ? *p.factor : 1.0f;
@@ -125,40 +159,58 @@ __device__ __forceinline__ void write_row(const PrepareArgs& p, int row, int64_t
     p.weight[row] = weight;
 }
 
-// One workgroup: rows in the order of the tokens (8192: 14 us).
+// One workgroup: rows in the order of the tokens, 512 consecutive ones a wavefront at a time (8192: 8 us; a barrier for each 1024 of them took 14).
 __global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
+    constexpr int kEach = 8;
     __shared__ int wave_count[16];
     __shared__ float wave_top[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int count = 0;
     float top = 0.0f;
-    for (int64_t base = 0; base < p.tokens; base += 1024) {
-        const int64_t i = base + threadIdx.x;
-        const int64_t t = i < p.tokens ? p.target[i] : p.ignore;
-        const bool valid = t != p.ignore;
-        const float g = valid && p.token_grads != nullptr ? p.token_grads[i] : 1.0f;
-        const uint64_t votes = __ballot(valid);
+    for (int64_t base = 0; base < p.tokens; base += 1024 * kEach) {
+        const int64_t first = base + wave * (64 * kEach) + lane;
+        int64_t t[kEach];
+        float g[kEach];
+        uint64_t votes[kEach];
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int64_t i = first + 64 * k;
+            t[k] = i < p.tokens ? p.target[i] : p.ignore;
+            g[k] = i < p.tokens && p.token_grads != nullptr ? p.token_grads[i] : 1.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            votes[k] = __ballot(t[k] != p.ignore);
+            mine += __popcll(votes[k]);
+        }
         __syncthreads();
-        if (lane == 0) wave_count[wave] = __popcll(votes);
+        if (lane == 0) wave_count[wave] = mine;
         __syncthreads();
-        int row = count + __popcll(votes & ((uint64_t(1) << lane) - 1));
+        int row = count;
         for (int w = 0; w < 16; ++w) {
             if (w < wave) row += wave_count[w];
             count += wave_count[w];
         }
-        if (valid) {
-            write_row(p, row, i, t, g);
-            top = fmaxf(top, fabsf(g));
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int64_t i = first + 64 * k;
+            const bool valid = (votes[k] >> lane) & 1;
+            const int at = row + __popcll(votes[k] & ((uint64_t(1) << lane) - 1));
+            if (valid) {
+                write_row(p, at, i, t[k], g[k]);
+                top = fmaxf(top, fabsf(g[k]));
+            }
+            if (i < p.tokens) p.place[i] = valid ? at : -1;
+            row += __popcll(votes[k]);
         }
-        if (i < p.tokens) p.place[i] = valid ? row : -1;
     }
     top = wave_max(top);
     if (lane == 0) wave_top[wave] = top;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 0; w < 16; ++w) top = fmaxf(top, wave_top[w]);
-        write_control(p, count, top);
-    }
+    if (wave != 0) return;
+    for (int w = 1; w < 16; ++w) top = fmaxf(top, wave_top[w]);
+    write_control(p, count, top, lane);
 }
 
 // `cols` elements from any boundary to a row of `ld`, zeros behind them; a wavefront.
@@ -246,9 +298,9 @@ __global__ __launch_bounds__(256) void prepare_few_kernel(PrepareArgs p, GatherA
     if (blockIdx.x == 0) top = wave_max(top);
     if (lane == 0) wave_before[wave] = before, wave_count[wave] = count, wave_top[wave] = top;
     __syncthreads();
-    if (blockIdx.x == 0 && threadIdx.x == 0)
+    if (blockIdx.x == 0 && wave == 0)
         write_control(p, (wave_count[0] + wave_count[1]) + (wave_count[2] + wave_count[3]),
-                      fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3])));
+                      fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3])), lane);
     const int token = first + wave;
     if (token >= tokens) return;
     int row = (wave_before[0] + wave_before[1]) + (wave_before[2] + wave_before[3]);
@@ -265,7 +317,7 @@ struct LogitArgs {
     const void* w;
     const void* bias;
     const int32_t* word;
-    float2* stats;      // [tile][row of the piece]: largest, sum of exponentials
+    float2* stats;      // [tile][row of the piece]: largest, sum of the other words' exponentials than the target's
     float* sums;        // the same: sum of the logits, or null without smoothing
     float* target;      // row -> its target's logit
     void* kept;         // [row of the piece][ldk] exponentials, or null
@@ -427,13 +479,13 @@ __global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) {
             const int at = (targets[i / 4] >> (8 * (i % 4))) & 255;
-            if (__any(at != 255)) {  // seldom: a wavefront's columns are a small part of the vocabulary
+            if (__builtin_expect(__any(at != 255), 0)) {  // seldom: a wavefront's columns are a small part of the vocabulary
                 float z = 0.0f;
 #pragma unroll
                 for (int j = 0; j < T::TN; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (at == 16 * j + 4 * q + e) z = acc[i][j][e];
+                        if (at == 16 * j + 4 * q + e) z = acc[i][j][e], acc[i][j][e] = -INFINITY;
                 if (at != 255 && ((at >> 2) & 3) == q && wm + 16 * i < rows) p.target[first + m + wm + 16 * i] = z;
             }
         }
@@ -498,7 +550,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
 
 // At most 16 tokens, without gradients: the read of W.  A workgroup of 8 waves forms 16 logits of
 // every token as the linear layer's thin kernel does, and their statistics.  1 x 4096 x 128256 in
-// bf16 takes 175 us (6.0 TB/s), 183 with the join; two or four groups of 16 a workgroup 215 and 191.
+// bf16 takes 175 to 180 us (5.8 to 6.0 TB/s), 183 to 188 with the join; two or four groups of 16 a workgroup 215 and 191.
 template <int D>
 __global__ __launch_bounds__(512) void thin_logit_kernel(const void* x_, int64_t ldx, const void* w_, int64_t ldw,
                                                          const void* bias, const int64_t* target, int tokens,
@@ -555,8 +607,8 @@ __global__ __launch_bounds__(512) void thin_logit_kernel(const void* x_, int64_t
     for (int e = 0; e < 4; ++e) {
         if (e < have) sum += acc[e];
         acc[e] = e < have ? in_units<D>(acc[e]) : -INFINITY;
-        if (at == e && e < have) target_logit[row] = acc[e];
         top = fmaxf(top, acc[e]);
+        if (at == e && e < have) target_logit[row] = acc[e], acc[e] = -INFINITY;
     }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
@@ -606,7 +658,7 @@ struct Running {
     }
 };
 
-__device__ __forceinline__ void finish_row(const JoinArgs& p, int row, const Running& r, double logits) {
+__device__ __forceinline__ void finish_row(const JoinArgs& p, int row, Running r, double logits) {
     const int64_t token = p.token != nullptr ? p.token[row] : row;
     bool known;
     if (p.word != nullptr) {
@@ -620,9 +672,13 @@ __device__ __forceinline__ void finish_row(const JoinArgs& p, int row, const Run
         }
         known = t >= 0 && t < p.vocab;
     }
-    // log p = (z_t - top) - log(sum): the two parts of a nearly certain target are both small
+    const float unit = static_cast<float>(p.unit), z = known ? p.target[row] : NAN;
+    const Running others = r;
+    if (known) r.add(z, 1.0, unit);
     const double log_sum = log(r.sum);
-    const double log_p = known ? (static_cast<double>(p.target[row]) - r.top) * p.unit - log_sum : NAN;
+    double log_p = (static_cast<double>(z) - r.top) * p.unit - log_sum;
+    if (z >= others.top && z < INFINITY)  // the others beside a 1, which would round them off
+        log_p = others.sum == 0.0 ? 0.0 : -log1p(others.sum * expf((others.top - z) * unit));
     double loss = -(1.0 - p.smoothing) * log_p;
     if (p.smoothing != 0.0f) loss += p.smoothing * ((r.top * p.unit + log_sum) - logits / static_cast<double>(p.vocab));
     if (p.loss != nullptr) p.loss[token] = static_cast<float>(loss);
@@ -670,7 +726,7 @@ __global__ __launch_bounds__(kJoinRows * kJoinGroups) void join_kernel(JoinArgs 
 }
 
 // Statistics [row][tile], many tiles and few rows: a workgroup a row, its lanes' parts joined in a tree
-// (8016 tiles: 8 us, where 256 lanes take 25).
+// (8016 tiles: 9 us, where 256 lanes take 25).
 __global__ __launch_bounds__(1024) void thin_join_kernel(JoinArgs p) {
     __shared__ float tops[1024];
     __shared__ double totals[1024], logit_sums[1024];
@@ -786,19 +842,9 @@ struct GradArgs {
     const int32_t* token;  // y's row for a row of the piece, or null: its own
     float* partial;        // [splits][m][ldp]
     int64_t lda, ldb, ldy, ldbefore, ldp, m, n, k, m_in, n_in;  // m_in, n_in: rows that the operands hold
-    int tile, tiles_n, blocks, splits;
+    int tiles_n, splits;   // splits: of dW, those of dx are the call's control's
     Piece piece;
 };
-
-// The tiles of a product over `m` rows and the parts of each one's sum.  The grid is made for as
-// many rows as there may be; where fewer carry a loss, a split sum takes the workgroups that they leave:
-// 1801 rows of 3001, 1000 x 32003: 6 parts of 32 tiles instead of 4, 168 us with its join where 4 take 215.
-template <bool kRows>
-__device__ __forceinline__ void tiles_and_splits(const GradArgs& p, int64_t m, int& tiles_m, int& splits) {
-    tiles_m = static_cast<int>((m + p.tile - 1) / p.tile);
-    splits = p.splits;
-    if (kRows && splits > 1 && tiles_m > 0) splits = max(splits, min(p.blocks / (tiles_m * p.tiles_n), 16));
-}
 
 // y = a b (dx: the rows of a are the piece's; dW: the sum runs over them), times the call's scale.
 template <int D, int OD, bool kRows>
@@ -824,9 +870,9 @@ __global__ __launch_bounds__(T::kThreads, 2) void grad_kernel(GradArgs p) {
     int first, count;
     piece_rows(p.piece, first, count);
     const int64_t m = kRows ? count : p.m, k = kRows ? p.k : count;
-    int tiles_m, splits, tm, tn;
-    tiles_and_splits<kRows>(p, m, tiles_m, splits);
+    const int tiles_m = static_cast<int>((m + T::BM - 1) / T::BM), splits = kRows ? p.piece.control->splits : p.splits;
     const int total = tiles_m * p.tiles_n, split = total > 0 ? static_cast<int>(blockIdx.x) / total : splits;
+    int tm, tn;
     if (split >= splits) return;
     band_order<8>(xcd_tile(static_cast<int>(blockIdx.x) - split * total, total), tiles_m, p.tiles_n, tm, tn);
     const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
@@ -838,7 +884,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void grad_kernel(GradArgs p) {
     tile_product<D, kRows, false, T, kAsync>(p.a, p.lda, m0, kRows ? m : p.m_in, b, p.ldb, n0, p.n_in, k0, k1, lds, acc);
     const int rows = static_cast<int>(min<int64_t>(m - m0, T::BM)), cols = static_cast<int>(min<int64_t>(p.n - n0, T::BN));
     const GradEpilogue<D, OD, kRows> tile{p, p.piece.control->scale_out, first};
-    float* partial = p.partial == nullptr ? nullptr : p.partial + (split * m + m0) * p.ldp + n0;
+    float* partial = splits == 1 ? nullptr : p.partial + (split * m + m0) * p.ldp + n0;
     finish_tile<T, kAsync, 2>(
         lds, acc,
         [&](int i, int j) {
@@ -859,8 +905,8 @@ __global__ __launch_bounds__(256) void grad_join_kernel(GradArgs p) {
     int first, count;
     piece_rows(p.piece, first, count);
     const int64_t m = kRows ? count : p.m, units = p.ldp / 4, total = m * units;
-    int tiles_m, splits;
-    tiles_and_splits<kRows>(p, m, tiles_m, splits);
+    const int splits = kRows ? p.piece.control->splits : p.splits;
+    if (splits == 1) return;
     const GradEpilogue<D, OD, kRows> tile{p, p.piece.control->scale_out, first};
     for (int64_t u = blockIdx.x * int64_t(256) + threadIdx.x; u < total; u += int64_t(gridDim.x) * 256) {
         const int64_t i = u / units, j = u % units * 4;
@@ -966,10 +1012,12 @@ __global__ __launch_bounds__(1024) void small_kernel(SmallArgs p) {
         for (int v = lane; v < p.vocab; v += 64) top = fmaxf(top, row[v]);
         top = wave_max(top);
         if (top == -INFINITY) top = 0.0f;
-        double sum = 0.0, logits = 0.0;
-        for (int v = lane; v < p.vocab; v += 64) sum += expf(row[v] - top), logits += row[v];
-        sum = wave_sum(sum), logits = wave_sum(logits);
-        const double log_sum = log(sum), log_p = known ? (static_cast<double>(row[word]) - top) - log_sum : NAN;
+        const float z_t = known ? row[word] : NAN;
+        double others = 0.0, logits = 0.0;  // without the target's exponential, which would round them off
+        for (int v = lane; v < p.vocab; v += 64) others += v == word ? 0.0f : expf(row[v] - top), logits += row[v];
+        others = wave_sum(others), logits = wave_sum(logits);
+        const double sum = known ? others + expf(z_t - top) : others, log_sum = log(sum);
+        const double log_p = z_t == top && top < INFINITY ? -log1p(others) : (static_cast<double>(z_t) - top) - log_sum;
         if (lane == 0) {
             losses[t] = -(1.0 - p.smoothing) * log_p;
             if (p.smoothing != 0.0f) losses[t] += p.smoothing * ((top + log_sum) - logits / p.vocab);
@@ -1053,6 +1101,7 @@ struct Plan {
     int tiles, pieces;
     int64_t most;           // rows of a piece, at most
     int64_t ld, ldk;        // gathered rows; exponentials
+    SplitArgs split;        // of dx
     int64_t control, place, token, word, weight, target, row, row_loss, rows, padded, stats, sums, kept, dw_sums, db_sums,
         parts, partial, bytes;
 };
@@ -1135,12 +1184,18 @@ Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants,
             p.db_sums = take(4 * vocab);
         }
         int64_t partial = 0;
-        const auto split = [&](int64_t m, int64_t n, int64_t k) {
-            const int splits = std::max(choose(m, n, k, dtype, true).splits, choose(m, n, k, dtype, false).splits);
-            if (splits > 1) partial = std::max(partial, 4 * splits * up(m, 256) * up(n, 4));
-        };
-        if ((wants & HBT_LINEAR_DX) && inner > 0) split(p.most, inner, vocab);
-        if ((wants & HBT_LINEAR_DW) && inner > 0) split(vocab, inner, p.most);
+        if ((wants & HBT_LINEAR_DX) && inner > 0) {
+            const int64_t tile = choose(p.most, inner, vocab, dtype, aligned).tile, across = (inner + tile - 1) / tile;
+            const int64_t tiles = (p.most + tile - 1) / tile * across, steps = (vocab + (size == 4 ? 31 : 63)) / (size == 4 ? 32 : 64);
+            const int64_t most = steps >= 8 && tiles <= kMostParts ? std::min(kMostParts, tiles * 16) : 0;
+            p.split = SplitArgs{inner, static_cast<int>(tile), static_cast<int>(across), static_cast<int>(steps),
+                                static_cast<int>(most), size == 4};
+            partial = 4 * most * tile * tile;
+        }
+        if ((wants & HBT_LINEAR_DW) && inner > 0) {
+            const int splits = choose(vocab, inner, p.most, dtype, true).splits;
+            if (splits > 1) partial = std::max(partial, 4 * splits * up(vocab, 256) * up(inner, 4));
+        }
         p.partial = take(partial);
     }
     p.bytes = at;
@@ -1171,12 +1226,11 @@ int32_t launch_logits(const char* who, LogitArgs p, int64_t rows, int64_t column
 }
 
 template <int D, int OD, bool kRows, class T, bool kAsync>
-int32_t launch_grad_tile(const char* who, GradArgs& p, hipStream_t s) {
+int32_t launch_grad_tile(const char* who, GradArgs& p, int64_t most_parts, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
-    p.tile = T::BM;
     p.tiles_n = static_cast<int>((p.n + T::BN - 1) / T::BN);
-    p.blocks = static_cast<int>((p.m + T::BM - 1) / T::BM * p.tiles_n * p.splits);
-    return launch<T, kAsync>(who, grad_kernel<D, OD, kRows, T, kAsync>, p, p.blocks, done, s);
+    const int64_t blocks = std::max((p.m + T::BM - 1) / T::BM * p.tiles_n * p.splits, most_parts);
+    return launch<T, kAsync>(who, grad_kernel<D, OD, kRows, T, kAsync>, p, blocks, done, s);
 }
 
 // dW in tiles of 256, its last rows or columns in tiles of 128 where that is estimated to be shorter
@@ -1186,7 +1240,7 @@ int32_t launch_cut(const char* who, const GradArgs& p, hipStream_t s) {
     const Cut cut = cut_of(p.m, p.n, p.k);
     GradArgs first = p, last = p;
     first.m = cut.m, first.n = cut.n;
-    const int32_t status = launch_grad_tile<D, OD, false, Tile256, true>(who, first, s);
+    const int32_t status = launch_grad_tile<D, OD, false, Tile256, true>(who, first, 0, s);
     if (status != HBT_OK || (cut.m == p.m && cut.n == p.n)) return status;
     const int64_t m0 = cut.m < p.m ? cut.m : 0, n0 = cut.n < p.n ? cut.n : 0;
     last.m -= m0, last.m_in -= m0, last.n -= n0, last.n_in -= n0;
@@ -1194,31 +1248,33 @@ int32_t launch_cut(const char* who, const GradArgs& p, hipStream_t s) {
     last.b = static_cast<const char*>(p.b) + n0 * elem_bytes<D>();
     last.y = static_cast<char*>(p.y) + (m0 * p.ldy + n0) * elem_bytes<OD>();
     if (p.before != nullptr) last.before = p.before + m0 * p.ldbefore + n0;
-    return launch_grad_tile<D, OD, false, Tile128, true>(who, last, s);
+    return launch_grad_tile<D, OD, false, Tile128, true>(who, last, 0, s);
 }
 
-// p.m or p.k is the most that the piece's rows may be.
+// p.m or p.k is the most that the piece's rows may be.  dx: `split` has its tile, and how many parts
+// there may be; dW's are chosen here.
 template <int D, int OD, bool kRows>
-int32_t launch_grad(const char* who, GradArgs& p, bool aligned, void* space, hipStream_t s) {
-    const Choice c = choose(p.m, p.n, p.k, D, aligned);
+int32_t launch_grad(const char* who, GradArgs& p, const SplitArgs& split, bool aligned, void* space, hipStream_t s) {
+    const Choice c = kRows ? Choice{split.tile, 1} : choose(p.m, p.n, p.k, D, aligned);
+    const int64_t parts = kRows ? split.most : 0;
     p.splits = c.splits;
     p.ldp = up(p.n, 4);
-    p.partial = c.splits > 1 ? static_cast<float*>(space) : nullptr;
+    p.partial = static_cast<float*>(space);
     int32_t status = HBT_OK;
     if (c.tile == 64) {
-        status = aligned ? launch_grad_tile<D, OD, kRows, Tile64, true>(who, p, s)
-                         : launch_grad_tile<D, OD, kRows, Tile64, false>(who, p, s);
+        status = aligned ? launch_grad_tile<D, OD, kRows, Tile64, true>(who, p, parts, s)
+                         : launch_grad_tile<D, OD, kRows, Tile64, false>(who, p, parts, s);
     } else if (c.tile == 128) {
-        status = aligned ? launch_grad_tile<D, OD, kRows, Tile128, true>(who, p, s)
-                         : launch_grad_tile<D, OD, kRows, Tile128, false>(who, p, s);
+        status = aligned ? launch_grad_tile<D, OD, kRows, Tile128, true>(who, p, parts, s)
+                         : launch_grad_tile<D, OD, kRows, Tile128, false>(who, p, parts, s);
     } else if constexpr (D != F32) {
         if constexpr (!kRows) {
-            status = c.splits == 1 ? launch_cut<D, OD>(who, p, s) : launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, s);
+            status = c.splits == 1 ? launch_cut<D, OD>(who, p, s) : launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, 0, s);
         } else {
-            status = launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, s);
+            status = launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, parts, s);
         }
     }
-    if (status != HBT_OK || c.splits == 1) return status;
+    if (status != HBT_OK || (c.splits == 1 && parts == 0)) return status;
     const int64_t blocks = std::min<int64_t>((p.m * (p.ldp / 4) + 255) / 256, 4096);
     grad_join_kernel<D, OD, kRows><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(p);
     return check_launch(who);
@@ -1311,7 +1367,7 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
     float* weight = static_cast<float*>(at(plan.weight));
     void* rows = at(plan.rows);
     const PrepareArgs prepare{c.target, c.token_grads, c.factor, control, place, token, word, weight, c.tokens, c.vocab, c.ignore, mean,
-                              D == F16 && plan.grads};
+                              D == F16 && plan.grads, plan.pieces, plan.split};
     const GatherArgs gather{c.x, place, rows, c.dx, token_loss, c.ldx, plan.ld, c.lddx, c.tokens, c.inner, OD == F32};
     const dim3 gathers(static_cast<unsigned>((c.tokens + 3) / 4));
     if (c.tokens <= kFewTokens) {
@@ -1366,7 +1422,7 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
             GradArgs g{};
             g.a = kept, g.b = w, g.y = c.dx, g.token = token, g.lda = plan.ldk, g.ldb = ldw, g.ldy = c.lddx;
             g.m = plan.most, g.n = c.inner, g.k = c.vocab, g.m_in = plan.most, g.n_in = plan.pad ? up(c.inner, 8) : c.inner, g.piece = piece;
-            if ((status = launch_grad<D, OD, true>(who, g, aligned, at(plan.partial), s)) != HBT_OK) return status;
+            if ((status = launch_grad<D, OD, true>(who, g, plan.split, aligned, at(plan.partial), s)) != HBT_OK) return status;
         }
         if ((c.wants & HBT_LINEAR_DW) && c.inner > 0) {
             GradArgs g{};
@@ -1378,10 +1434,10 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
             g.before = i > 0 ? carried : nullptr, g.ldbefore = ldcarried;
             if (last) {
                 g.y = c.dw, g.ldy = c.lddw;
-                status = launch_grad<D, OD, false>(who, g, true, at(plan.partial), s);
+                status = launch_grad<D, OD, false>(who, g, plan.split, true, at(plan.partial), s);
             } else {
                 g.y = carried, g.ldy = ldcarried;
-                status = launch_grad<D, F32, false>(who, g, true, at(plan.partial), s);
+                status = launch_grad<D, F32, false>(who, g, plan.split, true, at(plan.partial), s);
             }
             if (status != HBT_OK) return status;
         }

@@ -672,7 +672,7 @@ using Tile64 = Tile<64, 64, 2, 2, 4>;
 // (2048 x 768 by 768: 27, 14 and 9 us).  `fixed`: what a round costs beside its k-tiles.
 // Round lengths are fitted to such measurements over 17 shapes (256 CUs, one workgroup of 256 or
 // two of the others a CU), within about a fifth.
-inline double round_cost(int size, int64_t tiles, double steps, bool f32, double fixed) {
+__host__ __device__ inline double round_cost(int size, int64_t tiles, double steps, bool f32, double fixed) {
     constexpr int64_t kCus = 256;
     if (size == 256) return static_cast<double>((tiles + kCus - 1) / kCus) * (steps * 1.5 + fixed);
     const bool alone = tiles <= kCus;  // one workgroup a CU has the matrix cores for itself
@@ -682,6 +682,15 @@ inline double round_cost(int size, int64_t tiles, double steps, bool f32, double
     }
     const double step = size == 128 ? (alone ? 0.7 : 0.98) : 0.41;
     return static_cast<double>((tiles + 2 * kCus - 1) / (2 * kCus)) * (steps * step + fixed);
+}
+
+// The estimate for an m x n product of so many k-tiles whose sums are split into `splits` parts.  A split
+// sum writes and reads its fp32 parts (about 5 TB/s) in one more launch.
+__host__ __device__ inline double split_cost(int size, int64_t m, int64_t n, int64_t tiles, int64_t steps, int splits,
+                                             bool f32) {
+    const double fixed = size == 256 ? 9.0 : (size == 128 ? 6.0 : 3.5);
+    const double cost = round_cost(size, tiles * splits, static_cast<double>((steps + splits - 1) / splits), f32, fixed);
+    return splits == 1 ? cost : cost + (3.0 + 8.0 * m * n * splits / 5.0e6);
 }
 
 struct Choice {
@@ -694,8 +703,7 @@ inline int64_t tile_items(int64_t m, int64_t n, int size) {
     return ((m + size - 1) / size) * ((n + size - 1) / size) * (size == 256 ? 512 : 256);
 }
 
-// The cheapest tile and split by the estimate.  A split sum writes and reads its fp32 parts (about
-// 5 TB/s) in one more launch.  Tiles of 256 need operands that load straight into LDS.
+// The cheapest tile and split by the estimate.  Tiles of 256 need operands that load straight into LDS.
 inline Choice choose(int64_t m, int64_t n, int64_t k, int dtype, bool aligned) {
     const bool f32 = dtype == HBT_DTYPE_F32;
     const int64_t steps = (k + (f32 ? 31 : 63)) / (f32 ? 32 : 64);
@@ -703,12 +711,10 @@ inline Choice choose(int64_t m, int64_t n, int64_t k, int dtype, bool aligned) {
     double least = 0.0;
     for (const int size : {64, 128, 256}) {
         if ((size == 256 && (f32 || !aligned)) || tile_items(m, n, size) > kGridMaxItems) continue;
-        const double fixed = size == 256 ? 9.0 : (size == 128 ? 6.0 : 3.5);
         const int64_t tiles = ((m + size - 1) / size) * ((n + size - 1) / size);
         for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
             if (splits > 1 && (steps < 4 * splits || tiles * splits > 1024)) break;
-            double cost = round_cost(size, tiles * splits, static_cast<double>((steps + splits - 1) / splits), f32, fixed);
-            if (splits > 1) cost += 3.0 + 8.0 * m * n * splits / 5.0e6;
+            const double cost = split_cost(size, m, n, tiles, steps, splits, f32);
             if (least == 0.0 || cost < least) least = cost, best = {size, splits};
         }
     }

@@ -29,12 +29,14 @@ def test_working_storage():
     assert size(16, 32, 97, 0, 7, 0, 0.0, 1) == 0  # a small call's stands in LDS
     # one token over a large vocabulary: statistics alone
     assert 0 < size(1, 4096, 128256, 1, 0, 1, 0.0, 1) < 1 << 20
-    # evaluation never holds logits, training at most 2 GiB of exponentials beside rows and fp32 sums
+    # evaluation never holds logits, training at most 2 GiB of exponentials beside rows, fp32 sums and at most
+    # 1024 tiles' parts of dx's sums
     assert size(8192, 4096, 128256, 1, 0, 1, 0.0, 1) < 8192 * 4096 * 2 + (1 << 28) + (8 << 20)
     one = size(8192, 4096, 128256, 1, 3, 1, 0.0, 1)
-    assert one < 2 * GIB + 8192 * 4096 * 2 + (1 << 27)
+    parts = 1024 * 256 * 256 * 4
+    assert one < 2 * GIB + 8192 * 4096 * 2 + parts + (1 << 27)
     more = size(16384, 4096, 128256, 1, 3, 1, 0.0, 1)
-    assert more < 2 * GIB + 16384 * 4096 * 2 + 4 * 128256 * 4096 + (1 << 27)
+    assert more < 2 * GIB + 16384 * 4096 * 2 + 4 * 128256 * 4096 + parts + (1 << 27)
     assert size(32768, 4096, 128256, 1, 3, 1, 0.0, 1) - more < 16384 * 4096 * 2 + (4 << 20)
     # a 2-byte weight off 16 bytes is copied for many tokens, an fp32 one is not
     assert size(8192, 64, 50257, 1, 0, 1, 0.0, 0) - size(8192, 64, 50257, 1, 0, 1, 0.0, 1) > 50257 * 64 * 2 - (1 << 20)

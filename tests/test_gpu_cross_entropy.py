@@ -263,6 +263,29 @@ def test_a_nearly_certain_target_keeps_its_gradient():
     assert abs(float(loss.detach()) + float(torch.log1p(-missing).sum())) <= tokens * 2.0**-19
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens, vocab", [(3, 40), (4, 3000), (40, 3000), (300, 700)])
+@pytest.mark.parametrize("above", [11.5, 18.0, 25.0])
+def test_the_loss_of_a_nearly_certain_target_is_the_others_sum(dtype, tokens, vocab, above):
+    """log(1 + s) for an s down to 1e-11, which fp32 would lose beside the target's 1.  One logit z is not zero
+    and has one product; its unit, the difference of two tiles' largest and the exponentials are
+    off by at most 6 z + 16 float32 roundings."""
+    w = torch.zeros(vocab, 64, device=DEV, dtype=dtype)
+    w[1, 0] = 1.0
+    x = torch.zeros(tokens, 64, device=DEV, dtype=dtype)
+    x[:, 0] = math.log(vocab - 1) + above
+    target = torch.ones(tokens, dtype=torch.int64, device=DEV)
+    z = x[:, 0].double()
+    others = (vocab - 1) * torch.exp(-z)
+    off = (6 * z + 16) * 2.0**-24
+    loss = linear_cross_entropy(x, w, target, reduction="none")
+    assert ((loss.double() / torch.log1p(others) - 1).abs() <= off).all()
+    if dtype != torch.float16:  # whose dz of 1e-11 would be a subnormal
+        u = torch.finfo(dtype).eps / 2
+        dx, = torch.autograd.grad(linear_cross_entropy(x.requires_grad_(True), w, target, reduction="sum"), [x])
+        assert ((dx[:, 0].double() * (1 + others) / -others - 1).abs() <= off + 2 * u + 2.0**-22).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("tokens", [9, 150, 390])
 def test_layouts(dtype, tokens):
@@ -434,6 +457,48 @@ def test_equal_inputs_give_equal_bits():
         loss = linear_cross_entropy(x, w, target, b)
         runs.append([loss.detach(), *torch.autograd.grad(loss, leaves)])
     assert all(torch.equal(a, c) for other in runs[1:] for a, c in zip(runs[0], other))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(16, 32, 97), (16, 768, 5003), (130, 64, 257), (300, 501, 1000), (1801, 200, 4099), (700, 1, 9000)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_nothing_comes_from_unwritten_memory(dtype, shape, monkeypatch):
+    """Results and working storage that hold NaN before the call give the same bits."""
+    x, w, b, target = _inputs(*shape, dtype, bias=True, ignored=0.4)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def call():
+        loss = linear_cross_entropy(x, w, target, b, label_smoothing=0.1)
+        with torch.no_grad():
+            each = linear_cross_entropy(x, w, target, b, reduction="none")
+        return [loss.detach(), each, *torch.autograd.grad(loss, leaves)]
+
+    want = call()
+    empty = torch.empty
+
+    def poisoned(*args, **options):
+        t = empty(*args, **options)
+        return t.fill_(255 if t.dtype == torch.uint8 else math.nan)
+
+    monkeypatch.setattr(cross_entropy.torch, "empty", poisoned)
+    found = call()
+    monkeypatch.undo()
+    for a, c in zip(want, found):
+        assert torch.isfinite(a).all() and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("ignored", [0.0, 0.5, 0.9, 0.995])
+def test_few_rows_of_many_tokens(dtype, ignored):
+    """Sums of dx are split by how many tokens carry a loss, which only the device knows."""
+    x, w, _, target = _inputs(1500, 264, 9001, dtype, ignored=ignored)
+    target[3] = 5
+    c = torch.full(target.shape, 1.0, device=DEV)
+    _, _, grads, offs = _exact(x, w, None, target, grads=c)
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    found = torch.autograd.grad(linear_cross_entropy(x, w, target, reduction="sum"), leaves)
+    for g, want, off in zip(found, grads, offs):
+        _close(g, want, off)
 
 
 def test_two_streams_at_once():
