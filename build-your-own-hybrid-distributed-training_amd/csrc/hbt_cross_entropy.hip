@@ -783,9 +783,15 @@ struct SoftmaxArgs {
     int64_t cut;  // the words before it are in tiles of `tile` columns, the others in tiles of `last`
     int tile, last;
     float smoothing;
+    const double* row_loss;
+    float* loss;  // the call's, of which the first workgroup takes the sum, or null
+    int mean;
     Piece piece;
 };
 
+// Up to so many tokens the losses are added up beside the pass that follows them, a launch less (777 x 501
+// x 5003 in fp32: 175 us for 178); by one workgroup of 256 more would outlast it.
+constexpr int64_t kTotalTokens = 16384;
 constexpr int kSoftmaxUnits = 2;  // 16-byte units a lane
 // Bound by memory: a read and a write of 2 bytes (fp32: 4) an element, 8192 x 128256 in bf16 in 745 us
 // (5.6 TB/s), 8192 x 50257 in 297.  Two units a lane, read past the caches: as they are written 780 and 307;
@@ -793,11 +799,23 @@ constexpr int kSoftmaxUnits = 2;  // 16-byte units a lane
 template <int D>
 __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs p) {
     constexpr int E = unit_elems<D>(), B = elem_bytes<D>(), S = D == F32 ? F32 : F16;
+    int block = blockIdx.x;
+    if (p.loss != nullptr) {
+        if (block == 0) {
+            double sum = 0.0;
+            const int rows = p.piece.control->count;
+            for (int i = threadIdx.x; i < rows; i += 256) sum += p.row_loss[i];
+            sum = block_sum<256>(sum);
+            if (threadIdx.x == 0) p.loss[0] = static_cast<float>(p.mean ? sum / rows : sum);
+            return;
+        }
+        --block;
+    }
     int first, count;
     piece_rows(p.piece, first, count);
     constexpr int kSegment = 256 * kSoftmaxUnits * E;  // words a workgroup takes
     const int segments = static_cast<int>((p.ldk + kSegment - 1) / kSegment);
-    const int i = blockIdx.x / segments, part = blockIdx.x % segments;
+    const int i = block / segments, part = block % segments;
     if (i >= count) return;
     const Row row = p.row[first + i];
     const int word = p.word[first + i];
@@ -1412,12 +1430,14 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
         join_kernel<<<dim3(static_cast<unsigned>((plan.most + kJoinRows - 1) / kJoinRows)), kJoinRows * kJoinGroups, 0, s>>>(join);
         if ((status = check_launch(who)) != HBT_OK) return status;
         if (!plan.grads) continue;
+        const bool last = i + 1 == plan.pieces, totals = last && row_loss != nullptr && c.tokens <= kTotalTokens;
         const int64_t segment = 256 * kSoftmaxUnits * unit_elems<D>();
-        softmax_kernel<D><<<dim3(static_cast<unsigned>((plan.ldk + segment - 1) / segment * plan.most)), 256, 0, s>>>({kept, stats, row, word, plan.ldk,
-                                                                          c.vocab, plan.most, plan.cut, plan.size, 128,
-                                                                          c.smoothing, piece});
+        const int64_t blocks = (plan.ldk + segment - 1) / segment * plan.most + totals;
+        softmax_kernel<D><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(
+            {kept, stats, row, word, plan.ldk, c.vocab, plan.most, plan.cut, plan.size, 128, c.smoothing, row_loss,
+             totals ? c.loss : nullptr, mean, piece});
         if ((status = check_launch(who)) != HBT_OK) return status;
-        const bool last = i + 1 == plan.pieces;
+        if (totals) row_loss = nullptr;
         if ((c.wants & HBT_LINEAR_DX) && c.inner > 0) {
             GradArgs g{};
             g.a = kept, g.b = w, g.y = c.dx, g.token = token, g.lda = plan.ldk, g.ldb = ldw, g.ldy = c.lddx;
