@@ -1111,6 +1111,37 @@ __global__ __launch_bounds__(256) void scale_round_kernel(ScaleArgs p) {
 // ---- host ------------------------------------------------------------------------------------
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
+// dW in tiles of 256, its last rows or columns apart where that is estimated to be shorter: a round that
+// is mostly empty takes as long as a full one.  They are formed in tiles of 128 (splits 1), or in tiles of 256
+// whose sums are split so that they fill a round: 50257 x 768 over 8192 rows are two rounds and 79 tiles,
+// which take 94 us in three parts with their join, and 134 in tiles of 128 (bf16).
+struct DwCut {
+    int64_t m, n;  // the part in whole tiles of 256
+    int splits;
+};
+DwCut dw_cut(int64_t m, int64_t n, int64_t k) {
+    const int64_t rows = (m + 255) / 256, cols = (n + 255) / 256, steps = (k + 63) / 64;
+    DwCut best{m, n, 1};
+    double least = 0.97 * round_cost(256, rows * cols, steps, false, 9.0);
+    const auto consider = [&](int64_t whole, int64_t left, int64_t m_left, int64_t n_left, int64_t m_whole, int64_t n_whole) {
+        const double before = round_cost(256, whole, steps, false, 9.0) + 3.0;
+        if (before >= least) return;
+        const double small = before + round_cost(128, ((m_left + 127) / 128) * ((n_left + 127) / 128), steps, false, 6.0);
+        if (small < least) least = small, best = {m_whole, n_whole, 1};
+        const int splits = static_cast<int>(std::min<int64_t>(256 / left, 16));
+        if (splits < 2 || steps < 4 * splits) return;
+        const double split = before + split_cost(256, m_left, n_left, left, steps, splits, false);
+        if (split < least) least = split, best = {m_whole, n_whole, splits};
+    };
+    for (int64_t less = 1; less < 256; ++less) {  // tile rows or columns left to the second launch
+        if (less < rows && less * cols < 256)
+            consider((rows - less) * cols, less * cols, m - (rows - less) * 256, n, (rows - less) * 256, n);
+        if (less < cols && less * rows < 256)
+            consider(rows * (cols - less), less * rows, m, n - (cols - less) * 256, m, (cols - less) * 256);
+    }
+    return best;
+}
+
 // Everything a call's launches and working storage follow from.
 struct Plan {
     bool thin, grads, pad;  // pad: W is copied to rows on 16 bytes first
@@ -1120,6 +1151,8 @@ struct Plan {
     int64_t most;           // rows of a piece, at most
     int64_t ld, ldk;        // gathered rows; exponentials
     SplitArgs split;        // of dx
+    Choice dw;
+    DwCut cut_dw;
     int64_t control, place, token, word, weight, target, row, row_loss, rows, padded, stats, sums, kept, dw_sums, db_sums,
         parts, partial, bytes;
 };
@@ -1211,8 +1244,14 @@ Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants,
             partial = 4 * most * tile * tile;
         }
         if ((wants & HBT_LINEAR_DW) && inner > 0) {
-            const int splits = choose(vocab, inner, p.most, dtype, true).splits;
-            if (splits > 1) partial = std::max(partial, 4 * splits * up(vocab, 256) * up(inner, 4));
+            p.dw = choose(vocab, inner, p.most, dtype, true);
+            if (p.dw.splits > 1) {
+                partial = std::max(partial, 4 * p.dw.splits * up(vocab, 256) * up(inner, 4));
+            } else if (p.dw.tile == 256) {
+                p.cut_dw = dw_cut(vocab, inner, p.most);
+                const int64_t m = p.cut_dw.m < vocab ? vocab - p.cut_dw.m : vocab, n = p.cut_dw.n < inner ? inner - p.cut_dw.n : inner;
+                if (p.cut_dw.splits > 1) partial = std::max(partial, 4 * p.cut_dw.splits * up(m, 256) * up(n, 4));
+            }
         }
         p.partial = take(partial);
     }
@@ -1243,6 +1282,13 @@ int32_t launch_logits(const char* who, LogitArgs p, int64_t rows, int64_t column
     return launch<T, kAsync, kLds>(who, logit_kernel<D, T, kAsync>, p, tiles, done, s);
 }
 
+template <int D, int OD, bool kRows>
+int32_t join_parts(const char* who, const GradArgs& p, hipStream_t s) {
+    const int64_t blocks = std::min<int64_t>((p.m * (p.ldp / 4) + 255) / 256, 4096);
+    grad_join_kernel<D, OD, kRows><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(p);
+    return check_launch(who);
+}
+
 template <int D, int OD, bool kRows, class T, bool kAsync>
 int32_t launch_grad_tile(const char* who, GradArgs& p, int64_t most_parts, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
@@ -1251,14 +1297,13 @@ int32_t launch_grad_tile(const char* who, GradArgs& p, int64_t most_parts, hipSt
     return launch<T, kAsync>(who, grad_kernel<D, OD, kRows, T, kAsync>, p, blocks, done, s);
 }
 
-// dW in tiles of 256, its last rows or columns in tiles of 128 where that is estimated to be shorter
-// (cut_of, which has the measurements).
+// dW in tiles of 256, its last rows or columns in a launch of their own: in parts of their sums, or
+// in tiles of 128.
 template <int D, int OD>
-int32_t launch_cut(const char* who, const GradArgs& p, hipStream_t s) {
-    const Cut cut = cut_of(p.m, p.n, p.k);
+int32_t launch_cut(const char* who, const GradArgs& p, const DwCut& cut, hipStream_t s) {
     GradArgs first = p, last = p;
     first.m = cut.m, first.n = cut.n;
-    const int32_t status = launch_grad_tile<D, OD, false, Tile256, true>(who, first, 0, s);
+    int32_t status = launch_grad_tile<D, OD, false, Tile256, true>(who, first, 0, s);
     if (status != HBT_OK || (cut.m == p.m && cut.n == p.n)) return status;
     const int64_t m0 = cut.m < p.m ? cut.m : 0, n0 = cut.n < p.n ? cut.n : 0;
     last.m -= m0, last.m_in -= m0, last.n -= n0, last.n_in -= n0;
@@ -1266,14 +1311,19 @@ int32_t launch_cut(const char* who, const GradArgs& p, hipStream_t s) {
     last.b = static_cast<const char*>(p.b) + n0 * elem_bytes<D>();
     last.y = static_cast<char*>(p.y) + (m0 * p.ldy + n0) * elem_bytes<OD>();
     if (p.before != nullptr) last.before = p.before + m0 * p.ldbefore + n0;
-    return launch_grad_tile<D, OD, false, Tile128, true>(who, last, 0, s);
+    if (cut.splits == 1) return launch_grad_tile<D, OD, false, Tile128, true>(who, last, 0, s);
+    last.splits = cut.splits;
+    last.ldp = up(last.n, 4);
+    status = launch_grad_tile<D, OD, false, Tile256, true>(who, last, 0, s);
+    return status != HBT_OK ? status : join_parts<D, OD, false>(who, last, s);
 }
 
 // p.m or p.k is the most that the piece's rows may be.  dx: `split` has its tile, and how many parts
-// there may be; dW's are chosen here.
+// there may be; dW: its choice, and its cut in tiles of 256.
 template <int D, int OD, bool kRows>
-int32_t launch_grad(const char* who, GradArgs& p, const SplitArgs& split, bool aligned, void* space, hipStream_t s) {
-    const Choice c = kRows ? Choice{split.tile, 1} : choose(p.m, p.n, p.k, D, aligned);
+int32_t launch_grad(const char* who, GradArgs& p, const SplitArgs& split, const Choice& dw, const DwCut& cut, bool aligned,
+                    void* space, hipStream_t s) {
+    const Choice c = kRows ? Choice{split.tile, 1} : dw;
     const int64_t parts = kRows ? split.most : 0;
     p.splits = c.splits;
     p.ldp = up(p.n, 4);
@@ -1287,15 +1337,13 @@ int32_t launch_grad(const char* who, GradArgs& p, const SplitArgs& split, bool a
                          : launch_grad_tile<D, OD, kRows, Tile128, false>(who, p, parts, s);
     } else if constexpr (D != F32) {
         if constexpr (!kRows) {
-            status = c.splits == 1 ? launch_cut<D, OD>(who, p, s) : launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, 0, s);
+            status = c.splits == 1 ? launch_cut<D, OD>(who, p, cut, s) : launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, 0, s);
         } else {
             status = launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, parts, s);
         }
     }
     if (status != HBT_OK || (c.splits == 1 && parts == 0)) return status;
-    const int64_t blocks = std::min<int64_t>((p.m * (p.ldp / 4) + 255) / 256, 4096);
-    grad_join_kernel<D, OD, kRows><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(p);
-    return check_launch(who);
+    return join_parts<D, OD, kRows>(who, p, s);
 }
 
 int32_t refuse(const char* who, const char* what) {
@@ -1442,7 +1490,7 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
             GradArgs g{};
             g.a = kept, g.b = w, g.y = c.dx, g.token = token, g.lda = plan.ldk, g.ldb = ldw, g.ldy = c.lddx;
             g.m = plan.most, g.n = c.inner, g.k = c.vocab, g.m_in = plan.most, g.n_in = plan.pad ? up(c.inner, 8) : c.inner, g.piece = piece;
-            if ((status = launch_grad<D, OD, true>(who, g, plan.split, aligned, at(plan.partial), s)) != HBT_OK) return status;
+            if ((status = launch_grad<D, OD, true>(who, g, plan.split, plan.dw, plan.cut_dw, aligned, at(plan.partial), s)) != HBT_OK) return status;
         }
         if ((c.wants & HBT_LINEAR_DW) && c.inner > 0) {
             GradArgs g{};
@@ -1454,10 +1502,10 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
             g.before = i > 0 ? carried : nullptr, g.ldbefore = ldcarried;
             if (last) {
                 g.y = c.dw, g.ldy = c.lddw;
-                status = launch_grad<D, OD, false>(who, g, plan.split, true, at(plan.partial), s);
+                status = launch_grad<D, OD, false>(who, g, plan.split, plan.dw, plan.cut_dw, true, at(plan.partial), s);
             } else {
                 g.y = carried, g.ldy = ldcarried;
-                status = launch_grad<D, F32, false>(who, g, plan.split, true, at(plan.partial), s);
+                status = launch_grad<D, F32, false>(who, g, plan.split, plan.dw, plan.cut_dw, true, at(plan.partial), s);
             }
             if (status != HBT_OK) return status;
         }

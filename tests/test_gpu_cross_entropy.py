@@ -427,6 +427,19 @@ def test_a_weight_past_32_bits():
     _close(dx, want, near)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("inner, vocab", [(700, 28501), (28501, 700)])
+def test_a_last_round_of_few_tiles(dtype, inner, vocab):
+    """336 tiles of 256 of the weight's gradient: a round, and 81 whose sums are split."""
+    x, w, b, target = _inputs(8192, inner, vocab, dtype, bias=True, ignored=0.01)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    found = torch.autograd.grad(linear_cross_entropy(x, w, target, b, reduction="sum"), leaves)
+    ones = torch.ones(8192, device=DEV)
+    _, _, grads, offs = _exact(x.detach(), w.detach(), b.detach(), target, grads=ones)
+    for g, want, off in zip(found, grads, offs):
+        _close(g, want, off)
+
+
 def test_gradients_against_differences():
     x, w, b, target = _inputs(6, 8, 40, torch.float32, bias=True)
     x64, w64, b64 = x.double(), w.double(), b.double()
