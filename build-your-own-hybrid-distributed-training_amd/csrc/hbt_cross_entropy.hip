@@ -390,6 +390,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
     static_assert(T::TM <= 8 && 16 * T::TN <= 255, "a byte a row");
     const auto begin = [&]() {
         int tm;
+        // Tile rows in eights take 6825 and 748 us at the two sizes above, in fours 6753 and 755, in sixteens 7020 and 758.
         band_order<8>(xcd_tile(t, total), tiles_m, p.tiles_n, tm, tn);
         m0 = int64_t(tm) * T::BM, n0 = p.column + int64_t(tn) * T::BN;
         const int tid = thread();
@@ -892,7 +893,11 @@ __global__ __launch_bounds__(T::kThreads, 2) void grad_kernel(GradArgs p) {
     const int total = tiles_m * p.tiles_n, split = total > 0 ? static_cast<int>(blockIdx.x) / total : splits;
     int tm, tn;
     if (split >= splits) return;
-    band_order<8>(xcd_tile(static_cast<int>(blockIdx.x) - split * total, total), tiles_m, p.tiles_n, tm, tn);
+    // Tile rows walked together, in us (8192 x 4096 x 128256, 8192 x 768 x 50257): dW in fours 7305 and 563, in
+    // eights 7450 and 574; dx in fours 6540 and 586, in eights 6455 and 600, 1801 x 1000 x 32003 138 and 133.
+    const int at = xcd_tile(static_cast<int>(blockIdx.x) - split * total, total);
+    if (!kRows || p.tiles_n < 4) band_order<4>(at, tiles_m, p.tiles_n, tm, tn);
+    else band_order<8>(at, tiles_m, p.tiles_n, tm, tn);
     const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
     constexpr int BK = tile_k<D>();
     const int64_t part = ((k + splits - 1) / splits + BK - 1) / BK * BK;
