@@ -38,7 +38,7 @@ constexpr int64_t kThinProducts = int64_t(1) << 31;
 // 1324 us without the copy and 641 with it, all gradients 3884 and 2291; 200 tokens 73 either way.  In
 // fp32 the matrix cores are the bound and a copy gains nothing (2048 x 1001 x 32003: 3265 and 3185 us).
 constexpr int64_t kPadTokens = 256;
-constexpr int64_t kMostRows = int64_t(1) << 22;    // rows of a piece: a launch over them stays within a grid
+constexpr int64_t kMostRows = kMaxLd;               // rows of a piece: a row of the turned hidden states
 constexpr int64_t kMostTokens = int64_t(1) << 24;
 constexpr int64_t kMostParts = 1024;               // tiles' sums of dx that a call has room for
 constexpr float kLog2e = 1.44269504f;
@@ -774,6 +774,47 @@ __global__ __launch_bounds__(1024) void total_kernel(const double* row_loss, con
     if (threadIdx.x == 0) loss[0] = static_cast<float>(divide ? sum / valid : sum);
 }
 
+// ---- hidden states with the tokens along a row ---------------------------------------------
+// A dW in tiles of 256 reads its piece's hidden states so: of its operands, dz and x, both lie with the
+// sum's index down the columns, and the transposing reads from LDS that this takes are slower than straight ones:
+// dW at 8192 x 4096 x 128256 6970 us and 27 for this copy, 7290 without; at 8192 x 768 x 50257 551, 7 and 580.
+// 64 x 64 values a workgroup; the tokens are filled up with zeros to a multiple of 64, of which the k-tiles are made.
+struct TurnArgs {
+    const uint16_t* rows;
+    uint16_t* turned;    // [inner][ldt]
+    int64_t ld, ldt, inner;
+    Piece piece;
+};
+__device__ __forceinline__ int whole_tiles(int count) { return (count + 63) / 64 * 64; }
+__global__ __launch_bounds__(256) void turn_kernel(TurnArgs p) {
+    constexpr int kStride = 33;  // words of a row: a column's values fall on distinct banks
+    __shared__ uint32_t tile[64 * kStride];
+    int first, count;
+    piece_rows(p.piece, first, count);
+    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+    if (r0 >= count) return;
+    for (int u = threadIdx.x; u < 512; u += 256) {
+        const int r = u / 8, at = u % 8;
+        u32x4 v = {0, 0, 0, 0};  // rows end in zeros, at a multiple of 64
+        if (r0 + r < count) v = *reinterpret_cast<const u32x4*>(p.rows + (first + r0 + r) * p.ld + c0 + at * 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tile[r * kStride + at * 4 + e] = v[e];
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < 512; u += 256) {
+        const int c = u / 8, at = u % 8;
+        if (c0 + c >= p.inner) break;
+        u32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t* word = tile + (at * 8 + 2 * e) * kStride + c / 2;
+            const int shift = c % 2 * 16;
+            v[e] = ((word[0] >> shift) & 0xFFFFu) | ((word[kStride] >> shift) << 16);
+        }
+        *reinterpret_cast<u32x4*>(p.turned + (c0 + c) * p.ldt + r0 + at * 8) = v;
+    }
+}
+
 // ---- exponentials to dz, in place ----------------------------------------------------------
 struct SoftmaxArgs {
     void* kept;
@@ -787,6 +828,7 @@ struct SoftmaxArgs {
     const double* row_loss;
     float* loss;  // the call's, of which the first workgroup takes the sum, or null
     int mean;
+    int whole;    // the rows are filled up with zeros to a multiple of 64
     Piece piece;
 };
 
@@ -817,15 +859,23 @@ __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs p) {
     constexpr int kSegment = 256 * kSoftmaxUnits * E;  // words a workgroup takes
     const int segments = static_cast<int>((p.ldk + kSegment - 1) / kSegment);
     const int i = block / segments, part = block % segments;
-    if (i >= count) return;
+    char* line = static_cast<char*>(p.kept) + int64_t(i) * p.ldk * B;
+    const int64_t first_word = (int64_t(part) * 256 * kSoftmaxUnits + threadIdx.x) * E;
+    if (i >= count) {
+        if (!p.whole || i >= whole_tiles(count)) return;
+#pragma unroll
+        for (int u = 0; u < kSoftmaxUnits; ++u) {
+            const int64_t j = first_word + u * 256 * E;
+            if (j < p.ldk) *reinterpret_cast<u32x4*>(line + j * B) = u32x4{0, 0, 0, 0};
+        }
+        return;
+    }
     const Row row = p.row[first + i];
     const int word = p.word[first + i];
     const float even = p.smoothing / static_cast<float>(p.vocab) * row.weight;
     const float hit = (expm1f(row.log_p) + p.smoothing) * row.weight - even;
     const bool known = word >= 0;
-    char* line = static_cast<char*>(p.kept) + int64_t(i) * p.ldk * B;
     const float2* stats = p.stats + i;
-    const int64_t first_word = (int64_t(part) * 256 * kSoftmaxUnits + threadIdx.x) * E;
     u32x4 units[kSoftmaxUnits];
 #pragma unroll
     for (int u = 0; u < kSoftmaxUnits; ++u) {
@@ -865,7 +915,8 @@ struct GradArgs {
     Piece piece;
 };
 
-// y = a b (dx: the rows of a are the piece's; dW: the sum runs over them), times the call's scale.
+// y = a b (dx: the rows of a are the piece's; dW: the sum runs over them, kTurned along b's rows), times the
+// call's scale.
 template <int D, int OD, bool kRows>
 struct GradEpilogue {
     const GradArgs& p;
@@ -881,30 +932,32 @@ struct GradEpilogue {
     }
 };
 
-// Bound by the matrix cores: at 8192 x 4096 x 128256 in bf16 dx takes 6.6 ms (1.31 PFLOP/s; the
-// library 6.35) and dW 7.6 (1.14; the library 7.5), whose operands both come through transposing LDS reads.
-template <int D, int OD, bool kRows, class T, bool kAsync>
+// Bound by the matrix cores: at 8192 x 4096 x 128256 in bf16 dx takes 6.5 ms (1.32 PFLOP/s; the
+// library 6.35) and dW 7.0 (1.23; the library 7.5).
+template <int D, int OD, bool kRows, bool kTurned, class T, bool kAsync>
 __global__ __launch_bounds__(T::kThreads, 2) void grad_kernel(GradArgs p) {
     extern __shared__ __align__(16) char lds[];
     int first, count;
     piece_rows(p.piece, first, count);
-    const int64_t m = kRows ? count : p.m, k = kRows ? p.k : count;
+    const int64_t m = kRows ? count : p.m, k = kRows ? p.k : kTurned ? whole_tiles(count) : count;
     const int tiles_m = static_cast<int>((m + T::BM - 1) / T::BM), splits = kRows ? p.piece.control->splits : p.splits;
     const int total = tiles_m * p.tiles_n, split = total > 0 ? static_cast<int>(blockIdx.x) / total : splits;
     int tm, tn;
     if (split >= splits) return;
-    // Tile rows walked together, in us (8192 x 4096 x 128256, 8192 x 768 x 50257): dW in fours 7305 and 563, in
-    // eights 7450 and 574; dx in fours 6540 and 586, in eights 6455 and 600, 1801 x 1000 x 32003 138 and 133.
+    // Tile rows walked together, in us (8192 x 4096 x 128256, 8192 x 768 x 50257): dW in twos 7120 and 552, in
+    // fours 7175 and 556, in eights 7420 and 560; dx in fours 6540 and 586, in eights 6455 and 600, 1801 x 1000 x 32003
+    // 138 and 133.
     const int at = xcd_tile(static_cast<int>(blockIdx.x) - split * total, total);
-    if (!kRows || p.tiles_n < 4) band_order<4>(at, tiles_m, p.tiles_n, tm, tn);
+    if (!kRows) band_order<2>(at, tiles_m, p.tiles_n, tm, tn);
+    else if (p.tiles_n < 4) band_order<4>(at, tiles_m, p.tiles_n, tm, tn);
     else band_order<8>(at, tiles_m, p.tiles_n, tm, tn);
     const int64_t m0 = int64_t(tm) * T::BM, n0 = int64_t(tn) * T::BN;
     constexpr int BK = tile_k<D>();
     const int64_t part = ((k + splits - 1) / splits + BK - 1) / BK * BK;
     const int64_t k0 = min<int64_t>(k, split * part), k1 = min<int64_t>(k, k0 + part);
     f32x4 acc[T::TM][T::TN];
-    const char* b = static_cast<const char*>(p.b) + (kRows ? 0 : first * p.ldb * elem_bytes<D>());
-    tile_product<D, kRows, false, T, kAsync>(p.a, p.lda, m0, kRows ? m : p.m_in, b, p.ldb, n0, p.n_in, k0, k1, lds, acc);
+    const char* b = static_cast<const char*>(p.b) + (kRows || kTurned ? 0 : first * p.ldb * elem_bytes<D>());
+    tile_product<D, kRows, kTurned, T, kAsync>(p.a, p.lda, m0, kRows ? m : p.m_in, b, p.ldb, n0, p.n_in, k0, k1, lds, acc);
     const int rows = static_cast<int>(min<int64_t>(m - m0, T::BM)), cols = static_cast<int>(min<int64_t>(p.n - n0, T::BN));
     const GradEpilogue<D, OD, kRows> tile{p, p.piece.control->scale_out, first};
     float* partial = splits == 1 ? nullptr : p.partial + (split * m + m0) * p.ldp + n0;
@@ -1158,8 +1211,9 @@ struct Plan {
     SplitArgs split;        // of dx
     Choice dw;
     DwCut cut_dw;
+    bool turned;            // dW reads hidden states with the tokens along a row
     int64_t control, place, token, word, weight, target, row, row_loss, rows, padded, stats, sums, kept, dw_sums, db_sums,
-        parts, partial, bytes;
+        parts, partial, turned_rows, bytes;
 };
 
 // Where the last, mostly empty round of tiles of 256 is better formed in tiles of 128: the words from
@@ -1232,7 +1286,7 @@ Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants,
     }
     if (p.grads) {
         p.row = take(sizeof(Row) * tokens);
-        p.kept = take(size * p.most * p.ldk);
+        p.kept = take(size * up(p.most, 64) * p.ldk);
         const bool carried = p.pieces > 1;
         if ((wants & HBT_LINEAR_DW) && carried && grad_dtype != F32) p.dw_sums = take(4 * vocab * inner);
         if (wants & HBT_LINEAR_DBIAS) {
@@ -1250,6 +1304,8 @@ Plan plan_of(int64_t tokens, int64_t inner, int64_t vocab, int dtype, int wants,
         }
         if ((wants & HBT_LINEAR_DW) && inner > 0) {
             p.dw = choose(vocab, inner, p.most, dtype, true);
+            p.turned = p.dw.tile == 256;
+            if (p.turned) p.turned_rows = take(size * inner * up(p.most, 64));
             if (p.dw.splits > 1) {
                 partial = std::max(partial, 4 * p.dw.splits * up(vocab, 256) * up(inner, 4));
             } else if (p.dw.tile == 256) {
@@ -1294,12 +1350,12 @@ int32_t join_parts(const char* who, const GradArgs& p, hipStream_t s) {
     return check_launch(who);
 }
 
-template <int D, int OD, bool kRows, class T, bool kAsync>
+template <int D, int OD, bool kRows, bool kTurned, class T, bool kAsync>
 int32_t launch_grad_tile(const char* who, GradArgs& p, int64_t most_parts, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
     p.tiles_n = static_cast<int>((p.n + T::BN - 1) / T::BN);
     const int64_t blocks = std::max((p.m + T::BM - 1) / T::BM * p.tiles_n * p.splits, most_parts);
-    return launch<T, kAsync>(who, grad_kernel<D, OD, kRows, T, kAsync>, p, blocks, done, s);
+    return launch<T, kAsync>(who, grad_kernel<D, OD, kRows, kTurned, T, kAsync>, p, blocks, done, s);
 }
 
 // dW in tiles of 256, its last rows or columns in a launch of their own: in parts of their sums, or
@@ -1308,18 +1364,18 @@ template <int D, int OD>
 int32_t launch_cut(const char* who, const GradArgs& p, const DwCut& cut, hipStream_t s) {
     GradArgs first = p, last = p;
     first.m = cut.m, first.n = cut.n;
-    int32_t status = launch_grad_tile<D, OD, false, Tile256, true>(who, first, 0, s);
+    int32_t status = launch_grad_tile<D, OD, false, true, Tile256, true>(who, first, 0, s);
     if (status != HBT_OK || (cut.m == p.m && cut.n == p.n)) return status;
     const int64_t m0 = cut.m < p.m ? cut.m : 0, n0 = cut.n < p.n ? cut.n : 0;
     last.m -= m0, last.m_in -= m0, last.n -= n0, last.n_in -= n0;
     last.a = static_cast<const char*>(p.a) + m0 * elem_bytes<D>();
-    last.b = static_cast<const char*>(p.b) + n0 * elem_bytes<D>();
+    last.b = static_cast<const char*>(p.b) + n0 * p.ldb * elem_bytes<D>();
     last.y = static_cast<char*>(p.y) + (m0 * p.ldy + n0) * elem_bytes<OD>();
     if (p.before != nullptr) last.before = p.before + m0 * p.ldbefore + n0;
-    if (cut.splits == 1) return launch_grad_tile<D, OD, false, Tile128, true>(who, last, 0, s);
+    if (cut.splits == 1) return launch_grad_tile<D, OD, false, true, Tile128, true>(who, last, 0, s);
     last.splits = cut.splits;
     last.ldp = up(last.n, 4);
-    status = launch_grad_tile<D, OD, false, Tile256, true>(who, last, 0, s);
+    status = launch_grad_tile<D, OD, false, true, Tile256, true>(who, last, 0, s);
     return status != HBT_OK ? status : join_parts<D, OD, false>(who, last, s);
 }
 
@@ -1335,16 +1391,17 @@ int32_t launch_grad(const char* who, GradArgs& p, const SplitArgs& split, const 
     p.partial = static_cast<float*>(space);
     int32_t status = HBT_OK;
     if (c.tile == 64) {
-        status = aligned ? launch_grad_tile<D, OD, kRows, Tile64, true>(who, p, parts, s)
-                         : launch_grad_tile<D, OD, kRows, Tile64, false>(who, p, parts, s);
+        status = aligned ? launch_grad_tile<D, OD, kRows, false, Tile64, true>(who, p, parts, s)
+                         : launch_grad_tile<D, OD, kRows, false, Tile64, false>(who, p, parts, s);
     } else if (c.tile == 128) {
-        status = aligned ? launch_grad_tile<D, OD, kRows, Tile128, true>(who, p, parts, s)
-                         : launch_grad_tile<D, OD, kRows, Tile128, false>(who, p, parts, s);
+        status = aligned ? launch_grad_tile<D, OD, kRows, false, Tile128, true>(who, p, parts, s)
+                         : launch_grad_tile<D, OD, kRows, false, Tile128, false>(who, p, parts, s);
     } else if constexpr (D != F32) {
         if constexpr (!kRows) {
-            status = c.splits == 1 ? launch_cut<D, OD>(who, p, cut, s) : launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, 0, s);
+            status = c.splits == 1 ? launch_cut<D, OD>(who, p, cut, s)
+                                   : launch_grad_tile<D, OD, kRows, true, Tile256, true>(who, p, 0, s);
         } else {
-            status = launch_grad_tile<D, OD, kRows, Tile256, true>(who, p, parts, s);
+            status = launch_grad_tile<D, OD, kRows, false, Tile256, true>(who, p, parts, s);
         }
     }
     if (status != HBT_OK || (c.splits == 1 && parts == 0)) return status;
@@ -1485,10 +1542,10 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
         if (!plan.grads) continue;
         const bool last = i + 1 == plan.pieces, totals = last && row_loss != nullptr && c.tokens <= kTotalTokens;
         const int64_t segment = 256 * kSoftmaxUnits * unit_elems<D>();
-        const int64_t blocks = (plan.ldk + segment - 1) / segment * plan.most + totals;
+        const int64_t blocks = (plan.ldk + segment - 1) / segment * (plan.turned ? up(plan.most, 64) : plan.most) + totals;
         softmax_kernel<D><<<dim3(static_cast<unsigned>(blocks)), 256, 0, s>>>(
             {kept, stats, row, word, plan.ldk, c.vocab, plan.most, plan.cut, plan.size, 128, c.smoothing, row_loss,
-             totals ? c.loss : nullptr, mean, piece});
+             totals ? c.loss : nullptr, mean, plan.turned, piece});
         if ((status = check_launch(who)) != HBT_OK) return status;
         if (totals) row_loss = nullptr;
         if ((c.wants & HBT_LINEAR_DX) && c.inner > 0) {
@@ -1501,6 +1558,13 @@ int32_t run(const char* who, const Call& c, const Plan& plan, char* space, hipSt
             GradArgs g{};
             g.a = kept, g.b = rows, g.lda = plan.ldk, g.ldb = plan.ld;
             g.m = c.vocab, g.n = c.inner, g.k = plan.most, g.m_in = up(c.vocab, 8), g.n_in = up(c.inner, 8), g.piece = piece;
+            if (plan.turned) {
+                g.b = at(plan.turned_rows), g.ldb = up(plan.most, 64), g.n_in = c.inner;
+                const dim3 grid(static_cast<unsigned>(g.ldb / 64), static_cast<unsigned>((c.inner + 63) / 64));
+                turn_kernel<<<grid, 256, 0, s>>>({static_cast<const uint16_t*>(rows), static_cast<uint16_t*>(at(plan.turned_rows)),
+                                                  plan.ld, g.ldb, c.inner, piece});
+                if ((status = check_launch(who)) != HBT_OK) return status;
+            }
             // Between pieces the sums stand dense in fp32: in working storage, or in an fp32 result.
             float* carried = OD == F32 ? static_cast<float*>(c.dw) : static_cast<float*>(at(plan.dw_sums));
             const int64_t ldcarried = OD == F32 ? c.lddw : c.inner;
