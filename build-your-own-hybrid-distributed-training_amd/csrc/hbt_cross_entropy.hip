@@ -1025,8 +1025,8 @@ __global__ __launch_bounds__(256) void bias_join_kernel(const float* parts, floa
 
 // ---- small calls --------------------------------------------------------------------------
 // Few tokens of a small model over a small vocabulary are launch latency: one workgroup does all of
-// a call in LDS, in fp32, where the kernels above are eleven launches (16 x 32 x 97 with a bias: 11 us on
-// the device; forward and backward by the host's clock 62 to 112, where the eleven take 156).
+// a call in LDS, in fp32, where the kernels above are ten launches (16 x 32 x 97 with a bias: 11 us on
+// the device; forward and backward by the host's clock 62 to 112, where eleven launches took 156).
 constexpr int kSmallTokens = 64, kSmallLds = 128 << 10;
 constexpr int64_t kSmallProduct = int64_t(1) << 17;  // multiplications of each product
 int64_t small_lds(int64_t tokens, int64_t inner, int64_t vocab) {
