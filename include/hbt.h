@@ -791,7 +791,8 @@ int32_t hbt_moments8_decode(void* const* codes, void* const* scales, void* const
  * `workspace` (256-byte aligned) holds at least hbt_linear_cross_entropy_workspace's bytes (-1
  * for sizes that the call refuses; `wants`: HBT_LINEAR_DX / DW / DBIAS of the gradients given;
  * `aligned`: whether w, ldw and inner are multiples of 16 bytes): at most 2 GiB of exponentials, the gathered
- * rows, an fp32 dw where there are more, and a copy of a 2-byte w that is not aligned.
+ * rows, for a large dw those of a piece once more, at most 256 MiB of partial sums of dx and as much as its
+ * last tiles take of dw's, an fp32 dw where there are more pieces, and a copy of a 2-byte w that is not aligned.
  * ---------------------------------------------------------------------------- */
 #define HBT_LOSS_NONE 0
 #define HBT_LOSS_MEAN 1
