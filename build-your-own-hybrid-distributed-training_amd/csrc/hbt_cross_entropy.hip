@@ -11,14 +11,15 @@
 // The logits of a tile never leave the workgroup that forms them: it takes each row's largest and
 // the sum of exp(z - largest) over its columns, and a row's tiles are joined afterwards.  For
 // gradients the tile also stores exp(z - largest), which needs only 16 bits (fp16: 2^-11 of a value
-// whose gradient is rounded by 2^-8 or 2^-11 next; fp32 for fp32 tensors), for a piece of the rows
+// whose gradient is rounded by 2^-8 or 2^-11 next, or 2^-25 of the tile's largest; fp32 for fp32 tensors), for a piece of the rows
 // at a time (at most kPieceBytes); one pass over a piece turns them into dz, rounded to the tensors' dtype
 // for the matrix cores, and the two products follow.  So the logits are formed once, 6 T V D operations in
 // all, where forming them again for the gradients would take 8.
 //
-// What a sum over pieces needs (dW, db) is carried in fp32.  A target's exponential is left out of its
-// tile's sum and joins the others' in fp64, from its fp32 logit: both the loss and the gradient 1 - p of a
-// nearly certain target are the others' sum, which fp32 or fp16 would round off beside a 1.
+// What a sum over pieces needs (dW, db) is carried in fp32.  A target is left out of its tile's largest
+// and sum, and its exponential joins the others' in fp64, from its fp32 logit: both the loss and the gradient
+// 1 - p of a nearly certain target are the others' sum, which fp32 or fp16 would round off beside a 1, and the
+// other words' exponentials would be subnormal in fp16, or zero, beside the target's.
 #include "hbt_matmul.hpp"
 
 namespace hbt {
@@ -468,15 +469,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
                     for (int e = 0; e < 4; ++e)
                         if (16 * j + 4 * q + e >= left) acc[i][j][e] = -INFINITY;
         }
-#pragma unroll
-        for (int i = 0; i < T::TM; ++i) {
-            float top = fmaxf(fmaxf(acc[i][0][0], acc[i][0][1]), fmaxf(acc[i][0][2], acc[i][0][3]));
-#pragma unroll
-            for (int j = 1; j < T::TN; ++j)
-                top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
-            top = quarters_max(top);
-            if (q == 0) line[slot + 16 * i] = top;
-        }
+        // The target leaves before the largest is taken: far above the others, it would push their exponentials
+        // under fp16's smallest.
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) {
             const int at = (targets[i / 4] >> (8 * (i % 4))) & 255;
@@ -489,6 +483,15 @@ __global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
                         if (at == 16 * j + 4 * q + e) z = acc[i][j][e], acc[i][j][e] = -INFINITY;
                 if (at != 255 && ((at >> 2) & 3) == q && wm + 16 * i < rows) p.target[first + m + wm + 16 * i] = z;
             }
+        }
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
+            float top = fmaxf(fmaxf(acc[i][0][0], acc[i][0][1]), fmaxf(acc[i][0][2], acc[i][0][3]));
+#pragma unroll
+            for (int j = 1; j < T::TN; ++j)
+                top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
+            top = quarters_max(top);
+            if (q == 0) line[slot + 16 * i] = top;
         }
         __syncthreads();
 #pragma unroll
@@ -608,8 +611,8 @@ __global__ __launch_bounds__(512) void thin_logit_kernel(const void* x_, int64_t
     for (int e = 0; e < 4; ++e) {
         if (e < have) sum += acc[e];
         acc[e] = e < have ? in_units<D>(acc[e]) : -INFINITY;
-        top = fmaxf(top, acc[e]);
         if (at == e && e < have) target_logit[row] = acc[e], acc[e] = -INFINITY;
+        top = fmaxf(top, acc[e]);
     }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));

@@ -785,7 +785,10 @@ int32_t hbt_moments8_decode(void* const* codes, void* const* scales, void* const
  * number (gradients are zeros without any).  `factor`: NULL for 1, or one fp32 in device memory that
  * multiplies every c_i (the loss's own gradient).
  * dx, dw and dbias may each be NULL; they are of grad_dtype: dtype, or F32.  Sums and statistics are
- * fp32 or wider; dz is rounded to `dtype` once, for the matrix cores.  No atomics: results
+ * fp32 or wider; dz is rounded to `dtype` once, for the matrix cores.  Before that a 2-byte dtype's
+ * probabilities are held in fp16: to 2^-11 of themselves, or to 2^-25 of the largest one, the target's aside, of the
+ * up to 256 words beside it.  F16 dz stand at one power of two for the whole call, where the largest |c_i| is 2^13
+ * to 2^14: those under 2^-14 are held to 2^-25, so a token whose c_i is far under the largest keeps fewer digits.  No atomics: results
  * repeat bitwise.  Rows are at most 2^20 elements apart, vocab and inner at most 2^20 - 64, tokens
  * from 1 to 2^24.
  * `workspace` (256-byte aligned) holds at least hbt_linear_cross_entropy_workspace's bytes (-1
