@@ -681,7 +681,7 @@ __device__ __forceinline__ void finish_row(const JoinArgs& p, int row, Running r
     if (known) r.add(z, 1.0, unit);
     const double log_sum = log(r.sum);
     double log_p = (static_cast<double>(z) - r.top) * p.unit - log_sum;
-    if (z >= others.top && z < INFINITY)  // the others beside a 1, which would round them off
+    if (z >= others.top && fabsf(z) < INFINITY)  // the others beside a 1, which would round them off
         log_p = others.sum == 0.0 ? 0.0 : -log1p(others.sum * expf((others.top - z) * unit));
     double loss = -(1.0 - p.smoothing) * log_p;
     if (p.smoothing != 0.0f) loss += p.smoothing * ((r.top * p.unit + log_sum) - logits / static_cast<double>(p.vocab));

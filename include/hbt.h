@@ -778,7 +778,7 @@ int32_t hbt_moments8_decode(void* const* codes, void* const* scales, void* const
  *   dx = dz w,  dw = dz^T x,  dbias = column sums of dz
  * A token whose target is ignore_index has loss 0, a zero row of dx and no part in the rest,
  * whatever its row of x holds.  Any other target outside [0, vocab) makes its loss, and every
- * gradient that the token takes part in, NaN.
+ * gradient that the token takes part in, NaN; so does a row whose logits are all -inf.
  * reduction HBT_LOSS_NONE: loss is [tokens] fp32 (NULL for the gradients alone) and c_i =
  * token_grads[i] (fp32; NULL = 1).  HBT_LOSS_SUM: loss is one fp32, c_i = 1.  HBT_LOSS_MEAN:
  * its quotient by the number of tokens that are not ignored (0 / 0, NaN, without any), c_i one over that
