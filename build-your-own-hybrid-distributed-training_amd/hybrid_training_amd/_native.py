@@ -70,7 +70,7 @@ __all__ = [
     "stream_of",
 ]
 
-ABI_VERSION = 25
+ABI_VERSION = 26
 MAX_TENSORS_PER_LAUNCH = 16
 MAX_MATRICES = 32
 MAX_ADAMW8_TENSORS = 80
@@ -326,6 +326,11 @@ EXPORTED_SYMBOLS: dict[str, tuple[object, tuple[object, ...]]] = {
         _c_i32,
         (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_i32, _c_f32, _c_void_p, _c_f32,
          _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_void_p, _c_i32, _c_void_p),
+    ),
+    "hbt_adamw8_step_numbered": (
+        _c_i32,
+        (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_i32, _c_i32, _c_f32, _c_void_p, _c_f32,
+         _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, ctypes.c_uint32, _c_void_p, _c_i32, _c_void_p),
     ),
     "hbt_moments8_encode": (
         _c_i32, (_ptr_array, _ptr_array, _ptr_array, _ptr_array, _i64_array, _c_i32, _c_void_p)),

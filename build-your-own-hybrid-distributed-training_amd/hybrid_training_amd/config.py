@@ -182,7 +182,9 @@ class OptimizerConfig:
 
     ``state_format`` (no counterpart in the reference) says how AdamW's moments are held: ``"master"``
     in the parameter's dtype, as the reference does, or ``"8bit"`` in two bytes an element
-    with float32 scales for each 256 (float32, bfloat16 or float16 masters in device memory).
+    with float32 scales for each 256 (float32, bfloat16 or float16 masters in device memory).  Those
+    moments have 4 and 5 significant bits; from step 17 on, what rounding to nearest would lose from step to
+    step is rounded without bias instead (at the default ``betas`` all second moments).
     """
 
     name: str = "adamw"

@@ -1,11 +1,16 @@
 """AdamW's moments held in 8 bits: the state tensors of one parameter and the calls that read
-and write them (``hbt_adamw8_step``, ``hbt_moments8_encode``, ``hbt_moments8_decode``).
+and write them (``hbt_adamw8_step_numbered``, ``hbt_moments8_encode``, ``hbt_moments8_decode``).
 
 ``ShardedOptimizer`` holds its state this way with ``OptimizerConfig(state_format="8bit")``.  Every
 256 consecutive elements share two float32 scales, the largest first moment and the largest root of a second
 moment among them; beside these an element takes one byte for its first moment (e4m3, 4
 significant bits) and one for the root of its second (5 significant bits): 2.03 bytes of state an
 element instead of 8.
+
+A code is rounded to nearest where a step moves it by more than rounding can lose; elsewhere, as for
+the roots at the default beta2 of 0.999, without bias, by random numbers that follow from the step and the
+element's place: a root is then off by up to an eighth of itself, as often up as down, and equal runs
+stay equal bit by bit.
 """
 
 from __future__ import annotations

@@ -39,7 +39,7 @@ and the HBM traffic of a clipped fp32 step:
   written; ``.grad`` keeps the unclipped values.  32 B/element.
 
 With ``OptimizerConfig(state_format="8bit")`` AdamW's moments are held in 8 bits each
-(``hbt_adamw8_step``, :mod:`~hybrid_training_amd.moments8`): 16 B/element instead of 28 for the
+(``hbt_adamw8_step_numbered``, :mod:`~hybrid_training_amd.moments8`): 16 B/element instead of 28 for the
 update of fp32 masters.  The clip, its placements, the loss scaler and recorded steps work as above, and the
 state dict holds float32 moments, so a run can change between the formats.
 """
@@ -765,11 +765,11 @@ def _adamw_scalars(group: dict, step: float) -> tuple[float, ...]:
     return (decay, 1 - beta1, beta2, 1 - beta2, bias_correction2_sqrt, float(group["eps"]), -step_size)
 
 
-def _adamw8_scalars(scalars: tuple[float, ...]) -> tuple[float, ...]:
-    """:func:`_adamw_scalars` as ``hbt_adamw8_step`` takes them: the second bias correction as a
-    factor."""
-    decay, lerp, beta2, one_minus_beta2, root, eps, neg_step = scalars
-    return decay, lerp, beta2, one_minus_beta2, 1.0 / root, eps, neg_step
+def _adamw8_scalars(group: dict, step: float) -> tuple[float, ...]:
+    """:func:`_adamw_scalars` as ``hbt_adamw8_step_numbered`` takes them: the second bias correction as a
+    factor, and the step's number, by which moments are rounded."""
+    decay, lerp, beta2, one_minus_beta2, root, eps, neg_step = _adamw_scalars(group, step)
+    return decay, lerp, beta2, one_minus_beta2, 1.0 / root, eps, neg_step, int(max(0.0, min(step, 4294967295.0)))
 
 
 def _sgd_scalars(group: dict) -> tuple[tuple[float, ...], int]:
@@ -817,6 +817,7 @@ class _RecordedAdamW:
     eager step does to the host state: advance the parameters' step counters."""
 
     _KEYS: tuple[str, ...] = ("exp_avg", "exp_avg_sq")
+    _scalars = staticmethod(_adamw_scalars)
 
     def __init__(self, optimizer: "ShardedOptimizer", slot: torch.Tensor, record: int, params: list[nn.Parameter],
                  pdtype: torch.dtype, unscale: float, scalars: tuple[float, ...]) -> None:
@@ -842,7 +843,7 @@ class _RecordedAdamW:
         states = [opt._optimizer.state[p] for p in self._params]
         self._operands.check(states)
         nexts = [_next_step(s["step"]) for s in states]
-        found = {_adamw_scalars(groups[id(p)], step) for p in self._params for step in set(nexts)}
+        found = {self._scalars(groups[id(p)], step) for p in self._params for step in set(nexts)}
         if len(found) != 1:
             raise _replay_error("the parameters recorded in one launch no longer share their step scalars")
         scalars = found.pop()
@@ -869,13 +870,15 @@ class _RecordedAdamW:
 
 
 class _RecordedAdamW8(_RecordedAdamW):
-    """The same over moments in 8 bits, whose slot holds the call's eight scalars in order."""
+    """The same over moments in 8 bits, whose slot holds the call's eight scalars in order and the step's number."""
 
     _KEYS = moments8.STATE_KEYS
+    _scalars = staticmethod(_adamw8_scalars)
 
     def _format(self, scalars: tuple[float, ...]) -> None:
-        values = (self._unscale, *_adamw8_scalars(scalars))
-        ctypes.memmove(self._record, (ctypes.c_float * len(values))(*values), 4 * len(values))
+        *values, number = scalars
+        ctypes.memmove(self._record, (ctypes.c_float * 8)(self._unscale, *values), 32)
+        ctypes.memmove(self._record + 32, ctypes.byref(ctypes.c_uint32(number)), 4)
 
 
 class _RecordedSgd:
@@ -1335,6 +1338,7 @@ class ShardedOptimizer:
         lib = _native.library()
         recording = self._recording_check()
         batches: dict[tuple, list[tuple[nn.Parameter, torch.Tensor, dict]]] = {}
+        form = _adamw8_scalars if self._eight_bit else _adamw_scalars
         formed: dict[tuple[int, float], tuple[float, ...]] = {}  # scalars per group and step count
         for group, p, grad, state in self._stepped_parameters():
             if not state:
@@ -1356,7 +1360,7 @@ class ShardedOptimizer:
                 step = _next_step(step_t)  # the step each replay advances to
             scalars = formed.get((id(group), step))
             if scalars is None:
-                scalars = formed[(id(group), step)] = _adamw_scalars(group, step)
+                scalars = formed[(id(group), step)] = form(group, step)
             key = (scalars, p.dtype, grad.dtype, _pending_unscale(grad))
             batches.setdefault(key, []).append((p, grad, state))
         stream = _native.stream_of(self._device)
@@ -1397,16 +1401,15 @@ class ShardedOptimizer:
     def _launch_adamw8(self, batch, scalars, pdtype, gdtype, unscale, mul_ptr, flags, stream, slot) -> None:
         """The update of ``(parameter, gradient, state)`` entries that share their scalars."""
         lib = _native.library()
-        scalars = _adamw8_scalars(scalars)
         for start in range(0, len(batch), _native.MAX_ADAMW8_TENSORS):
             chunk = batch[start : start + _native.MAX_ADAMW8_TENSORS]
             params, states = [p for p, _, _ in chunk], [s for _, _, s in chunk]
-            _native.check(lib.hbt_adamw8_step(
+            _native.check(lib.hbt_adamw8_step_numbered(
                 _native.pointer_array([p.data_ptr() for p in params]),
                 _native.pointer_array([g.data_ptr() for _, g, _ in chunk]), *moments8.tables(states),
                 _native.int64_array([p.numel() for p in params]), len(chunk), _native.dtype_code(pdtype),
                 _native.dtype_code(gdtype), unscale, mul_ptr, *scalars, None if slot is None else slot.data_ptr(),
-                flags, stream), "optim.hbt_adamw8_step")
+                flags, stream), "optim.hbt_adamw8_step_numbered")
             increment_version(params + [s[key] for s in states for key in moments8.STATE_KEYS])
 
     def _recording_check(self) -> "_native.GraphRecording | None":

@@ -751,6 +751,12 @@ int32_t hbt_muon_step(void* const* params, const void* const* grads, float* cons
  * and m and r are encoded.  `slot`: NULL, or device memory holding the fp32 unscale, decay,
  * lerp_weight, beta2, one_minus_beta2, inverse_bias_correction2_sqrt, eps and neg_step_size,
  * read in place of the arguments when the kernels run, for a step recorded into a HIP graph.
+ * Nearest codes do not carry changes of less than half a code from step to step.
+ * hbt_adamw8_step_numbered: the same for step number `step` of a run, from 1 (in the slot a ninth
+ * word, uint32; 0: as hbt_adamw8_step).  From step 17 on it takes one of the two codes around a
+ * value, the upper one with the probability that leaves no bias, for first moments and roots under
+ * 2^-14 of their block's scale, for all first moments where |lerp_weight| < 1/16 and for all roots
+ * where one_minus_beta2 < 0.04; its random numbers follow from `step` and an element's index alone.
  * hbt_moments8_encode and hbt_moments8_decode convert fp32 moments to codes, and codes to
  * moments of out_dtype (F32, or BF16).  Encoding what was decoded to F32 gives the same codes and scales,
  * second moments under 2^-126 aside.
@@ -760,6 +766,11 @@ int32_t hbt_adamw8_step(void* const* params, void* const* grads, void* const* co
                         const float* grad_mul, float decay, float lerp_weight, float beta2, float one_minus_beta2,
                         float inverse_bias_correction2_sqrt, float eps, float neg_step_size, const float* slot,
                         int32_t flags, void* stream);
+int32_t hbt_adamw8_step_numbered(void* const* params, void* const* grads, void* const* codes, void* const* scales,
+                                 const int64_t* numels, int32_t count, int32_t param_dtype, int32_t grad_dtype,
+                                 float unscale, const float* grad_mul, float decay, float lerp_weight, float beta2,
+                                 float one_minus_beta2, float inverse_bias_correction2_sqrt, float eps,
+                                 float neg_step_size, uint32_t step, const float* slot, int32_t flags, void* stream);
 int32_t hbt_moments8_encode(const void* const* firsts, const void* const* seconds, void* const* codes,
                             void* const* scales, const int64_t* numels, int32_t count, void* stream);
 int32_t hbt_moments8_decode(void* const* codes, void* const* scales, void* const* firsts, void* const* seconds,
