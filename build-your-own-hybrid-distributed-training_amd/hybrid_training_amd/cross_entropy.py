@@ -42,9 +42,11 @@ _MAX_SIDE, _MAX_TOKENS = (1 << 20) - 64, 1 << 24
 _WHO = "cross_entropy.linear_cross_entropy"
 #: Gradients of float16 tensors are computed in the forward pass and held in float32 from so many tokens
 #: on, or for weights of fewer elements.  For few tokens of a large weight, writing and reading its
-#: gradient costs more than forming the logits again: 64 x 4096 x 128256 take 1732 us held and 1204 us
-#: not, 1024 tokens 3999 and 4171; 500 x 1000 x 5000 take 146 and 161.
-_HOLD_TOKENS, _HOLD_ELEMENTS = 768, 1 << 24
+#: gradient costs more than forming the logits again.  Held and not, in us, for 32, 512, 768 and 1024 tokens:
+#: 50257 x 768 (39M elements) 207 and 234, 353 and 376, 419 and 449, 480 and 532; 32768 x 2048 (67M) 294 and 260, 436
+#: and 408, 541 and 552, 610 and 641; 128256 x 2048 921 and 716, 1439 and 1356, 1801 and 1861, 2153 and 2295;
+#: 128256 x 4096 (525M) 1683 and 1219, 2635 and 2451, 3362 and 3405, 4017 and 4248.
+_HOLD_TOKENS, _HOLD_ELEMENTS = 768, 3 << 24
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None, reduction: str,
