@@ -23,7 +23,9 @@
 // and 10% each (26% while they fall 20 times).  What else there is is rounded to nearest, which holds each value closer and
 // where steps are as large as codes loses nothing: roots at beta2 = 0.95 0.7% off on average and 4.5% each (without
 // bias 0.1 and 6.4), at 0.97 2.0 and 5.6 (0.2 and 7.6), at 0.98 6.4 and 9.2 (0.4 and 8.6).  The first 16 steps, in which
-// a running sum grows by 1/(2t) a step, half a root's code or more, round to nearest too.
+// a running sum grows by 1/(2t) a step, half a root's code or more, round to nearest too.  (Up to beta2 = 0.96 a
+// root falls past its block's largest because that one, the scale, changes a little with every step, as gradients of
+// batches make it; beside one that never changes it could stop at a code of the octave where it began.)
 //
 // A block's largest element is held exactly (256 M / 256, 1 R), so a decay that all elements share
 // is carried by the scales without rounding, and encoding what was decoded gives the same codes.
@@ -244,11 +246,12 @@ __device__ __forceinline__ void wait_for_loads() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// A wavefront a block.  With fp32 gradients each stream is waited for before the next one is
-// asked for: 1,003,782,656 elements take 2647 us (6.1 TB/s), 2790 with all loads in flight together.
+// A wavefront a block; 1,003,782,656 elements in fp32 at betas (0.9, 0.95) take 2731 us (5.9 TB/s).  With fp32
+// gradients each stream is waited for before the next one is asked for (all to nearest: 2647 us, 2790 with all loads
+// in flight together).
 // 2-byte gradients leave less to move for the same arithmetic (a correctly rounded root and division an
-// element), which the loads then have to hide behind: 2335 us together and the gradient last (bf16, 6.0 TB/s),
-// 2475 one after another.
+// element), which the loads then have to hide behind (all to nearest: 2335 us together and the gradient last, 2475 one
+// after another; fp32 masters and bf16 gradients, 2^29 elements, now 1339 us, 5.6 TB/s).
 template <int PD, int GD, bool kWriteBack>
 __global__ __launch_bounds__(64) void adamw8_kernel(Table tab, Scalars s, uint32_t step, const Slot* __restrict__ slot,
                                                     bool numbered, const float* __restrict__ grad_mul, int64_t tile_base) {

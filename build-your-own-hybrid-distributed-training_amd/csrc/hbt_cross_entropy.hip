@@ -359,8 +359,8 @@ __device__ __forceinline__ void pair_columns(uint32_t& a, uint32_t& b) {
 // one workgroup a CU, and the first loads of its next tile are in flight while it reduces this one's logits
 // (8192 x 768 x 50257: a workgroup a tile takes 7% more).
 //
-// Bound by the matrix cores: in bf16 8192 x 4096 x 128256 takes 6.7 to 6.8 ms with the exponentials (1.28
-// PFLOP/s; the library's product alone 6.05), 8192 x 768 x 50257 760 to 800 us, 584 without them, an eighth
+// Bound by the matrix cores: in bf16 8192 x 4096 x 128256 takes 6.86 ms with the exponentials (1.25
+// PFLOP/s; the library's product alone 6.06), 8192 x 768 x 50257 763 us, 584 without them, an eighth
 // of it the reduction.  Logits passed through LDS, a row a wavefront, take 14 to 16 us a tile more.
 template <int D, class T, bool kAsync>
 __global__ __launch_bounds__(T::kThreads, 2) void logit_kernel(LogitArgs p) {
@@ -839,8 +839,8 @@ struct SoftmaxArgs {
 // x 5003 in fp32: 175 us for 178); by one workgroup of 256 more would outlast it.
 constexpr int64_t kTotalTokens = 16384;
 constexpr int kSoftmaxUnits = 2;  // 16-byte units a lane
-// Bound by memory: a read and a write of 2 bytes (fp32: 4) an element, 8192 x 128256 in bf16 in 745 us
-// (5.6 TB/s), 8192 x 50257 in 297.  Two units a lane, read past the caches: as they are written 780 and 307;
+// Bound by memory: a read and a write of 2 bytes (fp32: 4) an element, 8192 x 128256 in bf16 in 741 us
+// (5.6 TB/s), 8192 x 50257 in 293.  Two units a lane, read past the caches: as they are written 780 and 307;
 // four in a loop 815 and 317; one 710 and 315, but 52 for 44 where two fifths of the rows are none.
 template <int D>
 __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs p) {
@@ -935,8 +935,8 @@ struct GradEpilogue {
     }
 };
 
-// Bound by the matrix cores: at 8192 x 4096 x 128256 in bf16 dx takes 6.5 ms (1.32 PFLOP/s; the
-// library 6.35) and dW 7.0 (1.23; the library 7.5).
+// Bound by the matrix cores: at 8192 x 4096 x 128256 in bf16 dx takes 6.66 ms (1.29 PFLOP/s; the
+// library 6.54) and dW 7.09 (1.21; the library 7.58).
 template <int D, int OD, bool kRows, bool kTurned, class T, bool kAsync>
 __global__ __launch_bounds__(T::kThreads, 2) void grad_kernel(GradArgs p) {
     extern __shared__ __align__(16) char lds[];
