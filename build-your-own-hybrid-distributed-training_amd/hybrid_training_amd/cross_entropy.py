@@ -12,7 +12,9 @@ word and hidden value instead of 8.  Separate losses (``reduction="none"``), who
 known only then, and few float16 tokens of a large weight form the logits again in the backward pass.
 
 Sums and statistics are float32 or wider, and so is the loss.  The gradient of the logits is rounded once to the
-tensors' dtype, for the matrix cores.  Gradients of bfloat16 tensors are held rounded between
+tensors' dtype, for the matrix cores; before that the probabilities of 2-byte tensors are held in fp16, to 2^-11 of
+themselves or 2^-25 of the largest one beside them, the target's aside.  float16's gradients of separate losses share
+one power of two, so tokens whose loss counts far less than the largest one's keep fewer digits.  Gradients of bfloat16 tensors are held rounded between
 the passes, so a loss scaled by anything but a power of two rounds them twice; those of float16
 tensors are held in float32, and a loss scale keeps what float16 alone would flush to zero.  No
 atomics run, so equal inputs give equal bits.
@@ -235,7 +237,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     ``"sum"``, ``"none"``) and ``label_smoothing`` are ``torch.nn.functional.cross_entropy``'s.  An
     ignored token has no part in anything, whatever its row of ``x`` holds, and costs nothing but
     its look at the target; a mean over none is NaN, with zero gradients.  A target out of range makes its
-    loss and the gradients NaN.  Any strides are accepted, as by :func:`fused_linear`.
+    loss and the gradients NaN, and so does a row whose logits are all -inf.  Any strides are accepted, as by :func:`fused_linear`.
 
     With gradients wanted, a summed or averaged loss computes them here (see the module), so call
     it under ``torch.no_grad()`` to evaluate.  Before a step is recorded (:class:`StepGraph`), let go of the
